@@ -26,7 +26,8 @@ BD_OUT_BF16, BD_OUT_F16, BD_OUT_F32 = 0, 1, 2
 BD_EPI_NONE, BD_EPI_BIAS, BD_EPI_BIAS_RELU, BD_EPI_BIAS_SILU, BD_EPI_BIAS_GELU = 0, 1, 2, 3, 4
 BD_SPLIT_REDUCE, BD_SPLIT_PLANES, BD_SPLIT_ATOMIC = 0, 1, 2
 BD_GEMM_OVERLAP_PREV, BD_GEMM_WEIGHTS_STATIC, BD_GEMM_B_E4M3, BD_GEMM_SINGLE_CTA = 1, 2, 4, 8
-BD_IN_F32, BD_IN_BF16 = 0, 1
+BD_IN_F32, BD_IN_BF16, BD_IN_F16 = 0, 1, 2
+BD_FP4_NVFP4, BD_FP4_MXFP4 = 0, 1
 BD_DEVERR_WAIT_MASK, BD_DEVERR_WAIT_TMA, BD_DEVERR_NONFINITE, BD_DEVERR_RANGE = 0x1F, 0x01, 0x20, 0x40
 
 # name -> (restype, argtypes); mirrors include/bitdance_b200.h
@@ -54,6 +55,14 @@ SIGNATURES = {
     "bd_w4a6_gemm_ex": (_I, [_P, _P, _P, _P, _P, _F, _P, _I, _I, _I, _I, _I, _I, _I, _P, _SZ,
                              ctypes.c_uint, _P]),
     "bd_w4a6_gemm_noalloc": (_I, [_P, _P, _P, _P, _P, _F, _P, _I, _I, _I, _I, _I, _P]),
+    "bd_query_fp4_scales": (_SZ, [_I, _I, _I]),
+    "bd_quantize_fp4": (_I, [_P, _I, _I, _P, _P, _P, _P, _I, _I, ctypes.c_uint, _P]),
+    "bd_tile_scales_fp4": (_I, [_P, _P, _I, _I, _I, _P]),
+    "bd_dequantize_fp4": (_I, [_P, _P, _P, _F, _P, _I, _I, _I, _I, ctypes.c_uint, _P]),
+    "bd_w4a4_gemm": (_I, [_P, _P, _P, _P, _P, _P, _P, _F, _P, _I, _I, _I, _I, _I, _I,
+                          ctypes.c_uint, _P]),
+    "bd_query_w4a4_linear_workspace": (_SZ, [_I, _I, _I]),
+    "bd_w4a4_linear": (_I, [_P, _P, _I, _P, _P, _P, _F, _P, _I, _I, _I, _I, _I, _I, _P, _SZ, _P]),
     "bd_splitk_reduce": (_I, [_P, _P, _P, _F, _I, _I, _I, _I, _I, _P]),
 }
 

@@ -5,11 +5,12 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libbitdance_b200.so")
-SOURCES = [os.path.join(CSRC, "bitdance.cu")]
+SOURCES = [os.path.join(CSRC, f) for f in ("bitdance.cu", "fp4.cu")]
 HEADERS = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared"]
@@ -22,22 +23,35 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
+def _newest_header() -> float:
+    inc = os.path.join(os.path.dirname(HERE), "include", "bitdance_b200.h")
+    return max(os.path.getmtime(f) for f in HEADERS + [inc])
+
+
 def stale() -> bool:
     if not os.path.exists(LIB):
         return True
     t = os.path.getmtime(LIB)
-    inc = os.path.join(os.path.dirname(HERE), "include", "bitdance_b200.h")
-    return any(os.path.getmtime(f) > t for f in SOURCES + HEADERS + [inc])
+    return _newest_header() > t or any(os.path.getmtime(f) > t for f in SOURCES)
+
+
+def _run(cmd) -> str:
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"nvcc failed:\n{r.stdout}\n{r.stderr}")
+    return r.stderr
 
 
 def build_library(force: bool = False, verbose: bool = False) -> str:
     if force or stale():
-        cmd = [nvcc(), *NVCC_FLAGS, "-o", LIB, *SOURCES]
+        flags = [f for f in NVCC_FLAGS if f != "-shared"] + (["-Xptxas=-v"] if verbose else [])
+        objs = [os.path.splitext(f)[0] + ".o" for f in SOURCES]
+        with ThreadPoolExecutor(len(SOURCES)) as pool:  # one nvcc per source
+            logs = list(pool.map(lambda so: _run([nvcc(), *flags, "-c", "-o", so[1], so[0]]),
+                                 zip(SOURCES, objs)))
+        _run([nvcc(), *NVCC_FLAGS, "-o", LIB, *objs])
+        for o in objs:
+            os.remove(o)
         if verbose:
-            cmd.insert(1, "-Xptxas=-v")
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed:\n{r.stdout}\n{r.stderr}")
-        if verbose:
-            print(r.stderr)
+            print("".join(logs))
     return LIB

@@ -11,6 +11,7 @@
 
 #include "../../include/bitdance_b200.h"
 #include "gemm.cuh"
+#include "host.cuh"
 #include "probe.cuh"
 #include "quantize_b.cuh"
 #include "sm100.cuh"
@@ -22,24 +23,9 @@ namespace bd {
 __device__ uint32_t g_err_word;
 
 namespace {
-
-constexpr int kMaxDevices = 64;
-
-inline cudaStream_t as_stream(bd_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
-
-inline bool aligned(const void* p, uintptr_t a) {
-  return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
-}
-
-// Per-device facts, computed once.
-struct DeviceInfo {
-  int sm_count = 0;
-  bool is_sm100 = false;
-  uint32_t* err = nullptr;
-  bool ready = false;
-};
 DeviceInfo g_dev[kMaxDevices];
 std::mutex g_dev_mu;
+}  // namespace
 
 int device_info(DeviceInfo** out) {
   int dev = 0;
@@ -61,6 +47,8 @@ int device_info(DeviceInfo** out) {
   *out = &d;
   return d.is_sm100 ? BD_OK : BD_ERR_ARCH;
 }
+
+namespace {
 
 // Diagnostic of the bounded waits: warp 0 waits on an mbarrier that nothing arrives at, with
 // a limit of `limit` cycles, and so records kErrWaitTma and raises the abort flag; warp 1 waits
@@ -129,6 +117,8 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
+}  // namespace
+
 bool make_map_2d(CUtensorMap* m, CUtensorMapDataType dt, void* base, uint64_t d0, uint64_t d1,
                  uint64_t stride1_bytes, uint32_t b0, uint32_t b1, CUtensorMapSwizzle sw) {
   EncodeTiledFn fn = encode_fn();
@@ -140,6 +130,8 @@ bool make_map_2d(CUtensorMap* m, CUtensorMapDataType dt, void* base, uint64_t d0
   return fn(m, dt, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+namespace {
 
 bool make_map_3d(CUtensorMap* m, CUtensorMapDataType dt, void* base, uint64_t d0, uint64_t d1,
                  uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0,
@@ -154,12 +146,16 @@ bool make_map_3d(CUtensorMap* m, CUtensorMapDataType dt, void* base, uint64_t d0
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+}  // namespace
+
 int grid_for(int64_t work, int per_block, const DeviceInfo* d) {
   int64_t blocks = (work + per_block - 1) / per_block;
   const int64_t cap = static_cast<int64_t>(d->sm_count) * 8;
   if (blocks > cap) blocks = cap;
   return static_cast<int>(blocks < 1 ? 1 : blocks);
 }
+
+namespace {
 
 // Token rows loaded per tile (the MMA's M operand is 128 rows; a decode batch loads fewer).
 int token_tile(int M) {

@@ -1,0 +1,291 @@
+// gemm_fp4.cuh -- W4A4 GEMM for sm_100a: C = A4 . B4^T with both operands in microscaled 4-bit
+// floating point (NVFP4 or MXFP4), consumed by tcgen05.mma kind::mxf4nvf4 / kind::mxf4 as they
+// are: no transcode, codes and scale tiles go from HBM to shared memory by TMA / bulk copies,
+// scales on to tensor memory by tcgen05.cp.
+//
+//   C[m, n] = act(acc[m, n] * ((s_m * ts) * s_n) + bias[n]),  acc = sum_k a b in fp32
+//
+// w4a4_gemm_kernel: tiles of 128 weight rows (the MMA's M) x BN tokens (its N), so a decode batch
+// of 16 tokens pads to 16 columns instead of 128 rows. One CTA computes one K slice of one tile;
+// the `split` CTAs of a cluster share a tile, and exchange their fp32 partials through distributed
+// shared memory, each summing its share of the columns in rank order: no workspace, no atomics,
+// the same bits whatever the timing.
+//
+// Warps: 0 producer (TMA), 1 MMA, all four drain the accumulator (lane = weight row).
+#pragma once
+#include <cstdint>
+
+#include "epilogue.cuh"
+#include "fp4.cuh"
+#include "sm100.cuh"
+
+namespace bd {
+
+struct GemmFp4Params {
+  void* out;
+  const uint8_t* sf_t;        // scale tiles of the tokens / of the weights
+  const uint8_t* sf_w;
+  const float* row_scale_t;   // per token row / per weight row, may be null
+  const float* row_scale_w;
+  const __nv_bfloat16* bias;
+  float tensor_scale;
+  int M, N, K, words;
+  int n_tiles, m_tiles;
+  int out_dtype, epilogue;
+  int weights_early;
+  uint32_t* err;
+};
+
+constexpr int kF4ChunkK = 256;  // elements of K per stage: 128 bytes of codes, a swizzle row
+
+constexpr int cround_up(int x, int a) { return (x + a - 1) / a * a; }
+
+template <int BN, int kFmt>
+struct GemmFp4Cfg {
+  static constexpr int kWords = kFmt == kNvfp4 ? 4 : 2;  // scale words per row and chunk
+  static constexpr int kTBlocks = (BN + 127) / 128;
+  static constexpr int kWBytes = 128 * 128;              // weight codes of a stage
+  static constexpr int kTBytes = BN * 128;               // token codes
+  static constexpr int kSfBytes = 512 * kWords;          // scales of 128 rows
+  static constexpr int oT = kWBytes;
+  static constexpr int oSw = oT + kTBytes;
+  static constexpr int oSt = oSw + kSfBytes;
+  static constexpr int kStage = cround_up(oSt + kTBlocks * kSfBytes, 1024);
+  // two CTAs per SM up to 64 tokens (weight streaming: twice the independent schedules), one above
+  static constexpr int kCtasPerSm = BN <= 64 ? 2 : 1;
+  static constexpr int kBudget = (kCtasPerSm == 2 ? 113 : 226) * 1024 - 2048 - 1024;
+  static constexpr int kStages = kBudget / kStage > 8 ? 8 : kBudget / kStage;
+  static constexpr int kRing = kStages * kStage;
+  // column slices of the partial exchange: [split][BN / split][128] fp32, over the ring
+  static_assert(BN * 128 * 4 <= kRing, "exchange buffer fits the ring");
+  static constexpr int kSmemBytes = kRing + 2048 + 1024;
+  // tensor memory: accumulator, then two sets of scale words
+  static constexpr int kSfSet = 4 * kWords * (1 + kTBlocks);
+  static constexpr int kSfCol0 = BN < 64 ? 64 : BN;
+  static constexpr int kUsedCols = kSfCol0 + 2 * kSfSet;
+  static constexpr int kTmemCols = kUsedCols <= 128 ? 128 : kUsedCols <= 256 ? 256 : 512;
+  static_assert(kUsedCols <= 512, "tensor memory budget");
+  static_assert(BN % 16 == 0 && BN <= 256, "MMA N");
+  static_assert(kStage % 1024 == 0 && kWBytes % 1024 == 0 && kTBytes % 1024 == 0,
+                "1 KB swizzle atoms");
+};
+
+struct GemmFp4Ctl {
+  uint64_t full[8], empty[8], done;
+  uint32_t tmem_base, abort_flag;
+  float tok_scale[256];
+};
+
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+__device__ __forceinline__ float activate(float v, int epi) {
+  if (epi == 2) return fmaxf(v, 0.0f);
+  if (epi == 3) return silu_rn(v);
+  if (epi == 4) return gelu_tanh_rn(v);
+  return v;
+}
+
+template <int BN, int kFmt>
+__global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
+    w4a4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w,
+                     const __grid_constant__ CUtensorMap tm_t, const GemmFp4Params p, int split) {
+  using Cfg = GemmFp4Cfg<BN, kFmt>;
+  constexpr bool kNv = kFmt == kNvfp4;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  GemmFp4Ctl& ctl = *reinterpret_cast<GemmFp4Ctl*>(smem + Cfg::kRing);
+  static_assert(sizeof(GemmFp4Ctl) <= 2048, "control block");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile uint32_t* abort_flag = &ctl.abort_flag;
+
+  const int tile = blockIdx.x / split, rank = blockIdx.x % split;
+  const int mt = tile % p.m_tiles, nt = tile / p.m_tiles;
+  const int n0 = nt * 128, m0 = mt * BN;
+  const int chunks = (p.K + kF4ChunkK - 1) / kF4ChunkK;
+  const int k0 = static_cast<int>(static_cast<int64_t>(chunks) * rank / split);
+  const int k1 = static_cast<int>(static_cast<int64_t>(chunks) * (rank + 1) / split);
+
+  if (tid == 0) {
+    ctl.abort_flag = 0;
+    for (int s = 0; s < Cfg::kStages; ++s) {
+      mbar_init(smem_u32(&ctl.full[s]), 1);
+      mbar_init(smem_u32(&ctl.empty[s]), 1);
+    }
+    mbar_init(smem_u32(&ctl.done), 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&ctl.tmem_base), Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tb = ctl.tmem_base;
+  grid_dep_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tmap(&tm_w);
+      prefetch_tmap(&tm_t);
+      const int t_blocks = min(Cfg::kTBlocks, (p.M - m0 + 127) / 128);
+      // words of chunk k present in the tiles
+      auto words_of = [&](int k) { return min(Cfg::kWords, p.words - k * Cfg::kWords); };
+      auto load_weights = [&](int k, int slot) {
+        uint8_t* st = smem + slot * Cfg::kStage;
+        const uint32_t fb = smem_u32(&ctl.full[slot]);
+        const uint32_t sfb = 512u * words_of(k);
+        mbar_arrive_expect_tx(fb, Cfg::kWBytes + Cfg::kTBytes + sfb * (1 + t_blocks));
+        tma_load_2d(smem_u32(st), &tm_w, k * 128, n0, fb);
+        bulk_load(smem_u32(st + Cfg::oSw),
+                  p.sf_w + (static_cast<int64_t>(nt) * p.words + k * Cfg::kWords) * 512, sfb, fb);
+      };
+      auto load_tokens = [&](int k, int slot) {
+        uint8_t* st = smem + slot * Cfg::kStage;
+        const uint32_t fb = smem_u32(&ctl.full[slot]);
+        const uint32_t sfb = 512u * words_of(k);
+        tma_load_2d(smem_u32(st + Cfg::oT), &tm_t, k * 128, m0, fb);
+        for (int b = 0; b < t_blocks; ++b)
+          bulk_load(smem_u32(st + Cfg::oSt + b * Cfg::kSfBytes),
+                    p.sf_t + (static_cast<int64_t>(m0 / 128 + b) * p.words + k * Cfg::kWords) * 512,
+                    sfb, fb);
+      };
+      // the first ring of weights before the wait for the previous grid (when it does not write
+      // them), the tokens after it
+      const int first = min(k1 - k0, Cfg::kStages);
+      if (!p.weights_early) grid_dep_wait();
+      for (int i = 0; i < first; ++i) load_weights(k0 + i, i);
+      grid_dep_wait();
+      for (int i = 0; i < first; ++i) load_tokens(k0 + i, i);
+      RingPos<Cfg::kStages> r;
+      if (first == Cfg::kStages) r.phase = 1;
+      for (int k = k0 + first; k < k1; ++k) {
+        if (!mbar_wait(smem_u32(&ctl.empty[r.slot]), r.phase ^ 1u, p.err, kErrWaitEmpty,
+                       abort_flag))
+          break;
+        load_weights(k, r.slot);
+        load_tokens(k, r.slot);
+        r.next();
+      }
+      // every copy issued has landed before the CTA goes on (also after a wait ran out)
+      for (int i = max(0, k1 - k0 - Cfg::kStages); i < k1 - k0 && *abort_flag; ++i)
+        mbar_wait(smem_u32(&ctl.full[i % Cfg::kStages]), (i / Cfg::kStages) & 1, p.err, kErrWaitTma,
+                  nullptr);
+    }
+  } else if (warp == 1) {
+    RingPos<Cfg::kStages> r;
+    for (int k = k0; k < k1; ++k) {
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.full[r.slot]), r.phase, p.err,
+                                             kErrWaitTma, abort_flag)))
+        break;
+      tc_fence_after();
+      const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
+      const uint32_t sfw = tb + Cfg::kSfCol0 + ((k - k0) & 1) * Cfg::kSfSet;
+      const uint32_t sft = sfw + 4 * Cfg::kWords;
+      const int words = min(Cfg::kWords, p.words - k * Cfg::kWords);
+      const int steps = min(4, (p.K - k * kF4ChunkK + 63) / 64);
+      if (elect_one()) {
+        for (int w = 0; w < words; ++w) {
+          tmem_cp_32x128b_x4(sfw + 4 * w, sdesc_sf(st + Cfg::oSw + 512 * w));
+#pragma unroll
+          for (int b = 0; b < Cfg::kTBlocks; ++b)
+            tmem_cp_32x128b_x4(sft + 4 * (w * Cfg::kTBlocks + b),
+                               sdesc_sf(st + Cfg::oSt + b * Cfg::kSfBytes + 512 * w));
+        }
+        for (int kk = 0; kk < steps; ++kk) {
+          const int w = kNv ? kk : kk >> 1;
+          const uint32_t idesc = idesc_mxf4(128, BN, !kNv, kNv ? 0 : 2 * (kk & 1));
+          mma_mxf4_ss<kNv, false>(tb, sdesc_sw128(st + kk * 32), sdesc_sw128(st + Cfg::oT + kk * 32),
+                                  idesc, sfw + 4 * w, sft + 4 * Cfg::kTBlocks * w,
+                                  (k > k0 || kk > 0) ? 1u : 0u);
+        }
+        tc_commit(smem_u32(&ctl.empty[r.slot]));
+      }
+      __syncwarp();
+      r.next();
+    }
+    if (elect_one()) tc_commit(smem_u32(&ctl.done));
+    __syncwarp();
+  }
+  __syncwarp();
+  // ---- drain: every thread owns weight row n0 + 32 warp + lane of the tile
+  grid_dep_wait();
+  for (int j = tid; j < BN; j += 128) {
+    const int m = m0 + j;
+    ctl.tok_scale[j] = p.row_scale_t != nullptr && m < p.M
+                           ? __fmul_rn(p.row_scale_t[m], p.tensor_scale)
+                           : p.tensor_scale;
+  }
+  const int n = n0 + 32 * warp + lane;
+  const float wscale = p.row_scale_w != nullptr && n < p.N ? p.row_scale_w[n] : 1.0f;
+  const float bias = p.epilogue != 0 && n < p.N ? __bfloat162float(p.bias[n]) : 0.0f;
+  bool ok = mbar_wait(smem_u32(&ctl.done), 0, p.err, kErrWaitAccum, abort_flag);
+  // the barrier publishes tok_scale; nothing is stored after a wait that ran out (here, or in a
+  // peer of the cluster: its partial then holds whatever its accumulator held)
+  ok = __syncthreads_and(ok) && !*abort_flag;
+  tc_fence_after();
+  const uint32_t taddr = tb + (static_cast<uint32_t>(32 * warp) << 16);
+  auto finish = [&](int j, float acc) {
+    const int m = m0 + j;
+    if (m >= p.M || n >= p.N) return;
+    float v = __fmul_rn(acc, ctl.tok_scale[j]);
+    if (p.row_scale_w != nullptr) v = __fmul_rn(v, wscale);
+    if (p.epilogue != 0) v = activate(__fadd_rn(v, bias), p.epilogue);
+    store_out(p.out, static_cast<int64_t>(m) * p.N + n, v, p.out_dtype);
+  };
+  if (split == 1) {
+    if (ok) {
+      const int cols = min(BN, p.M - m0);
+#pragma unroll 1
+      for (int c0 = 0; c0 < cols; c0 += 16) {
+        uint32_t r[16];
+        tmem_ld_x16(taddr + c0, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) finish(c0 + j, __uint_as_float(r[j]));
+      }
+    }
+  } else {
+    // every CTA of the cluster is past its last MMA: the rings may be overwritten
+    cluster_arrive();
+    cluster_wait();
+    const int width = BN / split;  // columns per rank
+    float* part = reinterpret_cast<float*>(smem);
+#pragma unroll 1
+    for (int c0 = 0; c0 < BN; c0 += 16) {
+      uint32_t r[16];
+      tmem_ld_x16(taddr + c0, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int owner = (c0 + j) / width, col = (c0 + j) % width;
+        const uint32_t at = smem_u32(part + (rank * width + col) * 128 + 32 * warp + lane);
+        st_shared_cluster_f32(mapa_shared(at, owner), ok ? __uint_as_float(r[j]) : 0.0f);
+      }
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (ok)
+      for (int col = 0; col < width; ++col) {
+        float acc = 0.0f;
+        for (int s = 0; s < split; ++s) acc += part[(s * width + col) * 128 + 32 * warp + lane];
+        finish(rank * width + col, acc);
+      }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tb, Cfg::kTmemCols);
+  }
+}
+
+}  // namespace bd

@@ -287,6 +287,11 @@ __device__ __forceinline__ void tmem_cp_32x128b_x4(uint32_t taddr, uint64_t sdes
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc)
                : "memory");
 }
+// The same in both CTAs of a pair, each from its own shared memory at the same offset.
+__device__ __forceinline__ void tmem_cp_32x128b_x4_pair(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc)
+               : "memory");
+}
 // Shared -> tensor memory: 128 rows (lanes) x 16 bytes (4 columns).
 __device__ __forceinline__ void tmem_cp_128x128b(uint32_t taddr, uint64_t sdesc) {
   asm volatile("tcgen05.cp.cta_group::1.128x128b [%0], %1;" ::"r"(taddr), "l"(sdesc)
@@ -454,6 +459,49 @@ __device__ __forceinline__ void mma_mxf8f6f4_ts(uint32_t d_tmem, uint32_t a_tmem
           "r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
       : "memory");
+}
+
+// Shared-memory descriptor of a 512-byte scale-factor block (32 rows x 16 bytes, 8-row groups
+// 128 bytes apart) for tcgen05.cp 32x128b.
+__device__ __forceinline__ uint64_t sdesc_sf(uint32_t saddr) { return sdesc_plain(saddr, 0, 128); }
+
+// Instruction descriptor for tcgen05.mma.kind::mxf4 / mxf4nvf4.block_scale: E2M1 operands, two
+// codes per byte, K-major, K = 64, fp32 accumulation. e8m0: scales are E8M0 (else UE4M3); sf ids
+// pick the half of the 32-bit TMEM scale word a kind::mxf4 MMA takes (0 or 2).
+__host__ __device__ __forceinline__ uint32_t idesc_mxf4(uint32_t M, uint32_t N, bool e8m0,
+                                                        uint32_t sf_id) {
+  uint32_t d = 0;
+  d |= (sf_id & 3u) << 4;
+  d |= 1u << 7;   // A: E2M1
+  d |= 1u << 10;  // B: E2M1
+  d |= ((N >> 3) & 0x3Fu) << 17;
+  d |= (e8m0 ? 1u : 0u) << 23;
+  d |= ((M >> 4) & 0x1Fu) << 24;
+  d |= (sf_id & 3u) << 29;
+  return d;
+}
+
+// D[tmem] (+)= A[smem] * B[smem]^T of E2M1 codes with block scales from TMEM: kNv with four E4M3
+// scales per row (per 16 elements), else two E8M0 (per 32). kPair: the MMA of a CTA pair (M = 256,
+// rows of D, A and the A scales split between the CTAs, B's rows split in halves, the B scales of
+// all rows in each CTA), issued by rank 0.
+template <bool kNv, bool kPair>
+__device__ __forceinline__ void mma_mxf4_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t sfa_tmem, uint32_t sfb_tmem,
+                                            uint32_t accumulate) {
+#define BD_MMA_MXF4(GROUP, KIND, VEC)                                                            \
+  asm volatile(                                                                                  \
+      "{\n\t.reg .pred p;\n\t"                                                                   \
+      "setp.ne.b32 p, %4, 0;\n\t"                                                                \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" KIND ".block_scale.scale_vec::" VEC              \
+      " [%0], %1, %2, %3, [%5], [%6], p;\n\t}\n" ::"r"(d_tmem),                                  \
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)          \
+      : "memory")
+  if constexpr (kNv && !kPair) BD_MMA_MXF4("1", "mxf4nvf4", "4X");
+  else if constexpr (kNv) BD_MMA_MXF4("2", "mxf4nvf4", "4X");
+  else if constexpr (!kPair) BD_MMA_MXF4("1", "mxf4", "2X");
+  else BD_MMA_MXF4("2", "mxf4", "2X");
+#undef BD_MMA_MXF4
 }
 
 // Byte offset of 16-byte chunk `c` of row `r` inside a 128B-swizzled K-major tile whose

@@ -1,0 +1,233 @@
+"""Microscaled 4-bit floating point: quantiser, dequantiser and the W4A4 GEMM, tensor-level
+entry points over the C ABI (NVFP4 and MXFP4 operands, tcgen05 kind::mxf4nvf4 / kind::mxf4).
+
+Where ``ops.w4a6_gemm`` spends its time turning 4-bit weights into 6-bit operands on chip, the
+products here take both operands in 4 bits as they are: coarser activations, and twice the
+tensor-core rate. Weights quantised once by ``ops.quantize_nvfp4`` serve both paths.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import call
+from .ops import EPILOGUES, _OUT, _need, _p, _stream, quantize_nvfp4, tensor_scale_of
+
+FP4_FORMATS = {"nvfp4": _lib.BD_FP4_NVFP4, "mxfp4": _lib.BD_FP4_MXFP4}
+_BLOCK = {"nvfp4": 16, "mxfp4": 32}
+_IN4 = {torch.float32: _lib.BD_IN_F32, torch.bfloat16: _lib.BD_IN_BF16,
+        torch.float16: _lib.BD_IN_F16}
+
+
+@dataclass
+class Fp4Operand:
+    """A (rows, K) matrix in microscaled 4-bit floating point, either operand of ``w4a4_gemm``
+    (activations: rows are tokens; weights: rows are outputs). Its values are
+    code * block scale * (row_scale[row] * tensor_scale)."""
+    codes: torch.Tensor   # (rows, K/2) u8, element 2j in the low nibble of byte j
+    scales: torch.Tensor  # scale tiles (flat u8): [ceil(rows/128)][ceil(scales per row/4)][512]
+    rows: int
+    K: int
+    fmt: str              # "nvfp4": E4M3 per 16 elements; "mxfp4": E8M0 per 32
+    row_scale: Optional[torch.Tensor] = None  # (rows,) fp32
+    tensor_scale: float = 1.0
+
+
+def _fmt(fmt: str) -> int:
+    if fmt not in FP4_FORMATS:
+        raise ValueError(f"unknown 4-bit format {fmt!r}: 'nvfp4' or 'mxfp4'")
+    return FP4_FORMATS[fmt]
+
+
+def _scale_bytes(rows: int, K: int, fmt: str) -> int:
+    return (rows + 127) // 128 * ((K // _BLOCK[fmt] + 3) // 4) * 512
+
+
+def _on(stream, device):
+    """Context in which new tensors belong to the stream the kernels run on (their memory is
+    reused in that stream's order)."""
+    if stream is None:
+        return torch.cuda.stream(None)
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    return torch.cuda.stream(stream)
+
+
+def _check_x4(x: torch.Tensor):
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a 2-D tensor (M, K)")
+    if x.dtype not in _IN4:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    _need(x, x.dtype, "x")
+    M, K = x.shape
+    if K == 0 or K % 32:
+        raise ValueError(f"K must be a positive multiple of 32, got {K}")
+    return M, K
+
+
+def _check_operand(op: Fp4Operand, what: str) -> None:
+    _fmt(op.fmt)
+    if op.rows < 0 or op.K <= 0 or op.K % 32:
+        raise ValueError(f"{what}: K must be a positive multiple of 32, got {op.K}")
+    _need(op.codes, torch.uint8, f"{what}.codes", op.rows * op.K // 2)
+    _need(op.scales, torch.uint8, f"{what}.scales", _scale_bytes(op.rows, op.K, op.fmt))
+    if op.row_scale is not None:
+        _need(op.row_scale, torch.float32, f"{what}.row_scale", op.rows)
+
+
+def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", stream=None,
+                 overlap_prev: bool = False) -> Fp4Operand:
+    """x (M, K) fp32 / bf16 / fp16 -> Fp4Operand in one launch, K % 32 == 0. "nvfp4": E4M3 scales
+    per 16 elements under an fp32 scale per row (a token's codes do not depend on the rest of the
+    batch); "mxfp4": E8M0 scales per 32. A NaN or Inf sets BD_DEVERR_NONFINITE in the device error
+    word and leaves its row undefined."""
+    code = _fmt(fmt)
+    M, K = _check_x4(x)
+    with _on(stream, x.device):
+        codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
+        scales = torch.empty(_scale_bytes(M, K, fmt), dtype=torch.uint8, device=x.device)
+        row_scale = None
+        if fmt == "nvfp4":
+            row_scale = torch.empty(M, dtype=torch.float32, device=x.device)
+    call("bd_quantize_fp4", _p(x), _IN4[x.dtype], code, _p(codes), None, _p(scales), _p(row_scale),
+         M, K, _lib.BD_GEMM_OVERLAP_PREV if overlap_prev else 0, _stream(stream))
+    return Fp4Operand(codes, scales, M, K, fmt, row_scale)
+
+
+def quantize_mxfp4(x: torch.Tensor, stream=None):
+    """x (M, K) fp32 / bf16 / fp16 -> (codes (M, K/2) packed E2M1 nibbles, E8M0 (M, K/32) u8):
+    ``quantize_fp4(x, "mxfp4")`` in the natural layout (the reference's quantize(x, E8M0, E2M1),
+    vector_quant_error.py:283-319)."""
+    M, K = _check_x4(x)
+    with _on(stream, x.device):
+        codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
+        e8m0 = torch.empty((M, K // 32), dtype=torch.uint8, device=x.device)
+    call("bd_quantize_fp4", _p(x), _IN4[x.dtype], _lib.BD_FP4_MXFP4, _p(codes), _p(e8m0), None,
+         None, M, K, 0, _stream(stream))
+    return codes, e8m0
+
+
+def pack_fp4(codes: torch.Tensor, scales: torch.Tensor, fmt: str = "nvfp4",
+             tensor_scale: float = 1.0, row_scale: Optional[torch.Tensor] = None,
+             stream=None) -> Fp4Operand:
+    """Natural codes (rows, K/2) and block scales ((rows, K/16) E4M3 or (rows, K/32) E8M0 bytes) ->
+    Fp4Operand. The codes are the operand as they are (not copied); only the scales are re-laid."""
+    code = _fmt(fmt)
+    if codes.dim() != 2:
+        raise ValueError("codes must be 2-D (rows, K/2)")
+    rows, K = codes.shape[0], 2 * codes.shape[1]
+    if K == 0 or K % 32:
+        raise ValueError(f"K must be a positive multiple of 32, got {K}")
+    _need(codes, torch.uint8, "codes")
+    _need(scales, torch.uint8, "scales", rows * (K // _BLOCK[fmt]))
+    if row_scale is not None:
+        _need(row_scale, torch.float32, "row_scale", rows)
+    with _on(stream, codes.device):
+        tiled = torch.empty(_scale_bytes(rows, K, fmt), dtype=torch.uint8, device=codes.device)
+    call("bd_tile_scales_fp4", _p(scales), _p(tiled), rows, K, code, _stream(stream))
+    return Fp4Operand(codes, tiled, rows, K, fmt, row_scale, float(tensor_scale))
+
+
+def quantize_weights_fp4(w: torch.Tensor, fmt: str = "nvfp4", stream=None) -> Fp4Operand:
+    """Weights w (N, K) fp32 / bf16 -> Fp4Operand. "nvfp4": the codes of ``quantize_nvfp4`` (one
+    fp32 scale for the tensor, read back to the host once); "mxfp4": ``quantize_fp4``."""
+    if _fmt(fmt) == _lib.BD_FP4_MXFP4:
+        return quantize_fp4(w, fmt, stream)
+    with _on(stream, w.device):
+        codes, scales, tstat = quantize_nvfp4(w, stream)
+        return pack_fp4(codes, scales, fmt, tensor_scale_of(tstat), stream=stream)
+
+
+def dequantize_fp4(op: Fp4Operand, out_dtype=torch.float32, out: Optional[torch.Tensor] = None,
+                   stream=None) -> torch.Tensor:
+    """The values of an operand, (rows, K) in out_dtype (fp32, bf16 or fp16)."""
+    _check_operand(op, "operand")
+    if out_dtype not in _OUT:
+        raise TypeError(f"unsupported output dtype {out_dtype}")
+    if out is None:
+        with _on(stream, op.codes.device):
+            out = torch.empty((op.rows, op.K), dtype=out_dtype, device=op.codes.device)
+    _need(out, out_dtype, "out", op.rows * op.K)
+    call("bd_dequantize_fp4", _p(op.codes), _p(op.scales), _p(op.row_scale),
+         float(op.tensor_scale), _p(out), _OUT[out_dtype], FP4_FORMATS[op.fmt], op.rows, op.K, 0,
+         _stream(stream))
+    return out
+
+
+def _epilogue(epilogue: str, bias, N: int) -> int:
+    if epilogue not in EPILOGUES:
+        raise ValueError(f"unknown epilogue {epilogue!r}")
+    epi = EPILOGUES[epilogue]
+    if bias is not None:
+        _need(bias, torch.bfloat16, "bias", N)
+    if epi != _lib.BD_EPI_NONE and bias is None:
+        raise ValueError(f"epilogue {epilogue!r} needs a bias")
+    return epi
+
+
+def _output(out, M: int, N: int, out_dtype, device, stream):
+    if out_dtype not in _OUT:
+        raise TypeError(f"unsupported output dtype {out_dtype}")
+    if out is None:
+        with _on(stream, device):
+            return torch.empty((M, N), dtype=out_dtype, device=device)
+    _need(out, out_dtype, "out", M * N)
+    return out
+
+
+def w4a4_gemm(acts: Fp4Operand, weights: Fp4Operand, bias: Optional[torch.Tensor] = None,
+              out_dtype=torch.bfloat16, epilogue: str = "none",
+              out: Optional[torch.Tensor] = None, stream=None, overlap_prev: bool = False,
+              weights_static: bool = False) -> torch.Tensor:
+    """C[M, N] = act(A . B^T + bias) of two 4-bit operands of one format on the tensor cores (any
+    M and N, K % 32 == 0; no workspace). overlap_prev, weights_static: as in ``w4a6_gemm``."""
+    if acts.fmt != weights.fmt:
+        raise ValueError(f"format mismatch: activations {acts.fmt}, weights {weights.fmt}")
+    if acts.K != weights.K:
+        raise ValueError(f"K mismatch: activations {acts.K}, weights {weights.K}")
+    _check_operand(acts, "acts")
+    _check_operand(weights, "weights")
+    M, N, K = acts.rows, weights.rows, acts.K
+    epi = _epilogue(epilogue, bias, N)
+    out = _output(out, M, N, out_dtype, acts.codes.device, stream)
+    flags = (_lib.BD_GEMM_OVERLAP_PREV if overlap_prev else 0) | \
+        (_lib.BD_GEMM_WEIGHTS_STATIC if weights_static else 0)
+    call("bd_w4a4_gemm", _p(out), _p(acts.codes), _p(acts.scales), _p(acts.row_scale),
+         _p(weights.codes), _p(weights.scales), _p(weights.row_scale),
+         float(acts.tensor_scale) * float(weights.tensor_scale), _p(bias), M, N, K,
+         FP4_FORMATS[acts.fmt], _OUT[out_dtype], epi, flags, _stream(stream))
+    return out
+
+
+def w4a4_linear(x: torch.Tensor, weights: Fp4Operand, bias: Optional[torch.Tensor] = None,
+                out_dtype=torch.bfloat16, epilogue: str = "none",
+                out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """C = act(quantize_fp4(x) . W^T + bias) from raw activations x (M, K) fp32 / bf16 / fp16, in
+    the weights' format: the quantiser, then the W4A4 GEMM, which streams its first weights while
+    the quantiser runs (so the weights are not to be written by work still running on the
+    stream)."""
+    M, K = _check_x4(x)
+    if weights.K != K:
+        raise ValueError(f"K mismatch: activations {K}, weights {weights.K}")
+    _check_operand(weights, "weights")
+    N = weights.rows
+    epi = _epilogue(epilogue, bias, N)
+    out = _output(out, M, N, out_dtype, x.device, stream)
+    if M == 0:
+        return out
+    with _on(stream, x.device):
+        ws = torch.empty(_linear_workspace(M, K, weights.fmt), dtype=torch.uint8, device=x.device)
+    call("bd_w4a4_linear", _p(out), _p(x), _IN4[x.dtype], _p(weights.codes), _p(weights.scales),
+         _p(weights.row_scale), float(weights.tensor_scale), _p(bias), M, N, K,
+         FP4_FORMATS[weights.fmt], _OUT[out_dtype], epi, _p(ws), ws.numel(), _stream(stream))
+    return out
+
+
+def _linear_workspace(M: int, K: int, fmt: str) -> int:
+    """bd_query_w4a4_linear_workspace without the call."""
+    def up(v):
+        return (v + 255) // 256 * 256
+    return up(M * K // 2) + up(_scale_bytes(M, K, fmt)) + up(4 * M)

@@ -155,9 +155,11 @@ int bd_scales_e8m0_to_e4m3_pairs(const uint8_t* e8m0, uint8_t* e4m3_pairs, int64
 int bd_pack_a(const uint8_t* codes, const uint8_t* e8m0, uint8_t* a_packed,
               uint8_t* scales_tiled, int M, int K, bd_stream_t stream);
 
-/* Input element types of bd_quantize_a_mxfp6 and bd_quantize_b_nvfp4. */
+/* Input element types of bd_quantize_a_mxfp6 and bd_quantize_b_nvfp4 (BD_IN_F16: the 4-bit
+ * operators below only). */
 #define BD_IN_F32 0
 #define BD_IN_BF16 1
+#define BD_IN_F16 2
 
 /* Activations x (M, K) row-major, fp32 or bf16 -> MXFP6: E2M3 codes (M, K), one per byte (bits
  * 0..5; this is already the GEMM's `a` operand), and the E8M0 exponent of each 32-element
@@ -271,6 +273,66 @@ int bd_w4a6_gemm_noalloc(void* c, const uint8_t* a, const uint8_t* a_scales, con
  * plus bias/activation. Replaces the torch.sum over planes in kernel/bench_sweep.py:141-142. */
 int bd_splitk_reduce(const float* partials, void* c, const void* bias, float b_tensor_scale,
                      int M, int N, int split_k, int out_dtype, int epilogue, bd_stream_t stream);
+
+/* ---- 4-bit activations: W4A4 ----------------------------------------------------------------
+ * Operand formats: E2M1 codes (rows, K/2), element 2j in the low nibble of byte j, with
+ *   BD_FP4_NVFP4  one E4M3 scale byte per 16 elements, an fp32 scale per row and / or per tensor;
+ *   BD_FP4_MXFP4  one E8M0 scale byte per 32 elements.
+ * Scale tiles (what the GEMM reads; bd_query_fp4_scales bytes):
+ *   [ceil(rows/128)][ceil(scales per row / 4)][512]: row r of a tile at byte
+ *   16 (r % 32) + 4 (r / 32 % 4), its four scales side by side; zero bytes past the end of K, rows
+ *   past the last are not read into any result.
+ * K % 32 == 0, any number of rows (0: nothing is done). No reference counterpart: its w4a4 arm
+ * (psg_preshuffle_gemm.py in_dtype="w4a4_tc") transcodes both operands to MXFP6 instead. */
+#define BD_FP4_NVFP4 0
+#define BD_FP4_MXFP4 1
+
+/* Bytes of the scale tiles of a (rows, K) operand. */
+size_t bd_query_fp4_scales(int rows, int K, int fmt);
+
+/* x (M, K) row-major fp32 / bf16 / fp16 -> E2M1 codes (M, K/2) and block scales, natural (scales:
+ * (M, K/16) or (M, K/32)) and / or tiled (scales_tiled); either may be NULL, not both.
+ * NVFP4, every step in float32: row_scale[m] = s = max(amax(|x_m|) / 2688, 2^-120) (1 for a zero
+ * row); per 16-block top = amax * (1/s), B = the smallest E4M3 normal with 6 B >= top (448 at most,
+ * 1 for a zero block), code = nearest E2M1 of x * ((1/s) / B). MXFP4 (row_scale unused): e the
+ * smallest integer in [-40, 40] with 6 * 2^e >= amax of the 32-block (0 for a zero block), code =
+ * nearest E2M1 of x / 2^e. A tie goes to the lower magnitude, the sign is kept on non-zero codes
+ * only. NaN / Inf in a row sets BD_DEVERR_NONFINITE and leaves that row's outputs undefined.
+ * x, codes and scales_tiled 16-byte aligned. flags: BD_GEMM_OVERLAP_PREV. */
+int bd_quantize_fp4(const void* x, int x_dtype, int fmt, uint8_t* codes, uint8_t* scales,
+                    uint8_t* scales_tiled, float* row_scale, int M, int K, unsigned flags,
+                    bd_stream_t stream);
+
+/* Natural block scales (rows, K/16) E4M3 or (rows, K/32) E8M0 -> tiles (weights quantised by
+ * bd_quantize_b_nvfp4: their codes are the GEMM operand as they are). */
+int bd_tile_scales_fp4(const uint8_t* scales, uint8_t* scales_tiled, int rows, int K, int fmt,
+                       bd_stream_t stream);
+
+/* out (M, K) = code * block scale (exact) * (row_scale[m] * tensor_scale), rounded to out_dtype;
+ * row_scale may be NULL (1). out 16-byte aligned, codes 8. flags: BD_GEMM_OVERLAP_PREV. */
+int bd_dequantize_fp4(const uint8_t* codes, const uint8_t* scales_tiled, const float* row_scale,
+                      float tensor_scale, void* out, int out_dtype, int fmt, int M, int K,
+                      unsigned flags, bd_stream_t stream);
+
+/* C[M,N] = act((A . B^T) * (a_row_scale[m] * tensor_scale) * b_row_scale[n] + bias[n]): block-scaled
+ * 4-bit tensor-core MMAs, fp32 accumulation, both operands in format `fmt`, scales tiled; the row
+ * scales may be NULL (1). Any N >= 1; no workspace; results do not depend on timing. a, b and the
+ * scale tiles 16-byte aligned. flags: BD_GEMM_OVERLAP_PREV, BD_GEMM_WEIGHTS_STATIC (as for
+ * bd_w4a6_gemm_ex; b, b_scales). */
+int bd_w4a4_gemm(void* c, const uint8_t* a, const uint8_t* a_scales, const float* a_row_scale,
+                 const uint8_t* b, const uint8_t* b_scales, const float* b_row_scale,
+                 float tensor_scale, const void* bias, int M, int N, int K, int fmt,
+                 int out_dtype, int epilogue, unsigned flags, bd_stream_t stream);
+
+/* bd_quantize_fp4 of x (M, K), then bd_w4a4_gemm, launched so that the GEMM streams its first
+ * weights while the quantiser runs (b and b_scales must not be written by work still running
+ * on the stream). workspace: bd_query_w4a4_linear_workspace bytes, 256-byte aligned, contents
+ * irrelevant before and after; concurrent calls must not share one. */
+size_t bd_query_w4a4_linear_workspace(int M, int K, int fmt);
+int bd_w4a4_linear(void* c, const void* x, int x_dtype, const uint8_t* b, const uint8_t* b_scales,
+                   const float* b_row_scale, float tensor_scale, const void* bias, int M, int N,
+                   int K, int fmt, int out_dtype, int epilogue, void* workspace,
+                   size_t workspace_bytes, bd_stream_t stream);
 
 #ifdef __cplusplus
 }

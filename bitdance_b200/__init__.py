@@ -7,6 +7,7 @@ is its Python host side. ``psg`` mirrors the reference operator ``compile_preshu
 from ._lib import BitdanceError, load  # noqa: F401
 from .fp4 import (Fp4Operand, dequantize_fp4, pack_fp4, quantize_fp4,  # noqa: F401
                   quantize_mxfp4, quantize_weights_fp4, w4a4_gemm, w4a4_linear)
+from .moe import MoeWeights, moe_experts, moe_layer, quantize_moe_weights  # noqa: F401
 from .ops import (PackedActivations, PackedWeights, Workspace, device_error,  # noqa: F401
                   mma_peak_tflops,
                   pack_activations, pack_weights, quantize_activations, quantize_mxfp6,

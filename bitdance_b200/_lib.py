@@ -28,6 +28,7 @@ BD_SPLIT_REDUCE, BD_SPLIT_PLANES, BD_SPLIT_ATOMIC = 0, 1, 2
 BD_GEMM_OVERLAP_PREV, BD_GEMM_WEIGHTS_STATIC, BD_GEMM_B_E4M3, BD_GEMM_SINGLE_CTA = 1, 2, 4, 8
 BD_IN_F32, BD_IN_BF16, BD_IN_F16 = 0, 1, 2
 BD_FP4_NVFP4, BD_FP4_MXFP4 = 0, 1
+BD_MOE_SOFTMAX, BD_MOE_SIGMOID = 0, 1
 BD_DEVERR_WAIT_MASK, BD_DEVERR_WAIT_TMA, BD_DEVERR_NONFINITE, BD_DEVERR_RANGE = 0x1F, 0x01, 0x20, 0x40
 
 # name -> (restype, argtypes); mirrors include/bitdance_b200.h
@@ -63,6 +64,11 @@ SIGNATURES = {
                           ctypes.c_uint, _P]),
     "bd_query_w4a4_linear_workspace": (_SZ, [_I, _I, _I]),
     "bd_w4a4_linear": (_I, [_P, _P, _I, _P, _P, _P, _F, _P, _I, _I, _I, _I, _I, _I, _P, _SZ, _P]),
+    "bd_query_moe_workspace": (_SZ, [_I, _I, _I, _I, _I]),
+    "bd_moe_experts": (_I, [_P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
+                            _P, _SZ, _P]),
+    "bd_moe_layer": (_I, [_P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _F, _P, _P, _P, _P, _P, _P,
+                          _I, _I, _I, _I, _I, _I, _P, _SZ, _P]),
     "bd_splitk_reduce": (_I, [_P, _P, _P, _F, _I, _I, _I, _I, _I, _P]),
 }
 

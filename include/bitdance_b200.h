@@ -334,6 +334,43 @@ int bd_w4a4_linear(void* c, const void* x, int x_dtype, const uint8_t* b, const 
                    int K, int fmt, int out_dtype, int epilogue, void* workspace,
                    size_t workspace_bytes, bd_stream_t stream);
 
+/* ---- mixture of experts for a few tokens ----------------------------------------------------
+ * Expert weights in NVFP4, natural layout (what bd_quantize_b_nvfp4 writes, one expert after the
+ * other): gate_up (E, 2I, H/2) codes (I gate rows, then I up rows) and (E, 2I, H/16) E4M3 scales;
+ * down (E, H, I/2) and (E, H, I/16); one fp32 tensor scale per expert and matrix, device arrays.
+ * T <= 64 tokens, E <= 512, top_k <= min(16, E), H % 128 == 0, I % 128 == 0; T == 0: nothing is
+ * done. x bf16 or fp16 (T, H); y (T, H) in out_dtype. Products are of the exact weight and
+ * activation values, sums fp32, hidden values rounded once to bf16; results do not depend on
+ * timing. workspace: bd_query_moe_workspace bytes, 256-byte aligned, contents irrelevant before
+ * and after; concurrent calls must not share one. No reference counterpart. */
+#define BD_MOE_SOFTMAX 0
+#define BD_MOE_SIGMOID 1
+
+size_t bd_query_moe_workspace(int T, int H, int I, int E, int top_k);
+
+/* y[t] = sum over slots s of weights[t, s] * Wd_e (silu(Wg_e x_t) * (Wu_e x_t)), e = ids[t, s].
+ * An id of -1 is an empty slot (a token with none gets zeros); any other id outside [0, E) is
+ * taken as -1 and sets BD_DEVERR_RANGE. An expert named twice by a token counts with the sum of
+ * both weights. Two kernels. */
+int bd_moe_experts(void* y, const void* x, int x_dtype, const int* ids, const float* weights,
+                   const uint8_t* gate_up, const uint8_t* gate_up_scales,
+                   const float* gate_up_tensor_scale, const uint8_t* down,
+                   const uint8_t* down_scales, const float* down_tensor_scale, int T, int H,
+                   int I, int E, int top_k, int out_dtype, void* workspace,
+                   size_t workspace_bytes, bd_stream_t stream);
+
+/* The whole layer in two kernels: logits = x . router^T (router (E, H) in x's type or fp32), score =
+ * softmax over the experts or sigmoid; the top_k experts by score (+ selection_bias[e], NULL: none),
+ * ties to the lowest index, a NaN last; weights = score, divided by their sum when renormalize,
+ * times routed_scale. Writes ids and weights (T, top_k), best first, then y as bd_moe_experts. */
+int bd_moe_layer(void* y, int* ids, float* weights, const void* x, int x_dtype,
+                 const void* router, int router_dtype, const float* selection_bias, int scoring,
+                 int renormalize, float routed_scale, const uint8_t* gate_up,
+                 const uint8_t* gate_up_scales, const float* gate_up_tensor_scale,
+                 const uint8_t* down, const uint8_t* down_scales, const float* down_tensor_scale,
+                 int T, int H, int I, int E, int top_k, int out_dtype, void* workspace,
+                 size_t workspace_bytes, bd_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

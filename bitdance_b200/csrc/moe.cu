@@ -14,17 +14,24 @@ namespace {
 
 int last_status() { return cudaPeekAtLastError() == cudaSuccess ? BD_OK : BD_ERR_CUDA; }
 
-// Workspace: counters | fp16 image of x | its scales | hidden values, each 256-byte aligned.
+// Workspace: counters | row maxima of h | scales of x | fp16 image of x | h | partial sums, each
+// 256-byte aligned. Few pairs may split the down product: at least kPartRows rows of partials.
+constexpr int kPartRows = 256;
 struct MoeWs {
-  size_t xs, x_scale, h, total;
+  size_t hmax, x_scale, xs, h, part, total;
+  int part_rows;
 };
 MoeWs moe_ws(int T, int H, int I, int k) {
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  const size_t pairs = static_cast<size_t>(T) * k;
   MoeWs w;
-  w.xs = 256;
-  w.x_scale = w.xs + up(static_cast<size_t>(T) * H * 2);
-  w.h = w.x_scale + up(static_cast<size_t>(T) * 4);
-  w.total = w.h + up(static_cast<size_t>(T) * k * I * 2);
+  w.part_rows = std::max(T * k, kPartRows);
+  w.hmax = 256;
+  w.x_scale = w.hmax + up(pairs * 4);
+  w.xs = w.x_scale + up(static_cast<size_t>(T) * 4);
+  w.h = w.xs + up(static_cast<size_t>(T) * H * 2);
+  w.part = w.h + up(pairs * I * 4);
+  w.total = w.part + static_cast<size_t>(w.part_rows) * H * 4;
   return w;
 }
 
@@ -71,24 +78,21 @@ int launch_route_t(const MoeRouteParams& p, cudaStream_t s) {
   return launch_route<X, W, 4>(p, s);
 }
 
-template <int MAXT>
+template <int MB>
 int launch_experts(const MoeExpertsParams& p, const DeviceInfo* d, cudaStream_t s) {
   static std::atomic<uint64_t> configured{0};
-  constexpr int kMaxSmem =
-      kMoeWarps * 16 * 8 * MAXT * 4 + kMoeMaxExperts * 8 * MAXT * 2;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return BD_ERR_CUDA;
   const uint64_t bit = 1ull << (dev & 63);
   if (!(configured.load() & bit)) {
-    if (cudaFuncSetAttribute(moe_experts_kernel<MAXT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kMaxSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(moe_experts_kernel<MB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kMoeBBytes) != cudaSuccess)
       return BD_ERR_CUDA;
     configured.fetch_or(bit);
   }
-  const int smem = kMoeWarps * 16 * 8 * MAXT * 4 + std::min(p.E, p.T * p.k) * 8 * MAXT * 2;
   cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t cfg = config(2 * d->sm_count, smem, s, attr, 1);
-  return cudaLaunchKernelEx(&cfg, moe_experts_kernel<MAXT>, p) == cudaSuccess ? last_status()
+  const cudaLaunchConfig_t cfg = config(2 * d->sm_count, kMoeBBytes, s, attr, 1);
+  return cudaLaunchKernelEx(&cfg, moe_experts_kernel<MB>, p) == cudaSuccess ? last_status()
                                                                             : BD_ERR_CUDA;
 }
 
@@ -133,7 +137,11 @@ int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
   p.weights = weights;
   p.xs = reinterpret_cast<const __half*>(ws + w.xs);
   p.x_scale = reinterpret_cast<const float*>(ws + w.x_scale);
-  p.h = reinterpret_cast<__nv_bfloat16*>(ws + w.h);
+  p.h = reinterpret_cast<float*>(ws + w.h);
+  p.hmax = reinterpret_cast<uint32_t*>(ws + w.hmax);
+  p.part = reinterpret_cast<float*>(ws + w.part);
+  p.part_rows = w.part_rows;
+  p.vec_out = aligned(y, 16) ? 1 : 0;
   p.y = y;
   p.counters = reinterpret_cast<uint32_t*>(ws);
   p.T = T;
@@ -143,10 +151,11 @@ int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
   p.k = k;
   p.out_dtype = out_dtype;
   p.err = d->err;
-  if (T <= 8) return launch_experts<1>(p, d, s);
-  if (T <= 16) return launch_experts<2>(p, d, s);
-  if (T <= 32) return launch_experts<4>(p, d, s);
-  return launch_experts<8>(p, d, s);
+  // weight rows per task: 256 where the experts that can be touched give the machine two tasks per
+  // SM in the gate / up phase, else 128
+  const int64_t touched = std::min(E, T * k);
+  return touched * (I / 128) >= 2 * d->sm_count ? launch_experts<2>(p, d, s)
+                                                : launch_experts<1>(p, d, s);
 }
 
 }  // namespace
@@ -180,15 +189,17 @@ int bd_moe_experts(void* y, const void* x, int x_dtype, const int* ids, const fl
   __half* xs = reinterpret_cast<__half*>(ws + w.xs);
   float* x_scale = reinterpret_cast<float*>(ws + w.x_scale);
   uint32_t* counters = reinterpret_cast<uint32_t*>(ws);
+  uint32_t* hmax = reinterpret_cast<uint32_t*>(ws + w.hmax);
   cudaStream_t s = as_stream(stream);
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = config(T, 0, s, attr, 1);
   const cudaError_t e =
       x_dtype == BD_IN_BF16
           ? cudaLaunchKernelEx(&cfg, moe_prepare_kernel<__nv_bfloat16>,
-                               static_cast<const __nv_bfloat16*>(x), xs, x_scale, counters, H)
+                               static_cast<const __nv_bfloat16*>(x), xs, x_scale, counters, hmax, H,
+                               top_k)
           : cudaLaunchKernelEx(&cfg, moe_prepare_kernel<__half>, static_cast<const __half*>(x), xs,
-                               x_scale, counters, H);
+                               x_scale, counters, hmax, H, top_k);
   if (e != cudaSuccess) return BD_ERR_CUDA;
   return run_experts(y, out_dtype, ids, weights, a, T, H, I, E, top_k, ws, d, s);
 }
@@ -224,6 +235,7 @@ int bd_moe_layer(void* y, int* ids, float* weights, const void* x, int x_dtype,
   p.xs = reinterpret_cast<__half*>(ws + w.xs);
   p.x_scale = reinterpret_cast<float*>(ws + w.x_scale);
   p.counters = reinterpret_cast<uint32_t*>(ws);
+  p.hmax = reinterpret_cast<uint32_t*>(ws + w.hmax);
   p.T = T;
   p.H = H;
   p.E = E;

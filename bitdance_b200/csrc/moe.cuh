@@ -34,7 +34,15 @@ constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTopK = 16;
 constexpr int kMoeThreads = 256, kMoeWarps = kMoeThreads / 32;
 constexpr int kRouteCluster = 8;
 
-enum : int { kMoeShares = 0, kMoeDone = 1, kMoeDown = 2, kMoeCounters = 3 };
+// Counters in the workspace, zeroed by the first kernel: tickets and finished tasks per phase.
+enum : int {
+  kMoeGateUp = 0,
+  kMoeGateUpDone = 1,
+  kMoeDown = 2,
+  kMoeDownDone = 3,
+  kMoeCombine = 4,
+  kMoeCounters = 5
+};
 
 // Position of element k of a row in the scratch images of x and h. A thread of an MMA lane quad q
 // takes elements 32 q .. 32 q + 31 of a 128-block (one 16-byte piece of the weights' codes), in four
@@ -43,13 +51,6 @@ __host__ __device__ __forceinline__ int moe_perm(int k) {
   const int r = k & 127;
   return (k & ~127) + ((r >> 3) & 3) * 32 + (r >> 5) * 8 + (r & 7);
 }
-// h besides pairs elements m and m + 4 of a group of 8 (the pairs one shift of a word of codes
-// brings to the low ends of both 16-bit halves).
-__host__ __device__ __forceinline__ int moe_perm_h(int k) {
-  const int m = k & 7;
-  return (moe_perm(k) & ~7) + (m < 4 ? 2 * m : 2 * (m - 4) + 1);
-}
-
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -81,6 +82,7 @@ struct MoeRouteParams {
   __half* xs;              // (T, H) fp16 image, permuted
   float* x_scale;          // (T,) power of two
   uint32_t* counters;
+  uint32_t* hmax;
   int T, H, E, k;
   int sigmoid, renormalize;
   float routed_scale;
@@ -127,11 +129,13 @@ __device__ void moe_convert_token(const X* x, __half* xs, float* x_scale, int t,
 template <class X>
 __global__ void __launch_bounds__(kMoeThreads) moe_prepare_kernel(const X* x, __half* xs,
                                                                  float* x_scale,
-                                                                 uint32_t* counters, int H) {
+                                                                 uint32_t* counters,
+                                                                 uint32_t* hmax, int H, int k) {
   __shared__ uint32_t part[kMoeWarps];
   grid_dep_launch_dependents();
   grid_dep_wait();
   if (blockIdx.x == 0 && threadIdx.x < kMoeCounters) counters[threadIdx.x] = 0;
+  if (threadIdx.x < k) hmax[blockIdx.x * k + threadIdx.x] = 0;
   moe_convert_token(x, xs, x_scale, blockIdx.x, H, part);
 }
 
@@ -248,6 +252,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
       sum = 0.0;
       for (int r = 0; r < p.k; ++r) sum += sel[r];
     }
+    p.hmax[t * p.k + threadIdx.x] = 0;
     p.weights[t * p.k + threadIdx.x] =
         static_cast<float>(sel[threadIdx.x] / sum * static_cast<double>(p.routed_scale));
   }
@@ -266,11 +271,14 @@ struct MoeExpertsParams {
   const float* weights;
   const __half* xs;
   const float* x_scale;
-  __nv_bfloat16* h;          // (T k, I), permuted
+  float* h;                  // (T k, I) hidden values times weight and down scale
+  uint32_t* hmax;            // (T k,) bits of the largest |h| of a pair, zeroed by kernel 1
+  float* part;               // (slices, T k, H) partial sums; part_rows rows in all
   void* y;                   // (T, H)
   uint32_t* counters;
   int T, H, I, E, k;
-  int out_dtype;
+  int part_rows;
+  int out_dtype, vec_out;
   uint32_t* err;
 };
 
@@ -289,11 +297,6 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 __device__ __forceinline__ uint32_t byte_perm(uint32_t a, uint32_t b, uint32_t s) {
   return __byte_perm(a, b, s);
 }
@@ -304,14 +307,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 // Streaming load of 16 bytes of weights (read once: not kept in L1).
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
   uint4 v;
@@ -339,72 +334,30 @@ __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t scale, uint32_t (
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = mul_f16x2(cvt_e2m1x2_f16x2((w >> (8 * i)) & 0xFFu), scale);
 }
-// 8 codes -> four bf16x2 of code * scale * 2^-8, element pairs (i, i + 4). The code's three
-// magnitude bits sit as bf16 exponent and mantissa bits 8..6 = the value * 2^-126 (subnormals
-// included); the scale comes times 2^118.
-__device__ __forceinline__ void codes_bf16(uint32_t w, uint32_t scale, uint32_t (&o)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t sg = w << (12 - 4 * i);
-    const uint32_t mag = (i < 2 ? w << (6 - 4 * i) : w >> (4 * i - 6)) & 0x01C001C0u;
-    o[i] = mul_bf16x2((sg & 0x80008000u) | mag, scale);
-  }
-}
-// Two E4M3 scales (low byte first) times 2^118 as bf16, each in both halves of a word.
-__device__ __forceinline__ void scales_bf16(uint32_t pair, uint32_t& s0, uint32_t& s1) {
-  const uint32_t h = cvt_e4m3x2_f16x2(pair);
-  const __half2 hh = *reinterpret_cast<const __half2*>(&h);
-  const float up = __uint_as_float((127u + 118u) << 23);
-  const __nv_bfloat162 b =
-      __floats2bfloat162_rn(__low2float(hh) * up, __high2float(hh) * up);  // exact (4 bits)
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(&b);
-  s0 = byte_perm(w, w, 0x1010);
-  s1 = byte_perm(w, w, 0x3232);
-}
-
 struct MoePlan {
   int cnt[kMoeMaxExperts];           // pairs of an expert
   uint16_t off[kMoeMaxExperts];      // first pair of an expert in `pairs`
   uint16_t act[kMoeMaxExperts];      // experts with at least one pair, ascending
   uint16_t pairs[kMoeMaxTokens * kMoeMaxTopK];  // pairs t * k + slot, by expert
   float w[kMoeMaxTokens * kMoeMaxTopK];         // weight of a pair
-  uint8_t tiles[kMoeMaxExperts];     // by active expert: 8-token tiles with a pair (bit mask)
+  uint8_t used[kMoeMaxTokens * kMoeMaxTopK];    // the pair counts
   int nact;
   uint32_t ticket, flag;
+  uint32_t hmax[32];
 };
 
-// Batch of weight loads of a warp: kUnits units (128 elements of K) of two rows.
-constexpr int kMoeUnits = 4;
-struct MoeBatch {
-  uint4 a[kMoeUnits], b[kMoeUnits];
-  uint32_t sa[kMoeUnits], sb[kMoeUnits];
-};
-
-template <int MAXT>
-__global__ void __launch_bounds__(kMoeThreads, 2) moe_experts_kernel(const MoeExpertsParams p) {
-  extern __shared__ __align__(16) uint8_t dyn[];
-  __shared__ MoePlan pl;
-  constexpr int TP = 8 * MAXT;
-  // dynamic: partial sums of the down phase [warps][16][TP] fp32, then pair of (active expert,
-  // token) [nact][TP] int16, -1 where the token does not take the expert
-  float* red = reinterpret_cast<float*>(dyn);
-  int16_t* pair_of = reinterpret_cast<int16_t*>(dyn + kMoeWarps * 16 * TP * 4);
+// Pairs by expert. A token that names an expert twice keeps the first pair with the sum of the
+// weights; ids outside [0, E) are no pair (-1 quietly, others reported). Ends with a barrier.
+__device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, q = lane & 3;
   const int npairs = p.T * p.k;
-
-  for (int e = tid; e < p.E; e += kMoeThreads) pl.cnt[e] = 0;
-  __syncthreads();
-  grid_dep_wait();
-  if (tid == 0) pl.ticket = atomicAdd(p.counters + kMoeShares, 1u);
-
-  // ---- plan: pairs by expert. A token that names an expert twice keeps the first pair with the
-  // sum of the weights; ids outside [0, E) are no pair (-1 quietly, others reported).
-  int id[(kMoeMaxTokens * kMoeMaxTopK) / kMoeThreads], pos[(kMoeMaxTokens * kMoeMaxTopK) / kMoeThreads];
+  constexpr int kPer = kMoeMaxTokens * kMoeMaxTopK / kMoeThreads;
+  int id[kPer], pos[kPer];
 #pragma unroll
-  for (int i = 0; i < kMoeMaxTokens * kMoeMaxTopK / kMoeThreads; ++i) {
+  for (int i = 0; i < kPer; ++i) {
     const int pr = tid + i * kMoeThreads;
     id[i] = -1;
+    pos[i] = 0;
     if (pr < npairs) {
       int e = p.ids[pr];
       if (e < 0 || e >= p.E) {
@@ -422,6 +375,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_experts_kernel(const MoeEx
         pos[i] = atomicAdd(&pl.cnt[e], 1);
         pl.w[pr] = w;
       }
+      pl.used[pr] = e >= 0;
       id[i] = e;
     }
   }
@@ -438,10 +392,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_experts_kernel(const MoeEx
         if (lane >= o) inc += u;
       }
       if (c > 0) {
-        const int a = nact + __popc(has & ((1u << lane) - 1u));
-        pl.act[a] = static_cast<uint16_t>(e0 + lane);
+        pl.act[nact + __popc(has & ((1u << lane) - 1u))] = static_cast<uint16_t>(e0 + lane);
         pl.off[e0 + lane] = static_cast<uint16_t>(off + inc - c);
-        pl.tiles[a] = 0;
       }
       nact += __popc(has);
       off += __shfl_sync(0xFFFFFFFFu, inc, 31);
@@ -449,212 +401,364 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_experts_kernel(const MoeEx
     if (lane == 0) pl.nact = nact;
   }
   __syncthreads();
-  const int nact = pl.nact;
+  // the place of a pair within its expert's list is the order of arrival: it picks an MMA
+  // column, not a value
 #pragma unroll
-  for (int i = 0; i < kMoeMaxTokens * kMoeMaxTopK / kMoeThreads; ++i)
+  for (int i = 0; i < kPer; ++i)
     if (id[i] >= 0) pl.pairs[pl.off[id[i]] + pos[i]] = static_cast<uint16_t>(tid + i * kMoeThreads);
-  for (int i = tid; i < nact * TP; i += kMoeThreads) pair_of[i] = -1;
   __syncthreads();
-  for (int a = warp; a < nact; a += kMoeWarps) {
-    const int e = pl.act[a], n = pl.cnt[e];
-    uint32_t mask = 0;
-    for (int c = lane; c < n; c += 32) {
-      const int pr = pl.pairs[pl.off[e] + c];
-      pair_of[a * TP + pr / p.k] = static_cast<int16_t>(pr);
-      mask |= 1u << (pr / p.k / 8);
-    }
-    mask = __reduce_or_sync(0xFFFFFFFFu, mask);
-    if (lane == 0) pl.tiles[a] = static_cast<uint8_t>(mask);
-  }
+}
 
-  // ---- gate / up: granules of 8 hidden units (rows g: gate, g + 8: up of the MMA) over all of H
-  const int gpe = p.I / 8;
-  const int64_t granules = static_cast<int64_t>(nact) * gpe;
-  const int shares = gridDim.x;
-  __syncthreads();
-  uint32_t share = pl.ticket;
-  while (share < static_cast<uint32_t>(shares)) {
-    const int64_t g0 = granules * share / shares, g1 = granules * (share + 1) / shares;
-    for (int64_t gi = g0 + warp; gi < g1; gi += kMoeWarps) {
-      const int a = static_cast<int>(gi / gpe), gl = static_cast<int>(gi % gpe);
-      const int e = pl.act[a], n = pl.cnt[e], off = pl.off[e];
-      const int nt = (n + 7) / 8;
-      const int64_t row = static_cast<int64_t>(e) * 2 * p.I + 8 * gl + g;
-      const uint8_t* ca = p.w13 + row * (p.H / 2) + 16 * q;
-      const uint8_t* cb = ca + static_cast<int64_t>(p.I) * (p.H / 2);
-      const uint8_t* sa = p.s13 + row * (p.H / 16) + 2 * q;
-      const uint8_t* sb = sa + static_cast<int64_t>(p.I) * (p.H / 16);
-      const __half* xt[MAXT];
-#pragma unroll
-      for (int i = 0; i < MAXT; ++i) {
-        const int c = 8 * i + g;
-        xt[i] = c < n ? p.xs + static_cast<int64_t>(pl.pairs[off + c] / p.k) * p.H + 8 * q : nullptr;
+// tid 0: until *counter >= target (bounded); the others take the answer from pl.flag after a
+// barrier. The writes counted before are visible to the CTA afterwards.
+__device__ __forceinline__ bool moe_wait(const uint32_t* counter, uint32_t target, MoePlan& pl,
+                                         uint32_t* err) {
+  if (threadIdx.x == 0) {
+    uint32_t ok = 1;
+    const long long c0 = clock64();
+    while (ld_acquire_gpu(counter) < target) {
+      if (static_cast<unsigned long long>(clock64() - c0) > kWaitLimitCycles) {
+        atomicOr(err, kErrWaitOperand);
+        ok = 0;
+        break;
       }
-      float acc[MAXT][4] = {};
-      const int units = p.H / 128;
-      MoeBatch cur, nxt;
-      auto fetch = [&](MoeBatch& b, int u0) {
+    }
+    pl.flag = ok;
+  }
+  __syncthreads();
+  return pl.flag != 0;
+}
+
+// Exponent that takes a row whose largest magnitude has these bits to [2^14, 2^15) (fp16): the row
+// times 2^(14 - E).
+__device__ __forceinline__ int moe_row_exp(uint32_t amax_bits) {
+  return amax_bits >= 0x7F800000u ? 14 : max(-100, static_cast<int>(amax_bits >> 23) - 127);
+}
+__device__ __forceinline__ float pow2f(int e) {
+  return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
+// Weights of one unit (128 elements of K) of a warp's 16 MB rows: per MMA row block the 16 code
+// bytes and two scale bytes of this lane in rows g and g + 8.
+template <int MB>
+struct MoeUnit {
+  uint4 a[MB], b[MB];
+  uint32_t sa[MB], sb[MB];
+};
+struct MoeRows {
+  const uint8_t *codes, *scales;  // this lane's place in row g of the warp's first row block
+  int64_t block, second;          // bytes of codes from row block to row block, from row g to g + 8
+};
+template <int MB>
+__device__ __forceinline__ void moe_fetch(MoeUnit<MB>& w, const MoeRows& r, int u) {
 #pragma unroll
-        for (int i = 0; i < kMoeUnits; ++i)
-          if (u0 + i < units) {
-            b.a[i] = ld_stream(ca + (u0 + i) * 64);
-            b.b[i] = ld_stream(cb + (u0 + i) * 64);
-            b.sa[i] = __ldg(reinterpret_cast<const unsigned short*>(sa + (u0 + i) * 8));
-            b.sb[i] = __ldg(reinterpret_cast<const unsigned short*>(sb + (u0 + i) * 8));
-          }
-      };
-      fetch(cur, 0);
-      for (int u0 = 0; u0 < units; u0 += kMoeUnits) {
-        fetch(nxt, u0 + kMoeUnits);
+  for (int m = 0; m < MB; ++m) {
+    const uint8_t* c = r.codes + m * r.block + u * 64;
+    const uint8_t* s = r.scales + (m * r.block >> 3) + u * 8;
+    w.a[m] = ld_stream(c);
+    w.b[m] = ld_stream(c + r.second);
+    w.sa[m] = __ldg(reinterpret_cast<const unsigned short*>(s));
+    w.sb[m] = __ldg(reinterpret_cast<const unsigned short*>(s + (r.second >> 3)));
+  }
+}
+
+constexpr int kMoeTiles = 4;                // token tiles (8 columns each) per pass over the weights
+constexpr int kMoeBBytes = 72 * 1024;       // staged activations
+constexpr int kMoePad = 64;                 // bytes between token rows: conflict-free 16-byte reads
+
+// One unit against nt staged token tiles: tok is this lane's place in the staged block (token row g
+// of tile 0, 16 bytes per MMA pair), `tile` bytes on to the next tile.
+template <int MB>
+__device__ __forceinline__ void moe_unit(float (&acc)[MB][kMoeTiles][4], const MoeUnit<MB>& w,
+                                         uint32_t tok, uint32_t tile, int nt) {
+  uint32_t ha[MB], hb[MB];
 #pragma unroll
-        for (int i = 0; i < kMoeUnits; ++i) {
-          if (u0 + i >= units) break;
-          const uint32_t ha = cvt_e4m3x2_f16x2(cur.sa[i]), hb = cvt_e4m3x2_f16x2(cur.sb[i]);
-          const uint32_t wa[4] = {cur.a[i].x, cur.a[i].y, cur.a[i].z, cur.a[i].w};
-          const uint32_t wb[4] = {cur.b[i].x, cur.b[i].y, cur.b[i].z, cur.b[i].w};
+  for (int m = 0; m < MB; ++m) {
+    ha[m] = cvt_e4m3x2_f16x2(w.sa[m]);
+    hb[m] = cvt_e4m3x2_f16x2(w.sb[m]);
+  }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t sel = j < 2 ? 0x1010 : 0x3232;
-            uint32_t ga[4], ua[4];
-            codes_f16(wa[j], byte_perm(ha, ha, sel), ga);
-            codes_f16(wb[j], byte_perm(hb, hb, sel), ua);
+  for (int j = 0; j < 4; ++j) {
+    uint4 xb[kMoeTiles];
 #pragma unroll
-            for (int m = 0; m < MAXT; ++m) {
-              if (m >= nt) break;
-              uint4 xb = make_uint4(0, 0, 0, 0);
-              if (xt[m] != nullptr)
-                xb = __ldg(reinterpret_cast<const uint4*>(xt[m] + (u0 + i) * 128 + 32 * j));
-              mma_f16(acc[m], ga[0], ua[0], ga[1], ua[1], xb.x, xb.y);
-              mma_f16(acc[m], ga[2], ua[2], ga[3], ua[3], xb.z, xb.w);
-            }
+    for (int t = 0; t < kMoeTiles; ++t)
+      if (t < nt) {
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(xb[t].x), "=r"(xb[t].y), "=r"(xb[t].z), "=r"(xb[t].w)
+                     : "r"(tok + t * tile + 64 * j));
+      }
+    const uint32_t sel = j < 2 ? 0x1010 : 0x3232;
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      const uint32_t wa = j == 0 ? w.a[m].x : j == 1 ? w.a[m].y : j == 2 ? w.a[m].z : w.a[m].w;
+      const uint32_t wb = j == 0 ? w.b[m].x : j == 1 ? w.b[m].y : j == 2 ? w.b[m].z : w.b[m].w;
+      uint32_t fa[4], fb[4];
+      codes_f16(wa, byte_perm(ha[m], ha[m], sel), fa);
+      codes_f16(wb, byte_perm(hb[m], hb[m], sel), fb);
+#pragma unroll
+      for (int t = 0; t < kMoeTiles; ++t)
+        if (t < nt) {
+          mma_f16(acc[m][t], fa[0], fb[0], fa[1], fb[1], xb[t].x, xb[t].y);
+          mma_f16(acc[m][t], fa[2], fb[2], fa[3], fb[3], xb[t].z, xb[t].w);
+        }
+    }
+  }
+}
+
+// The experts' kernel. Tasks of 8 warps x 16 MB weight rows of one expert, all of the expert's tokens
+// (in passes of 32 where more take it), K streamed: weights from global memory to registers one unit
+// ahead, activations staged in shared memory for all eight warps, as much of K at a time as fits.
+//   gate / up: 64 MB hidden units (MMA row g: gate, g + 8: up of one unit, so one thread holds both
+//              values of the same token); h = silu(gate) up w ts in fp32, and its row maximum;
+//   down:      128 MB output rows of one expert and a slice of I; h staged as fp16 times the power of
+//              two that brings its row's maximum to [2^14, 2^15); partial sums per (slice, pair);
+//   combine:   y = the partial sums of a token's pairs in slot order.
+// Each phase's tasks wait for the phase before (see the ticket argument at the top).
+template <int MB>
+__global__ void __launch_bounds__(kMoeThreads, 2) moe_experts_kernel(const MoeExpertsParams p) {
+  extern __shared__ __align__(16) uint8_t stage[];
+  __shared__ MoePlan pl;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, q = lane & 3;
+
+  for (int e = tid; e < p.E; e += kMoeThreads) pl.cnt[e] = 0;
+  __syncthreads();
+  grid_dep_wait();
+  if (tid == 0) pl.ticket = atomicAdd(p.counters + kMoeGateUp, 1u);
+  moe_plan(p, pl);
+  const int nact = pl.nact;
+
+  const int blocks1 = p.I / (64 * MB);
+  const uint32_t total1 = static_cast<uint32_t>(nact) * blocks1;
+  const int blocks2 = (p.H + 128 * MB - 1) / (128 * MB);
+  const int units2 = p.I / 128;
+  // slices of I per down task: while the tasks do not fill the grid and the partials fit
+  int slices = 1;
+  while (nact * blocks2 * slices < static_cast<int>(gridDim.x) &&
+         2 * slices * p.T * p.k <= p.part_rows && units2 >= 4 * slices)
+    slices *= 2;
+  const uint32_t total2 = static_cast<uint32_t>(nact) * blocks2 * slices;
+
+  // tokens [c0, c0 + n) of an expert: geometry of the staged block
+  auto chunk_units = [](int n8) { return min((kMoeBBytes / n8 - kMoePad) / 256, 1 << 20); };
+  const uint32_t stage_u = smem_u32(stage);
+
+  // ------------------------------------------------------------------------------ gate / up
+  while (true) {
+    const uint32_t task = pl.ticket;
+    if (task >= total1) break;
+    const int a = task / blocks1, blk = task % blocks1;
+    const int e = pl.act[a], cnt = pl.cnt[e], off = pl.off[e];
+    const int i0 = blk * 64 * MB + warp * 8 * MB;  // this warp's first hidden unit
+    const int units = p.H / 128;
+    MoeRows rows;
+    {
+      const int64_t row = static_cast<int64_t>(e) * 2 * p.I + i0 + g;
+      rows.codes = p.w13 + row * (p.H / 2) + 16 * q;
+      rows.scales = p.s13 + row * (p.H / 16) + 2 * q;
+      rows.block = static_cast<int64_t>(8) * (p.H / 2);
+      rows.second = static_cast<int64_t>(p.I) * (p.H / 2);
+    }
+    const float ts13 = p.ts13[e], ts2 = p.ts2[e];
+    for (int c0 = 0; c0 < cnt; c0 += 8 * kMoeTiles) {
+      const int n = min(cnt - c0, 8 * kMoeTiles), nt = (n + 7) / 8;
+      const int cu = chunk_units(8 * nt);
+      float acc[MB][kMoeTiles][4] = {};
+      MoeUnit<MB> cur, nxt;
+      moe_fetch(cur, rows, 0);
+      for (int u0 = 0; u0 < units; u0 += cu) {
+        const int uc = min(cu, units - u0);
+        const uint32_t pitch = uc * 256 + kMoePad;
+        if (u0 > 0) __syncthreads();  // the block staged before is read
+        for (int c = warp; c < 8 * nt; c += kMoeWarps) {
+          const int4* src = reinterpret_cast<const int4*>(
+              c < n ? p.xs + static_cast<int64_t>(pl.pairs[off + c0 + c] / p.k) * p.H + u0 * 128
+                    : nullptr);
+          for (int i = lane; i < uc * 16; i += 32) {
+            const uint32_t dst = stage_u + c * pitch + i * 16;
+            if (src != nullptr)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src + i)
+                           : "memory");
+            else
+              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst), "r"(0) : "memory");
           }
         }
-        cur = nxt;
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
+        uint32_t tok = stage_u + g * pitch + 16 * q;
+#pragma unroll 1
+        for (int u = u0; u < u0 + uc; ++u, tok += 256) {
+          if (u + 1 < units) moe_fetch(nxt, rows, u + 1);
+          moe_unit<MB>(acc, cur, tok, 8 * pitch, nt);
+          cur = nxt;
+        }
       }
-      const float ts13 = p.ts13[e], ts2 = p.ts2[e];
-      const int at = moe_perm_h(8 * gl + g);
+      if (tid < 32) pl.hmax[tid] = 0;
+      __syncthreads();
 #pragma unroll
-      for (int m = 0; m < MAXT; ++m)
+      for (int t = 0; t < kMoeTiles; ++t) {
+        if (t >= nt) break;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int col = 8 * m + 2 * q + c;
+          const int col = 8 * t + 2 * q + c;
+          uint32_t hm = 0;
           if (col < n) {
-            const int pr = pl.pairs[off + col];
-            const float s = p.x_scale[pr / p.k] * ts13;
-            const float gate = acc[m][c] * s, up = acc[m][2 + c] * s;
-            const float hv = silu_rn(gate) * up * (pl.w[pr] * ts2);
-            p.h[static_cast<int64_t>(pr) * p.I + at] = __float2bfloat16_rn(hv);
+            const int pr = pl.pairs[off + c0 + col];
+            const float s = p.x_scale[pr / p.k] * ts13, wt = pl.w[pr] * ts2;
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+              const float h = silu_rn(acc[m][t][c] * s) * (acc[m][t][2 + c] * s) * wt;
+              p.h[static_cast<int64_t>(pr) * p.I + i0 + 8 * m + g] = h;
+              hm = max(hm, __float_as_uint(h) & 0x7FFFFFFFu);
+            }
           }
+          hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, 4));
+          hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, 8));
+          hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, 16));
+          if (g == 0 && col < n) atomicMax(&pl.hmax[col], hm);
         }
-    }
-    __syncthreads();  // the share's hidden values are written (and the ticket is read)
-    if (tid == 0) {
-      __threadfence();
-      atomicAdd(p.counters + kMoeDone, 1u);
-      pl.ticket = atomicAdd(p.counters + kMoeShares, 1u);
+      }
+      __syncthreads();
+      if (tid < n) atomicMax(p.hmax + pl.pairs[off + c0 + tid], pl.hmax[tid]);
     }
     __syncthreads();
-    share = pl.ticket;
+    if (tid == 0) {
+      __threadfence();
+      atomicAdd(p.counters + kMoeGateUpDone, 1u);
+      pl.ticket = atomicAdd(p.counters + kMoeGateUp, 1u);
+    }
+    __syncthreads();
   }
 
-  // ---- down: tasks of 16 output rows over all active experts and all of I, units (expert,
-  // 128-block) dealt to the warps in turn; columns are the tokens, so one accumulator collects
-  // every expert's part
-  const int tasks = p.H / 16, upe = p.I / 128, units = nact * upe;
-  const int per_warp = units > warp ? (units - warp + kMoeWarps - 1) / kMoeWarps : 0;
+  // ---------------------------------------------------------------------------------- down
   bool ready = false;
   while (true) {
     __syncthreads();
     if (tid == 0) pl.ticket = atomicAdd(p.counters + kMoeDown, 1u);
     __syncthreads();
     const uint32_t task = pl.ticket;
-    if (task >= static_cast<uint32_t>(tasks)) break;
-    const int64_t row = 16 * static_cast<int64_t>(task) + g;
-    MoeBatch cur, nxt;
-    auto fetch = [&](MoeBatch& b, int v0) {  // v0: number of the unit within this warp's
+    if (task >= total2) break;
+    const int z = task % slices, ab = task / slices;
+    const int a = ab / blocks2, blk = ab % blocks2;
+    const int e = pl.act[a], cnt = pl.cnt[e], off = pl.off[e];
+    const int r0 = blk * 128 * MB + warp * 16 * MB;  // this warp's first output row
+    const bool active = r0 < p.H;                   // H % 128 == 0: whole warps
+    const int ub = static_cast<int>(static_cast<int64_t>(units2) * z / slices);
+    const int ue = static_cast<int>(static_cast<int64_t>(units2) * (z + 1) / slices);
+    MoeRows rows;
+    {
+      const int64_t row = static_cast<int64_t>(e) * p.H + (active ? r0 : 0) + g;
+      rows.codes = p.w2 + row * (p.I / 2) + 16 * q;
+      rows.scales = p.s2 + row * (p.I / 16) + 2 * q;
+      rows.block = static_cast<int64_t>(16) * (p.I / 2);
+      rows.second = static_cast<int64_t>(8) * (p.I / 2);
+    }
+    for (int c0 = 0; c0 < cnt; c0 += 8 * kMoeTiles) {
+      const int n = min(cnt - c0, 8 * kMoeTiles), nt = (n + 7) / 8;
+      const int cu = chunk_units(8 * nt);
+      float acc[MB][kMoeTiles][4] = {};
+      MoeUnit<MB> cur, nxt;
+      moe_fetch(cur, rows, ub);
+      if (!ready) {
+        if (!moe_wait(p.counters + kMoeGateUpDone, total1, pl, p.err)) return;
+        ready = true;
+      }
+      for (int u0 = ub; u0 < ue; u0 += cu) {
+        const int uc = min(cu, ue - u0);
+        const uint32_t pitch = uc * 256 + kMoePad;
+        __syncthreads();
+        for (int c = warp; c < 8 * nt; c += kMoeWarps) {
+          const int pr = c < n ? pl.pairs[off + c0 + c] : -1;
+          const float* src = pr >= 0 ? p.h + static_cast<int64_t>(pr) * p.I + u0 * 128 : nullptr;
+          const float up = pr >= 0 ? pow2f(14 - moe_row_exp(__ldcg(p.hmax + pr))) : 0.0f;
+          for (int i = lane; i < uc * 16; i += 32) {
+            // piece i of the permuted row: elements 32 q + 8 j .. + 7 of block i / 16
+            uint32_t w[4] = {0, 0, 0, 0};
+            if (src != nullptr) {
+              const float* s = src + (i >> 4) * 128 + 32 * (i & 3) + 8 * ((i >> 2) & 3);
+              const uint4 lo = ld_cg(s), hi = ld_cg(s + 4);
+              const uint32_t v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-      for (int i = 0; i < kMoeUnits; ++i)
-        if (v0 + i < per_warp) {
-          const int u = warp + (v0 + i) * kMoeWarps;
-          const int a = u / upe, blk = u - a * upe;
-          const int64_t r = static_cast<int64_t>(pl.act[a]) * p.H + row;
-          const uint8_t* c = p.w2 + r * (p.I / 2) + blk * 64 + 16 * q;
-          const uint8_t* s = p.s2 + r * (p.I / 16) + blk * 8 + 2 * q;
-          b.a[i] = ld_stream(c);
-          b.b[i] = ld_stream(c + static_cast<int64_t>(8) * (p.I / 2));
-          b.sa[i] = __ldg(reinterpret_cast<const unsigned short*>(s));
-          b.sb[i] = __ldg(reinterpret_cast<const unsigned short*>(s + static_cast<int64_t>(8) * (p.I / 16)));
-        }
-    };
-    fetch(cur, 0);
-    if (!ready) {
-      // all hidden values (bounded: every share is held by a running CTA)
-      if (tid == 0) {
-        uint32_t ok = 1;
-        const long long c0 = clock64();
-        while (ld_acquire_gpu(p.counters + kMoeDone) < static_cast<uint32_t>(shares)) {
-          if (static_cast<unsigned long long>(clock64() - c0) > kWaitLimitCycles) {
-            atomicOr(p.err, kErrWaitOperand);
-            ok = 0;
-            break;
+              for (int j = 0; j < 4; ++j) {
+                const __half2 hh = __floats2half2_rn(__uint_as_float(v[2 * j]) * up,
+                                                     __uint_as_float(v[2 * j + 1]) * up);
+                w[j] = *reinterpret_cast<const uint32_t*>(&hh);
+              }
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stage_u + c * pitch + i * 16),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
           }
         }
-        pl.flag = ok;
+        __syncthreads();
+        uint32_t tok = stage_u + g * pitch + 16 * q;
+        if (active) {
+#pragma unroll 1
+          for (int u = u0; u < u0 + uc; ++u, tok += 256) {
+            if (u + 1 < ue) moe_fetch(nxt, rows, u + 1);
+            moe_unit<MB>(acc, cur, tok, 8 * pitch, nt);
+            cur = nxt;
+          }
+        }
       }
-      __syncthreads();
-      if (pl.flag == 0) return;
+      if (active) {
+#pragma unroll
+        for (int t = 0; t < kMoeTiles; ++t) {
+          if (t >= nt) break;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int col = 8 * t + 2 * q + c;
+            if (col < n) {
+              const int pr = pl.pairs[off + c0 + col];
+              const float back = pow2f(moe_row_exp(__ldcg(p.hmax + pr)) - 14);
+              float* dst = p.part + (static_cast<int64_t>(z) * p.T * p.k + pr) * p.H + r0 + g;
+#pragma unroll
+              for (int m = 0; m < MB; ++m) {
+                dst[16 * m] = acc[m][t][c] * back;
+                dst[16 * m + 8] = acc[m][t][2 + c] * back;
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (tid == 0) {
+      __threadfence();
+      atomicAdd(p.counters + kMoeDownDone, 1u);
+    }
+  }
+
+  // -------------------------------------------------------------------------------- combine
+  const int cols = 4 * kMoeThreads;  // outputs per task
+  const int blocks3 = (p.H + cols - 1) / cols;
+  ready = false;
+  while (true) {
+    __syncthreads();
+    if (tid == 0) pl.ticket = atomicAdd(p.counters + kMoeCombine, 1u);
+    __syncthreads();
+    const uint32_t task = pl.ticket;
+    if (task >= static_cast<uint32_t>(p.T * blocks3)) break;
+    if (!ready) {
+      if (!moe_wait(p.counters + kMoeDownDone, total2, pl, p.err)) return;
       ready = true;
     }
-    float acc[MAXT][4] = {};
-    for (int v0 = 0; v0 < per_warp; v0 += kMoeUnits) {
-      fetch(nxt, v0 + kMoeUnits);
-#pragma unroll
-      for (int i = 0; i < kMoeUnits; ++i) {
-        if (v0 + i >= per_warp) break;
-        const int u = warp + (v0 + i) * kMoeWarps;
-        const int a = u / upe, blk = u - a * upe;
-        const uint32_t tiles = pl.tiles[a];
-        uint32_t s00, s01, s10, s11;
-        scales_bf16(cur.sa[i], s00, s01);
-        scales_bf16(cur.sb[i], s10, s11);
-        const uint32_t wa[4] = {cur.a[i].x, cur.a[i].y, cur.a[i].z, cur.a[i].w};
-        const uint32_t wb[4] = {cur.b[i].x, cur.b[i].y, cur.b[i].z, cur.b[i].w};
-        const __nv_bfloat16* ht[MAXT];
-#pragma unroll
-        for (int m = 0; m < MAXT; ++m) {
-          const int pr = pair_of[a * TP + 8 * m + g];
-          ht[m] = pr >= 0 ? p.h + static_cast<int64_t>(pr) * p.I + blk * 128 + 8 * q : nullptr;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t ra[4], rb[4];
-          codes_bf16(wa[j], j < 2 ? s00 : s01, ra);
-          codes_bf16(wb[j], j < 2 ? s10 : s11, rb);
-#pragma unroll
-          for (int m = 0; m < MAXT; ++m) {
-            if (MAXT > 1 && !((tiles >> m) & 1u)) continue;
-            uint4 hb = make_uint4(0, 0, 0, 0);
-            if (ht[m] != nullptr) hb = ld_cg(ht[m] + 32 * j);
-            mma_bf16(acc[m], ra[0], rb[0], ra[1], rb[1], hb.x, hb.y);
-            mma_bf16(acc[m], ra[2], rb[2], ra[3], rb[3], hb.z, hb.w);
-          }
-        }
+    const int t = task / blocks3, h0 = (task % blocks3) * cols + 4 * tid;
+    if (h0 >= p.H) continue;
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < p.k; ++s) {
+      const int pr = t * p.k + s;
+      if (!pl.used[pr]) continue;
+      for (int z = 0; z < slices; ++z) {
+        const uint4 v =
+            ld_cg(p.part + (static_cast<int64_t>(z) * p.T * p.k + pr) * p.H + h0);
+        o[0] += __uint_as_float(v.x);
+        o[1] += __uint_as_float(v.y);
+        o[2] += __uint_as_float(v.z);
+        o[3] += __uint_as_float(v.w);
       }
-      cur = nxt;
     }
-#pragma unroll
-    for (int m = 0; m < MAXT; ++m)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        red[(warp * 16 + g + 8 * (c >> 1)) * TP + 8 * m + 2 * q + (c & 1)] = acc[m][c];
-    __syncthreads();
-    for (int i = tid; i < 16 * p.T; i += kMoeThreads) {
-      const int t = i / 16, r = i % 16;
-      float s = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kMoeWarps; ++w) s += red[(w * 16 + r) * TP + t];
-      store_out(p.y, static_cast<int64_t>(t) * p.H + 16 * task + r, s * 256.0f, p.out_dtype);
-    }
+    store_row<4>(p.y, static_cast<int64_t>(t) * p.H + h0, o, p.out_dtype, p.vec_out);
   }
 }
 

@@ -82,7 +82,11 @@ def _workspace_bytes(T: int, H: int, inter: int, top_k: int) -> int:
     """bd_query_moe_workspace without the call."""
     def up(v):
         return (v + 255) // 256 * 256
-    return 256 + up(2 * T * H) + up(4 * T) + up(2 * T * top_k * inter)
+    if T == 0:
+        return 0
+    pairs = T * top_k
+    return 256 + up(4 * pairs) + up(4 * T) + up(2 * T * H) + up(4 * pairs * inter) + \
+        4 * H * max(pairs, 256)
 
 
 def _out_tensor(out, x: torch.Tensor, out_dtype):

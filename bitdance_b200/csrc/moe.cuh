@@ -282,10 +282,14 @@ struct MoeExpertsParams {
   uint32_t* err;
 };
 
-__device__ __forceinline__ uint32_t cvt_e2m1x2_f16x2(uint32_t byte) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 b;\n\tcvt.u8.u32 b, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(r) : "r"(byte));
-  return r;
+// 8 codes (four bytes) -> four f16x2.
+__device__ __forceinline__ void cvt_e2m1x8_f16(uint32_t w, uint32_t (&o)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+      : "r"(w));
 }
 __device__ __forceinline__ uint32_t cvt_e4m3x2_f16x2(uint32_t pair) {
   uint32_t r;
@@ -331,8 +335,9 @@ __device__ __forceinline__ uint32_t ld_acquire_gpu(const uint32_t* p) {
 
 // 8 codes -> four f16x2 of code * scale (adjacent elements), scale in both halves.
 __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t scale, uint32_t (&o)[4]) {
+  cvt_e2m1x8_f16(w, o);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = mul_f16x2(cvt_e2m1x2_f16x2((w >> (8 * i)) & 0xFFu), scale);
+  for (int i = 0; i < 4; ++i) o[i] = mul_f16x2(o[i], scale);
 }
 struct MoePlan {
   int cnt[kMoeMaxExperts];           // pairs of an expert
@@ -468,9 +473,9 @@ constexpr int kMoePad = 64;                 // bytes between token rows: conflic
 
 // One unit against nt staged token tiles: tok is this lane's place in the staged block (token row g
 // of tile 0, 16 bytes per MMA pair), `tile` bytes on to the next tile.
-template <int MB>
+template <int MB, int NT>
 __device__ __forceinline__ void moe_unit(float (&acc)[MB][kMoeTiles][4], const MoeUnit<MB>& w,
-                                         uint32_t tok, uint32_t tile, int nt) {
+                                         uint32_t tok, uint32_t tile) {
   uint32_t ha[MB], hb[MB];
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
@@ -479,14 +484,12 @@ __device__ __forceinline__ void moe_unit(float (&acc)[MB][kMoeTiles][4], const M
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint4 xb[kMoeTiles];
+    uint4 xb[NT];
 #pragma unroll
-    for (int t = 0; t < kMoeTiles; ++t)
-      if (t < nt) {
-        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(xb[t].x), "=r"(xb[t].y), "=r"(xb[t].z), "=r"(xb[t].w)
-                     : "r"(tok + t * tile + 64 * j));
-      }
+    for (int t = 0; t < NT; ++t)
+      asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(xb[t].x), "=r"(xb[t].y), "=r"(xb[t].z), "=r"(xb[t].w)
+                   : "r"(tok + t * tile + 64 * j));
     const uint32_t sel = j < 2 ? 0x1010 : 0x3232;
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
@@ -496,13 +499,43 @@ __device__ __forceinline__ void moe_unit(float (&acc)[MB][kMoeTiles][4], const M
       codes_f16(wa, byte_perm(ha[m], ha[m], sel), fa);
       codes_f16(wb, byte_perm(hb[m], hb[m], sel), fb);
 #pragma unroll
-      for (int t = 0; t < kMoeTiles; ++t)
-        if (t < nt) {
-          mma_f16(acc[m][t], fa[0], fb[0], fa[1], fb[1], xb[t].x, xb[t].y);
-          mma_f16(acc[m][t], fa[2], fb[2], fa[3], fb[3], xb[t].z, xb[t].w);
-        }
+      for (int t = 0; t < NT; ++t) {
+        mma_f16(acc[m][t], fa[0], fb[0], fa[1], fb[1], xb[t].x, xb[t].y);
+        mma_f16(acc[m][t], fa[2], fb[2], fa[3], fb[3], xb[t].z, xb[t].w);
+      }
     }
   }
+}
+
+// Units [u0, u1) of a warp's rows against the staged block that begins with unit u0; w holds the
+// weights of u0 and ends with those of u1 (when u1 < end).
+template <int MB, int NT>
+__device__ __forceinline__ void moe_run(float (&acc)[MB][kMoeTiles][4], MoeUnit<MB>& w,
+                                        const MoeRows& rows, int u0, int u1, int end,
+                                        uint32_t tok, uint32_t tile) {
+  MoeUnit<MB> nxt;
+  int u = u0;
+#pragma unroll 1
+  for (; u + 2 <= u1; u += 2, tok += 512) {
+    moe_fetch(nxt, rows, u + 1);
+    moe_unit<MB, NT>(acc, w, tok, tile);
+    if (u + 2 < end) moe_fetch(w, rows, u + 2);
+    moe_unit<MB, NT>(acc, nxt, tok + 256, tile);
+  }
+  if (u < u1) {
+    if (u + 1 < end) moe_fetch(nxt, rows, u + 1);
+    moe_unit<MB, NT>(acc, w, tok, tile);
+    w = nxt;
+  }
+}
+template <int MB>
+__device__ __forceinline__ void moe_run(float (&acc)[MB][kMoeTiles][4], MoeUnit<MB>& w,
+                                        const MoeRows& rows, int u0, int u1, int end,
+                                        uint32_t tok, uint32_t tile, int nt) {
+  if (nt == 1) moe_run<MB, 1>(acc, w, rows, u0, u1, end, tok, tile);
+  else if (nt == 2) moe_run<MB, 2>(acc, w, rows, u0, u1, end, tok, tile);
+  else if (nt == 3) moe_run<MB, 3>(acc, w, rows, u0, u1, end, tok, tile);
+  else moe_run<MB, 4>(acc, w, rows, u0, u1, end, tok, tile);
 }
 
 // The experts' kernel. Tasks of 8 warps x 16 MB weight rows of one expert, all of the expert's tokens
@@ -564,7 +597,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_experts_kernel(const MoeEx
       const int n = min(cnt - c0, 8 * kMoeTiles), nt = (n + 7) / 8;
       const int cu = chunk_units(8 * nt);
       float acc[MB][kMoeTiles][4] = {};
-      MoeUnit<MB> cur, nxt;
+      MoeUnit<MB> cur;
       moe_fetch(cur, rows, 0);
       for (int u0 = 0; u0 < units; u0 += cu) {
         const int uc = min(cu, units - u0);
@@ -585,13 +618,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_experts_kernel(const MoeEx
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
-        uint32_t tok = stage_u + g * pitch + 16 * q;
-#pragma unroll 1
-        for (int u = u0; u < u0 + uc; ++u, tok += 256) {
-          if (u + 1 < units) moe_fetch(nxt, rows, u + 1);
-          moe_unit<MB>(acc, cur, tok, 8 * pitch, nt);
-          cur = nxt;
-        }
+        moe_run<MB>(acc, cur, rows, u0, u0 + uc, units, stage_u + g * pitch + 16 * q, 8 * pitch, nt);
       }
       if (tid < 32) pl.hmax[tid] = 0;
       __syncthreads();
@@ -657,7 +684,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_experts_kernel(const MoeEx
       const int n = min(cnt - c0, 8 * kMoeTiles), nt = (n + 7) / 8;
       const int cu = chunk_units(8 * nt);
       float acc[MB][kMoeTiles][4] = {};
-      MoeUnit<MB> cur, nxt;
+      MoeUnit<MB> cur;
       moe_fetch(cur, rows, ub);
       if (!ready) {
         if (!moe_wait(p.counters + kMoeGateUpDone, total1, pl, p.err)) return;
@@ -691,15 +718,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_experts_kernel(const MoeEx
           }
         }
         __syncthreads();
-        uint32_t tok = stage_u + g * pitch + 16 * q;
-        if (active) {
-#pragma unroll 1
-          for (int u = u0; u < u0 + uc; ++u, tok += 256) {
-            if (u + 1 < ue) moe_fetch(nxt, rows, u + 1);
-            moe_unit<MB>(acc, cur, tok, 8 * pitch, nt);
-            cur = nxt;
-          }
-        }
+        if (active)
+          moe_run<MB>(acc, cur, rows, u0, u0 + uc, ue, stage_u + g * pitch + 16 * q, 8 * pitch, nt);
       }
       if (active) {
 #pragma unroll

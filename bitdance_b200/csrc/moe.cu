@@ -14,11 +14,11 @@ namespace {
 
 int last_status() { return cudaPeekAtLastError() == cudaSuccess ? BD_OK : BD_ERR_CUDA; }
 
-// Workspace: counters | row maxima of h | scales of x | fp16 image of x | h | partial sums, each
-// 256-byte aligned. Few pairs may split the down product: at least kPartRows rows of partials.
+// Workspace: counters | images of x | images of h | partial sums, each 256-byte aligned. Few pairs
+// may split the down product: at least kPartRows rows of partials.
 constexpr int kPartRows = 256;
 struct MoeWs {
-  size_t hmax, x_scale, xs, h, part, total;
+  size_t xs, h, part, total;
   int part_rows;
 };
 MoeWs moe_ws(int T, int H, int I, int k) {
@@ -26,25 +26,24 @@ MoeWs moe_ws(int T, int H, int I, int k) {
   const size_t pairs = static_cast<size_t>(T) * k;
   MoeWs w;
   w.part_rows = std::max(T * k, kPartRows);
-  w.hmax = 256;
-  w.x_scale = w.hmax + up(pairs * 4);
-  w.xs = w.x_scale + up(static_cast<size_t>(T) * 4);
-  w.h = w.xs + up(static_cast<size_t>(T) * H * 2);
-  w.part = w.h + up(pairs * I * 4);
+  w.xs = 256;
+  w.h = w.xs + up(T * moe_image_row(H));
+  w.part = w.h + up(pairs * moe_image_row(I));
   w.total = w.part + static_cast<size_t>(w.part_rows) * H * 4;
   return w;
 }
 
 bool bad_shape(int T, int H, int I, int E, int k) {
   return T < 0 || T > kMoeMaxTokens || H <= 0 || I <= 0 || H % 128 || I % 128 || H > (1 << 20) ||
-         I > (1 << 20) || E <= 0 || E > kMoeMaxExperts || k <= 0 || k > kMoeMaxTopK || k > E;
+         I > (1 << 20) || E <= 0 || E > kMoeMaxExperts || k <= 0 || k > kMoeMaxTopK || k > E ||
+         static_cast<int64_t>(E) * std::max(H, 2 * I) > 0x7FFFFFFF;
 }
 
-cudaLaunchConfig_t config(int grid, int smem, cudaStream_t s, cudaLaunchAttribute* attr,
+cudaLaunchConfig_t config(int grid, int threads, int smem, cudaStream_t s, cudaLaunchAttribute* attr,
                           int cluster) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kMoeThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -62,7 +61,7 @@ cudaLaunchConfig_t config(int grid, int smem, cudaStream_t s, cudaLaunchAttribut
 template <class X, class W, int TB>
 int launch_route(const MoeRouteParams& p, cudaStream_t s) {
   cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t cfg = config((p.T + TB - 1) / TB * kRouteCluster,
+  const cudaLaunchConfig_t cfg = config((p.T + TB - 1) / TB * kRouteCluster, kMoeThreads,
                                         2 * p.E * static_cast<int>(sizeof(double)), s, attr,
                                         kRouteCluster);
   return cudaLaunchKernelEx(&cfg, moe_route_kernel<X, W, TB>, p) == cudaSuccess ? last_status()
@@ -76,24 +75,6 @@ int launch_route_t(const MoeRouteParams& p, cudaStream_t s) {
   if (p.T <= 16) return launch_route<X, W, 1>(p, s);
   if (p.T <= 32) return launch_route<X, W, 2>(p, s);
   return launch_route<X, W, 4>(p, s);
-}
-
-template <int MB>
-int launch_experts(const MoeExpertsParams& p, const DeviceInfo* d, cudaStream_t s) {
-  static std::atomic<uint64_t> configured{0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return BD_ERR_CUDA;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(configured.load() & bit)) {
-    if (cudaFuncSetAttribute(moe_experts_kernel<MB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kMoeBBytes) != cudaSuccess)
-      return BD_ERR_CUDA;
-    configured.fetch_or(bit);
-  }
-  cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t cfg = config(2 * d->sm_count, kMoeBBytes, s, attr, 1);
-  return cudaLaunchKernelEx(&cfg, moe_experts_kernel<MB>, p) == cudaSuccess ? last_status()
-                                                                            : BD_ERR_CUDA;
 }
 
 struct MoeExpertArgs {
@@ -116,10 +97,15 @@ int check_experts(const void* y, const void* x, int x_dtype, int out_dtype, cons
     return BD_ERR_INVALID_ARG;
   if (!ws || ws_bytes < moe_ws(T, H, I, k).total) return BD_ERR_WORKSPACE;
   if (!aligned(ws, 256) || !aligned(x, 16) || !aligned(a.w13, 16) || !aligned(a.w2, 16) ||
-      !aligned(a.s13, 2) || !aligned(a.s2, 2) || !aligned(a.ts13, 4) || !aligned(a.ts2, 4) ||
+      !aligned(a.s13, 8) || !aligned(a.s2, 8) || !aligned(a.ts13, 4) || !aligned(a.ts2, 4) ||
       !aligned(ids, 4) || !aligned(weights, 4) || !aligned(y, out_dtype == BD_OUT_F32 ? 4 : 2))
     return BD_ERR_ALIGNMENT;
   return BD_OK;
+}
+
+bool codes_map(CUtensorMap* m, const uint8_t* codes, int64_t rows, int K) {
+  return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<uint8_t*>(codes), K / 2, rows,
+                     K / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
@@ -127,21 +113,15 @@ int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
                 const DeviceInfo* d, cudaStream_t s) {
   const MoeWs w = moe_ws(T, H, I, k);
   MoeExpertsParams p;
-  p.w13 = a.w13;
   p.s13 = a.s13;
-  p.ts13 = a.ts13;
-  p.w2 = a.w2;
   p.s2 = a.s2;
+  p.ts13 = a.ts13;
   p.ts2 = a.ts2;
   p.ids = ids;
   p.weights = weights;
-  p.xs = reinterpret_cast<const __half*>(ws + w.xs);
-  p.x_scale = reinterpret_cast<const float*>(ws + w.x_scale);
-  p.h = reinterpret_cast<float*>(ws + w.h);
-  p.hmax = reinterpret_cast<uint32_t*>(ws + w.hmax);
+  p.xs = ws + w.xs;
+  p.h = ws + w.h;
   p.part = reinterpret_cast<float*>(ws + w.part);
-  p.part_rows = w.part_rows;
-  p.vec_out = aligned(y, 16) ? 1 : 0;
   p.y = y;
   p.counters = reinterpret_cast<uint32_t*>(ws);
   p.T = T;
@@ -149,13 +129,28 @@ int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
   p.I = I;
   p.E = E;
   p.k = k;
+  p.part_rows = w.part_rows;
   p.out_dtype = out_dtype;
+  p.vec_out = aligned(y, 16) ? 1 : 0;
   p.err = d->err;
-  // weight rows per task: 256 where the experts that can be touched give the machine two tasks per
-  // SM in the gate / up phase, else 128
-  const int64_t touched = std::min(E, T * k);
-  return touched * (I / 128) >= 2 * d->sm_count ? launch_experts<2>(p, d, s)
-                                                : launch_experts<1>(p, d, s);
+  CUtensorMap m13, m2;
+  if (!codes_map(&m13, a.w13, static_cast<int64_t>(E) * 2 * I, H) ||
+      !codes_map(&m2, a.w2, static_cast<int64_t>(E) * H, I))
+    return BD_ERR_CUDA;
+  static std::atomic<uint64_t> configured{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return BD_ERR_CUDA;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    if (cudaFuncSetAttribute(moe_experts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kMoeSmem) != cudaSuccess)
+      return BD_ERR_CUDA;
+    configured.fetch_or(bit);
+  }
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = config(d->sm_count, kMoeExpertThreads, kMoeSmem, s, attr, 1);
+  return cudaLaunchKernelEx(&cfg, moe_experts_kernel, m13, m2, p) == cudaSuccess ? last_status()
+                                                                                 : BD_ERR_CUDA;
 }
 
 }  // namespace
@@ -186,20 +181,16 @@ int bd_moe_experts(void* y, const void* x, int x_dtype, const int* ids, const fl
   if (st != BD_OK) return st;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const MoeWs w = moe_ws(T, H, I, top_k);
-  __half* xs = reinterpret_cast<__half*>(ws + w.xs);
-  float* x_scale = reinterpret_cast<float*>(ws + w.x_scale);
   uint32_t* counters = reinterpret_cast<uint32_t*>(ws);
-  uint32_t* hmax = reinterpret_cast<uint32_t*>(ws + w.hmax);
   cudaStream_t s = as_stream(stream);
   cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t cfg = config(T, 0, s, attr, 1);
+  const cudaLaunchConfig_t cfg = config(T, kMoeThreads, 0, s, attr, 1);
   const cudaError_t e =
       x_dtype == BD_IN_BF16
           ? cudaLaunchKernelEx(&cfg, moe_prepare_kernel<__nv_bfloat16>,
-                               static_cast<const __nv_bfloat16*>(x), xs, x_scale, counters, hmax, H,
-                               top_k)
-          : cudaLaunchKernelEx(&cfg, moe_prepare_kernel<__half>, static_cast<const __half*>(x), xs,
-                               x_scale, counters, hmax, H, top_k);
+                               static_cast<const __nv_bfloat16*>(x), ws + w.xs, counters, H)
+          : cudaLaunchKernelEx(&cfg, moe_prepare_kernel<__half>, static_cast<const __half*>(x),
+                               ws + w.xs, counters, H);
   if (e != cudaSuccess) return BD_ERR_CUDA;
   return run_experts(y, out_dtype, ids, weights, a, T, H, I, E, top_k, ws, d, s);
 }
@@ -232,10 +223,8 @@ int bd_moe_layer(void* y, int* ids, float* weights, const void* x, int x_dtype,
   p.bias = selection_bias;
   p.ids = ids;
   p.weights = weights;
-  p.xs = reinterpret_cast<__half*>(ws + w.xs);
-  p.x_scale = reinterpret_cast<float*>(ws + w.x_scale);
+  p.xs = ws + w.xs;
   p.counters = reinterpret_cast<uint32_t*>(ws);
-  p.hmax = reinterpret_cast<uint32_t*>(ws + w.hmax);
   p.T = T;
   p.H = H;
   p.E = E;

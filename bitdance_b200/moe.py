@@ -85,7 +85,7 @@ def _workspace_bytes(T: int, H: int, inter: int, top_k: int) -> int:
     if T == 0:
         return 0
     pairs = T * top_k
-    return 256 + up(4 * pairs) + up(4 * T) + up(2 * T * H) + up(4 * pairs * inter) + \
+    return 256 + up(T * (H // 128) * 272) + up(pairs * (inter // 128) * 272) + \
         4 * H * max(pairs, 256)
 
 

@@ -14,11 +14,12 @@ namespace {
 
 int last_status() { return cudaPeekAtLastError() == cudaSuccess ? BD_OK : BD_ERR_CUDA; }
 
-// Workspace: counters | images of x | images of h | partial sums, each 256-byte aligned. Few pairs
-// may split the down product: at least kPartRows rows of partials.
+// Workspace: counters | row maxima of h | row factors of x | digits of x | h | digits of h | partial
+// sums, each 256-byte aligned. Few pairs may split the down product: at least kPartRows rows of
+// partials.
 constexpr int kPartRows = 256;
 struct MoeWs {
-  size_t xs, h, part, total;
+  size_t hmax, x_scale, xs, h, hs, part, total;
   int part_rows;
 };
 MoeWs moe_ws(int T, int H, int I, int k) {
@@ -26,9 +27,12 @@ MoeWs moe_ws(int T, int H, int I, int k) {
   const size_t pairs = static_cast<size_t>(T) * k;
   MoeWs w;
   w.part_rows = std::max(T * k, kPartRows);
-  w.xs = 256;
+  w.hmax = 256;
+  w.x_scale = w.hmax + up(pairs * 4);
+  w.xs = w.x_scale + up(static_cast<size_t>(T) * 4);
   w.h = w.xs + up(T * moe_image_row(H));
-  w.part = w.h + up(pairs * moe_image_row(I));
+  w.hs = w.h + up(pairs * I * 4);
+  w.part = w.hs + up(pairs * moe_image_row(I));
   w.total = w.part + static_cast<size_t>(w.part_rows) * H * 4;
   return w;
 }
@@ -97,7 +101,7 @@ int check_experts(const void* y, const void* x, int x_dtype, int out_dtype, cons
     return BD_ERR_INVALID_ARG;
   if (!ws || ws_bytes < moe_ws(T, H, I, k).total) return BD_ERR_WORKSPACE;
   if (!aligned(ws, 256) || !aligned(x, 16) || !aligned(a.w13, 16) || !aligned(a.w2, 16) ||
-      !aligned(a.s13, 8) || !aligned(a.s2, 8) || !aligned(a.ts13, 4) || !aligned(a.ts2, 4) ||
+      !aligned(a.s13, 4) || !aligned(a.s2, 4) || !aligned(a.ts13, 4) || !aligned(a.ts2, 4) ||
       !aligned(ids, 4) || !aligned(weights, 4) || !aligned(y, out_dtype == BD_OUT_F32 ? 4 : 2))
     return BD_ERR_ALIGNMENT;
   return BD_OK;
@@ -106,6 +110,27 @@ int check_experts(const void* y, const void* x, int x_dtype, int out_dtype, cons
 bool codes_map(CUtensorMap* m, const uint8_t* codes, int64_t rows, int K) {
   return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<uint8_t*>(codes), K / 2, rows,
                      K / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int TOK>
+int launch_experts(const CUtensorMap& m13, const CUtensorMap& m2, const MoeExpertsParams& p,
+                   const DeviceInfo* d, cudaStream_t s) {
+  static std::atomic<uint64_t> configured{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return BD_ERR_CUDA;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    if (cudaFuncSetAttribute(moe_experts_kernel<TOK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             MoeCfg<TOK>::kSmem) != cudaSuccess)
+      return BD_ERR_CUDA;
+    configured.fetch_or(bit);
+  }
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg =
+      config(d->sm_count, kMoeExpertThreads, MoeCfg<TOK>::kSmem, s, attr, 1);
+  return cudaLaunchKernelEx(&cfg, moe_experts_kernel<TOK>, m13, m2, p) == cudaSuccess
+             ? last_status()
+             : BD_ERR_CUDA;
 }
 
 int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
@@ -120,7 +145,10 @@ int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
   p.ids = ids;
   p.weights = weights;
   p.xs = ws + w.xs;
-  p.h = ws + w.h;
+  p.x_scale = reinterpret_cast<const float*>(ws + w.x_scale);
+  p.h = reinterpret_cast<float*>(ws + w.h);
+  p.hmax = reinterpret_cast<uint32_t*>(ws + w.hmax);
+  p.hs = ws + w.hs;
   p.part = reinterpret_cast<float*>(ws + w.part);
   p.y = y;
   p.counters = reinterpret_cast<uint32_t*>(ws);
@@ -137,20 +165,10 @@ int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
   if (!codes_map(&m13, a.w13, static_cast<int64_t>(E) * 2 * I, H) ||
       !codes_map(&m2, a.w2, static_cast<int64_t>(E) * H, I))
     return BD_ERR_CUDA;
-  static std::atomic<uint64_t> configured{0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return BD_ERR_CUDA;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(configured.load() & bit)) {
-    if (cudaFuncSetAttribute(moe_experts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kMoeSmem) != cudaSuccess)
-      return BD_ERR_CUDA;
-    configured.fetch_or(bit);
-  }
-  cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t cfg = config(d->sm_count, kMoeExpertThreads, kMoeSmem, s, attr, 1);
-  return cudaLaunchKernelEx(&cfg, moe_experts_kernel, m13, m2, p) == cudaSuccess ? last_status()
-                                                                                 : BD_ERR_CUDA;
+  // passes of 8 tokens (deeper weight ring) where an expert is expected to have few, of 24 else;
+  // an expert with more takes several passes either way
+  return T <= 8 || T * k <= 4 * E ? launch_experts<8>(m13, m2, p, d, s)
+                                  : launch_experts<24>(m13, m2, p, d, s);
 }
 
 }  // namespace
@@ -182,15 +200,18 @@ int bd_moe_experts(void* y, const void* x, int x_dtype, const int* ids, const fl
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const MoeWs w = moe_ws(T, H, I, top_k);
   uint32_t* counters = reinterpret_cast<uint32_t*>(ws);
+  uint32_t* hmax = reinterpret_cast<uint32_t*>(ws + w.hmax);
+  float* x_scale = reinterpret_cast<float*>(ws + w.x_scale);
   cudaStream_t s = as_stream(stream);
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = config(T, kMoeThreads, 0, s, attr, 1);
   const cudaError_t e =
       x_dtype == BD_IN_BF16
           ? cudaLaunchKernelEx(&cfg, moe_prepare_kernel<__nv_bfloat16>,
-                               static_cast<const __nv_bfloat16*>(x), ws + w.xs, counters, H)
+                               static_cast<const __nv_bfloat16*>(x), ws + w.xs, x_scale, hmax, counters,
+                               H, top_k)
           : cudaLaunchKernelEx(&cfg, moe_prepare_kernel<__half>, static_cast<const __half*>(x),
-                               ws + w.xs, counters, H);
+                               ws + w.xs, x_scale, hmax, counters, H, top_k);
   if (e != cudaSuccess) return BD_ERR_CUDA;
   return run_experts(y, out_dtype, ids, weights, a, T, H, I, E, top_k, ws, d, s);
 }
@@ -224,6 +245,8 @@ int bd_moe_layer(void* y, int* ids, float* weights, const void* x, int x_dtype,
   p.ids = ids;
   p.weights = weights;
   p.xs = ws + w.xs;
+  p.x_scale = reinterpret_cast<float*>(ws + w.x_scale);
+  p.hmax = reinterpret_cast<uint32_t*>(ws + w.hmax);
   p.counters = reinterpret_cast<uint32_t*>(ws);
   p.T = T;
   p.H = H;

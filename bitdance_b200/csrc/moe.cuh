@@ -4,22 +4,24 @@
 //   logits = x Wr^T;  s = softmax or sigmoid(logits);  top-k by s (+ bias);  w = s (renormalised)
 //   y_t = sum over the chosen experts e of w_e * Wd_e (silu(Wg_e x_t) * (Wu_e x_t))
 //
-// A few tokens read far more weights than they compute with, so the experts' kernel streams the
-// touched experts' 4-bit weights once through a ring in shared memory (TMA), turns them into fp16
-// MMA fragments in registers (exactly: an E2M1 times an E4M3 value has at most 6 significant bits)
-// and multiplies by all tokens of the expert with mma.sync (weights are the 16 rows, tokens the 8
-// columns; the tensor work is far below what the weights' bytes cost, so the legacy MMA, whose
-// fragments come from registers, saves the trip of converted weights through shared memory).
-// Activations are fp16 images with a power-of-two scale per token and 128 elements: exact for x
-// (down to 2^-29 of a token's largest value), one rounding to 11 bits for the hidden values. Sums
-// are fp32.
+// A few tokens read far more weights than they compute with: the time is that of streaming the touched
+// experts' 4-bit weights once. So no thread touches a weight: codes and scales go by TMA and
+// cp.async to shared memory and from there to tcgen05.mma kind::mxf4nvf4 as they are. What that MMA
+// wants besides is a second operand in 4 bits, and it has columns to spare: a token becomes eight
+// columns, six of them digits of its values. With s = 2^e the scale of a 16-block (amax <= 4 s),
+//   x = s (d_0 + d_1 / 8 + ... + d_5 / 8^5) + r,   d_p = E2M1 round of what is left, |r| <= s 2^-16,
+// each digit's scale 2^(e - 3 p) an E4M3 power of two, and the columns' sum is the product with x
+// to 2^-17 of the block's largest value (digits whose scale would fall below E4M3's 2^-9 are dropped:
+// 2^-20 of the row's largest): activations of 16 bits against 4-bit weights (W4A16) on the FP4
+// tensor cores without unpacking a weight. (Unpacking them into fp16 fragments for mma.sync took
+// 140 to 175 instructions per 2048 weights and ran at 40 % of the memory rate.)
 //
 // Kernel 1 (moe_route_kernel, or moe_prepare_kernel where the caller brings the routing): router
-// products, selection, image of x, counters to zero.
-// Kernel 2 (moe_experts_kernel): gate / up, down and combine phases in one grid. Work is handed out
-// by tickets (atomic counters), all tasks of a phase before those of the next: a CTA that waits for a
-// phase to finish knows that each of its tasks is held by a CTA that already runs, so the wait ends
-// without any guarantee that the whole grid is resident at once.
+// products, selection, digits of x, counters to zero.
+// Kernel 2 (moe_experts_kernel): gate / up, digits of the hidden values, down and combine phases in
+// one grid. Work is handed out by tickets (atomic counters), all tasks of a phase before those of
+// the next: a CTA that waits for a phase to finish knows that each of its tasks is held by a CTA
+// that already runs, so the wait ends without any guarantee that the whole grid is resident.
 #pragma once
 #include <cstdint>
 
@@ -38,24 +40,22 @@ constexpr int kRouteCluster = 8;
 // Counters in the workspace, zeroed by the first kernel: tickets and finished tasks per phase.
 enum : int {
   kMoeGateUp = 0,
-  kMoeGateUpDone = 1,
-  kMoeDown = 2,
-  kMoeDownDone = 3,
-  kMoeCombine = 4,
-  kMoeCounters = 5
+  kMoeGateUpDone,
+  kMoeDigits,
+  kMoeDigitsDone,
+  kMoeDown,
+  kMoeDownDone,
+  kMoeCombine,
+  kMoeCounters
 };
 
-// Image of a row of activations: per 128 elements 256 bytes of fp16, one fp32 factor (what the fp16
-// values are multiplied by) and 12 unused bytes. A thread of an MMA lane quad q takes elements
-// 32 q .. 32 q + 31 of a block (one 16-byte piece of the weights' codes) in four loads of 8; (q, load)
-// are exchanged so that a quad's load is 64 contiguous bytes.
-constexpr int kMoeBlock = 272;
-__host__ __device__ __forceinline__ int moe_image_offset(int k) {  // bytes, of element k
-  const int r = k & 127;
-  return (k >> 7) * kMoeBlock + ((r >> 3) & 3) * 64 + (r >> 5) * 16 + (r & 7) * 2;
-}
+// Digits of a row of K activations: per 256 elements the 8 x 128 bytes of codes (row p: digit p; rows
+// 6 and 7 are zero), 128B-swizzled as the MMA's operand tile, then 8 x 4 words of scales.
+constexpr int kMoeDigitRows = 8, kMoeDigitCount = 6;
+constexpr int kMoeChunkCodes = 1024;
+constexpr int kMoeChunk = kMoeChunkCodes + 128;
 __host__ __device__ __forceinline__ int64_t moe_image_row(int K) {
-  return static_cast<int64_t>(K / 128) * kMoeBlock;
+  return static_cast<int64_t>((K + 255) / 256) * kMoeChunk;
 }
 
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -86,26 +86,84 @@ struct MoeRouteParams {
   const float* bias;       // (E,) added for the selection only, may be null
   int* ids;                // (T, k)
   float* weights;          // (T, k)
-  uint8_t* xs;             // images of x
+  uint8_t* xs;             // digits of x
+  float* x_scale;          // (T,) row factors
+  uint32_t* hmax;          // (T, k) zeroed here
   uint32_t* counters;
   int T, H, E, k;
   int sigmoid, renormalize;
   float routed_scale;
 };
 
-// Exponent that takes values whose largest magnitude has these bits to [2^14, 2^15): times
-// 2^(14 - E). A NaN or Inf stays one under E = 14.
-__device__ __forceinline__ int moe_exp(uint32_t amax_bits) {
-  return amax_bits >= 0x7F800000u ? 14 : max(-100, static_cast<int>(amax_bits >> 23) - 127);
-}
 __device__ __forceinline__ float pow2f(int e) {
   return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
+// Row factor: with 2^E <= amax < 2^(E+1) the row times 2^(9 - E) is below 2^10 = 4 * 2^8, so that its
+// largest block's scale is E4M3's 2^8. Returns 9 - E; the factor back is 2^(E - 9), and NaN for a
+// row with a NaN or Inf (its digits are finite: the factor carries the NaN into every product).
+__device__ __forceinline__ int moe_row_shift(uint32_t amax_bits) {
+  return 9 - min(127, max(-100, static_cast<int>(amax_bits >> 23) - 127));
+}
+__device__ __forceinline__ float moe_row_factor(uint32_t amax_bits) {
+  return amax_bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u)
+                                  : pow2f(-moe_row_shift(amax_bits));
+}
 
-// Image of token t of x, one scale for the whole row: a bf16 or fp16 value keeps all its bits down
-// to 2^-29 of the row's largest, and below that errs by at most 2^-40 of it.
+// E2M1 codes of (lo, hi), round to nearest, and their values.
+__device__ __forceinline__ uint32_t e2m1_pair(float lo, float hi, float& vlo, float& vhi) {
+  uint32_t code, val;
+  asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %3, %2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.u32.u8 %0, b;\n\t}"
+      : "=r"(code), "=r"(val)
+      : "f"(lo), "f"(hi));
+  const __half2 h = *reinterpret_cast<const __half2*>(&val);
+  vlo = __low2float(h);
+  vhi = __high2float(h);
+  return code;
+}
+
+// Digits of the 16-block `blk` of a row (values v already times the row's 2^shift) into its image.
+// Lanes 4 i .. 4 i + 3 hold four consecutive blocks (one scale word); all lanes of a group come
+// together.
+__device__ __forceinline__ void moe_digits(float (&v)[16], uint8_t* img, int blk) {
+  float a = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) a = fmaxf(a, fabsf(v[j]));
+  const int e = max(-9, min(8, static_cast<int>(__float_as_uint(a) >> 23) - 128));  // amax <= 4 2^e
+  const float down = pow2f(-e);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] *= down;
+  uint8_t* chunk = img + static_cast<int64_t>(blk >> 4) * kMoeChunk;
+  const int piece = (blk & 15) >> 1;  // 16-byte piece of the 128-byte row; this block is half of it
+  const uint32_t group = 0xFu << (threadIdx.x & 28);
+#pragma unroll
+  for (int p = 0; p < kMoeDigitRows; ++p) {
+    const int ep = e - 3 * p;
+    uint32_t w[2] = {0, 0}, byte = 0;
+    if (p < kMoeDigitCount && ep >= -9) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float d0, d1;
+        w[j >> 2] |= e2m1_pair(v[2 * j], v[2 * j + 1], d0, d1) << (8 * (j & 3));
+        v[2 * j] = (v[2 * j] - d0) * 8.0f;
+        v[2 * j + 1] = (v[2 * j + 1] - d1) * 8.0f;
+      }
+      byte = ep >= -6 ? static_cast<uint32_t>(ep + 7) << 3 : 1u << (ep + 9);
+    }
+    *reinterpret_cast<uint2*>(chunk + p * 128 + ((piece ^ p) << 4) + (blk & 1) * 8) =
+        make_uint2(w[0], w[1]);
+    uint32_t word = byte << (8 * (blk & 3));
+    word |= __shfl_xor_sync(group, word, 1);
+    word |= __shfl_xor_sync(group, word, 2);
+    if ((blk & 3) == 0)
+      *reinterpret_cast<uint32_t*>(chunk + kMoeChunkCodes + p * 16 + (blk & 15)) = word;
+  }
+}
+
+// Digits of token t of x, by one CTA.
 template <class X>
-__device__ void moe_convert_token(const X* x, uint8_t* xs, int t, int H, uint32_t* part) {
+__device__ void moe_convert_token(const X* x, uint8_t* xs, float* x_scale, int t, int H,
+                                  uint32_t* part) {
   const X* row = x + static_cast<int64_t>(t) * H;
   uint8_t* img = xs + t * moe_image_row(H);
   uint32_t am = 0;
@@ -121,32 +179,29 @@ __device__ void moe_convert_token(const X* x, uint8_t* xs, int t, int H, uint32_
   am = 0;
 #pragma unroll
   for (int i = 0; i < kMoeWarps; ++i) am = max(am, part[i]);
-  const int E = moe_exp(am);
-  const float up = pow2f(14 - E);
-  for (int c = threadIdx.x; c < H / 8; c += kMoeThreads) {
-    float v[8];
-    load8(row + 8 * c, v);
-    uint32_t w[4];
+  const float up = pow2f(moe_row_shift(am));
+  for (int b = threadIdx.x; b < H / 16; b += kMoeThreads) {  // H / 16 is a multiple of 8
+    float v[16];
+    load8(row + 16 * b, *reinterpret_cast<float(*)[8]>(v));
+    load8(row + 16 * b + 8, *reinterpret_cast<float(*)[8]>(v + 8));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const __half2 h = __floats2half2_rn(v[2 * j] * up, v[2 * j + 1] * up);
-      w[j] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    *reinterpret_cast<uint4*>(img + moe_image_offset(8 * c)) = make_uint4(w[0], w[1], w[2], w[3]);
-    if ((c & 15) == 0)
-      *reinterpret_cast<float*>(img + (c >> 4) * kMoeBlock + 256) = pow2f(E - 14);
+    for (int j = 0; j < 16; ++j) v[j] *= up;
+    moe_digits(v, img, b);
   }
+  if (threadIdx.x == 0) x_scale[t] = moe_row_factor(am);
 }
 
 // One CTA per token, where the caller brings ids and weights.
 template <class X>
-__global__ void __launch_bounds__(kMoeThreads) moe_prepare_kernel(const X* x, uint8_t* xs,
-                                                                 uint32_t* counters, int H) {
+__global__ void __launch_bounds__(kMoeThreads)
+    moe_prepare_kernel(const X* x, uint8_t* xs, float* x_scale, uint32_t* hmax, uint32_t* counters,
+                       int H, int k) {
   __shared__ uint32_t part[kMoeWarps];
   grid_dep_launch_dependents();
   grid_dep_wait();
   if (blockIdx.x == 0 && threadIdx.x < kMoeCounters) counters[threadIdx.x] = 0;
-  moe_convert_token(x, xs, blockIdx.x, H, part);
+  if (threadIdx.x < k) hmax[blockIdx.x * k + threadIdx.x] = 0;
+  moe_convert_token(x, xs, x_scale, blockIdx.x, H, part);
 }
 
 // max (kMax) or sum over the CTA's threads, the same value in all of them, in a fixed order
@@ -215,9 +270,9 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
       }
     }
   }
-  // the image of token i by CTA 7 - i, while the others may still multiply
+  // the digits of token i by CTA 7 - i, while the others may still multiply
   const int mine = kRouteCluster - 1 - static_cast<int>(rank);
-  if (mine < TB && t0 + mine < p.T) moe_convert_token(x, p.xs, t0 + mine, p.H, upart);
+  if (mine < TB && t0 + mine < p.T) moe_convert_token(x, p.xs, p.x_scale, t0 + mine, p.H, upart);
   cluster_sync_all();
   const int t = t0 + static_cast<int>(rank);
   if (static_cast<int>(rank) >= TB || t >= p.T) return;
@@ -262,6 +317,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
       sum = 0.0;
       for (int r = 0; r < p.k; ++r) sum += sel[r];
     }
+    p.hmax[t * p.k + threadIdx.x] = 0;
     p.weights[t * p.k + threadIdx.x] =
         static_cast<float>(sel[threadIdx.x] / sum * static_cast<double>(p.routed_scale));
   }
@@ -276,8 +332,11 @@ struct MoeExpertsParams {
   const float* ts2;
   const int* ids;
   const float* weights;
-  const uint8_t* xs;         // images of x, one per token
-  uint8_t* h;                // images of the hidden values (times weight and down scale), per pair
+  const uint8_t* xs;         // digits of x, per token, and their row factors
+  const float* x_scale;
+  float* h;                  // (T k, I) hidden values (times weight and down scale)
+  uint32_t* hmax;            // (T k,) bits of the largest |h| of a pair
+  uint8_t* hs;               // digits of h, per pair
   float* part;               // (slices, T k, H) partial sums; part_rows rows in all
   void* y;                   // (T, H)
   uint32_t* counters;
@@ -287,36 +346,6 @@ struct MoeExpertsParams {
   uint32_t* err;
 };
 
-// 8 codes (four bytes) -> four f16x2.
-__device__ __forceinline__ void cvt_e2m1x8_f16(uint32_t w, uint32_t (&o)[4]) {
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
-      : "r"(w));
-}
-__device__ __forceinline__ uint32_t cvt_e4m3x2_f16x2(uint32_t pair) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<unsigned short>(pair)));
-  return r;
-}
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t byte_perm(uint32_t a, uint32_t b, uint32_t s) {
-  return __byte_perm(a, b, s);
-}
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                        uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // Data written earlier in this grid: not through the read-only path.
 __device__ __forceinline__ uint4 ld_cg(const void* p) {
   uint4 v;
@@ -331,12 +360,6 @@ __device__ __forceinline__ uint32_t ld_acquire_gpu(const uint32_t* p) {
   return v;
 }
 
-// 8 codes -> four f16x2 of code * scale (adjacent elements), scale in both halves.
-__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t scale, uint32_t (&o)[4]) {
-  cvt_e2m1x8_f16(w, o);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = mul_f16x2(o[i], scale);
-}
 struct MoePlan {
   int cnt[kMoeMaxExperts];           // pairs of an expert
   uint16_t off[kMoeMaxExperts];      // first pair of an expert in `pairs`
@@ -411,62 +434,62 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
   __syncthreads();
 }
 
-// ---- the experts' kernel. Tasks of 256 weight rows of one expert, all tokens of the expert (in
-// passes of 32 where more take it), K in stages of 256:
-//   gate / up: 128 hidden units (128 gate rows, 128 up rows; MMA rows g: gate, g + 8: up of one
-//              unit, so one thread holds both values of the same token);
-//              h = silu(gate) up w ts, scaled per token by the 128 units' largest, as fp16 image;
+// ---- the experts' kernel. Tasks of 256 weight rows (two MMA tiles of 128) of one expert against
+// all tokens of the expert, in passes of TOK tokens; K in stages of 256:
+//   gate / up: 128 hidden units, tile 0 the gate rows, tile 1 the up rows: lane i of both tiles is
+//              hidden unit i. h = silu(gate) up w ts in fp32, and the pair's maximum;
+//   digits:    h -> digits, once every h is there (their row factor needs the row's maximum);
 //   down:      256 output rows of one expert and a slice of I; partial sums per (slice, pair);
 //   combine:   y = the partial sums of a token's pairs in slot order.
-// Warps: 16 consumers of 16 MMA rows each; a weight producer, which takes the tickets, publishes the
-// tasks in a small queue and keeps the weight ring full across tasks and phases (TMA boxes of
-// 128 rows x 128 bytes for the codes, cp.async for the scales, whose row pitch need not suit TMA);
-// an activation producer, which copies the tokens' images (bulk copies, a lane per token) into a
-// ring of two slots, waiting for the gate / up phase to end before the first hidden values.
-// Bound by the weights' bytes where the tokens per expert are few: per 2048 weights a warp issues
-// about 140 instructions, 35 cycles of an SM against 49 for the bytes.
-constexpr int kMoeConsumers = 16;
-constexpr int kMoeExpertThreads = 32 * (kMoeConsumers + 2);
-constexpr int kMoeTiles = 4;                              // token tiles (8 columns) per pass
-constexpr int kMoeStages = 4;
-constexpr int kMoeCodes = 256 * 128;                      // codes of a stage: 256 rows, 256 of K
-constexpr int kMoeStage = kMoeCodes + 256 * 16;           // and the rows' 16 scales
-constexpr int kMoeActSlot = 32 * 1024;                    // activations of one chunk of K
+// Warps: 0 weight codes (takes the tickets and publishes the tasks in a queue), 1 and 2 weight scales
+// of the two tiles (4-byte cp.async straight into the tiles tcgen05.cp wants: no repacking of the
+// natural layout), 3 activation digits (waits for the digits phase before the first down task, while
+// the weights of the next stages already arrive), 4 MMA, 5..12 epilogue (and the digits and combine
+// phases). Two builds: TOK = 8 (four stages, accumulators double-buffered) where an expert has few
+// tokens, TOK = 24.
+constexpr int kMoeEpiWarp0 = 5, kMoeEpiWarps = 8;
+constexpr int kMoeExpertThreads = 32 * (kMoeEpiWarp0 + kMoeEpiWarps);
 constexpr int kMoeQueue = 4;
-constexpr int oMoeAct = kMoeStages * kMoeStage;
-constexpr int kMoeSmem = oMoeAct + 2 * kMoeActSlot + 1024;
+
+template <int TOK>
+struct MoeCfg {
+  static constexpr int kN = TOK * kMoeDigitRows;             // MMA columns of a full pass
+  static constexpr int kBlocks = (kN + 127) / 128;           // 128-row blocks of the digit scales
+  static constexpr int kCodes = 2 * 128 * 128;
+  static constexpr int oSw = kCodes;                         // weight scales [tile][word][512]
+  static constexpr int oB = oSw + 2 * 4 * 512;               // digits
+  static constexpr int oSb = oB + TOK * kMoeChunkCodes;      // digit scales [block][word][512]
+  static constexpr int kStage = oSb + kBlocks * 4 * 512;
+  static constexpr int kStages = TOK <= 8 ? 4 : 3;
+  static constexpr int kSmem = kStages * kStage + 1024;
+  static constexpr int kAccs = TOK <= 8 ? 2 : 1;             // accumulator pairs
+  static constexpr int kSfCol0 = kAccs * 2 * kN;
+  static constexpr int kSfSet = 2 * 16 + kBlocks * 16;       // scale words of a stage in tensor memory
+  static_assert(kSfCol0 + 2 * kSfSet <= 512, "tensor memory budget");
+  static_assert(kStage % 1024 == 0 && oB % 1024 == 0, "1 KB swizzle atoms");
+  // a full stage: the code and digit copies' tx arrives, 64 + 32 lanes' scale copies
+  static constexpr int kFullCount = 2 + 96;
+};
 
 struct MoeCtl {
-  uint64_t wfull[kMoeStages], wempty[kMoeStages], afull[2], aempty[2], qfull[kMoeQueue],
-      qempty[kMoeQueue], cbar;
+  uint64_t full[4], empty[4], acc_full[2], acc_empty[2], qfull[kMoeQueue], qempty[kMoeQueue], drain;
   uint32_t queue[kMoeQueue];
-  uint32_t abort_flag, ticket;
-  uint32_t hmax[2][32];
+  uint32_t abort_flag, tmem_base;
 };
+constexpr int kMoeQueueReaders = kMoeEpiWarp0 - 1 + kMoeEpiWarps;
 
 // A queue entry: phase in the top two bits (0 gate / up, 1 down, 2 end), task below.
 struct MoeTask {
   uint32_t phase, index;
 };
 
-// The chunks of K (in units of 128) in which nt tiles of activations are staged: as many units as a
-// slot holds, an even number (a weight stage is two units).
-__device__ __forceinline__ int moe_chunk_units(int nt) {
-  return ((kMoeActSlot / (8 * nt) - 112) / kMoeBlock) & ~1;
-}
-// Bytes from token row to token row of a staged chunk of uc units: 64 mod 128, so that the 16-byte
-// reads of two token rows by a lane quad each fall on different banks.
-__device__ __forceinline__ uint32_t moe_pitch(int uc) {
-  const uint32_t n = static_cast<uint32_t>(uc) * kMoeBlock;
-  return n + ((64u - n) & 127u);
-}
-
 // Geometry of a task.
 struct MoeGeom {
   int e, cnt, off;      // expert, its pairs
-  int u0, u1;           // units of K
-  int row0;             // first hidden unit / output row
-  int z;                // slice
+  int c0, c1;           // stages of K
+  int K, row0, z;       // first hidden unit / output row, slice
+  int64_t ra, rb;       // first weight rows of the two tiles
+  bool two;             // the second tile exists
 };
 struct MoeShape {
   int blocks1, blocks2, slices;
@@ -475,20 +498,27 @@ struct MoeShape {
                                           const MoeTask& t) const {
     MoeGeom g;
     if (t.phase == 0) {
-      const int a = t.index / blocks1;
-      g.e = pl.act[a];
+      g.e = pl.act[t.index / blocks1];
       g.row0 = (t.index % blocks1) * 128;
-      g.u0 = 0;
-      g.u1 = p.H / 128;
       g.z = 0;
+      g.c0 = 0;
+      g.c1 = (p.H + 255) / 256;
+      g.K = p.H;
+      g.ra = static_cast<int64_t>(g.e) * 2 * p.I + g.row0;
+      g.rb = g.ra + p.I;
+      g.two = true;
     } else {
       const int ab = t.index / slices;
       g.z = t.index % slices;
       g.e = pl.act[ab / blocks2];
       g.row0 = (ab % blocks2) * 256;
-      const int pairs = (p.I / 128 + 1) / 2;  // slices begin on whole stages
-      g.u0 = 2 * (pairs * g.z / slices);
-      g.u1 = min(p.I / 128, 2 * (pairs * (g.z + 1) / slices));
+      const int n = (p.I + 255) / 256;
+      g.c0 = n * g.z / slices;
+      g.c1 = n * (g.z + 1) / slices;
+      g.K = p.I;
+      g.ra = static_cast<int64_t>(g.e) * p.H + g.row0;
+      g.rb = g.ra + 128;
+      g.two = g.row0 + 128 < p.H;
     }
     g.cnt = pl.cnt[g.e];
     g.off = pl.off[g.e];
@@ -496,172 +526,109 @@ struct MoeShape {
   }
 };
 
-// One unit against NT staged token tiles. A quad reads pieces 4 (u & 1) + q of its rows' 128 bytes,
-// 128B-swizzled; lane group g holds row rho(g) of its 8, rho alternating between rows 0..3 and 4..7
-// so that the two rows of a read phase use different banks.
-template <int NT>
-__device__ __forceinline__ void moe_unit(float (&acc)[kMoeTiles][4], uint32_t codes_a,
-                                         uint32_t codes_b, uint32_t scale_a, uint32_t scale_b,
-                                         uint32_t tok, uint32_t tile, uint32_t fac) {
-  uint32_t a[4], b[4], sa, sb;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(codes_a));
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "r"(codes_b));
-  asm volatile("ld.shared.u16 %0, [%1];" : "=r"(sa) : "r"(scale_a));
-  asm volatile("ld.shared.u16 %0, [%1];" : "=r"(sb) : "r"(scale_b));
-  float f[NT][2], d[NT][4];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[t][0]) : "r"(fac + t * tile));
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[t][1]) : "r"(fac + t * tile + tile / 8));
-#pragma unroll
-    for (int c = 0; c < 4; ++c) d[t][c] = 0.0f;
-  }
-  const uint32_t ha = cvt_e4m3x2_f16x2(sa), hb = cvt_e4m3x2_f16x2(sb);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint4 xb[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(xb[t].x), "=r"(xb[t].y), "=r"(xb[t].z), "=r"(xb[t].w)
-                   : "r"(tok + t * tile + 64 * j));
-    const uint32_t sel = j < 2 ? 0x1010 : 0x3232;
-    uint32_t fa[4], fb[4];
-    codes_f16(a[j], byte_perm(ha, ha, sel), fa);
-    codes_f16(b[j], byte_perm(hb, hb, sel), fb);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      mma_f16(d[t], fa[0], fb[0], fa[1], fb[1], xb[t].x, xb[t].y);
-      mma_f16(d[t], fa[2], fb[2], fa[3], fb[3], xb[t].z, xb[t].w);
-    }
-  }
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int c = 0; c < 4; ++c)  // volatile: issued before the caller releases the slot
-      asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc[t][c]) : "f"(d[t][c]), "f"(f[t][c & 1]));
-}
-
 // A whole warp's bounded wait: the same answer in every lane.
 __device__ __forceinline__ bool moe_warp_wait(uint64_t& bar, uint32_t parity, uint32_t code,
                                               MoeCtl& ctl, uint32_t* err) {
   return __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&bar), parity, err, code, &ctl.abort_flag));
 }
 
-// Ring positions of a role.
-struct MoeRings {
-  RingPos<kMoeStages> w;
-  RingPos<2> a;
-  RingPos<kMoeQueue> q;
-};
-
-// A consumer warp's part of one pass: units [u0, u1) against NT tiles.
-template <int NT>
-__device__ __forceinline__ bool moe_consume(float (&acc)[kMoeTiles][4], const uint8_t* smem,
-                                            MoeCtl& ctl, MoeRings& r, int u0, int u1, int row_a,
-                                            int row_b, bool active, uint32_t* err) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int cu = moe_chunk_units(NT);
-  const uint32_t base = smem_u32(smem);
-  const uint32_t xa = base + row_a * 128, xb = base + row_b * 128;
-  const uint32_t ya = base + kMoeCodes + row_a * 16 + 2 * q, yb = base + kMoeCodes + row_b * 16 + 2 * q;
-  for (int c0 = u0; c0 < u1; c0 += cu) {
-    const int uc = min(cu, u1 - c0);
-    const uint32_t pitch = moe_pitch(uc);
-    if (!moe_warp_wait(ctl.afull[r.a.slot], r.a.phase, kErrWaitOperand, ctl, err)) return false;
-    const uint32_t act = base + oMoeAct + r.a.slot * kMoeActSlot;
-    const uint32_t tok = act + g * pitch + 16 * q, fac = act + 2 * q * pitch + 256;
-    for (int u = 0; u < uc; u += 2) {
-      if (!moe_warp_wait(ctl.wfull[r.w.slot], r.w.phase, kErrWaitTma, ctl, err)) return false;
-      const uint32_t st = r.w.slot * kMoeStage;
-      if (active) {
-#pragma unroll
-        for (int v = 0; v < 2; ++v)
-          if (u + v < uc)
-            moe_unit<NT>(acc, xa + st + (((4 * v + q) ^ (row_a & 7)) << 4),
-                         xb + st + (((4 * v + q) ^ (row_b & 7)) << 4), ya + st + 8 * v,
-                         yb + st + 8 * v, tok + (u + v) * kMoeBlock, 8 * pitch,
-                         fac + (u + v) * kMoeBlock);
-      }
-      // the MMAs that took the stage's words are issued (volatile, in order), so the loads are done
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctl.wempty[r.w.slot]));
-      r.w.next();
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&ctl.aempty[r.a.slot]));
-    r.a.next();
-  }
-  return true;
-}
-
-// Barrier of the consumer warps: an mbarrier, so that the wait is bounded and ends when another role
-// has given up.
-__device__ __forceinline__ bool moe_consumer_sync(MoeCtl& ctl, uint32_t& parity, uint32_t* err) {
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl.cbar));
-  const bool ok = moe_warp_wait(ctl.cbar, parity, kErrWaitAccum, ctl, err);
-  parity ^= 1u;
-  return ok;
-}
-
-// The next queue entry (lane 0 reads it, and the shuffle waits for that read before the release).
-__device__ __forceinline__ bool moe_next_task(MoeTask& t, MoeCtl& ctl, MoeRings& r, uint32_t* err) {
-  if (!moe_warp_wait(ctl.qfull[r.q.slot], r.q.phase, kErrWaitTma, ctl, err)) return false;
-  uint32_t v = *reinterpret_cast<volatile uint32_t*>(&ctl.queue[r.q.slot]);
+// The next queue entry (the shuffle waits for the read before the release).
+__device__ __forceinline__ bool moe_next_task(MoeTask& t, RingPos<kMoeQueue>& q, MoeCtl& ctl,
+                                              uint32_t* err) {
+  if (!moe_warp_wait(ctl.qfull[q.slot], q.phase, kErrWaitTma, ctl, err)) return false;
+  uint32_t v = *reinterpret_cast<volatile uint32_t*>(&ctl.queue[q.slot]);
   v = __shfl_sync(0xFFFFFFFFu, v, 0);
-  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl.qempty[r.q.slot]));
-  r.q.next();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl.qempty[q.slot]));
+  q.next();
   t.phase = v >> 30;
   t.index = v & 0x3FFFFFFFu;
   return true;
 }
 
-// Until *counter >= target, bounded.
+// A whole warp: until *counter >= target, bounded.
 __device__ __forceinline__ bool moe_wait(const uint32_t* counter, uint32_t target, MoeCtl& ctl,
                                          uint32_t* err) {
+  bool ok = true;
   const long long c0 = clock64();
   while (ld_acquire_gpu(counter) < target) {
-    if (*reinterpret_cast<volatile uint32_t*>(&ctl.abort_flag)) return false;
+    if (*reinterpret_cast<volatile uint32_t*>(&ctl.abort_flag)) {
+      ok = false;
+      break;
+    }
     if (static_cast<unsigned long long>(clock64() - c0) > kWaitLimitCycles) {
       atomicOr(err, kErrWaitOperand);
       *reinterpret_cast<volatile uint32_t*>(&ctl.abort_flag) = 1u;
-      return false;
+      ok = false;
+      break;
     }
   }
-  return true;
+  return __all_sync(0xFFFFFFFFu, ok);
 }
 
+__device__ __forceinline__ uint32_t moe_ticket(uint32_t* counter) {
+  uint32_t k = 0;
+  if ((threadIdx.x & 31) == 0) k = atomicAdd(counter, 1u);
+  return __shfl_sync(0xFFFFFFFFu, k, 0);
+}
+// A warp's part of a task is done: its stores before the count.
+__device__ __forceinline__ void moe_count(uint32_t* counter) {
+  __threadfence();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) atomicAdd(counter, 1u);
+}
+
+// Sum of a token's eight digit columns.
+__device__ __forceinline__ float moe_sum8(const uint32_t* r) {
+  float s = __uint_as_float(r[kMoeDigitCount - 1]);
+#pragma unroll
+  for (int p = kMoeDigitCount - 2; p >= 0; --p) s += __uint_as_float(r[p]);
+  return s;
+}
+
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+template <int TOK>
 __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w13,
                        const __grid_constant__ CUtensorMap tm_w2, const MoeExpertsParams p) {
+  using Cfg = MoeCfg<TOK>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ MoePlan pl;
   __shared__ MoeCtl ctl;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile uint32_t* abort_flag = &ctl.abort_flag;
   if (tid == 0) {
     ctl.abort_flag = 0;
-    for (int s = 0; s < kMoeStages; ++s) {
-      mbar_init(smem_u32(&ctl.wfull[s]), 33);  // the tx arrive and 32 lanes' scale copies
-      mbar_init(smem_u32(&ctl.wempty[s]), kMoeConsumers);
+    for (int s = 0; s < Cfg::kStages; ++s) {
+      mbar_init(smem_u32(&ctl.full[s]), Cfg::kFullCount);
+      mbar_init(smem_u32(&ctl.empty[s]), 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(smem_u32(&ctl.afull[s]), 1);
-      mbar_init(smem_u32(&ctl.aempty[s]), kMoeConsumers);
+    for (int s = 0; s < Cfg::kAccs; ++s) {
+      mbar_init(smem_u32(&ctl.acc_full[s]), 1);
+      mbar_init(smem_u32(&ctl.acc_empty[s]), kMoeEpiWarps);
     }
     for (int s = 0; s < kMoeQueue; ++s) {
       mbar_init(smem_u32(&ctl.qfull[s]), 1);
-      mbar_init(smem_u32(&ctl.qempty[s]), kMoeConsumers + 1);
+      mbar_init(smem_u32(&ctl.qempty[s]), kMoeQueueReaders);
     }
-    mbar_init(smem_u32(&ctl.cbar), kMoeConsumers);
+    mbar_init(smem_u32(&ctl.drain), 1);
     fence_mbar_init();
   }
-  if (tid < 64) ctl.hmax[tid >> 5][tid & 31] = 0;
+  if (warp == 4) {
+    tmem_alloc(smem_u32(&ctl.tmem_base), 512);
+    tmem_relinquish();
+  }
   for (int e = tid; e < p.E; e += kMoeExpertThreads) pl.cnt[e] = 0;
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tb = ctl.tmem_base;
   grid_dep_wait();
   moe_plan<kMoeExpertThreads>(p, pl);
   const int nact = pl.nact;
@@ -673,27 +640,30 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
   // slices of I per down task: while the tasks do not fill the grid and the partials fit
   sh.slices = 1;
   while (nact * sh.blocks2 * sh.slices < static_cast<int>(gridDim.x) &&
-         2 * sh.slices * p.T * p.k <= p.part_rows && p.I / 128 >= 4 * sh.slices)
+         2 * sh.slices * p.T * p.k <= p.part_rows && p.I / 256 >= 2 * sh.slices)
     sh.slices *= 2;
   sh.total2 = static_cast<uint32_t>(nact) * sh.blocks2 * sh.slices;
+  // digits: a warp task is 32 blocks of 16 hidden values, over all pairs
+  const int blocks_h = p.I / 16;
+  const uint32_t total_d = static_cast<uint32_t>(p.T * p.k * blocks_h + 31) / 32;
 
-  MoeRings r;
-  volatile uint32_t* abort_flag = &ctl.abort_flag;
-  if (warp == kMoeConsumers) {
-    // ------------------------------------------------------------------ weight producer
+  RingPos<kMoeQueue> q;
+  RingPos<Cfg::kStages> r;
+  MoeTask t;
+  if (warp == 0) {
+    // -------------------------------------------------------------------- weight codes, tickets
     if (lane == 0) {
       prefetch_tmap(&tm_w13);
       prefetch_tmap(&tm_w2);
     }
     uint32_t phase = 0;
-    int issued = 0;
-    while (true) {
+    bool ok = true;
+    while (ok) {
       // the next task: the phase's tickets, then the next phase's
-      MoeTask t{2, 0};
+      t.phase = 2;
+      t.index = 0;
       while (phase < 2) {
-        uint32_t k = 0;
-        if (lane == 0) k = atomicAdd(p.counters + (phase == 0 ? kMoeGateUp : kMoeDown), 1u);
-        k = __shfl_sync(0xFFFFFFFFu, k, 0);
+        const uint32_t k = moe_ticket(p.counters + (phase == 0 ? kMoeGateUp : kMoeDown));
         if (k < (phase == 0 ? sh.total1 : sh.total2)) {
           t.phase = phase;
           t.index = k;
@@ -701,227 +671,284 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
         }
         ++phase;
       }
-      if (!moe_warp_wait(ctl.qempty[r.q.slot], r.q.phase ^ 1u, kErrWaitEmpty, ctl, p.err)) break;
+      if (!(ok = moe_warp_wait(ctl.qempty[q.slot], q.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
       if (lane == 0) {
-        ctl.queue[r.q.slot] = t.phase << 30 | t.index;
-        mbar_arrive(smem_u32(&ctl.qfull[r.q.slot]));
+        ctl.queue[q.slot] = t.phase << 30 | t.index;
+        mbar_arrive(smem_u32(&ctl.qfull[q.slot]));
       }
-      r.q.next();
+      q.next();
       if (t.phase == 2) break;
       const MoeGeom gm = sh.geom(p, pl, t);
-      const bool up = t.phase == 0;
-      const int K = up ? p.H : p.I;
-      const uint8_t* sc = up ? p.s13 : p.s2;
-      // rows 0..127 and 128..255 of the tile
-      const int64_t ra = up ? static_cast<int64_t>(gm.e) * 2 * p.I + gm.row0
-                            : static_cast<int64_t>(gm.e) * p.H + gm.row0;
-      const int64_t rb = up ? ra + p.I : ra + 128;
-      const bool two = up || gm.row0 + 128 < p.H;
-      bool ok = true;
-      for (int c0 = 0; c0 < gm.cnt && ok; c0 += 8 * kMoeTiles) {
-        for (int u = gm.u0; u < gm.u1; u += 2) {
-          if (!moe_warp_wait(ctl.wempty[r.w.slot], r.w.phase ^ 1u, kErrWaitEmpty, ctl, p.err)) {
-            ok = false;
-            break;
-          }
-          uint8_t* st = smem + r.w.slot * kMoeStage;
-          const uint32_t fb = smem_u32(&ctl.wfull[r.w.slot]);
+      const CUtensorMap* tm = t.phase == 0 ? &tm_w13 : &tm_w2;
+      for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK)
+        for (int c = gm.c0; c < gm.c1; ++c) {
+          if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
           if (lane == 0) {
-            const CUtensorMap* tm = up ? &tm_w13 : &tm_w2;
-            mbar_arrive_expect_tx(fb, two ? kMoeCodes : kMoeCodes / 2);
-            tma_load_2d(smem_u32(st), tm, u * 64, static_cast<int32_t>(ra), fb);
-            if (two)
-              tma_load_2d(smem_u32(st + kMoeCodes / 2), tm, u * 64, static_cast<int32_t>(rb), fb);
+            const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
+            const uint32_t fb = smem_u32(&ctl.full[r.slot]);
+            mbar_arrive_expect_tx(fb, gm.two ? Cfg::kCodes : Cfg::kCodes / 2);
+            tma_load_2d(st, tm, c * 128, static_cast<int32_t>(gm.ra), fb);
+            if (gm.two)
+              tma_load_2d(st + Cfg::kCodes / 2, tm, c * 128, static_cast<int32_t>(gm.rb), fb);
           }
-          const bool second = u + 1 < gm.u1;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int row = lane + 32 * i;
-            if (i >= 4 && !two) break;
-            const uint8_t* src = sc + ((i < 4 ? ra : rb) + (row & 127)) * (K / 16) + u * 8;
-            const uint32_t dst = smem_u32(st + kMoeCodes + row * 16);
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-            if (second)
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + 8), "l"(src + 8)
-                           : "memory");
-          }
-          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(fb) : "memory");
-          r.w.next();
-          ++issued;
+          __syncwarp();
+          r.next();
         }
-      }
+    }
+  } else if (warp <= 2) {
+    // ----------------------------------------------------------------- weight scales of a tile
+    const int m = warp - 1;
+    while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
+      const MoeGeom gm = sh.geom(p, pl, t);
+      const int w = lane & 3;
+      const uint8_t* src0 = (t.phase == 0 ? p.s13 : p.s2) +
+                            ((m == 0 ? gm.ra : gm.rb) + (lane >> 2)) * (gm.K / 16) + 4 * w;
+      bool ok = true;
+      for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK)
+        for (int c = gm.c0; c < gm.c1; ++c) {
+          if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
+          if ((m == 0 || gm.two) && c * 4 + w < gm.K / 64) {
+            const uint32_t dst =
+                smem_u32(smem + r.slot * Cfg::kStage + Cfg::oSw + (m * 4 + w) * 512);
+            const uint8_t* src = src0 + c * 16;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int row = 8 * i + (lane >> 2);
+              cp_async4(dst + (row & 31) * 16 + (row >> 5) * 4, src + 8 * i * (gm.K / 16));
+            }
+          }
+          cp_async_arrive(smem_u32(&ctl.full[r.slot]));
+          r.next();
+        }
       if (!ok) break;
     }
-    // every copy issued has landed before the CTA exits (also after a wait ran out)
-    for (int j = max(0, issued - kMoeStages); j < issued; ++j)
-      mbar_wait(smem_u32(&ctl.wfull[j % kMoeStages]), (j / kMoeStages) & 1, p.err, kErrWaitTma,
-                nullptr);
-  } else if (warp == kMoeConsumers + 1) {
-    // -------------------------------------------------------------- activation producer
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------------- activation digits
     bool ready = false;
-    int issued = 0;
-    MoeTask t;
-    while (moe_next_task(t, ctl, r, p.err) && t.phase != 2) {
+    while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
       if (t.phase == 1 && !ready) {
-        if (!__all_sync(0xFFFFFFFFu,
-                        moe_wait(p.counters + kMoeGateUpDone, sh.total1, ctl, p.err)))
-          break;
-        // the hidden values were written by ordinary stores; the copies read through the async proxy
+        if (!moe_wait(p.counters + kMoeDigitsDone, total_d, ctl, p.err)) break;
+        // written by ordinary stores of this grid; the bulk copies read through the async proxy
         asm volatile("fence.proxy.async;" ::: "memory");
         ready = true;
       }
       const MoeGeom gm = sh.geom(p, pl, t);
       bool ok = true;
-      for (int c0 = 0; c0 < gm.cnt && ok; c0 += 8 * kMoeTiles) {
-        const int n = min(gm.cnt - c0, 8 * kMoeTiles), nt = (n + 7) / 8;
-        const int cu = moe_chunk_units(nt);
-        const uint8_t* src = nullptr;
+      for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK) {
+        const int n = min(gm.cnt - n0, TOK);
+        int64_t at = 0;  // this lane's token
         if (lane < n) {
-          const int pr = pl.pairs[gm.off + c0 + lane];
-          src = t.phase == 0 ? p.xs + (pr / p.k) * moe_image_row(p.H)
-                             : p.h + pr * moe_image_row(p.I);
+          const int pr = pl.pairs[gm.off + n0 + lane];
+          at = (t.phase == 0 ? pr / p.k : pr) * moe_image_row(gm.K);
         }
-        for (int u = gm.u0; u < gm.u1; u += cu) {
-          const int uc = min(cu, gm.u1 - u);
-          if (!moe_warp_wait(ctl.aempty[r.a.slot], r.a.phase ^ 1u, kErrWaitEmpty, ctl, p.err)) {
-            ok = false;
-            break;
-          }
-          const uint32_t fb = smem_u32(&ctl.afull[r.a.slot]);
-          if (lane == 0) mbar_arrive_expect_tx(fb, static_cast<uint32_t>(n * uc) * kMoeBlock);
+        const uint8_t* base = t.phase == 0 ? p.xs : p.hs;
+        for (int c = gm.c0; c < gm.c1; ++c) {
+          if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
+          const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
+          const uint32_t fb = smem_u32(&ctl.full[r.slot]);
+          if (lane == 0) mbar_arrive_expect_tx(fb, n * kMoeChunkCodes);
           __syncwarp();
-          if (lane < n)
-            bulk_load(smem_u32(smem + oMoeAct + r.a.slot * kMoeActSlot) + lane * moe_pitch(uc),
-                      src + static_cast<int64_t>(u) * kMoeBlock, uc * kMoeBlock, fb);
-          r.a.next();
-          ++issued;
+          const uint8_t* src = base + at + static_cast<int64_t>(c) * kMoeChunk;
+          if (lane < n) bulk_load(st + Cfg::oB + lane * kMoeChunkCodes, src, kMoeChunkCodes, fb);
+          // scale words of token i: lane = 4 digit + word
+          for (int i = 0; i < n; ++i) {
+            const uint8_t* si = base + __shfl_sync(0xFFFFFFFFu, at, i) +
+                                static_cast<int64_t>(c) * kMoeChunk + kMoeChunkCodes + 4 * lane;
+            const int row = i * kMoeDigitRows + (lane >> 2);
+            if (c * 4 + (lane & 3) < gm.K / 64)
+              cp_async4(st + Cfg::oSb + (row >> 7) * 2048 + (lane & 3) * 512 + (row & 31) * 16 +
+                            ((row >> 5) & 3) * 4,
+                        si);
+          }
+          cp_async_arrive(fb);
+          r.next();
         }
       }
       if (!ok) break;
     }
-    for (int j = max(0, issued - 2); j < issued; ++j)
-      mbar_wait(smem_u32(&ctl.afull[j % 2]), (j / 2) & 1, p.err, kErrWaitTma, nullptr);
-  } else {
-    // ---------------------------------------------------------------------------- consumers
-    const int g = lane >> 2, q = lane & 3;
-    const int rho = (g >> 1) | ((g & 1) << 2);
-    int flip = 0;
-    uint32_t cph = 0;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == 4) {
+    // ----------------------------------------------------------------------------------- MMA
+    RingPos<Cfg::kAccs> ac;
+    uint32_t set = 0;
     bool ok = true;
-    MoeTask t;
-    // any wait that runs out ends the role (ok false): the abort flag ends the other roles' waits
-    while ((ok = moe_next_task(t, ctl, r, p.err)) && t.phase != 2) {
+    while (ok && moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
       const MoeGeom gm = sh.geom(p, pl, t);
-      const bool up = t.phase == 0;
-      const int row_a = up ? 8 * warp + rho : 16 * warp + rho;
-      const int row_b = up ? row_a + 128 : row_a + 8;
-      const bool active = up || gm.row0 + 16 * warp < p.H;
-      for (int c0 = 0; c0 < gm.cnt && ok; c0 += 8 * kMoeTiles) {
-        const int n = min(gm.cnt - c0, 8 * kMoeTiles), nt = (n + 7) / 8;
-        float acc[kMoeTiles][4] = {};
-        if (nt == 1) ok = moe_consume<1>(acc, smem, ctl, r, gm.u0, gm.u1, row_a, row_b, active, p.err);
-        else if (nt == 2) ok = moe_consume<2>(acc, smem, ctl, r, gm.u0, gm.u1, row_a, row_b, active, p.err);
-        else if (nt == 3) ok = moe_consume<3>(acc, smem, ctl, r, gm.u0, gm.u1, row_a, row_b, active, p.err);
-        else ok = moe_consume<4>(acc, smem, ctl, r, gm.u0, gm.u1, row_a, row_b, active, p.err);
-        if (!ok) break;
-        if (up) {
-          const float ts13 = p.ts13[gm.e], ts2 = p.ts2[gm.e];
-          const int i = gm.row0 + 8 * warp + rho;
-#pragma unroll
-          for (int tl = 0; tl < kMoeTiles; ++tl) {
-            if (tl >= nt) break;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int col = 8 * tl + 2 * q + c;
-              float hv = 0.0f;
-              if (col < n)
-                hv = silu_rn(acc[tl][c] * ts13) * (acc[tl][2 + c] * ts13) *
-                     (pl.w[pl.pairs[gm.off + c0 + col]] * ts2);
-              acc[tl][c] = hv;
-              uint32_t hm = __float_as_uint(hv) & 0x7FFFFFFFu;
-              hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, 4));
-              hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, 8));
-              hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, 16));
-              if (g == 0 && col < n) atomicMax(&ctl.hmax[flip][col], hm);
+      for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK) {
+        const int n = min(gm.cnt - n0, TOK);
+        const uint32_t N = static_cast<uint32_t>(n * kMoeDigitRows + 15) & ~15u;
+        const uint32_t idesc = idesc_mxf4(128, N, false, 0);
+        const int blocks = N > 128 ? 2 : 1;
+        if (!(ok = moe_warp_wait(ctl.acc_empty[ac.slot], ac.phase ^ 1u, kErrWaitAccum, ctl, p.err)))
+          break;
+        tc_fence_after();
+        const uint32_t acc = tb + ac.slot * 2 * Cfg::kN;
+        for (int c = gm.c0; c < gm.c1; ++c) {
+          if (!(ok = moe_warp_wait(ctl.full[r.slot], r.phase, kErrWaitTma, ctl, p.err))) break;
+          // the scales were written by cp.async (generic proxy): before tcgen05.cp reads them
+          fence_proxy_async_smem();
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
+          const uint32_t sf = tb + Cfg::kSfCol0 + set * Cfg::kSfSet;
+          const int steps = min(4, gm.K / 64 - c * 4);
+          if (elect_one()) {
+            for (int kk = 0; kk < steps; ++kk) {
+              tmem_cp_32x128b_x4(sf + 4 * kk, sdesc_sf(st + Cfg::oSw + kk * 512));
+              if (gm.two)
+                tmem_cp_32x128b_x4(sf + 16 + 4 * kk, sdesc_sf(st + Cfg::oSw + (4 + kk) * 512));
+              tmem_cp_32x128b_x4(sf + 32 + kk * 4 * Cfg::kBlocks,
+                                 sdesc_sf(st + Cfg::oSb + kk * 512));
+              if (Cfg::kBlocks > 1 && blocks > 1)
+                tmem_cp_32x128b_x4(sf + 32 + kk * 4 * Cfg::kBlocks + 4,
+                                   sdesc_sf(st + Cfg::oSb + 2048 + kk * 512));
             }
-          }
-          if (!(ok = moe_consumer_sync(ctl, cph, p.err))) break;
-          if (tid < 32) ctl.hmax[flip ^ 1][tid] = 0;
-#pragma unroll
-          for (int tl = 0; tl < kMoeTiles; ++tl) {
-            if (tl >= nt) break;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int col = 8 * tl + 2 * q + c;
-              if (col < n) {
-                const int E = moe_exp(ctl.hmax[flip][col]);
-                uint8_t* img = p.h + pl.pairs[gm.off + c0 + col] * moe_image_row(p.I);
-                *reinterpret_cast<__half*>(img + moe_image_offset(i)) =
-                    __float2half_rn(acc[tl][c] * pow2f(14 - E));
-                if (warp == 0 && g == 0)
-                  *reinterpret_cast<float*>(img + gm.row0 / 128 * kMoeBlock + 256) = pow2f(E - 14);
-              }
+            for (int kk = 0; kk < steps; ++kk) {
+              const uint32_t accumulate = (c > gm.c0 || kk > 0) ? 1u : 0u;
+              const uint64_t bd = sdesc_sw128(st + Cfg::oB + kk * 32);
+              const uint32_t sfb = sf + 32 + kk * 4 * Cfg::kBlocks;
+              mma_mxf4_ss<true, false>(acc, sdesc_sw128(st + kk * 32), bd, idesc, sf + 4 * kk, sfb,
+                                       accumulate);
+              if (gm.two)
+                mma_mxf4_ss<true, false>(acc + Cfg::kN, sdesc_sw128(st + Cfg::kCodes / 2 + kk * 32),
+                                         bd, idesc, sf + 16 + 4 * kk, sfb, accumulate);
             }
+            tc_commit(smem_u32(&ctl.empty[r.slot]));
+            if (c + 1 == gm.c1) tc_commit(smem_u32(&ctl.acc_full[ac.slot]));
           }
-          flip ^= 1;
-          // hmax is read, the other copy cleared, the images written
-          if (!(ok = moe_consumer_sync(ctl, cph, p.err))) break;
-        } else if (active) {
-#pragma unroll
-          for (int tl = 0; tl < kMoeTiles; ++tl) {
-            if (tl >= nt) break;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int col = 8 * tl + 2 * q + c;
-              if (col < n) {
-                const int pr = pl.pairs[gm.off + c0 + col];
-                float* dst = p.part + (static_cast<int64_t>(gm.z) * p.T * p.k + pr) * p.H + gm.row0;
-                dst[row_a] = acc[tl][c];
-                dst[row_b] = acc[tl][2 + c];
-              }
-            }
-          }
+          __syncwarp();
+          r.next();
+          set ^= 1u;
         }
-      }
-      if (!ok || (!up && !(ok = moe_consumer_sync(ctl, cph, p.err)))) break;
-      if (tid == 0) {
-        if (up) asm volatile("fence.proxy.async;" ::: "memory");
-        __threadfence();
-        atomicAdd(p.counters + (up ? kMoeGateUpDone : kMoeDownDone), 1u);
+        ac.next();
       }
     }
+    // arrives once every tcgen05 operation this warp issued has completed
+    if (elect_one()) tc_commit(smem_u32(&ctl.drain));
+    __syncwarp();
+    mbar_wait(smem_u32(&ctl.drain), 0, p.err, kErrWaitMma, nullptr);
+  } else {
+    // ------------------------------------------------------------------------------ epilogue
+    const int group = (warp - kMoeEpiWarp0) / 4, quarter = warp & 3;
+    const int row = 32 * quarter + lane;  // row of the MMA tile
+    const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
+    RingPos<Cfg::kAccs> ac;
+    bool ok = true, digits = false;
+    // digits of the hidden values, by tickets, between this CTA's last gate / up and first down
+    auto make_digits = [&]() {
+      digits = true;
+      bool ready = false;
+      while (true) {
+        const uint32_t k = moe_ticket(p.counters + kMoeDigits);
+        if (k >= total_d) return true;
+        if (!ready && !moe_wait(p.counters + kMoeGateUpDone, sh.total1 * kMoeEpiWarps, ctl, p.err))
+          return false;
+        ready = true;
+        const int b = static_cast<int>(k) * 32 + lane;  // blocks of a pair: a multiple of eight
+        const int pr = b / blocks_h;
+        if (pr < p.T * p.k && pl.used[pr]) {
+          const int blk = b - pr * blocks_h;
+          const float up = pow2f(moe_row_shift(__ldcg(p.hmax + pr)));
+          const float* src = p.h + static_cast<int64_t>(pr) * p.I + 16 * blk;
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 u = ld_cg(src + 4 * j);
+            v[4 * j] = __uint_as_float(u.x) * up;
+            v[4 * j + 1] = __uint_as_float(u.y) * up;
+            v[4 * j + 2] = __uint_as_float(u.z) * up;
+            v[4 * j + 3] = __uint_as_float(u.w) * up;
+          }
+          moe_digits(v, p.hs + pr * moe_image_row(p.I), blk);
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");
+        moe_count(p.counters + kMoeDigitsDone);
+      }
+    };
+    while ((ok = moe_next_task(t, q, ctl, p.err)) && t.phase != 2) {
+      if (t.phase == 1 && !digits && !(ok = make_digits())) break;
+      const MoeGeom gm = sh.geom(p, pl, t);
+      const float ts13 = p.ts13[gm.e], ts2 = p.ts2[gm.e];
+      for (int n0 = 0; n0 < gm.cnt; n0 += TOK) {
+        const int n = min(gm.cnt - n0, TOK);
+        if (!(ok = moe_warp_wait(ctl.acc_full[ac.slot], ac.phase, kErrWaitAccum, ctl, p.err))) break;
+        tc_fence_after();
+        const uint32_t acc = tb + lanes + ac.slot * 2 * Cfg::kN;
+        if (t.phase == 0) {
+          // tokens of this group of four warps: every other one
+          for (int c = group; c < n; c += 2) {
+            uint32_t ga[8], ua[8];
+            tmem_ld_x8(acc + c * kMoeDigitRows, ga);
+            tmem_ld_x8(acc + Cfg::kN + c * kMoeDigitRows, ua);
+            tmem_ld_wait();
+            const int pr = pl.pairs[gm.off + n0 + c];
+            const float s = p.x_scale[pr / p.k] * ts13;
+            const float h = silu_rn(moe_sum8(ga) * s) * (moe_sum8(ua) * s) * (pl.w[pr] * ts2);
+            p.h[static_cast<int64_t>(pr) * p.I + gm.row0 + row] = h;
+            const uint32_t hm =
+                __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h) & 0x7FFFFFFFu);
+            if (lane == 0) atomicMax(p.hmax + pr, hm);
+          }
+        } else if (group == 0 || gm.two) {
+          for (int c = 0; c < n; ++c) {
+            uint32_t d[8];
+            tmem_ld_x8(acc + group * Cfg::kN + c * kMoeDigitRows, d);
+            tmem_ld_wait();
+            const int pr = pl.pairs[gm.off + n0 + c];
+            p.part[(static_cast<int64_t>(gm.z) * p.T * p.k + pr) * p.H + gm.row0 + 128 * group + row] =
+                moe_sum8(d) * moe_row_factor(__ldcg(p.hmax + pr));
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.acc_empty[ac.slot]));
+        ac.next();
+      }
+      if (!ok) break;
+      moe_count(p.counters + (t.phase == 0 ? kMoeGateUpDone : kMoeDownDone));
+    }
+    if (ok && !digits) ok = make_digits();
 
-    // ------------------------------------------------------------------------------ combine
-    const int cols = 4 * 32 * kMoeConsumers;  // outputs per task
-    const int blocks3 = (p.H + cols - 1) / cols;
+    // combine: a warp task is 256 outputs of a token
+    const int blocks3 = (p.H + 255) / 256;
     bool ready = false;
     while (ok) {
-      if (!moe_consumer_sync(ctl, cph, p.err)) break;
-      if (tid == 0) {
-        ctl.ticket = atomicAdd(p.counters + kMoeCombine, 1u);
-        if (!ready && ctl.ticket < static_cast<uint32_t>(p.T * blocks3))
-          moe_wait(p.counters + kMoeDownDone, sh.total2, ctl, p.err);  // raises the abort flag
-      }
-      if (!moe_consumer_sync(ctl, cph, p.err) || *abort_flag) break;
-      const uint32_t task = ctl.ticket;
+      const uint32_t task = moe_ticket(p.counters + kMoeCombine);
       if (task >= static_cast<uint32_t>(p.T * blocks3)) break;
+      if (!ready && !moe_wait(p.counters + kMoeDownDone, sh.total2 * kMoeEpiWarps, ctl, p.err)) break;
       ready = true;
-      const int t = task / blocks3, h0 = (task % blocks3) * cols + 4 * tid;
-      if (h0 >= p.H) continue;
-      float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int s = 0; s < p.k; ++s) {
-        const int pr = t * p.k + s;
-        if (!pl.used[pr]) continue;
-        for (int z = 0; z < sh.slices; ++z) {
-          const uint4 v = ld_cg(p.part + (static_cast<int64_t>(z) * p.T * p.k + pr) * p.H + h0);
-          o[0] += __uint_as_float(v.x);
-          o[1] += __uint_as_float(v.y);
-          o[2] += __uint_as_float(v.z);
-          o[3] += __uint_as_float(v.w);
+      const int tok = task / blocks3;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int h0 = (task % blocks3) * 256 + half * 128 + 4 * lane;
+        if (h0 >= p.H) break;
+        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < p.k; ++s) {
+          const int pr = tok * p.k + s;
+          if (!pl.used[pr]) continue;
+          for (int z = 0; z < sh.slices; ++z) {
+            const uint4 v = ld_cg(p.part + (static_cast<int64_t>(z) * p.T * p.k + pr) * p.H + h0);
+            o[0] += __uint_as_float(v.x);
+            o[1] += __uint_as_float(v.y);
+            o[2] += __uint_as_float(v.z);
+            o[3] += __uint_as_float(v.w);
+          }
         }
+        store_row<4>(p.y, static_cast<int64_t>(tok) * p.H + h0, o, p.out_dtype, p.vec_out);
       }
-      store_row<4>(p.y, static_cast<int64_t>(t) * p.H + h0, o, p.out_dtype, p.vec_out);
     }
+  }
+  // ------------------------------------------------------------------------------- teardown
+  __syncwarp();
+  if (*abort_flag && warp == 0) {  // a wait ran out: the copies issued land before the CTA exits
+    for (int s = 0; s < Cfg::kStages; ++s)
+      mbar_wait(smem_u32(&ctl.full[s]), 0, p.err, kErrWaitTma, nullptr, kWaitLimitCycles / 8);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tb, 512);
   }
 }
 

@@ -85,8 +85,8 @@ def _workspace_bytes(T: int, H: int, inter: int, top_k: int) -> int:
     if T == 0:
         return 0
     pairs = T * top_k
-    return 256 + up(T * (H // 128) * 272) + up(pairs * (inter // 128) * 272) + \
-        4 * H * max(pairs, 256)
+    return 256 + up(4 * pairs) + up(4 * T) + up(T * ((H + 255) // 256) * 1152) + \
+        up(4 * pairs * inter) + up(pairs * ((inter + 255) // 256) * 1152) + 4 * H * max(pairs, 256)
 
 
 def _out_tensor(out, x: torch.Tensor, out_dtype):

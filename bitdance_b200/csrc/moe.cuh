@@ -34,7 +34,7 @@
 namespace bd {
 
 constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTopK = 16;
-constexpr int kMoeThreads = 256, kMoeWarps = kMoeThreads / 32;
+constexpr int kMoeThreads = 512, kMoeWarps = kMoeThreads / 32;
 constexpr int kRouteCluster = 8;
 
 // Counters in the workspace, zeroed by the first kernel: tickets and finished tasks per phase.
@@ -45,7 +45,6 @@ enum : int {
   kMoeDigitsDone,
   kMoeDown,
   kMoeDownDone,
-  kMoeCombine,
   kMoeCounters
 };
 
@@ -245,7 +244,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
   for (int e = rank + kRouteCluster * warp; e < p.E; e += kRouteCluster * kMoeWarps) {
     double acc[TB] = {};
     const W* row = wr + static_cast<int64_t>(e) * p.H;
-#pragma unroll 4
+#pragma unroll(TB == 1 ? 8 : 4)
     for (int c = lane; c < pieces; c += 32) {
       float w[8];
       load8(row + 8 * c, w);
@@ -365,65 +364,78 @@ struct MoePlan {
   uint16_t off[kMoeMaxExperts];      // first pair of an expert in `pairs`
   uint16_t act[kMoeMaxExperts];      // experts with at least one pair, ascending
   uint16_t pairs[kMoeMaxTokens * kMoeMaxTopK];  // pairs t * k + slot, by expert
+  int16_t id[kMoeMaxTokens * kMoeMaxTopK];      // expert of a pair, -1 for none
   float w[kMoeMaxTokens * kMoeMaxTopK];         // weight of a pair
   uint8_t used[kMoeMaxTokens * kMoeMaxTopK];    // the pair counts
+  uint32_t totals[kMoeMaxExperts / 32];         // experts << 16 | pairs of 32 experts
   int nact;
 };
 
-// Pairs by expert. A token that names an expert twice keeps the first pair with the sum of the
-// weights; ids outside [0, E) are no pair (-1 quietly, others reported). Ends with a barrier.
+// Pairs by expert, by kThreads >= kMoeMaxExperts threads; pl.cnt is zero and visible before. A token
+// that names an expert twice keeps the first pair with the sum of the weights; ids outside [0, E) are
+// no pair (-1 quietly, others reported). Ends with a barrier.
 template <int kThreads>
 __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
+  static_assert(kThreads >= kMoeMaxExperts, "an expert per thread");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int npairs = p.T * p.k;
   constexpr int kPer = (kMoeMaxTokens * kMoeMaxTopK + kThreads - 1) / kThreads;
+  float w[kPer] = {};
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int pr = tid + i * kThreads;
+    if (pr >= npairs) continue;
+    int e = p.ids[pr];
+    w[i] = p.weights[pr];
+    if (e < 0 || e >= p.E) {
+      if (e != -1) atomicOr(p.err, kErrRange);
+      e = -1;
+    }
+    pl.id[pr] = static_cast<int16_t>(e);
+    pl.w[pr] = w[i];
+  }
+  __syncthreads();
   int id[kPer], pos[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int pr = tid + i * kThreads;
     id[i] = -1;
     pos[i] = 0;
-    if (pr < npairs) {
-      int e = p.ids[pr];
-      if (e < 0 || e >= p.E) {
-        if (e != -1) atomicOr(p.err, kErrRange);
-        e = -1;
-      }
-      float w = p.weights[pr];
-      const int first = pr / p.k * p.k;
-      for (int s = first; s < first + p.k && e >= 0; ++s) {
-        if (s == pr || p.ids[s] != e) continue;
-        if (s < pr) e = -1;
-        else w += p.weights[s];
-      }
-      if (e >= 0) {
-        pos[i] = atomicAdd(&pl.cnt[e], 1);
-        pl.w[pr] = w;
-      }
-      pl.used[pr] = e >= 0;
-      id[i] = e;
+    if (pr >= npairs) continue;
+    int e = pl.id[pr];
+    const int first = pr / p.k * p.k;
+    for (int s = first; s < first + p.k && e >= 0; ++s) {
+      if (s == pr || pl.id[s] != e) continue;
+      if (s < pr) e = -1;
+      else w[i] += pl.w[s];
     }
+    if (e >= 0) pos[i] = atomicAdd(&pl.cnt[e], 1);
+    pl.used[pr] = e >= 0;
+    id[i] = e;
   }
   __syncthreads();
-  if (warp == 0) {
-    int nact = 0, off = 0;
-    for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int c = e0 + lane < p.E ? pl.cnt[e0 + lane] : 0;
-      const uint32_t has = __ballot_sync(0xFFFFFFFFu, c > 0);
-      int inc = c;
+  // expert of this thread: its place among the touched ones, and its first pair
+  const int c = tid < p.E ? pl.cnt[tid] : 0;
+  uint32_t inc = static_cast<uint32_t>(c) + (c > 0 ? 0x10000u : 0u);
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-        if (lane >= o) inc += u;
-      }
-      if (c > 0) {
-        pl.act[nact + __popc(has & ((1u << lane) - 1u))] = static_cast<uint16_t>(e0 + lane);
-        pl.off[e0 + lane] = static_cast<uint16_t>(off + inc - c);
-      }
-      nact += __popc(has);
-      off += __shfl_sync(0xFFFFFFFFu, inc, 31);
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  if (lane == 31 && warp < kMoeMaxExperts / 32) pl.totals[warp] = inc;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (id[i] >= 0) pl.w[tid + i * kThreads] = w[i];
+  __syncthreads();
+  if (warp < kMoeMaxExperts / 32) {
+    uint32_t before = 0;
+    for (int i = 0; i < warp; ++i) before += pl.totals[i];
+    const uint32_t end = before + inc;
+    if (c > 0) {
+      pl.act[(end >> 16) - 1] = static_cast<uint16_t>(tid);
+      pl.off[tid] = static_cast<uint16_t>((end & 0xFFFFu) - c);
     }
-    if (lane == 0) pl.nact = nact;
+    if (tid == kMoeMaxExperts - 1) pl.nact = end >> 16;
   }
   __syncthreads();
   // the place of a pair within its expert's list is the order of arrival: it picks an MMA
@@ -441,13 +453,16 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
 //   digits:    h -> digits, once every h is there (their row factor needs the row's maximum);
 //   down:      256 output rows of one expert and a slice of I; partial sums per (slice, pair);
 //   combine:   y = the partial sums of a token's pairs in slot order.
-// Warps: 0 weight codes (takes the tickets and publishes the tasks in a queue), 1 and 2 weight scales
-// of the two tiles (4-byte cp.async straight into the tiles tcgen05.cp wants: no repacking of the
-// natural layout), 3 activation digits (waits for the digits phase before the first down task, while
-// the weights of the next stages already arrive), 4 MMA, 5..12 epilogue (and the digits and combine
-// phases). Two builds: TOK = 8 (four stages, accumulators double-buffered) where an expert has few
+// Warps: 0 weight codes (takes the tickets and publishes the tasks in a queue), 1..4 weight scales
+// (64 rows each, 4-byte cp.async straight into the tiles tcgen05.cp wants: no repacking of the natural
+// layout), 5 activation digits, 6..8 their scales (5..8 wait for the digits phase before the first down
+// task, while the weights of the next stages already arrive; with one warp for 5..8 it was the
+// slowest role and the layer up to twice as slow), 9 MMA, 10..17 epilogue (and the digits and
+// combine phases). Two builds: TOK = 8 (four stages, accumulators double-buffered) where an expert has few
 // tokens, TOK = 24.
-constexpr int kMoeEpiWarp0 = 5, kMoeEpiWarps = 8;
+constexpr int kMoeScaleWarps = 4, kMoeDigitScaleWarps = 3;
+constexpr int kMoeMmaWarp = 2 + kMoeScaleWarps + kMoeDigitScaleWarps;
+constexpr int kMoeEpiWarp0 = kMoeMmaWarp + 1, kMoeEpiWarps = 8;
 constexpr int kMoeExpertThreads = 32 * (kMoeEpiWarp0 + kMoeEpiWarps);
 constexpr int kMoeQueue = 4;
 
@@ -467,14 +482,15 @@ struct MoeCfg {
   static constexpr int kSfSet = 2 * 16 + kBlocks * 16;       // scale words of a stage in tensor memory
   static_assert(kSfCol0 + 2 * kSfSet <= 512, "tensor memory budget");
   static_assert(kStage % 1024 == 0 && oB % 1024 == 0, "1 KB swizzle atoms");
-  // a full stage: the code and digit copies' tx arrives, 64 + 32 lanes' scale copies
-  static constexpr int kFullCount = 2 + 96;
+  // a full stage: the code and digit copies' tx arrives, the scale warps' lanes
+  static constexpr int kFullCount = 2 + 32 * (kMoeScaleWarps + kMoeDigitScaleWarps);
 };
 
 struct MoeCtl {
-  uint64_t full[4], empty[4], acc_full[2], acc_empty[2], qfull[kMoeQueue], qempty[kMoeQueue], drain;
+  uint64_t full[4], empty[4], acc_full[2], acc_empty[2], qfull[kMoeQueue], qempty[kMoeQueue], drain, ebar;
   uint32_t queue[kMoeQueue];
-  uint32_t abort_flag, tmem_base;
+  uint32_t abort_flag, tmem_base, ticket;
+  uint32_t warps[2];  // epilogue warps that finished a part of a task: products, digits
 };
 constexpr int kMoeQueueReaders = kMoeEpiWarp0 - 1 + kMoeEpiWarps;
 
@@ -570,11 +586,26 @@ __device__ __forceinline__ uint32_t moe_ticket(uint32_t* counter) {
   if ((threadIdx.x & 31) == 0) k = atomicAdd(counter, 1u);
   return __shfl_sync(0xFFFFFFFFu, k, 0);
 }
-// A warp's part of a task is done: its stores before the count.
-__device__ __forceinline__ void moe_count(uint32_t* counter) {
+// An epilogue warp's part of a task is done: its stores before the count. The last of the eight
+// counts for the CTA (atomics on one address pass one after the other: eight times as many, and a
+// ticket per warp in the digits phase, held the phases up by 10 to 20 us).
+__device__ __forceinline__ void moe_count(uint32_t* counter, uint32_t* warps) {
   __threadfence();
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) atomicAdd(counter, 1u);
+  if ((threadIdx.x & 31) == 0 && (atomicAdd(warps, 1u) & (kMoeEpiWarps - 1)) == kMoeEpiWarps - 1) {
+    __threadfence();
+    atomicAdd(counter, 1u);
+  }
+}
+
+// Barrier of the epilogue warps: an mbarrier, so that the wait is bounded and ends when another role
+// has given up.
+__device__ __forceinline__ bool moe_epi_sync(MoeCtl& ctl, uint32_t& parity, uint32_t* err) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl.ebar));
+  const bool ok = moe_warp_wait(ctl.ebar, parity, kErrWaitAccum, ctl, err);
+  parity ^= 1u;
+  return ok;
 }
 
 // Sum of a token's eight digit columns.
@@ -618,9 +649,11 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
       mbar_init(smem_u32(&ctl.qempty[s]), kMoeQueueReaders);
     }
     mbar_init(smem_u32(&ctl.drain), 1);
+    mbar_init(smem_u32(&ctl.ebar), kMoeEpiWarps);
+    ctl.warps[0] = ctl.warps[1] = 0;
     fence_mbar_init();
   }
-  if (warp == 4) {
+  if (warp == kMoeMmaWarp) {
     tmem_alloc(smem_u32(&ctl.tmem_base), 512);
     tmem_relinquish();
   }
@@ -630,6 +663,8 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
   tc_fence_after();
   const uint32_t tb = ctl.tmem_base;
   grid_dep_wait();
+  uint32_t first_ticket = 0;  // taken while the plan is made
+  if (tid == 0) first_ticket = atomicAdd(p.counters + kMoeGateUp, 1u);
   moe_plan<kMoeExpertThreads>(p, pl);
   const int nact = pl.nact;
 
@@ -643,9 +678,10 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
          2 * sh.slices * p.T * p.k <= p.part_rows && p.I / 256 >= 2 * sh.slices)
     sh.slices *= 2;
   sh.total2 = static_cast<uint32_t>(nact) * sh.blocks2 * sh.slices;
-  // digits: a warp task is 32 blocks of 16 hidden values, over all pairs
+  // digits: a task is a 16-block of hidden values per epilogue thread, over all pairs
   const int blocks_h = p.I / 16;
-  const uint32_t total_d = static_cast<uint32_t>(p.T * p.k * blocks_h + 31) / 32;
+  const uint32_t total_d =
+      static_cast<uint32_t>(p.T * p.k * blocks_h + 32 * kMoeEpiWarps - 1) / (32 * kMoeEpiWarps);
 
   RingPos<kMoeQueue> q;
   RingPos<Cfg::kStages> r;
@@ -657,13 +693,19 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
       prefetch_tmap(&tm_w2);
     }
     uint32_t phase = 0;
-    bool ok = true;
+    bool ok = true, first = true;
     while (ok) {
       // the next task: the phase's tickets, then the next phase's
       t.phase = 2;
       t.index = 0;
       while (phase < 2) {
-        const uint32_t k = moe_ticket(p.counters + (phase == 0 ? kMoeGateUp : kMoeDown));
+        uint32_t k;
+        if (first) {
+          k = __shfl_sync(0xFFFFFFFFu, first_ticket, 0);
+          first = false;
+        } else {
+          k = moe_ticket(p.counters + (phase == 0 ? kMoeGateUp : kMoeDown));
+        }
         if (k < (phase == 0 ? sh.total1 : sh.total2)) {
           t.phase = phase;
           t.index = k;
@@ -695,14 +737,14 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
           r.next();
         }
     }
-  } else if (warp <= 2) {
-    // ----------------------------------------------------------------- weight scales of a tile
-    const int m = warp - 1;
+  } else if (warp <= kMoeScaleWarps) {
+    // ------------------------------------------------- weight scales: half the rows of a tile
+    const int m = (warp - 1) >> 1, r0 = ((warp - 1) & 1) * 64 + (lane >> 2);
     while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
       const MoeGeom gm = sh.geom(p, pl, t);
       const int w = lane & 3;
       const uint8_t* src0 = (t.phase == 0 ? p.s13 : p.s2) +
-                            ((m == 0 ? gm.ra : gm.rb) + (lane >> 2)) * (gm.K / 16) + 4 * w;
+                            ((m == 0 ? gm.ra : gm.rb) + r0) * (gm.K / 16) + 4 * w;
       bool ok = true;
       for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK)
         for (int c = gm.c0; c < gm.c1; ++c) {
@@ -712,8 +754,8 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
                 smem_u32(smem + r.slot * Cfg::kStage + Cfg::oSw + (m * 4 + w) * 512);
             const uint8_t* src = src0 + c * 16;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int row = 8 * i + (lane >> 2);
+            for (int i = 0; i < 8; ++i) {
+              const int row = r0 + 8 * i;
               cp_async4(dst + (row & 31) * 16 + (row >> 5) * 4, src + 8 * i * (gm.K / 16));
             }
           }
@@ -723,8 +765,9 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
       if (!ok) break;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == 3) {
-    // ---------------------------------------------------------------------- activation digits
+  } else if (warp < kMoeMmaWarp) {
+    // ------------------------------------------ activation digits: codes (warp 5), scales (6..8)
+    const int part = warp - kMoeScaleWarps - 2;  // -1: codes
     bool ready = false;
     while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
       if (t.phase == 1 && !ready) {
@@ -734,6 +777,7 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
         ready = true;
       }
       const MoeGeom gm = sh.geom(p, pl, t);
+      const uint8_t* base = t.phase == 0 ? p.xs : p.hs;
       bool ok = true;
       for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK) {
         const int n = min(gm.cnt - n0, TOK);
@@ -742,33 +786,38 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
           const int pr = pl.pairs[gm.off + n0 + lane];
           at = (t.phase == 0 ? pr / p.k : pr) * moe_image_row(gm.K);
         }
-        const uint8_t* base = t.phase == 0 ? p.xs : p.hs;
         for (int c = gm.c0; c < gm.c1; ++c) {
           if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
           const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
           const uint32_t fb = smem_u32(&ctl.full[r.slot]);
-          if (lane == 0) mbar_arrive_expect_tx(fb, n * kMoeChunkCodes);
-          __syncwarp();
-          const uint8_t* src = base + at + static_cast<int64_t>(c) * kMoeChunk;
-          if (lane < n) bulk_load(st + Cfg::oB + lane * kMoeChunkCodes, src, kMoeChunkCodes, fb);
-          // scale words of token i: lane = 4 digit + word
-          for (int i = 0; i < n; ++i) {
-            const uint8_t* si = base + __shfl_sync(0xFFFFFFFFu, at, i) +
-                                static_cast<int64_t>(c) * kMoeChunk + kMoeChunkCodes + 4 * lane;
-            const int row = i * kMoeDigitRows + (lane >> 2);
-            if (c * 4 + (lane & 3) < gm.K / 64)
-              cp_async4(st + Cfg::oSb + (row >> 7) * 2048 + (lane & 3) * 512 + (row & 31) * 16 +
-                            ((row >> 5) & 3) * 4,
-                        si);
+          const uint8_t* src = base + static_cast<int64_t>(c) * kMoeChunk;
+          if (part < 0) {
+            if (lane == 0) mbar_arrive_expect_tx(fb, n * kMoeChunkCodes);
+            __syncwarp();
+            if (lane < n)
+              bulk_load(st + Cfg::oB + lane * kMoeChunkCodes, src + at, kMoeChunkCodes, fb);
+          } else {
+            // scale words of token i: lane = 4 digit + word
+            const bool in = c * 4 + (lane & 3) < gm.K / 64;
+#pragma unroll
+            for (int j = 0; j < TOK / kMoeDigitScaleWarps + 1; ++j) {
+              const int i = part + j * kMoeDigitScaleWarps;
+              const int64_t ai = __shfl_sync(0xFFFFFFFFu, at, i & 31);
+              const int row = i * kMoeDigitRows + (lane >> 2);
+              if (i < n && in)
+                cp_async4(st + Cfg::oSb + (row >> 7) * 2048 + (lane & 3) * 512 + (row & 31) * 16 +
+                              ((row >> 5) & 3) * 4,
+                          src + ai + kMoeChunkCodes + 4 * lane);
+            }
+            cp_async_arrive(fb);
           }
-          cp_async_arrive(fb);
           r.next();
         }
       }
       if (!ok) break;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == 4) {
+  } else if (warp == kMoeMmaWarp) {
     // ----------------------------------------------------------------------------------- MMA
     RingPos<Cfg::kAccs> ac;
     uint32_t set = 0;
@@ -835,16 +884,22 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     RingPos<Cfg::kAccs> ac;
     bool ok = true, digits = false;
     // digits of the hidden values, by tickets, between this CTA's last gate / up and first down
+    uint32_t eph = 0;
     auto make_digits = [&]() {
       digits = true;
       bool ready = false;
       while (true) {
-        const uint32_t k = moe_ticket(p.counters + kMoeDigits);
+        if (warp == kMoeEpiWarp0) {
+          const uint32_t k = moe_ticket(p.counters + kMoeDigits);
+          if (lane == 0) ctl.ticket = k;
+        }
+        if (!moe_epi_sync(ctl, eph, p.err)) return false;
+        const uint32_t k = *reinterpret_cast<volatile uint32_t*>(&ctl.ticket);
         if (k >= total_d) return true;
-        if (!ready && !moe_wait(p.counters + kMoeGateUpDone, sh.total1 * kMoeEpiWarps, ctl, p.err))
-          return false;
+        if (!ready && !moe_wait(p.counters + kMoeGateUpDone, sh.total1, ctl, p.err)) return false;
         ready = true;
-        const int b = static_cast<int>(k) * 32 + lane;  // blocks of a pair: a multiple of eight
+        // blocks of a pair: a multiple of eight
+        const int b = (static_cast<int>(k) * kMoeEpiWarps + warp - kMoeEpiWarp0) * 32 + lane;
         const int pr = b / blocks_h;
         if (pr < p.T * p.k && pl.used[pr]) {
           const int blk = b - pr * blocks_h;
@@ -862,7 +917,8 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
           moe_digits(v, p.hs + pr * moe_image_row(p.I), blk);
         }
         asm volatile("fence.proxy.async;" ::: "memory");
-        moe_count(p.counters + kMoeDigitsDone);
+        moe_count(p.counters + kMoeDigitsDone, &ctl.warps[1]);
+        if (!moe_epi_sync(ctl, eph, p.err)) return false;  // the ticket is read
       }
     };
     while ((ok = moe_next_task(t, q, ctl, p.err)) && t.phase != 2) {
@@ -874,49 +930,60 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
         if (!(ok = moe_warp_wait(ctl.acc_full[ac.slot], ac.phase, kErrWaitAccum, ctl, p.err))) break;
         tc_fence_after();
         const uint32_t acc = tb + lanes + ac.slot * 2 * Cfg::kN;
-        if (t.phase == 0) {
-          // tokens of this group of four warps: every other one
-          for (int c = group; c < n; c += 2) {
-            uint32_t ga[8], ua[8];
-            tmem_ld_x8(acc + c * kMoeDigitRows, ga);
-            tmem_ld_x8(acc + Cfg::kN + c * kMoeDigitRows, ua);
+        // the columns' sums into registers, then the accumulator is free. Up: this group of four warps
+        // takes every other token, both tiles; down: all tokens of its own tile.
+        const bool up = t.phase == 0;
+        float sum[TOK];
+#pragma unroll
+        for (int j = 0; j < TOK / 2; ++j) {
+          const int c = up ? 2 * j + group : 2 * j;
+          if (c < n && (up || group == 0 || gm.two)) {
+            uint32_t d0[8], d1[8];
+            tmem_ld_x8(acc + (up ? 0 : group * Cfg::kN) + c * kMoeDigitRows, d0);
+            tmem_ld_x8(acc + (up ? Cfg::kN + c * kMoeDigitRows
+                                 : group * Cfg::kN + (c + 1) * kMoeDigitRows), d1);
             tmem_ld_wait();
-            const int pr = pl.pairs[gm.off + n0 + c];
-            const float s = p.x_scale[pr / p.k] * ts13;
-            const float h = silu_rn(moe_sum8(ga) * s) * (moe_sum8(ua) * s) * (pl.w[pr] * ts2);
-            p.h[static_cast<int64_t>(pr) * p.I + gm.row0 + row] = h;
-            const uint32_t hm =
-                __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h) & 0x7FFFFFFFu);
-            if (lane == 0) atomicMax(p.hmax + pr, hm);
-          }
-        } else if (group == 0 || gm.two) {
-          for (int c = 0; c < n; ++c) {
-            uint32_t d[8];
-            tmem_ld_x8(acc + group * Cfg::kN + c * kMoeDigitRows, d);
-            tmem_ld_wait();
-            const int pr = pl.pairs[gm.off + n0 + c];
-            p.part[(static_cast<int64_t>(gm.z) * p.T * p.k + pr) * p.H + gm.row0 + 128 * group + row] =
-                moe_sum8(d) * moe_row_factor(__ldcg(p.hmax + pr));
+            sum[2 * j] = moe_sum8(d0);
+            sum[2 * j + 1] = moe_sum8(d1);
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&ctl.acc_empty[ac.slot]));
         ac.next();
+        if (up) {
+#pragma unroll
+          for (int j = 0; j < TOK / 2; ++j) {
+            const int c = 2 * j + group;
+            if (c >= n) break;
+            const int pr = pl.pairs[gm.off + n0 + c];
+            const float s = p.x_scale[pr / p.k] * ts13;
+            const float h = silu_rn(sum[2 * j] * s) * (sum[2 * j + 1] * s) * (pl.w[pr] * ts2);
+            p.h[static_cast<int64_t>(pr) * p.I + gm.row0 + row] = h;
+            const uint32_t hm =
+                __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h) & 0x7FFFFFFFu);
+            if (lane == 0) atomicMax(p.hmax + pr, hm);
+          }
+        } else if (group == 0 || gm.two) {
+#pragma unroll
+          for (int c = 0; c < TOK; ++c) {
+            if (c >= n) break;
+            const int pr = pl.pairs[gm.off + n0 + c];
+            p.part[(static_cast<int64_t>(gm.z) * p.T * p.k + pr) * p.H + gm.row0 + 128 * group + row] =
+                sum[c] * moe_row_factor(__ldcg(p.hmax + pr));
+          }
+        }
       }
       if (!ok) break;
-      moe_count(p.counters + (t.phase == 0 ? kMoeGateUpDone : kMoeDownDone));
+      moe_count(p.counters + (t.phase == 0 ? kMoeGateUpDone : kMoeDownDone), &ctl.warps[0]);
     }
     if (ok && !digits) ok = make_digits();
 
-    // combine: a warp task is 256 outputs of a token
+    // combine: 256 outputs of a token per warp and turn, dealt by index (no one waits for these)
     const int blocks3 = (p.H + 255) / 256;
-    bool ready = false;
-    while (ok) {
-      const uint32_t task = moe_ticket(p.counters + kMoeCombine);
-      if (task >= static_cast<uint32_t>(p.T * blocks3)) break;
-      if (!ready && !moe_wait(p.counters + kMoeDownDone, sh.total2 * kMoeEpiWarps, ctl, p.err)) break;
-      ready = true;
+    ok = ok && moe_wait(p.counters + kMoeDownDone, sh.total2, ctl, p.err);
+    for (int task = blockIdx.x + gridDim.x * (warp - kMoeEpiWarp0); ok && task < p.T * blocks3;
+         task += gridDim.x * kMoeEpiWarps) {
       const int tok = task / blocks3;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -946,7 +1013,7 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == kMoeMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tb, 512);
   }

@@ -22,12 +22,12 @@ struct MoeWs {
   size_t hmax, x_scale, xs, h, hs, part, total;
   int part_rows;
 };
-MoeWs moe_ws(int T, int H, int I, int k) {
+MoeWs moe_ws(int T, int H, int I, int E, int k) {
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   const size_t pairs = static_cast<size_t>(T) * k;
   MoeWs w;
   w.part_rows = std::max(T * k, kPartRows);
-  w.hmax = 256;
+  w.hmax = up(static_cast<size_t>(moe_counters(E)) * 4);
   w.x_scale = w.hmax + up(pairs * 4);
   w.xs = w.x_scale + up(static_cast<size_t>(T) * 4);
   w.h = w.xs + up(T * moe_image_row(H));
@@ -99,7 +99,7 @@ int check_experts(const void* y, const void* x, int x_dtype, int out_dtype, cons
   if (T == 0) return BD_OK;
   if (!y || !x || !ids || !weights || !a.w13 || !a.s13 || !a.ts13 || !a.w2 || !a.s2 || !a.ts2)
     return BD_ERR_INVALID_ARG;
-  if (!ws || ws_bytes < moe_ws(T, H, I, k).total) return BD_ERR_WORKSPACE;
+  if (!ws || ws_bytes < moe_ws(T, H, I, E, k).total) return BD_ERR_WORKSPACE;
   if (!aligned(ws, 256) || !aligned(x, 16) || !aligned(a.w13, 16) || !aligned(a.w2, 16) ||
       !aligned(a.s13, 4) || !aligned(a.s2, 4) || !aligned(a.ts13, 4) || !aligned(a.ts2, 4) ||
       !aligned(ids, 4) || !aligned(weights, 4) || !aligned(y, out_dtype == BD_OUT_F32 ? 4 : 2))
@@ -136,7 +136,7 @@ int launch_experts(const CUtensorMap& m13, const CUtensorMap& m2, const MoeExper
 int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
                 const MoeExpertArgs& a, int T, int H, int I, int E, int k, uint8_t* ws,
                 const DeviceInfo* d, cudaStream_t s) {
-  const MoeWs w = moe_ws(T, H, I, k);
+  const MoeWs w = moe_ws(T, H, I, E, k);
   MoeExpertsParams p;
   p.s13 = a.s13;
   p.s2 = a.s2;
@@ -180,7 +180,7 @@ extern "C" {
 
 size_t bd_query_moe_workspace(int T, int H, int I, int E, int top_k) {
   if (bad_shape(T, H, I, E, top_k) || T == 0) return 0;
-  return moe_ws(T, H, I, top_k).total;
+  return moe_ws(T, H, I, E, top_k).total;
 }
 
 int bd_moe_experts(void* y, const void* x, int x_dtype, const int* ids, const float* weights,
@@ -198,7 +198,7 @@ int bd_moe_experts(void* y, const void* x, int x_dtype, const int* ids, const fl
   st = device_info(&d);
   if (st != BD_OK) return st;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const MoeWs w = moe_ws(T, H, I, top_k);
+  const MoeWs w = moe_ws(T, H, I, E, top_k);
   uint32_t* counters = reinterpret_cast<uint32_t*>(ws);
   uint32_t* hmax = reinterpret_cast<uint32_t*>(ws + w.hmax);
   float* x_scale = reinterpret_cast<float*>(ws + w.x_scale);
@@ -209,9 +209,9 @@ int bd_moe_experts(void* y, const void* x, int x_dtype, const int* ids, const fl
       x_dtype == BD_IN_BF16
           ? cudaLaunchKernelEx(&cfg, moe_prepare_kernel<__nv_bfloat16>,
                                static_cast<const __nv_bfloat16*>(x), ws + w.xs, x_scale, hmax, counters,
-                               H, top_k)
+                               H, E, top_k)
           : cudaLaunchKernelEx(&cfg, moe_prepare_kernel<__half>, static_cast<const __half*>(x),
-                               ws + w.xs, x_scale, hmax, counters, H, top_k);
+                               ws + w.xs, x_scale, hmax, counters, H, E, top_k);
   if (e != cudaSuccess) return BD_ERR_CUDA;
   return run_experts(y, out_dtype, ids, weights, a, T, H, I, E, top_k, ws, d, s);
 }
@@ -237,7 +237,7 @@ int bd_moe_layer(void* y, int* ids, float* weights, const void* x, int x_dtype,
   st = device_info(&d);
   if (st != BD_OK) return st;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const MoeWs w = moe_ws(T, H, I, top_k);
+  const MoeWs w = moe_ws(T, H, I, E, top_k);
   MoeRouteParams p;
   p.x = x;
   p.router = router;

@@ -19,9 +19,10 @@
 // Kernel 1 (moe_route_kernel, or moe_prepare_kernel where the caller brings the routing): router
 // products, selection, digits of x, counters to zero.
 // Kernel 2 (moe_experts_kernel): gate / up, digits of the hidden values, down and combine phases in
-// one grid. Work is handed out by tickets (atomic counters), all tasks of a phase before those of
-// the next: a CTA that waits for a phase to finish knows that each of its tasks is held by a CTA
-// that already runs, so the wait ends without any guarantee that the whole grid is resident.
+// one grid. Work is handed out by tickets (atomic counters) in the order of the experts, and a task
+// waits only for the tasks of its own expert. All gate / up tickets go before the first down ticket,
+// and no gate / up task waits for anything: whatever a CTA waits for is held by a CTA that already
+// runs, so the waits end without any guarantee that the whole grid is resident.
 #pragma once
 #include <cstdint>
 
@@ -37,16 +38,17 @@ constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTopK = 16;
 constexpr int kMoeThreads = 512, kMoeWarps = kMoeThreads / 32;
 constexpr int kRouteCluster = 8;
 
-// Counters in the workspace, zeroed by the first kernel: tickets and finished tasks per phase.
+// Counters in the workspace, zeroed by the first kernel: tickets and finished tasks, then per touched
+// expert its finished gate / up tasks [E] and digit tasks [E].
 enum : int {
   kMoeGateUp = 0,
-  kMoeGateUpDone,
   kMoeDigits,
   kMoeDigitsDone,
   kMoeDown,
   kMoeDownDone,
   kMoeCounters
 };
+__host__ __device__ constexpr int moe_counters(int E) { return kMoeCounters + 2 * E; }
 
 // Digits of a row of K activations: per 256 elements the 8 x 128 bytes of codes (row p: digit p; rows
 // 6 and 7 are zero), 128B-swizzled as the MMA's operand tile, then 8 x 4 words of scales.
@@ -194,11 +196,12 @@ __device__ void moe_convert_token(const X* x, uint8_t* xs, float* x_scale, int t
 template <class X>
 __global__ void __launch_bounds__(kMoeThreads)
     moe_prepare_kernel(const X* x, uint8_t* xs, float* x_scale, uint32_t* hmax, uint32_t* counters,
-                       int H, int k) {
+                       int H, int E, int k) {
   __shared__ uint32_t part[kMoeWarps];
   grid_dep_launch_dependents();
   grid_dep_wait();
-  if (blockIdx.x == 0 && threadIdx.x < kMoeCounters) counters[threadIdx.x] = 0;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < moe_counters(E); i += kMoeThreads) counters[i] = 0;
   if (threadIdx.x < k) hmax[blockIdx.x * k + threadIdx.x] = 0;
   moe_convert_token(x, xs, x_scale, blockIdx.x, H, part);
 }
@@ -238,7 +241,8 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
   const W* wr = static_cast<const W*>(p.router);
   grid_dep_launch_dependents();
   grid_dep_wait();
-  if (blockIdx.x == 0 && threadIdx.x < kMoeCounters) p.counters[threadIdx.x] = 0;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < moe_counters(p.E); i += kMoeThreads) p.counters[i] = 0;
   cluster_sync_all();  // every CTA of the cluster runs: its shared memory may be written
   const int pieces = p.H / 8;
   for (int e = rank + kRouteCluster * warp; e < p.E; e += kRouteCluster * kMoeWarps) {
@@ -368,8 +372,10 @@ struct MoePlan {
   float w[kMoeMaxTokens * kMoeMaxTopK];         // weight of a pair
   uint8_t used[kMoeMaxTokens * kMoeMaxTopK];    // the pair counts
   uint32_t totals[kMoeMaxExperts / 32];         // experts << 16 | pairs of 32 experts
+  uint32_t dig[kMoeMaxExperts + 1];  // first digit task of a touched expert, and their number
   int nact;
 };
+constexpr int kMoeDigitBlocks = 256;  // 16-blocks of hidden values per digit task
 
 // Pairs by expert, by kThreads >= kMoeMaxExperts threads; pl.cnt is zero and visible before. A token
 // that names an expert twice keeps the first pair with the sum of the weights; ids outside [0, E) are
@@ -438,11 +444,40 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
     if (tid == kMoeMaxExperts - 1) pl.nact = end >> 16;
   }
   __syncthreads();
-  // the place of a pair within its expert's list is the order of arrival: it picks an MMA
-  // column, not a value
+  // a pair's place in its expert's list: by its number (every CTA has the same lists)
+  uint16_t* unsorted = reinterpret_cast<uint16_t*>(pl.id);
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
-    if (id[i] >= 0) pl.pairs[pl.off[id[i]] + pos[i]] = static_cast<uint16_t>(tid + i * kThreads);
+    if (id[i] >= 0) unsorted[pl.off[id[i]] + pos[i]] = static_cast<uint16_t>(tid + i * kThreads);
+  // digit tasks before each touched expert's
+  const int nact = pl.nact;
+  const int mine = tid < nact ? pl.cnt[pl.act[tid]] : 0;
+  const uint32_t tasks =
+      (static_cast<uint32_t>(mine) * (p.I / 16) + kMoeDigitBlocks - 1) / kMoeDigitBlocks;
+  uint32_t sum = tasks;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+    if (lane >= o) sum += u;
+  }
+  __syncthreads();  // totals is read
+  if (lane == 31 && warp < kMoeMaxExperts / 32) pl.totals[warp] = sum;
+  __syncthreads();
+  if (warp < kMoeMaxExperts / 32) {
+    uint32_t before = 0;
+    for (int i = 0; i < warp; ++i) before += pl.totals[i];
+    if (tid <= nact) pl.dig[tid] = before + sum - tasks;
+    if (tid + 1 == nact) pl.dig[nact] = before + sum;
+    if (nact == 0 && tid == 0) pl.dig[0] = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (id[i] >= 0) {
+      const int pr = tid + i * kThreads, o = pl.off[id[i]], n = pl.cnt[id[i]];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += unsorted[o + j] < pr ? 1 : 0;
+      pl.pairs[o + rank] = static_cast<uint16_t>(pr);
+    }
   __syncthreads();
 }
 
@@ -450,15 +485,15 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
 // all tokens of the expert, in passes of TOK tokens; K in stages of 256:
 //   gate / up: 128 hidden units, tile 0 the gate rows, tile 1 the up rows: lane i of both tiles is
 //              hidden unit i. h = silu(gate) up w ts in fp32, and the pair's maximum;
-//   digits:    h -> digits, once every h is there (their row factor needs the row's maximum);
+//   digits:    h -> digits, once every h of an expert is there (the row factor needs the row's
+//              maximum), by whichever epilogue warps come past;
 //   down:      256 output rows of one expert and a slice of I; partial sums per (slice, pair);
 //   combine:   y = the partial sums of a token's pairs in slot order.
 // Warps: 0 weight codes (takes the tickets and publishes the tasks in a queue), 1..4 weight scales
 // (64 rows each, 4-byte cp.async straight into the tiles tcgen05.cp wants: no repacking of the natural
-// layout), 5 activation digits, 6..8 their scales (5..8 wait for the digits phase before the first down
-// task, while the weights of the next stages already arrive; with one warp for 5..8 it was the
-// slowest role and the layer up to twice as slow), 9 MMA, 10..17 epilogue (and the digits and
-// combine phases). Two builds: TOK = 8 (four stages, accumulators double-buffered) where an expert has few
+// layout), 5 activation digits, 6..8 their scales (5..8 wait for the digits of a down task's expert,
+// while the weights of the next stages already arrive; with one warp for 5..8 it was the slowest role
+// and the layer up to twice as slow), 9 MMA, 10..17 epilogue (and the digits and combine phases). Two builds: TOK = 8 (four stages, accumulators double-buffered) where an expert has few
 // tokens, TOK = 24.
 constexpr int kMoeScaleWarps = 4, kMoeDigitScaleWarps = 3;
 constexpr int kMoeMmaWarp = 2 + kMoeScaleWarps + kMoeDigitScaleWarps;
@@ -489,8 +524,8 @@ struct MoeCfg {
 struct MoeCtl {
   uint64_t full[4], empty[4], acc_full[2], acc_empty[2], qfull[kMoeQueue], qempty[kMoeQueue], drain, ebar;
   uint32_t queue[kMoeQueue];
-  uint32_t abort_flag, tmem_base, ticket;
-  uint32_t warps[2];  // epilogue warps that finished a part of a task: products, digits
+  uint32_t abort_flag, tmem_base, ticket, ticket_expert;
+  uint32_t warps;  // epilogue warps that finished their part of a down task
 };
 constexpr int kMoeQueueReaders = kMoeEpiWarp0 - 1 + kMoeEpiWarps;
 
@@ -501,7 +536,7 @@ struct MoeTask {
 
 // Geometry of a task.
 struct MoeGeom {
-  int e, cnt, off;      // expert, its pairs
+  int a, e, cnt, off;   // touched expert, expert, its pairs
   int c0, c1;           // stages of K
   int K, row0, z;       // first hidden unit / output row, slice
   int64_t ra, rb;       // first weight rows of the two tiles
@@ -514,7 +549,8 @@ struct MoeShape {
                                           const MoeTask& t) const {
     MoeGeom g;
     if (t.phase == 0) {
-      g.e = pl.act[t.index / blocks1];
+      g.a = t.index / blocks1;
+      g.e = pl.act[g.a];
       g.row0 = (t.index % blocks1) * 128;
       g.z = 0;
       g.c0 = 0;
@@ -526,7 +562,8 @@ struct MoeShape {
     } else {
       const int ab = t.index / slices;
       g.z = t.index % slices;
-      g.e = pl.act[ab / blocks2];
+      g.a = ab / blocks2;
+      g.e = pl.act[g.a];
       g.row0 = (ab % blocks2) * 256;
       const int n = (p.I + 255) / 256;
       g.c0 = n * g.z / slices;
@@ -586,10 +623,9 @@ __device__ __forceinline__ uint32_t moe_ticket(uint32_t* counter) {
   if ((threadIdx.x & 31) == 0) k = atomicAdd(counter, 1u);
   return __shfl_sync(0xFFFFFFFFu, k, 0);
 }
-// An epilogue warp's part of a task is done: its stores before the count. The last of the eight
-// counts for the CTA (atomics on one address pass one after the other: eight times as many, and a
-// ticket per warp in the digits phase, held the phases up by 10 to 20 us).
-__device__ __forceinline__ void moe_count(uint32_t* counter, uint32_t* warps) {
+// An epilogue warp's part of a down task is done: its stores before the count. The last of eight
+// parts counts for the CTA (parts of two tasks may mix; the phase's total is what is waited for).
+__device__ __forceinline__ void moe_count_down(uint32_t* counter, uint32_t* warps) {
   __threadfence();
   __syncwarp();
   if ((threadIdx.x & 31) == 0 && (atomicAdd(warps, 1u) & (kMoeEpiWarps - 1)) == kMoeEpiWarps - 1) {
@@ -650,7 +686,7 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     }
     mbar_init(smem_u32(&ctl.drain), 1);
     mbar_init(smem_u32(&ctl.ebar), kMoeEpiWarps);
-    ctl.warps[0] = ctl.warps[1] = 0;
+    ctl.warps = 0;
     fence_mbar_init();
   }
   if (warp == kMoeMmaWarp) {
@@ -678,10 +714,10 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
          2 * sh.slices * p.T * p.k <= p.part_rows && p.I / 256 >= 2 * sh.slices)
     sh.slices *= 2;
   sh.total2 = static_cast<uint32_t>(nact) * sh.blocks2 * sh.slices;
-  // digits: a task is a 16-block of hidden values per epilogue thread, over all pairs
   const int blocks_h = p.I / 16;
-  const uint32_t total_d =
-      static_cast<uint32_t>(p.T * p.k * blocks_h + 32 * kMoeEpiWarps - 1) / (32 * kMoeEpiWarps);
+  const uint32_t total_d = pl.dig[nact];
+  uint32_t* gate_up_done = p.counters + kMoeCounters;
+  uint32_t* digits_done = gate_up_done + p.E;
 
   RingPos<kMoeQueue> q;
   RingPos<Cfg::kStages> r;
@@ -768,15 +804,15 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
   } else if (warp < kMoeMmaWarp) {
     // ------------------------------------------ activation digits: codes (warp 5), scales (6..8)
     const int part = warp - kMoeScaleWarps - 2;  // -1: codes
-    bool ready = false;
+    bool ready = false;  // the digits of all experts
     while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
+      const MoeGeom gm = sh.geom(p, pl, t);
       if (t.phase == 1 && !ready) {
-        if (!moe_wait(p.counters + kMoeDigitsDone, total_d, ctl, p.err)) break;
+        ready = __all_sync(0xFFFFFFFFu, ld_acquire_gpu(p.counters + kMoeDigitsDone) >= total_d);
+        if (!ready && !moe_wait(digits_done + gm.a, pl.dig[gm.a + 1] - pl.dig[gm.a], ctl, p.err)) break;
         // written by ordinary stores of this grid; the bulk copies read through the async proxy
         asm volatile("fence.proxy.async;" ::: "memory");
-        ready = true;
       }
-      const MoeGeom gm = sh.geom(p, pl, t);
       const uint8_t* base = t.phase == 0 ? p.xs : p.hs;
       bool ok = true;
       for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK) {
@@ -883,26 +919,47 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
     RingPos<Cfg::kAccs> ac;
     bool ok = true, digits = false;
-    // digits of the hidden values, by tickets, between this CTA's last gate / up and first down
     uint32_t eph = 0;
-    auto make_digits = [&]() {
-      digits = true;
-      bool ready = false;
-      while (true) {
-        if (warp == kMoeEpiWarp0) {
-          const uint32_t k = moe_ticket(p.counters + kMoeDigits);
-          if (lane == 0) ctl.ticket = k;
+    // A digit task by the eight warps, or none: with `wait` the next ticket, waiting for its expert's
+    // hidden values; else only if that expert has them all already. False when a wait ran out; none
+    // (ticket at or past the total) ends the caller's loop.
+    auto digit_task = [&](bool wait, bool& none) {
+      if (warp == kMoeEpiWarp0) {
+        uint32_t k = wait ? moe_ticket(p.counters + kMoeDigits)
+                          : __shfl_sync(0xFFFFFFFFu, ld_acquire_gpu(p.counters + kMoeDigits), 0);
+        int a = 0;
+        if (k < total_d) {
+          for (int lo = 0, hi = nact; hi - lo > 1;) {  // dig[a] <= k < dig[a + 1]
+            const int mid = (lo + hi) >> 1;
+            if (pl.dig[mid] <= k) lo = mid;
+            else hi = mid;
+            a = lo;
+          }
+          if (wait) {
+            if (!moe_wait(gate_up_done + a, sh.blocks1, ctl, p.err)) k = 0xFFFFFFFFu;
+          } else {
+            uint32_t got = k;
+            if (lane == 0)
+              got = ld_acquire_gpu(gate_up_done + a) < static_cast<uint32_t>(sh.blocks1)
+                        ? ~k
+                        : atomicCAS(p.counters + kMoeDigits, k, k + 1);
+            if (__shfl_sync(0xFFFFFFFFu, got, 0) != k) k = 0xFFFFFFFFu;
+          }
         }
-        if (!moe_epi_sync(ctl, eph, p.err)) return false;
-        const uint32_t k = *reinterpret_cast<volatile uint32_t*>(&ctl.ticket);
-        if (k >= total_d) return true;
-        if (!ready && !moe_wait(p.counters + kMoeGateUpDone, sh.total1, ctl, p.err)) return false;
-        ready = true;
-        // blocks of a pair: a multiple of eight
-        const int b = (static_cast<int>(k) * kMoeEpiWarps + warp - kMoeEpiWarp0) * 32 + lane;
-        const int pr = b / blocks_h;
-        if (pr < p.T * p.k && pl.used[pr]) {
-          const int blk = b - pr * blocks_h;
+        if (lane == 0) {
+          ctl.ticket = k;
+          ctl.ticket_expert = a;
+        }
+      }
+      if (!moe_epi_sync(ctl, eph, p.err)) return false;
+      const uint32_t k = *reinterpret_cast<volatile uint32_t*>(&ctl.ticket);
+      const int a = *reinterpret_cast<volatile uint32_t*>(&ctl.ticket_expert);
+      none = k >= total_d;
+      if (!none) {
+        const int e = pl.act[a];
+        const int b = static_cast<int>(k - pl.dig[a]) * kMoeDigitBlocks + 32 * (warp - kMoeEpiWarp0) + lane;
+        if (b < pl.cnt[e] * blocks_h) {  // a multiple of eight
+          const int pr = pl.pairs[pl.off[e] + b / blocks_h], blk = b % blocks_h;
           const float up = pow2f(moe_row_shift(__ldcg(p.hmax + pr)));
           const float* src = p.h + static_cast<int64_t>(pr) * p.I + 16 * blk;
           float v[16];
@@ -917,12 +974,24 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
           moe_digits(v, p.hs + pr * moe_image_row(p.I), blk);
         }
         asm volatile("fence.proxy.async;" ::: "memory");
-        moe_count(p.counters + kMoeDigitsDone, &ctl.warps[1]);
-        if (!moe_epi_sync(ctl, eph, p.err)) return false;  // the ticket is read
       }
+      if (!moe_epi_sync(ctl, eph, p.err)) return false;  // stored; the ticket is read
+      if (!none && tid == 32 * kMoeEpiWarp0) {
+        __threadfence();
+        atomicAdd(digits_done + a, 1u);
+        atomicAdd(p.counters + kMoeDigitsDone, 1u);
+      }
+      return true;
+    };
+    auto all_digits = [&]() {
+      digits = true;
+      bool none = false;
+      while (!none)
+        if (!digit_task(true, none)) return false;
+      return true;
     };
     while ((ok = moe_next_task(t, q, ctl, p.err)) && t.phase != 2) {
-      if (t.phase == 1 && !digits && !(ok = make_digits())) break;
+      if (t.phase == 1 && !digits && !(ok = all_digits())) break;
       const MoeGeom gm = sh.geom(p, pl, t);
       const float ts13 = p.ts13[gm.e], ts2 = p.ts2[gm.e];
       for (int n0 = 0; n0 < gm.cnt; n0 += TOK) {
@@ -975,9 +1044,20 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
         }
       }
       if (!ok) break;
-      moe_count(p.counters + (t.phase == 0 ? kMoeGateUpDone : kMoeDownDone), &ctl.warps[0]);
+      if (t.phase == 1) {
+        moe_count_down(p.counters + kMoeDownDone, &ctl.warps);
+        continue;
+      }
+      if (!(ok = moe_epi_sync(ctl, eph, p.err))) break;  // every warp's hidden values are stored
+      if (tid == 32 * kMoeEpiWarp0) {
+        __threadfence();
+        atomicAdd(gate_up_done + gm.a, 1u);
+      }
+      bool none = false;
+      for (int i = 0; i < 2 && !none && ok; ++i) ok = digit_task(false, none);
+      if (!ok) break;
     }
-    if (ok && !digits) ok = make_digits();
+    if (ok && !digits) ok = all_digits();
 
     // combine: 256 outputs of a token per warp and turn, dealt by index (no one waits for these)
     const int blocks3 = (p.H + 255) / 256;

@@ -78,14 +78,14 @@ def _check(x: torch.Tensor, w: MoeWeights, top_k: int):
     return T, H, inter, E
 
 
-def _workspace_bytes(T: int, H: int, inter: int, top_k: int) -> int:
+def _workspace_bytes(T: int, H: int, inter: int, E: int, top_k: int) -> int:
     """bd_query_moe_workspace without the call."""
     def up(v):
         return (v + 255) // 256 * 256
     if T == 0:
         return 0
     pairs = T * top_k
-    return 256 + up(4 * pairs) + up(4 * T) + up(T * ((H + 255) // 256) * 1152) + \
+    return up(4 * (5 + 2 * E)) + up(4 * pairs) + up(4 * T) + up(T * ((H + 255) // 256) * 1152) + \
         up(4 * pairs * inter) + up(pairs * ((inter + 255) // 256) * 1152) + 4 * H * max(pairs, 256)
 
 
@@ -120,7 +120,7 @@ def moe_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Ten
     _need(topk_weights, torch.float32, "topk_weights")
     with _on(stream, x.device):
         out = _out_tensor(out, x, out_dtype)
-        ws = torch.empty(_workspace_bytes(T, H, inter, top_k), dtype=torch.uint8, device=x.device)
+        ws = torch.empty(_workspace_bytes(T, H, inter, E, top_k), dtype=torch.uint8, device=x.device)
     call("bd_moe_experts", _p(out), _p(x), _IN_MOE[x.dtype], _p(topk_ids), _p(topk_weights),
          *_weight_args(experts), T, H, inter, E, top_k, _OUT[out.dtype], _p(ws), ws.numel(),
          _stream(stream))
@@ -152,7 +152,7 @@ def moe_layer(x: torch.Tensor, router: torch.Tensor, experts: MoeWeights, top_k:
         out = _out_tensor(out, x, out_dtype)
         ids = torch.empty((T, top_k), dtype=torch.int32, device=x.device)
         weights = torch.empty((T, top_k), dtype=torch.float32, device=x.device)
-        ws = torch.empty(_workspace_bytes(T, H, inter, top_k), dtype=torch.uint8, device=x.device)
+        ws = torch.empty(_workspace_bytes(T, H, inter, E, top_k), dtype=torch.uint8, device=x.device)
     call("bd_moe_layer", _p(out), _p(ids), _p(weights), _p(x), _IN_MOE[x.dtype], _p(router),
          _IN_MOE[router.dtype], _p(selection_bias), SCORINGS[scoring], 1 if renormalize else 0,
          float(routed_scale), *_weight_args(experts), T, H, inter, E, top_k, _OUT[out.dtype],

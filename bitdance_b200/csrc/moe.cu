@@ -101,7 +101,7 @@ int check_experts(const void* y, const void* x, int x_dtype, int out_dtype, cons
     return BD_ERR_INVALID_ARG;
   if (!ws || ws_bytes < moe_ws(T, H, I, E, k).total) return BD_ERR_WORKSPACE;
   if (!aligned(ws, 256) || !aligned(x, 16) || !aligned(a.w13, 16) || !aligned(a.w2, 16) ||
-      !aligned(a.s13, 4) || !aligned(a.s2, 4) || !aligned(a.ts13, 4) || !aligned(a.ts2, 4) ||
+      !aligned(a.s13, 8) || !aligned(a.s2, 8) || !aligned(a.ts13, 4) || !aligned(a.ts2, 4) ||
       !aligned(ids, 4) || !aligned(weights, 4) || !aligned(y, out_dtype == BD_OUT_F32 ? 4 : 2))
     return BD_ERR_ALIGNMENT;
   return BD_OK;

@@ -490,12 +490,13 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
 //   down:      256 output rows of one expert and a slice of I; partial sums per (slice, pair);
 //   combine:   y = the partial sums of a token's pairs in slot order.
 // Warps: 0 weight codes (takes the tickets and publishes the tasks in a queue), 1..4 weight scales
-// (64 rows each, 4-byte cp.async straight into the tiles tcgen05.cp wants: no repacking of the natural
-// layout), 5 activation digits, 6..8 their scales (5..8 wait for the digits of a down task's expert,
-// while the weights of the next stages already arrive; with one warp for 5..8 it was the slowest role
-// and the layer up to twice as slow), 9 MMA, 10..17 epilogue (and the digits and combine phases). Two builds: TOK = 8 (four stages, accumulators double-buffered) where an expert has few
+// (64 rows each: from the natural layout through registers, three stages ahead, to the tiles
+// tcgen05.cp wants; 4-byte cp.async took 26 shared-memory cycles an instruction, 1300 of a stage's
+// 2000 cycles), 5 activation digits, 6..9 their scales (5..9 wait for the digits of a down task's
+// expert, while the weights of the next stages already arrive), 10 MMA, 11..18 epilogue (and the
+// digits and combine phases). Two builds: TOK = 8 (four stages, accumulators double-buffered) where an expert has few
 // tokens, TOK = 24.
-constexpr int kMoeScaleWarps = 4, kMoeDigitScaleWarps = 3;
+constexpr int kMoeScaleWarps = 4, kMoeDigitScaleWarps = 4;
 constexpr int kMoeMmaWarp = 2 + kMoeScaleWarps + kMoeDigitScaleWarps;
 constexpr int kMoeEpiWarp0 = kMoeMmaWarp + 1, kMoeEpiWarps = 8;
 constexpr int kMoeExpertThreads = 32 * (kMoeEpiWarp0 + kMoeEpiWarps);
@@ -517,8 +518,8 @@ struct MoeCfg {
   static constexpr int kSfSet = 2 * 16 + kBlocks * 16;       // scale words of a stage in tensor memory
   static_assert(kSfCol0 + 2 * kSfSet <= 512, "tensor memory budget");
   static_assert(kStage % 1024 == 0 && oB % 1024 == 0, "1 KB swizzle atoms");
-  // a full stage: the code and digit copies' tx arrives, the scale warps' lanes
-  static constexpr int kFullCount = 2 + 32 * (kMoeScaleWarps + kMoeDigitScaleWarps);
+  // a full stage: the code and digit copies' tx arrives, the scale warps
+  static constexpr int kFullCount = 2 + kMoeScaleWarps + kMoeDigitScaleWarps;
 };
 
 struct MoeCtl {
@@ -652,12 +653,20 @@ __device__ __forceinline__ float moe_sum8(const uint32_t* r) {
   return s;
 }
 
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+// Four scale words (a row's 16 scales of a stage) into their tiles, 512 bytes apart.
+__device__ __forceinline__ void moe_store_scales(uint32_t dst, const uint2& lo, const uint2& hi) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(lo.x) : "memory");
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + 512), "r"(lo.y) : "memory");
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + 1024), "r"(hi.x) : "memory");
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + 1536), "r"(hi.y) : "memory");
 }
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+// A scale warp's part of a stage is stored: the tensor core reads it through the async proxy.
+__device__ __forceinline__ void moe_scales_ready(uint64_t& full) {
+  fence_proxy_async_smem();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&full));
 }
+constexpr int kMoeAhead = 3;  // stages whose scales are in registers
 
 template <int TOK>
 __global__ void __launch_bounds__(kMoeExpertThreads, 1)
@@ -775,35 +784,57 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     }
   } else if (warp <= kMoeScaleWarps) {
     // ------------------------------------------------- weight scales: half the rows of a tile
-    const int m = (warp - 1) >> 1, r0 = ((warp - 1) & 1) * 64 + (lane >> 2);
+    // Lane (i, j) = (lane / 8, lane % 8) holds rows 32 i + 16 h + j and + 8, h the half: the four
+    // row groups of one j are side by side in a tile, so the stores have no bank conflicts.
+    const int m = (warp - 1) >> 1;
+    const int row = 32 * (lane >> 3) + 16 * ((warp - 1) & 1) + (lane & 7);
+    const uint32_t at = Cfg::oSw + m * 2048 + (row & 31) * 16 + (row >> 5) * 4;
     while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
       const MoeGeom gm = sh.geom(p, pl, t);
-      const int w = lane & 3;
-      const uint8_t* src0 = (t.phase == 0 ? p.s13 : p.s2) +
-                            ((m == 0 ? gm.ra : gm.rb) + r0) * (gm.K / 16) + 4 * w;
-      bool ok = true;
-      for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK)
-        for (int c = gm.c0; c < gm.c1; ++c) {
-          if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
-          if ((m == 0 || gm.two) && c * 4 + w < gm.K / 64) {
-            const uint32_t dst =
-                smem_u32(smem + r.slot * Cfg::kStage + Cfg::oSw + (m * 4 + w) * 512);
-            const uint8_t* src = src0 + c * 16;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int row = r0 + 8 * i;
-              cp_async4(dst + (row & 31) * 16 + (row >> 5) * 4, src + 8 * i * (gm.K / 16));
-            }
+      const int pitch = gm.K / 16;
+      const uint8_t* src = (t.phase == 0 ? p.s13 : p.s2) + ((m == 0 ? gm.ra : gm.rb) + row) * pitch;
+      const bool have = m == 0 || gm.two;
+      uint2 w[kMoeAhead][4];
+      auto load = [&](uint2 (&v)[4], int c) {  // 16 scales of two rows, the last stage maybe 8
+        const uint2* s0 = reinterpret_cast<const uint2*>(src + c * 16);
+        const uint2* s1 = reinterpret_cast<const uint2*>(src + 8 * pitch + c * 16);
+        if (have && c < gm.c1) {
+          v[0] = __ldg(s0);
+          v[2] = __ldg(s1);
+          if (c * 16 + 8 < pitch) {
+            v[1] = __ldg(s0 + 1);
+            v[3] = __ldg(s1 + 1);
           }
-          cp_async_arrive(smem_u32(&ctl.full[r.slot]));
-          r.next();
         }
+      };
+      bool ok = true;
+      for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK) {
+#pragma unroll
+        for (int j = 0; j < kMoeAhead; ++j) load(w[j], gm.c0 + j);
+        for (int c0 = gm.c0; c0 < gm.c1 && ok; c0 += kMoeAhead) {
+#pragma unroll
+          for (int j = 0; j < kMoeAhead; ++j) {
+            if (c0 + j >= gm.c1) break;
+            if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
+            const uint32_t dst = smem_u32(smem + r.slot * Cfg::kStage) + at;
+            if (have) {
+              moe_store_scales(dst, w[j][0], w[j][1]);
+              moe_store_scales(dst + 128, w[j][2], w[j][3]);
+            }
+            moe_scales_ready(ctl.full[r.slot]);
+            load(w[j], c0 + j + kMoeAhead);
+            r.next();
+          }
+        }
+      }
       if (!ok) break;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp < kMoeMmaWarp) {
-    // ------------------------------------------ activation digits: codes (warp 5), scales (6..8)
+    // ------------------------------------------ activation digits: codes (warp 5), scales (6..9)
+    // Scale warp `part`: tokens part + 4 i (+ 16), lane = 8 i + digit: again the four row groups of a
+    // line side by side.
     const int part = warp - kMoeScaleWarps - 2;  // -1: codes
+    constexpr int kSets = Cfg::kBlocks;
     bool ready = false;  // the digits of all experts
     while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
       const MoeGeom gm = sh.geom(p, pl, t);
@@ -817,42 +848,59 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
       bool ok = true;
       for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK) {
         const int n = min(gm.cnt - n0, TOK);
-        int64_t at = 0;  // this lane's token
-        if (lane < n) {
-          const int pr = pl.pairs[gm.off + n0 + lane];
-          at = (t.phase == 0 ? pr / p.k : pr) * moe_image_row(gm.K);
-        }
-        for (int c = gm.c0; c < gm.c1; ++c) {
-          if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
-          const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
-          const uint32_t fb = smem_u32(&ctl.full[r.slot]);
-          const uint8_t* src = base + static_cast<int64_t>(c) * kMoeChunk;
-          if (part < 0) {
+        auto image = [&](int i) {
+          const int pr = pl.pairs[gm.off + n0 + i];
+          return base + (t.phase == 0 ? pr / p.k : pr) * moe_image_row(gm.K);
+        };
+        if (part < 0) {
+          const uint8_t* src = lane < n ? image(lane) : nullptr;
+          for (int c = gm.c0; c < gm.c1; ++c) {
+            if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
+            const uint32_t fb = smem_u32(&ctl.full[r.slot]);
             if (lane == 0) mbar_arrive_expect_tx(fb, n * kMoeChunkCodes);
             __syncwarp();
             if (lane < n)
-              bulk_load(st + Cfg::oB + lane * kMoeChunkCodes, src + at, kMoeChunkCodes, fb);
-          } else {
-            // scale words of token i: lane = 4 digit + word
-            const bool in = c * 4 + (lane & 3) < gm.K / 64;
-#pragma unroll
-            for (int j = 0; j < TOK / kMoeDigitScaleWarps + 1; ++j) {
-              const int i = part + j * kMoeDigitScaleWarps;
-              const int64_t ai = __shfl_sync(0xFFFFFFFFu, at, i & 31);
-              const int row = i * kMoeDigitRows + (lane >> 2);
-              if (i < n && in)
-                cp_async4(st + Cfg::oSb + (row >> 7) * 2048 + (lane & 3) * 512 + (row & 31) * 16 +
-                              ((row >> 5) & 3) * 4,
-                          src + ai + kMoeChunkCodes + 4 * lane);
-            }
-            cp_async_arrive(fb);
+              bulk_load(smem_u32(smem + r.slot * Cfg::kStage) + Cfg::oB + lane * kMoeChunkCodes,
+                        src + static_cast<int64_t>(c) * kMoeChunk, kMoeChunkCodes, fb);
+            r.next();
           }
-          r.next();
+          continue;
+        }
+        const uint8_t* src[kSets];
+        uint32_t at[kSets];
+        uint4 w[kMoeAhead][kSets];
+#pragma unroll
+        for (int k = 0; k < kSets; ++k) {
+          const int i = 16 * k + part + 4 * (lane >> 3);
+          src[k] = i < n && i < TOK ? image(i) + kMoeChunkCodes + 16 * (lane & 7) : nullptr;
+          at[k] = Cfg::oSb + k * 2048 + (part * 8 + (lane & 7)) * 16 + (lane >> 3) * 4;
+        }
+        auto load = [&](uint4 (&v)[kSets], int c) {
+#pragma unroll
+          for (int k = 0; k < kSets; ++k)
+            if (src[k] != nullptr && c < gm.c1) v[k] = ld_cg(src[k] + static_cast<int64_t>(c) * kMoeChunk);
+        };
+#pragma unroll
+        for (int j = 0; j < kMoeAhead; ++j) load(w[j], gm.c0 + j);
+        for (int c0 = gm.c0; c0 < gm.c1 && ok; c0 += kMoeAhead) {
+#pragma unroll
+          for (int j = 0; j < kMoeAhead; ++j) {
+            if (c0 + j >= gm.c1) break;
+            if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
+            const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
+#pragma unroll
+            for (int k = 0; k < kSets; ++k)
+              if (src[k] != nullptr)
+                moe_store_scales(st + at[k], make_uint2(w[j][k].x, w[j][k].y),
+                                 make_uint2(w[j][k].z, w[j][k].w));
+            moe_scales_ready(ctl.full[r.slot]);
+            load(w[j], c0 + j + kMoeAhead);
+            r.next();
+          }
         }
       }
       if (!ok) break;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kMoeMmaWarp) {
     // ----------------------------------------------------------------------------------- MMA
     RingPos<Cfg::kAccs> ac;
@@ -871,8 +919,6 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
         const uint32_t acc = tb + ac.slot * 2 * Cfg::kN;
         for (int c = gm.c0; c < gm.c1; ++c) {
           if (!(ok = moe_warp_wait(ctl.full[r.slot], r.phase, kErrWaitTma, ctl, p.err))) break;
-          // the scales were written by cp.async (generic proxy): before tcgen05.cp reads them
-          fence_proxy_async_smem();
           tc_fence_after();
           const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
           const uint32_t sf = tb + Cfg::kSfCol0 + set * Cfg::kSfSet;
@@ -1059,30 +1105,33 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     }
     if (ok && !digits) ok = all_digits();
 
-    // combine: 256 outputs of a token per warp and turn, dealt by index (no one waits for these)
-    const int blocks3 = (p.H + 255) / 256;
+    // combine: 128 outputs of a token per warp and turn, dealt by index (no one waits for these),
+    // eight partial sums in flight
+    const int blocks3 = p.H / 128, terms = p.k * sh.slices;
     ok = ok && moe_wait(p.counters + kMoeDownDone, sh.total2, ctl, p.err);
     for (int task = blockIdx.x + gridDim.x * (warp - kMoeEpiWarp0); ok && task < p.T * blocks3;
          task += gridDim.x * kMoeEpiWarps) {
-      const int tok = task / blocks3;
+      const int tok = task / blocks3, h0 = (task % blocks3) * 128 + 4 * lane;
+      float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i0 = 0; i0 < terms; i0 += 8) {
+        uint4 v[8];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int h0 = (task % blocks3) * 256 + half * 128 + 4 * lane;
-        if (h0 >= p.H) break;
-        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < p.k; ++s) {
+        for (int j = 0; j < 8; ++j) {
+          const int i = i0 + j, s = i / sh.slices, z = i - s * sh.slices;
           const int pr = tok * p.k + s;
-          if (!pl.used[pr]) continue;
-          for (int z = 0; z < sh.slices; ++z) {
-            const uint4 v = ld_cg(p.part + (static_cast<int64_t>(z) * p.T * p.k + pr) * p.H + h0);
-            o[0] += __uint_as_float(v.x);
-            o[1] += __uint_as_float(v.y);
-            o[2] += __uint_as_float(v.z);
-            o[3] += __uint_as_float(v.w);
-          }
+          v[j] = i < terms && pl.used[pr]
+                     ? ld_cg(p.part + (static_cast<int64_t>(z) * p.T * p.k + pr) * p.H + h0)
+                     : make_uint4(0, 0, 0, 0);
         }
-        store_row<4>(p.y, static_cast<int64_t>(tok) * p.H + h0, o, p.out_dtype, p.vec_out);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          o[0] += __uint_as_float(v[j].x);
+          o[1] += __uint_as_float(v[j].y);
+          o[2] += __uint_as_float(v[j].z);
+          o[3] += __uint_as_float(v[j].w);
+        }
       }
+      store_row<4>(p.y, static_cast<int64_t>(tok) * p.H + h0, o, p.out_dtype, p.vec_out);
     }
   }
   // ------------------------------------------------------------------------------- teardown

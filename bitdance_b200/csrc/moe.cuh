@@ -489,15 +489,16 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
 //              maximum), by whichever epilogue warps come past;
 //   down:      256 output rows of one expert and a slice of I; partial sums per (slice, pair);
 //   combine:   y = the partial sums of a token's pairs in slot order.
-// Warps: 0 weight codes (takes the tickets and publishes the tasks in a queue), 1..4 weight scales
-// (64 rows each: from the natural layout through registers, three stages ahead, to the tiles
-// tcgen05.cp wants; 4-byte cp.async took 26 shared-memory cycles an instruction, 1300 of a stage's
-// 2000 cycles), 5 activation digits, 6..9 their scales (5..9 wait for the digits of a down task's
-// expert, while the weights of the next stages already arrive), 10 MMA, 11..18 epilogue (and the
-// digits and combine phases). Two builds: TOK = 8 (four stages, accumulators double-buffered) where an expert has few
+// Warps: 0 weight codes (takes the tickets and publishes the tasks in a queue), 1 weight scales as they
+// are (cp.async, 16 bytes a row), 2..5 these into the tiles tcgen05.cp wants, 64 rows each (4-byte
+// cp.async straight into the tiles took 26 shared-memory cycles an instruction, 1300 of a stage's
+// 2000 cycles; loads to registers three stages ahead did not cover the memory's latency), 6 activation
+// digits, 7..10 their scales (6..10 wait for the digits of a down task's expert, while the weights of
+// the next stages already arrive), 11 MMA, 12..19 epilogue (and the digits and combine phases). Two builds: TOK = 8 (four stages, accumulators double-buffered) where an expert has few
 // tokens, TOK = 24.
 constexpr int kMoeScaleWarps = 4, kMoeDigitScaleWarps = 4;
-constexpr int kMoeMmaWarp = 2 + kMoeScaleWarps + kMoeDigitScaleWarps;
+constexpr int kMoeDigitWarp = 2 + kMoeScaleWarps;
+constexpr int kMoeMmaWarp = kMoeDigitWarp + 1 + kMoeDigitScaleWarps;
 constexpr int kMoeEpiWarp0 = kMoeMmaWarp + 1, kMoeEpiWarps = 8;
 constexpr int kMoeExpertThreads = 32 * (kMoeEpiWarp0 + kMoeEpiWarps);
 constexpr int kMoeQueue = 4;
@@ -512,7 +513,9 @@ struct MoeCfg {
   static constexpr int oSb = oB + TOK * kMoeChunkCodes;      // digit scales [block][word][512]
   static constexpr int kStage = oSb + kBlocks * 4 * 512;
   static constexpr int kStages = TOK <= 8 ? 4 : 3;
-  static constexpr int kSmem = kStages * kStage + 1024;
+  static constexpr int kRaw = 256 * 16;                      // natural weight scales of a stage
+  static constexpr int oRaw = kStages * kStage;
+  static constexpr int kSmem = oRaw + kStages * kRaw + 1024;
   static constexpr int kAccs = TOK <= 8 ? 2 : 1;             // accumulator pairs
   static constexpr int kSfCol0 = kAccs * 2 * kN;
   static constexpr int kSfSet = 2 * 16 + kBlocks * 16;       // scale words of a stage in tensor memory
@@ -523,7 +526,7 @@ struct MoeCfg {
 };
 
 struct MoeCtl {
-  uint64_t full[4], empty[4], acc_full[2], acc_empty[2], qfull[kMoeQueue], qempty[kMoeQueue], drain, ebar;
+  uint64_t full[4], empty[4], raw_full[4], raw_empty[4], acc_full[2], acc_empty[2], qfull[kMoeQueue], qempty[kMoeQueue], drain, ebar;
   uint32_t queue[kMoeQueue];
   uint32_t abort_flag, tmem_base, ticket, ticket_expert;
   uint32_t warps;  // epilogue warps that finished their part of a down task
@@ -684,6 +687,8 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     for (int s = 0; s < Cfg::kStages; ++s) {
       mbar_init(smem_u32(&ctl.full[s]), Cfg::kFullCount);
       mbar_init(smem_u32(&ctl.empty[s]), 1);
+      mbar_init(smem_u32(&ctl.raw_full[s]), 32);
+      mbar_init(smem_u32(&ctl.raw_empty[s]), kMoeScaleWarps);
     }
     for (int s = 0; s < Cfg::kAccs; ++s) {
       mbar_init(smem_u32(&ctl.acc_full[s]), 1);
@@ -782,58 +787,70 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
           r.next();
         }
     }
-  } else if (warp <= kMoeScaleWarps) {
-    // ------------------------------------------------- weight scales: half the rows of a tile
-    // Lane (i, j) = (lane / 8, lane % 8) holds rows 32 i + 16 h + j and + 8, h the half: the four
-    // row groups of one j are side by side in a tile, so the stores have no bank conflicts.
-    const int m = (warp - 1) >> 1;
-    const int row = 32 * (lane >> 3) + 16 * ((warp - 1) & 1) + (lane & 7);
+  } else if (warp == 1) {
+    // --------------------------------------------------------- weight scales, natural, 16 bytes a row
+    while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
+      const MoeGeom gm = sh.geom(p, pl, t);
+      const int pitch = gm.K / 16, half = 8 * (lane & 1);
+      const uint8_t* base = (t.phase == 0 ? p.s13 : p.s2) + (lane >> 1) * pitch + half;
+      const uint8_t *sa = base + gm.ra * pitch, *sb = base + gm.rb * pitch;
+      bool ok = true;
+      for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK)
+        for (int c = gm.c0; c < gm.c1; ++c) {
+          if (!(ok = moe_warp_wait(ctl.raw_empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
+          if (c * 16 + half < pitch) {  // the last stage may have 8 scales a row
+            const uint32_t dst = smem_u32(smem + Cfg::oRaw + r.slot * Cfg::kRaw) + 8 * lane;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + 256 * i),
+                           "l"(sa + c * 16 + 16 * i * pitch)
+                           : "memory");
+              if (gm.two)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + 2048 + 256 * i),
+                             "l"(sb + c * 16 + 16 * i * pitch)
+                             : "memory");
+            }
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
+                           smem_u32(&ctl.raw_full[r.slot]))
+                       : "memory");
+          r.next();
+        }
+      if (!ok) break;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp < kMoeDigitWarp) {
+    // ---------------------------------------- weight scales into their tiles: half the rows of a tile
+    // Lane (i, j) = (lane / 8, lane % 8) takes rows 32 i + 16 h + j and + 8, h the half: the four row
+    // groups of one j are side by side in a tile, so neither loads nor stores have bank conflicts.
+    const int m = (warp - 2) >> 1;
+    const int row = 32 * (lane >> 3) + 16 * (warp & 1) + (lane & 7);
     const uint32_t at = Cfg::oSw + m * 2048 + (row & 31) * 16 + (row >> 5) * 4;
     while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
       const MoeGeom gm = sh.geom(p, pl, t);
-      const int pitch = gm.K / 16;
-      const uint8_t* src = (t.phase == 0 ? p.s13 : p.s2) + ((m == 0 ? gm.ra : gm.rb) + row) * pitch;
-      const bool have = m == 0 || gm.two;
-      uint2 w[kMoeAhead][4];
-      auto load = [&](uint2 (&v)[4], int c) {  // 16 scales of two rows, the last stage maybe 8
-        const uint2* s0 = reinterpret_cast<const uint2*>(src + c * 16);
-        const uint2* s1 = reinterpret_cast<const uint2*>(src + 8 * pitch + c * 16);
-        if (have && c < gm.c1) {
-          v[0] = __ldg(s0);
-          v[2] = __ldg(s1);
-          if (c * 16 + 8 < pitch) {
-            v[1] = __ldg(s0 + 1);
-            v[3] = __ldg(s1 + 1);
-          }
-        }
-      };
       bool ok = true;
-      for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK) {
-#pragma unroll
-        for (int j = 0; j < kMoeAhead; ++j) load(w[j], gm.c0 + j);
-        for (int c0 = gm.c0; c0 < gm.c1 && ok; c0 += kMoeAhead) {
-#pragma unroll
-          for (int j = 0; j < kMoeAhead; ++j) {
-            if (c0 + j >= gm.c1) break;
-            if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
-            const uint32_t dst = smem_u32(smem + r.slot * Cfg::kStage) + at;
-            if (have) {
-              moe_store_scales(dst, w[j][0], w[j][1]);
-              moe_store_scales(dst + 128, w[j][2], w[j][3]);
-            }
-            moe_scales_ready(ctl.full[r.slot]);
-            load(w[j], c0 + j + kMoeAhead);
-            r.next();
-          }
+      for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK)
+        for (int c = gm.c0; c < gm.c1; ++c) {
+          if (!(ok = moe_warp_wait(ctl.raw_full[r.slot], r.phase, kErrWaitTma, ctl, p.err))) break;
+          const uint8_t* raw = smem + Cfg::oRaw + r.slot * Cfg::kRaw + m * 2048 + row * 16;
+          const uint4 lo = *reinterpret_cast<const uint4*>(raw);
+          const uint4 hi = *reinterpret_cast<const uint4*>(raw + 128);
+          if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
+          const uint32_t dst = smem_u32(smem + r.slot * Cfg::kStage) + at;
+          moe_store_scales(dst, make_uint2(lo.x, lo.y), make_uint2(lo.z, lo.w));
+          moe_store_scales(dst + 128, make_uint2(hi.x, hi.y), make_uint2(hi.z, hi.w));
+          moe_scales_ready(ctl.full[r.slot]);
+          // (the stores depend on the loads: the raw slot is read)
+          if (lane == 0) mbar_arrive(smem_u32(&ctl.raw_empty[r.slot]));
+          r.next();
         }
-      }
       if (!ok) break;
     }
   } else if (warp < kMoeMmaWarp) {
-    // ------------------------------------------ activation digits: codes (warp 5), scales (6..9)
+    // ----------------------------------------- activation digits: codes (warp 6), scales (7..10)
     // Scale warp `part`: tokens part + 4 i (+ 16), lane = 8 i + digit: again the four row groups of a
     // line side by side.
-    const int part = warp - kMoeScaleWarps - 2;  // -1: codes
+    const int part = warp - kMoeDigitWarp - 1;  // -1: codes
     constexpr int kSets = Cfg::kBlocks;
     bool ready = false;  // the digits of all experts
     while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {

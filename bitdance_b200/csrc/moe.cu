@@ -165,10 +165,10 @@ int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
   if (!codes_map(&m13, a.w13, static_cast<int64_t>(E) * 2 * I, H) ||
       !codes_map(&m2, a.w2, static_cast<int64_t>(E) * H, I))
     return BD_ERR_CUDA;
-  // passes of 8 tokens (deeper weight ring) where an expert is expected to have few, of 24 else;
-  // an expert with more takes several passes either way
-  return T <= 8 || T * k <= 4 * E ? launch_experts<8>(m13, m2, p, d, s)
-                                  : launch_experts<24>(m13, m2, p, d, s);
+  // passes of 16 tokens (half the MMAs) where an expert is expected to have at most about ten, of 24
+  // else; an expert with more takes several passes either way
+  return T <= 16 || T * k <= 10 * E ? launch_experts<16>(m13, m2, p, d, s)
+                                    : launch_experts<24>(m13, m2, p, d, s);
 }
 
 }  // namespace

@@ -375,7 +375,7 @@ struct MoePlan {
   uint32_t dig[kMoeMaxExperts + 1];  // first digit task of a touched expert, and their number
   int nact;
 };
-constexpr int kMoeDigitBlocks = 256;  // 16-blocks of hidden values per digit task
+constexpr int kMoeDigitBlocks = 64;  // 16-blocks of hidden values per digit task
 
 // Pairs by expert, by kThreads >= kMoeMaxExperts threads; pl.cnt is zero and visible before. A token
 // that names an expert twice keeps the first pair with the sum of the weights; ids outside [0, E) are
@@ -486,52 +486,58 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
 //   gate / up: 128 hidden units, tile 0 the gate rows, tile 1 the up rows: lane i of both tiles is
 //              hidden unit i. h = silu(gate) up w ts in fp32, and the pair's maximum;
 //   digits:    h -> digits, once every h of an expert is there (the row factor needs the row's
-//              maximum), by whichever epilogue warps come past;
+//              maximum);
 //   down:      256 output rows of one expert and a slice of I; partial sums per (slice, pair);
 //   combine:   y = the partial sums of a token's pairs in slot order.
-// Warps: 0 weight codes (takes the tickets and publishes the tasks in a queue), 1 weight scales as they
-// are (cp.async, 16 bytes a row), 2..5 these into the tiles tcgen05.cp wants, 64 rows each (4-byte
-// cp.async straight into the tiles took 26 shared-memory cycles an instruction, 1300 of a stage's
-// 2000 cycles; loads to registers three stages ahead did not cover the memory's latency), 6 activation
-// digits, 7..10 their scales (6..10 wait for the digits of a down task's expert, while the weights of
-// the next stages already arrive), 11 MMA, 12..19 epilogue (and the digits and combine phases). Two builds: TOK = 8 (four stages, accumulators double-buffered) where an expert has few
-// tokens, TOK = 24.
-constexpr int kMoeScaleWarps = 4, kMoeDigitScaleWarps = 4;
-constexpr int kMoeDigitWarp = 2 + kMoeScaleWarps;
-constexpr int kMoeMmaWarp = kMoeDigitWarp + 1 + kMoeDigitScaleWarps;
-constexpr int kMoeEpiWarp0 = kMoeMmaWarp + 1, kMoeEpiWarps = 8;
+// Warps: 0 weight codes (TMA) and scales as they are (cp.async, 16 bytes a row); it takes the tickets
+// and publishes the tasks in a queue. 1..4 the scales into the tiles tcgen05.cp wants, 64 rows each
+// (4-byte cp.async straight into the tiles took 26 shared-memory cycles an instruction, 1300 of a
+// stage's 2000 cycles; loads to registers three stages ahead did not cover the memory's latency).
+// 5..8 activation digits, waiting for those of a down task's expert while the weights of the next
+// stages already arrive. 9 MMA. 10, 11 digits of the hidden values, as experts finish. 12..19 epilogue
+// and combine.
+// An MMA of this kind takes the same time (about 128 cycles) for 16 columns as for 256, so the weights
+// are its 256 columns and the digits its 128 rows where a pass has at most 16 tokens (kSwap: half the
+// MMAs a stage; the digits' sum then runs over lanes); with 24 tokens a pass the weights are two
+// tiles of 128 rows and the digits 192 columns.
+constexpr int kMoeScaleWarp0 = 1, kMoeScaleWarps = 4;
+constexpr int kMoeDigitWarp0 = kMoeScaleWarp0 + kMoeScaleWarps, kMoeDigitWarps = 4;
+constexpr int kMoeMmaWarp = kMoeDigitWarp0 + kMoeDigitWarps;
+constexpr int kMoeMakeWarp0 = kMoeMmaWarp + 1, kMoeMakeWarps = 2;
+constexpr int kMoeEpiWarp0 = kMoeMakeWarp0 + kMoeMakeWarps, kMoeEpiWarps = 8;
 constexpr int kMoeExpertThreads = 32 * (kMoeEpiWarp0 + kMoeEpiWarps);
 constexpr int kMoeQueue = 4;
 
 template <int TOK>
 struct MoeCfg {
-  static constexpr int kN = TOK * kMoeDigitRows;             // MMA columns of a full pass
-  static constexpr int kBlocks = (kN + 127) / 128;           // 128-row blocks of the digit scales
+  static constexpr bool kSwap = TOK <= 16;
+  static constexpr int kN = kSwap ? 128 : TOK * kMoeDigitRows;  // accumulator columns of a tile
+  static constexpr int kBlocks = (TOK * kMoeDigitRows + 127) / 128;  // 128-row blocks of digit scales
   static constexpr int kCodes = 2 * 128 * 128;
   static constexpr int oSw = kCodes;                         // weight scales [tile][word][512]
   static constexpr int oB = oSw + 2 * 4 * 512;               // digits
   static constexpr int oSb = oB + TOK * kMoeChunkCodes;      // digit scales [block][word][512]
   static constexpr int kStage = oSb + kBlocks * 4 * 512;
-  static constexpr int kStages = TOK <= 8 ? 4 : 3;
+  static constexpr int kStages = 3;
   static constexpr int kRaw = 256 * 16;                      // natural weight scales of a stage
   static constexpr int oRaw = kStages * kStage;
   static constexpr int kSmem = oRaw + kStages * kRaw + 1024;
-  static constexpr int kAccs = TOK <= 8 ? 2 : 1;             // accumulator pairs
-  static constexpr int kSfCol0 = kAccs * 2 * kN;
+  static constexpr int kSfCol0 = 2 * kN;                     // after the two tiles' accumulators
   static constexpr int kSfSet = 2 * 16 + kBlocks * 16;       // scale words of a stage in tensor memory
   static_assert(kSfCol0 + 2 * kSfSet <= 512, "tensor memory budget");
+  static_assert(!kSwap || TOK == 16, "128 rows of digits");
   static_assert(kStage % 1024 == 0 && oB % 1024 == 0, "1 KB swizzle atoms");
   // a full stage: the code and digit copies' tx arrives, the scale warps
-  static constexpr int kFullCount = 2 + kMoeScaleWarps + kMoeDigitScaleWarps;
+  static constexpr int kFullCount = 2 + kMoeScaleWarps + kMoeDigitWarps;
 };
 
 struct MoeCtl {
-  uint64_t full[4], empty[4], raw_full[4], raw_empty[4], acc_full[2], acc_empty[2], qfull[kMoeQueue], qempty[kMoeQueue], drain, ebar;
+  uint64_t full[4], empty[4], raw_full[4], acc_full, acc_empty, qfull[kMoeQueue], qempty[kMoeQueue], drain;
   uint32_t queue[kMoeQueue];
-  uint32_t abort_flag, tmem_base, ticket, ticket_expert;
+  uint32_t abort_flag, tmem_base;
   uint32_t warps;  // epilogue warps that finished their part of a down task
 };
-constexpr int kMoeQueueReaders = kMoeEpiWarp0 - 1 + kMoeEpiWarps;
+constexpr int kMoeQueueReaders = kMoeScaleWarps + kMoeDigitWarps + 1 + kMoeEpiWarps;
 
 // A queue entry: phase in the top two bits (0 gate / up, 1 down, 2 end), task below.
 struct MoeTask {
@@ -638,22 +644,35 @@ __device__ __forceinline__ void moe_count_down(uint32_t* counter, uint32_t* warp
   }
 }
 
-// Barrier of the epilogue warps: an mbarrier, so that the wait is bounded and ends when another role
-// has given up.
-__device__ __forceinline__ bool moe_epi_sync(MoeCtl& ctl, uint32_t& parity, uint32_t* err) {
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl.ebar));
-  const bool ok = moe_warp_wait(ctl.ebar, parity, kErrWaitAccum, ctl, err);
-  parity ^= 1u;
-  return ok;
-}
-
 // Sum of a token's eight digit columns.
 __device__ __forceinline__ float moe_sum8(const uint32_t* r) {
   float s = __uint_as_float(r[kMoeDigitCount - 1]);
 #pragma unroll
   for (int p = kMoeDigitCount - 2; p >= 0; --p) s += __uint_as_float(r[p]);
   return s;
+}
+
+// 16 columns of eight lanes' digits: lane p of the eight gets the sums over the eight lanes of columns
+// p and 8 + p (each step halves the columns a lane keeps, adding what the other half's lane had).
+__device__ __forceinline__ void moe_lane_sums(const uint32_t (&d)[16], float& s0, float& s1) {
+  const int lane = threadIdx.x & 31;
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(d[i]);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    const bool high = (lane & o) != 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < o; ++i) {
+        const float keep = high ? v[8 * h + o + i] : v[8 * h + i];
+        const float give = high ? v[8 * h + i] : v[8 * h + o + i];
+        v[8 * h + i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
+      }
+  }
+  s0 = v[0];
+  s1 = v[8];
 }
 
 // Four scale words (a row's 16 scales of a stage) into their tiles, 512 bytes apart.
@@ -688,18 +707,14 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
       mbar_init(smem_u32(&ctl.full[s]), Cfg::kFullCount);
       mbar_init(smem_u32(&ctl.empty[s]), 1);
       mbar_init(smem_u32(&ctl.raw_full[s]), 32);
-      mbar_init(smem_u32(&ctl.raw_empty[s]), kMoeScaleWarps);
     }
-    for (int s = 0; s < Cfg::kAccs; ++s) {
-      mbar_init(smem_u32(&ctl.acc_full[s]), 1);
-      mbar_init(smem_u32(&ctl.acc_empty[s]), kMoeEpiWarps);
-    }
+    mbar_init(smem_u32(&ctl.acc_full), 1);
+    mbar_init(smem_u32(&ctl.acc_empty), kMoeEpiWarps);
     for (int s = 0; s < kMoeQueue; ++s) {
       mbar_init(smem_u32(&ctl.qfull[s]), 1);
       mbar_init(smem_u32(&ctl.qempty[s]), kMoeQueueReaders);
     }
     mbar_init(smem_u32(&ctl.drain), 1);
-    mbar_init(smem_u32(&ctl.ebar), kMoeEpiWarps);
     ctl.warps = 0;
     fence_mbar_init();
   }
@@ -772,8 +787,12 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
       if (t.phase == 2) break;
       const MoeGeom gm = sh.geom(p, pl, t);
       const CUtensorMap* tm = t.phase == 0 ? &tm_w13 : &tm_w2;
+      const int pitch = gm.K / 16, half = 8 * (lane & 1);
+      const uint8_t* base = (t.phase == 0 ? p.s13 : p.s2) + (lane >> 1) * pitch + half;
+      const uint8_t *sa = base + gm.ra * pitch, *sb = base + gm.rb * pitch;
       for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK)
         for (int c = gm.c0; c < gm.c1; ++c) {
+          // (an empty stage's raw scales are read too: they were repacked before its MMAs)
           if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
           if (lane == 0) {
             const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
@@ -784,20 +803,6 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
               tma_load_2d(st + Cfg::kCodes / 2, tm, c * 128, static_cast<int32_t>(gm.rb), fb);
           }
           __syncwarp();
-          r.next();
-        }
-    }
-  } else if (warp == 1) {
-    // --------------------------------------------------------- weight scales, natural, 16 bytes a row
-    while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
-      const MoeGeom gm = sh.geom(p, pl, t);
-      const int pitch = gm.K / 16, half = 8 * (lane & 1);
-      const uint8_t* base = (t.phase == 0 ? p.s13 : p.s2) + (lane >> 1) * pitch + half;
-      const uint8_t *sa = base + gm.ra * pitch, *sb = base + gm.rb * pitch;
-      bool ok = true;
-      for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK)
-        for (int c = gm.c0; c < gm.c1; ++c) {
-          if (!(ok = moe_warp_wait(ctl.raw_empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
           if (c * 16 + half < pitch) {  // the last stage may have 8 scales a row
             const uint32_t dst = smem_u32(smem + Cfg::oRaw + r.slot * Cfg::kRaw) + 8 * lane;
 #pragma unroll
@@ -816,15 +821,14 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
                        : "memory");
           r.next();
         }
-      if (!ok) break;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp < kMoeDigitWarp) {
+  } else if (warp < kMoeDigitWarp0) {
     // ---------------------------------------- weight scales into their tiles: half the rows of a tile
     // Lane (i, j) = (lane / 8, lane % 8) takes rows 32 i + 16 h + j and + 8, h the half: the four row
     // groups of one j are side by side in a tile, so neither loads nor stores have bank conflicts.
-    const int m = (warp - 2) >> 1;
-    const int row = 32 * (lane >> 3) + 16 * (warp & 1) + (lane & 7);
+    const int m = (warp - kMoeScaleWarp0) >> 1;
+    const int row = 32 * (lane >> 3) + 16 * ((warp - kMoeScaleWarp0) & 1) + (lane & 7);
     const uint32_t at = Cfg::oSw + m * 2048 + (row & 31) * 16 + (row >> 5) * 4;
     while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
       const MoeGeom gm = sh.geom(p, pl, t);
@@ -835,22 +839,20 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
           const uint8_t* raw = smem + Cfg::oRaw + r.slot * Cfg::kRaw + m * 2048 + row * 16;
           const uint4 lo = *reinterpret_cast<const uint4*>(raw);
           const uint4 hi = *reinterpret_cast<const uint4*>(raw + 128);
-          if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
+          // (raw scales arrive only in a stage whose MMAs are done: its tiles are free)
           const uint32_t dst = smem_u32(smem + r.slot * Cfg::kStage) + at;
           moe_store_scales(dst, make_uint2(lo.x, lo.y), make_uint2(lo.z, lo.w));
           moe_store_scales(dst + 128, make_uint2(hi.x, hi.y), make_uint2(hi.z, hi.w));
           moe_scales_ready(ctl.full[r.slot]);
-          // (the stores depend on the loads: the raw slot is read)
-          if (lane == 0) mbar_arrive(smem_u32(&ctl.raw_empty[r.slot]));
           r.next();
         }
       if (!ok) break;
     }
   } else if (warp < kMoeMmaWarp) {
-    // ----------------------------------------- activation digits: codes (warp 6), scales (7..10)
-    // Scale warp `part`: tokens part + 4 i (+ 16), lane = 8 i + digit: again the four row groups of a
-    // line side by side.
-    const int part = warp - kMoeDigitWarp - 1;  // -1: codes
+    // ---------------------------------------------- activation digits: scales; codes by the first
+    // Warp `part`: tokens part + 4 i (+ 16), lane = 8 i + digit: again the four row groups of a line
+    // side by side.
+    const int part = warp - kMoeDigitWarp0;
     constexpr int kSets = Cfg::kBlocks;
     bool ready = false;  // the digits of all experts
     while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
@@ -869,20 +871,7 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
           const int pr = pl.pairs[gm.off + n0 + i];
           return base + (t.phase == 0 ? pr / p.k : pr) * moe_image_row(gm.K);
         };
-        if (part < 0) {
-          const uint8_t* src = lane < n ? image(lane) : nullptr;
-          for (int c = gm.c0; c < gm.c1; ++c) {
-            if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
-            const uint32_t fb = smem_u32(&ctl.full[r.slot]);
-            if (lane == 0) mbar_arrive_expect_tx(fb, n * kMoeChunkCodes);
-            __syncwarp();
-            if (lane < n)
-              bulk_load(smem_u32(smem + r.slot * Cfg::kStage) + Cfg::oB + lane * kMoeChunkCodes,
-                        src + static_cast<int64_t>(c) * kMoeChunk, kMoeChunkCodes, fb);
-            r.next();
-          }
-          continue;
-        }
+        const uint8_t* codes = part == 0 && lane < n ? image(lane) : nullptr;
         const uint8_t* src[kSets];
         uint32_t at[kSets];
         uint4 w[kMoeAhead][kSets];
@@ -905,6 +894,14 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
             if (c0 + j >= gm.c1) break;
             if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
             const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
+            if (part == 0) {
+              const uint32_t fb = smem_u32(&ctl.full[r.slot]);
+              if (lane == 0) mbar_arrive_expect_tx(fb, n * kMoeChunkCodes);
+              __syncwarp();
+              if (codes != nullptr)
+                bulk_load(st + Cfg::oB + lane * kMoeChunkCodes,
+                          codes + static_cast<int64_t>(c0 + j) * kMoeChunk, kMoeChunkCodes, fb);
+            }
 #pragma unroll
             for (int k = 0; k < kSets; ++k)
               if (src[k] != nullptr)
@@ -920,107 +917,80 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     }
   } else if (warp == kMoeMmaWarp) {
     // ----------------------------------------------------------------------------------- MMA
-    RingPos<Cfg::kAccs> ac;
-    uint32_t set = 0;
+    uint32_t aph = 0, set = 0;
     bool ok = true;
     while (ok && moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
       const MoeGeom gm = sh.geom(p, pl, t);
       for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK) {
         const int n = min(gm.cnt - n0, TOK);
-        const uint32_t N = static_cast<uint32_t>(n * kMoeDigitRows + 15) & ~15u;
+        const uint32_t N = Cfg::kSwap ? (gm.two ? 256u : 128u)
+                                      : static_cast<uint32_t>(n * kMoeDigitRows + 15) & ~15u;
         const uint32_t idesc = idesc_mxf4(128, N, false, 0);
-        const int blocks = N > 128 ? 2 : 1;
-        if (!(ok = moe_warp_wait(ctl.acc_empty[ac.slot], ac.phase ^ 1u, kErrWaitAccum, ctl, p.err)))
-          break;
+        const int blocks = !Cfg::kSwap && N > 128 ? 2 : 1;
+        if (!(ok = moe_warp_wait(ctl.acc_empty, aph ^ 1u, kErrWaitAccum, ctl, p.err))) break;
+        aph ^= 1u;
         tc_fence_after();
-        const uint32_t acc = tb + ac.slot * 2 * Cfg::kN;
         for (int c = gm.c0; c < gm.c1; ++c) {
           if (!(ok = moe_warp_wait(ctl.full[r.slot], r.phase, kErrWaitTma, ctl, p.err))) break;
           tc_fence_after();
           const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
-          const uint32_t sf = tb + Cfg::kSfCol0 + set * Cfg::kSfSet;
+          // scale words in tensor memory: weights [word][tile] (kSwap: one 256-row operand) or
+          // [tile][word], digits [word][block]
+          const uint32_t sfw = tb + Cfg::kSfCol0 + set * Cfg::kSfSet, sfd = sfw + 32;
+          constexpr uint32_t kWord = Cfg::kSwap ? 8 : 4, kTile = Cfg::kSwap ? 4 : 16;
           const int steps = min(4, gm.K / 64 - c * 4);
           if (elect_one()) {
             for (int kk = 0; kk < steps; ++kk) {
-              tmem_cp_32x128b_x4(sf + 4 * kk, sdesc_sf(st + Cfg::oSw + kk * 512));
+              tmem_cp_32x128b_x4(sfw + kWord * kk, sdesc_sf(st + Cfg::oSw + kk * 512));
               if (gm.two)
-                tmem_cp_32x128b_x4(sf + 16 + 4 * kk, sdesc_sf(st + Cfg::oSw + (4 + kk) * 512));
-              tmem_cp_32x128b_x4(sf + 32 + kk * 4 * Cfg::kBlocks,
-                                 sdesc_sf(st + Cfg::oSb + kk * 512));
+                tmem_cp_32x128b_x4(sfw + kWord * kk + kTile, sdesc_sf(st + Cfg::oSw + (4 + kk) * 512));
+              tmem_cp_32x128b_x4(sfd + kk * 4 * Cfg::kBlocks, sdesc_sf(st + Cfg::oSb + kk * 512));
               if (Cfg::kBlocks > 1 && blocks > 1)
-                tmem_cp_32x128b_x4(sf + 32 + kk * 4 * Cfg::kBlocks + 4,
+                tmem_cp_32x128b_x4(sfd + kk * 4 * Cfg::kBlocks + 4,
                                    sdesc_sf(st + Cfg::oSb + 2048 + kk * 512));
             }
             for (int kk = 0; kk < steps; ++kk) {
               const uint32_t accumulate = (c > gm.c0 || kk > 0) ? 1u : 0u;
-              const uint64_t bd = sdesc_sw128(st + Cfg::oB + kk * 32);
-              const uint32_t sfb = sf + 32 + kk * 4 * Cfg::kBlocks;
-              mma_mxf4_ss<true, false>(acc, sdesc_sw128(st + kk * 32), bd, idesc, sf + 4 * kk, sfb,
-                                       accumulate);
-              if (gm.two)
-                mma_mxf4_ss<true, false>(acc + Cfg::kN, sdesc_sw128(st + Cfg::kCodes / 2 + kk * 32),
-                                         bd, idesc, sf + 16 + 4 * kk, sfb, accumulate);
+              const uint64_t wd = sdesc_sw128(st + kk * 32), dd = sdesc_sw128(st + Cfg::oB + kk * 32);
+              const uint32_t sd = sfd + kk * 4 * Cfg::kBlocks;
+              if constexpr (Cfg::kSwap) {
+                mma_mxf4_ss<true, false>(tb, dd, wd, idesc, sd, sfw + kWord * kk, accumulate);
+              } else {
+                mma_mxf4_ss<true, false>(tb, wd, dd, idesc, sfw + kWord * kk, sd, accumulate);
+                if (gm.two)
+                  mma_mxf4_ss<true, false>(tb + Cfg::kN, sdesc_sw128(st + Cfg::kCodes / 2 + kk * 32),
+                                           dd, idesc, sfw + kWord * kk + kTile, sd, accumulate);
+              }
             }
             tc_commit(smem_u32(&ctl.empty[r.slot]));
-            if (c + 1 == gm.c1) tc_commit(smem_u32(&ctl.acc_full[ac.slot]));
+            if (c + 1 == gm.c1) tc_commit(smem_u32(&ctl.acc_full));
           }
           __syncwarp();
           r.next();
           set ^= 1u;
         }
-        ac.next();
       }
     }
     // arrives once every tcgen05 operation this warp issued has completed
     if (elect_one()) tc_commit(smem_u32(&ctl.drain));
     __syncwarp();
     mbar_wait(smem_u32(&ctl.drain), 0, p.err, kErrWaitMma, nullptr);
-  } else {
-    // ------------------------------------------------------------------------------ epilogue
-    const int group = (warp - kMoeEpiWarp0) / 4, quarter = warp & 3;
-    const int row = 32 * quarter + lane;  // row of the MMA tile
-    const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
-    RingPos<Cfg::kAccs> ac;
-    bool ok = true, digits = false;
-    uint32_t eph = 0;
-    // A digit task by the eight warps, or none: with `wait` the next ticket, waiting for its expert's
-    // hidden values; else only if that expert has them all already. False when a wait ran out; none
-    // (ticket at or past the total) ends the caller's loop.
-    auto digit_task = [&](bool wait, bool& none) {
-      if (warp == kMoeEpiWarp0) {
-        uint32_t k = wait ? moe_ticket(p.counters + kMoeDigits)
-                          : __shfl_sync(0xFFFFFFFFu, ld_acquire_gpu(p.counters + kMoeDigits), 0);
-        int a = 0;
-        if (k < total_d) {
-          for (int lo = 0, hi = nact; hi - lo > 1;) {  // dig[a] <= k < dig[a + 1]
-            const int mid = (lo + hi) >> 1;
-            if (pl.dig[mid] <= k) lo = mid;
-            else hi = mid;
-            a = lo;
-          }
-          if (wait) {
-            if (!moe_wait(gate_up_done + a, sh.blocks1, ctl, p.err)) k = 0xFFFFFFFFu;
-          } else {
-            uint32_t got = k;
-            if (lane == 0)
-              got = ld_acquire_gpu(gate_up_done + a) < static_cast<uint32_t>(sh.blocks1)
-                        ? ~k
-                        : atomicCAS(p.counters + kMoeDigits, k, k + 1);
-            if (__shfl_sync(0xFFFFFFFFu, got, 0) != k) k = 0xFFFFFFFFu;
-          }
-        }
-        if (lane == 0) {
-          ctl.ticket = k;
-          ctl.ticket_expert = a;
-        }
+  } else if (warp < kMoeEpiWarp0) {
+    // ------------------------------------------------------------- digits of the hidden values
+    while (true) {
+      const uint32_t k = moe_ticket(p.counters + kMoeDigits);
+      if (k >= total_d) break;
+      int a = 0;
+      for (int hi = nact; hi - a > 1;) {  // dig[a] <= k < dig[a + 1]
+        const int mid = (a + hi) >> 1;
+        if (pl.dig[mid] <= k) a = mid;
+        else hi = mid;
       }
-      if (!moe_epi_sync(ctl, eph, p.err)) return false;
-      const uint32_t k = *reinterpret_cast<volatile uint32_t*>(&ctl.ticket);
-      const int a = *reinterpret_cast<volatile uint32_t*>(&ctl.ticket_expert);
-      none = k >= total_d;
-      if (!none) {
-        const int e = pl.act[a];
-        const int b = static_cast<int>(k - pl.dig[a]) * kMoeDigitBlocks + 32 * (warp - kMoeEpiWarp0) + lane;
+      if (!moe_wait(gate_up_done + a, sh.blocks1 * kMoeEpiWarps, ctl, p.err)) break;
+      const int e = pl.act[a];
+#pragma unroll 1
+      for (int i = 0; i < kMoeDigitBlocks; i += 32) {
+        const int b = static_cast<int>(k - pl.dig[a]) * kMoeDigitBlocks + i + lane;
         if (b < pl.cnt[e] * blocks_h) {  // a multiple of eight
           const int pr = pl.pairs[pl.off[e] + b / blocks_h], blk = b % blocks_h;
           const float up = pow2f(moe_row_shift(__ldcg(p.hmax + pr)));
@@ -1036,91 +1006,148 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
           }
           moe_digits(v, p.hs + pr * moe_image_row(p.I), blk);
         }
-        asm volatile("fence.proxy.async;" ::: "memory");
       }
-      if (!moe_epi_sync(ctl, eph, p.err)) return false;  // stored; the ticket is read
-      if (!none && tid == 32 * kMoeEpiWarp0) {
-        __threadfence();
+      asm volatile("fence.proxy.async;" ::: "memory");
+      __threadfence();
+      __syncwarp();
+      if (lane == 0) {
         atomicAdd(digits_done + a, 1u);
         atomicAdd(p.counters + kMoeDigitsDone, 1u);
       }
-      return true;
-    };
-    auto all_digits = [&]() {
-      digits = true;
-      bool none = false;
-      while (!none)
-        if (!digit_task(true, none)) return false;
-      return true;
-    };
+    }
+  } else {
+    // ------------------------------------------------------------------------------ epilogue
+    const int group = (warp - kMoeEpiWarp0) / 4, quarter = warp & 3;
+    const int row = 32 * quarter + lane;  // row of the MMA tile
+    const uint32_t acc = tb + (static_cast<uint32_t>(32 * quarter) << 16);
+    uint32_t aph = 0;
+    bool ok = true;
     while ((ok = moe_next_task(t, q, ctl, p.err)) && t.phase != 2) {
-      if (t.phase == 1 && !digits && !(ok = all_digits())) break;
       const MoeGeom gm = sh.geom(p, pl, t);
       const float ts13 = p.ts13[gm.e], ts2 = p.ts2[gm.e];
       for (int n0 = 0; n0 < gm.cnt; n0 += TOK) {
         const int n = min(gm.cnt - n0, TOK);
-        if (!(ok = moe_warp_wait(ctl.acc_full[ac.slot], ac.phase, kErrWaitAccum, ctl, p.err))) break;
-        tc_fence_after();
-        const uint32_t acc = tb + lanes + ac.slot * 2 * Cfg::kN;
-        // the columns' sums into registers, then the accumulator is free. Up: this group of four warps
-        // takes every other token, both tiles; down: all tokens of its own tile.
+        // what the tokens need besides, by lane: loaded before the wait
         const bool up = t.phase == 0;
-        float sum[TOK];
-#pragma unroll
-        for (int j = 0; j < TOK / 2; ++j) {
-          const int c = up ? 2 * j + group : 2 * j;
-          if (c < n && (up || group == 0 || gm.two)) {
-            uint32_t d0[8], d1[8];
-            tmem_ld_x8(acc + (up ? 0 : group * Cfg::kN) + c * kMoeDigitRows, d0);
-            tmem_ld_x8(acc + (up ? Cfg::kN + c * kMoeDigitRows
-                                 : group * Cfg::kN + (c + 1) * kMoeDigitRows), d1);
-            tmem_ld_wait();
-            sum[2 * j] = moe_sum8(d0);
-            sum[2 * j + 1] = moe_sum8(d1);
+        float f0 = 0.0f, f1 = 0.0f;
+        int pr_l = 0;
+        if (lane < n) {
+          pr_l = pl.pairs[gm.off + n0 + lane];
+          if (up) {
+            f0 = p.x_scale[pr_l / p.k] * ts13;
+            f1 = pl.w[pr_l] * ts2;
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ctl.acc_empty[ac.slot]));
-        ac.next();
-        if (up) {
+        if (!(ok = moe_warp_wait(ctl.acc_full, aph, kErrWaitAccum, ctl, p.err))) break;
+        aph ^= 1u;
+        // (a pair's maximum is final once its expert's down product runs, not before)
+        if (!up && lane < n) f0 = moe_row_factor(__ldcg(p.hmax + pr_l));
+        tc_fence_after();
+        auto release = [&]() {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ctl.acc_empty));
+        };
+        if constexpr (Cfg::kSwap) {
+          // Lanes 8 i .. 8 i + 7 of a quarter: the digits of token 4 quarter + i; columns: weight
+          // rows. Up: this group of four warps takes 64 hidden units, both tiles; down: the 128
+          // rows of its own tile. Four pieces of 16 + 16 columns, summed over the digits so that
+          // lane p of eight ends with columns p and 8 + p of each 16.
+          const int c = 4 * quarter + (lane >> 3);
+          const bool work = 4 * quarter < n && (up || group == 0 || gm.two);
+          float v[16];
+          if (work) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t d0[16], d1[16];
+              tmem_ld_x16(acc + (up ? 64 * group + 16 * j : 128 * group + 32 * j), d0);
+              tmem_ld_x16(acc + (up ? 128 + 64 * group + 16 * j : 128 * group + 32 * j + 16), d1);
+              tmem_ld_wait();
+              moe_lane_sums(d0, v[4 * j], v[4 * j + 1]);
+              moe_lane_sums(d1, v[4 * j + 2], v[4 * j + 3]);
+            }
+          }
+          release();
+          if (work) {
+            const int pr = __shfl_sync(0xFFFFFFFFu, pr_l, c);
+            const float g0 = __shfl_sync(0xFFFFFFFFu, f0, c), g1 = __shfl_sync(0xFFFFFFFFu, f1, c);
+            uint32_t hm = 0;
+            float* dst = up ? p.h + static_cast<int64_t>(pr) * p.I + gm.row0 + 64 * group
+                            : p.part + (static_cast<int64_t>(gm.z) * p.T * p.k + pr) * p.H + gm.row0 +
+                                  128 * group;
+            dst += lane & 7;
+            if (c < n) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  if (up) {
+                    const float h = silu_rn(v[4 * j + half] * g0) * (v[4 * j + 2 + half] * g0) * g1;
+                    dst[16 * j + 8 * half] = h;
+                    hm = max(hm, __float_as_uint(h) & 0x7FFFFFFFu);
+                  } else {
+                    dst[32 * j + 8 * half] = v[4 * j + half] * g0;
+                    dst[32 * j + 16 + 8 * half] = v[4 * j + 2 + half] * g0;
+                  }
+                }
+            }
+            if (up) {
+#pragma unroll
+              for (int o = 1; o < 8; o <<= 1) hm = max(hm, __shfl_xor_sync(0xFFFFFFFFu, hm, o));
+              if ((lane & 7) == 0 && c < n) atomicMax(p.hmax + pr, hm);
+            }
+          }
+        } else {
+          // Lane: weight row; columns: the tokens' digits. Up: this group of four warps takes every
+          // other token, both tiles; down: all tokens of its own tile.
+          float sum[TOK];
 #pragma unroll
           for (int j = 0; j < TOK / 2; ++j) {
-            const int c = 2 * j + group;
-            if (c >= n) break;
-            const int pr = pl.pairs[gm.off + n0 + c];
-            const float s = p.x_scale[pr / p.k] * ts13;
-            const float h = silu_rn(sum[2 * j] * s) * (sum[2 * j + 1] * s) * (pl.w[pr] * ts2);
-            p.h[static_cast<int64_t>(pr) * p.I + gm.row0 + row] = h;
-            const uint32_t hm =
-                __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h) & 0x7FFFFFFFu);
-            if (lane == 0) atomicMax(p.hmax + pr, hm);
+            const int c = up ? 2 * j + group : 2 * j;
+            if (c < n && (up || group == 0 || gm.two)) {
+              uint32_t d0[8], d1[8];
+              tmem_ld_x8(acc + (up ? 0 : group * Cfg::kN) + c * kMoeDigitRows, d0);
+              tmem_ld_x8(acc + (up ? Cfg::kN + c * kMoeDigitRows
+                                   : group * Cfg::kN + (c + 1) * kMoeDigitRows), d1);
+              tmem_ld_wait();
+              sum[2 * j] = moe_sum8(d0);
+              sum[2 * j + 1] = moe_sum8(d1);
+            }
           }
-        } else if (group == 0 || gm.two) {
+          release();
+          if (up) {
 #pragma unroll
-          for (int c = 0; c < TOK; ++c) {
-            if (c >= n) break;
-            const int pr = pl.pairs[gm.off + n0 + c];
-            p.part[(static_cast<int64_t>(gm.z) * p.T * p.k + pr) * p.H + gm.row0 + 128 * group + row] =
-                sum[c] * moe_row_factor(__ldcg(p.hmax + pr));
+            for (int j = 0; j < TOK / 2; ++j) {
+              const int c = 2 * j + group;
+              if (c >= n) break;
+              const int pr = __shfl_sync(0xFFFFFFFFu, pr_l, c);
+              const float s = __shfl_sync(0xFFFFFFFFu, f0, c), wt = __shfl_sync(0xFFFFFFFFu, f1, c);
+              const float h = silu_rn(sum[2 * j] * s) * (sum[2 * j + 1] * s) * wt;
+              p.h[static_cast<int64_t>(pr) * p.I + gm.row0 + row] = h;
+              const uint32_t hm =
+                  __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(h) & 0x7FFFFFFFu);
+              if (lane == 0) atomicMax(p.hmax + pr, hm);
+            }
+          } else if (group == 0 || gm.two) {
+            float* dst = p.part + static_cast<int64_t>(gm.z) * p.T * p.k * p.H + gm.row0 + 128 * group + row;
+#pragma unroll
+            for (int c = 0; c < TOK; ++c) {
+              if (c >= n) break;
+              dst[static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, pr_l, c)) * p.H] =
+                  sum[c] * __shfl_sync(0xFFFFFFFFu, f0, c);
+            }
           }
         }
       }
       if (!ok) break;
-      if (t.phase == 1) {
-        moe_count_down(p.counters + kMoeDownDone, &ctl.warps);
-        continue;
-      }
-      if (!(ok = moe_epi_sync(ctl, eph, p.err))) break;  // every warp's hidden values are stored
-      if (tid == 32 * kMoeEpiWarp0) {
+      if (t.phase == 0) {
         __threadfence();
-        atomicAdd(gate_up_done + gm.a, 1u);
+        __syncwarp();
+        if (lane == 0) atomicAdd(gate_up_done + gm.a, 1u);
+      } else {
+        moe_count_down(p.counters + kMoeDownDone, &ctl.warps);
       }
-      bool none = false;
-      for (int i = 0; i < 2 && !none && ok; ++i) ok = digit_task(false, none);
-      if (!ok) break;
     }
-    if (ok && !digits) ok = all_digits();
 
     // combine: 128 outputs of a token per warp and turn, dealt by index (no one waits for these),
     // eight partial sums in flight

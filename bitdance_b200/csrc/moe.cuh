@@ -223,11 +223,12 @@ __device__ __forceinline__ double block_reduce(double v, double* part) {
   return v;
 }
 
-// Router: a cluster of eight CTAs per TB tokens; CTA r takes experts r, r + 8, ..., one per warp at
-// a time, for all TB tokens; the logits of token i of the group go to CTA i's shared memory, which
-// selects for it. Two logits may be arbitrarily close, so they are kept in 64 bits: eight products
-// are summed in fp32 and added to a double, an error near 1e-8 of the logits' spread. Bound by the
-// latency of one pass over the router weights.
+// Router: a cluster of eight CTAs per TB tokens; a CTA takes every eighth expert (every seventh, and
+// the last CTA none, where one token's digits keep that CTA busy), one per warp at a time, for all TB
+// tokens; the logits of token i of the group go to CTA i's shared memory, which selects for it. Two
+// logits may be arbitrarily close, so they are kept in 64 bits: eight products are summed in fp32 and
+// added to a double, an error near 1e-8 of the logits' spread. Bound by the latency of one pass over
+// the router weights and of the selection's steps.
 template <class X, class W, int TB>
 __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRouteParams p) {
   extern __shared__ double sh[];  // scores [E] (logits of this CTA's token), keys [E]
@@ -245,7 +246,8 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
     for (int i = threadIdx.x; i < moe_counters(p.E); i += kMoeThreads) p.counters[i] = 0;
   cluster_sync_all();  // every CTA of the cluster runs: its shared memory may be written
   const int pieces = p.H / 8;
-  for (int e = rank + kRouteCluster * warp; e < p.E; e += kRouteCluster * kMoeWarps) {
+  constexpr int kRanks = TB == 1 ? kRouteCluster - 1 : kRouteCluster;
+  for (int e = rank + kRanks * warp; rank < kRanks && e < p.E; e += kRanks * kMoeWarps) {
     double acc[TB] = {};
     const W* row = wr + static_cast<int64_t>(e) * p.H;
 #pragma unroll(TB == 1 ? 8 : 4)
@@ -279,50 +281,67 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
   cluster_sync_all();
   const int t = t0 + static_cast<int>(rank);
   if (static_cast<int>(rank) >= TB || t >= p.T) return;
-  double* logit = sh;
+  // Scores and keys. The key ranks: the logit itself (softmax without bias: the same order, nothing
+  // rounds), else score + bias; a NaN ranks last. Where the weights are renormalised softmax scores
+  // ranked by logit, exp(logit - largest) of the chosen ones is all that is needed.
+  double* score = sh;
   double* key = sh + p.E;
-  double m = -INFINITY;
-  for (int e = threadIdx.x; e < p.E; e += kMoeThreads) m = fmax(m, logit[e]);
-  double z = 1.0;
-  if (!p.sigmoid) {
-    m = block_reduce<true>(m, part);
-    z = 0.0;
-    for (int e = threadIdx.x; e < p.E; e += kMoeThreads) z += exp(logit[e] - m);
-    z = block_reduce<false>(z, part);
-  }
-  // score in place of the logit; the key ranks: the logit itself (softmax without bias: the same
-  // order, nothing rounds), else score + bias; a NaN ranks last
-  for (int e = threadIdx.x; e < p.E; e += kMoeThreads) {
-    const double l = logit[e];
-    const double s = p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / z;
-    const double v = p.bias != nullptr ? s + static_cast<double>(p.bias[e]) : l;
-    logit[e] = s;
-    key[e] = v == v ? v : -INFINITY;
-  }
-  __syncthreads();
-  // rank of an expert: how many stand before it (ties to the lowest index); ranks are distinct
-  for (int e = threadIdx.x; e < p.E; e += kMoeThreads) {
-    const double v = key[e];
-    int r = 0;
-    for (int j = 0; j < p.E; ++j) {
-      const double u = key[j];
-      r += (u > v || (u == v && j < e)) ? 1 : 0;
+  const bool lazy = !p.sigmoid && p.bias == nullptr && p.renormalize;
+  if (!lazy) {
+    double m = 0.0, z = 1.0;
+    if (!p.sigmoid) {
+      m = -INFINITY;
+      for (int e = threadIdx.x; e < p.E; e += kMoeThreads) m = fmax(m, score[e]);
+      m = block_reduce<true>(m, part);
+      z = 0.0;
+      for (int e = threadIdx.x; e < p.E; e += kMoeThreads) z += exp(score[e] - m);
+      z = block_reduce<false>(z, part);
     }
-    if (r < p.k) {
+    for (int e = threadIdx.x; e < p.E; e += kMoeThreads) {
+      const double l = score[e];
+      const double s = p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / z;
+      const double v = p.bias != nullptr ? s + static_cast<double>(p.bias[e]) : l;
+      score[e] = s;
+      key[e] = v == v ? v : -INFINITY;
+    }
+    __syncthreads();
+  }
+  // rank of an expert: how many stand before it (ties to the lowest index); ranks are distinct.
+  // `team` threads (a power of two up to 32) share an expert.
+  int team = 32;
+  while (team > 1 && team * p.E > kMoeThreads) team >>= 1;
+  const int sub = threadIdx.x & (team - 1);
+  const double* by = lazy ? score : key;
+  for (int e0 = 0; e0 < p.E; e0 += kMoeThreads / team) {
+    const int e = e0 + threadIdx.x / team;
+    int r = 0;
+    if (e < p.E) {
+      double v = by[e];
+      if (v != v) v = -INFINITY;
+      for (int j = sub; j < p.E; j += team) {
+        double u = by[j];
+        if (u != u) u = -INFINITY;
+        r += (u > v || (u == v && j < e)) ? 1 : 0;
+      }
+    }
+    for (int o = team >> 1; o > 0; o >>= 1) r += __shfl_xor_sync(0xFFFFFFFFu, r, o);
+    if (e < p.E && sub == 0 && r < p.k) {
       p.ids[t * p.k + r] = e;
-      sel[r] = logit[e];
+      sel[r] = score[e];
     }
   }
   __syncthreads();
   if (threadIdx.x < p.k) {
+    // lazy: sel holds logits, the first the largest (all NaN or -inf: the weights are NaN, as theirs)
+    const double mine = lazy ? exp(sel[threadIdx.x] - sel[0]) : sel[threadIdx.x];
     double sum = 1.0;
     if (p.renormalize) {
       sum = 0.0;
-      for (int r = 0; r < p.k; ++r) sum += sel[r];
+      for (int r = 0; r < p.k; ++r) sum += lazy ? exp(sel[r] - sel[0]) : sel[r];
     }
     p.hmax[t * p.k + threadIdx.x] = 0;
     p.weights[t * p.k + threadIdx.x] =
-        static_cast<float>(sel[threadIdx.x] / sum * static_cast<double>(p.routed_scale));
+        static_cast<float>(mine / sum * static_cast<double>(p.routed_scale));
   }
 }
 
@@ -527,8 +546,8 @@ struct MoeCfg {
   static_assert(kSfCol0 + 2 * kSfSet <= 512, "tensor memory budget");
   static_assert(!kSwap || TOK == 16, "128 rows of digits");
   static_assert(kStage % 1024 == 0 && oB % 1024 == 0, "1 KB swizzle atoms");
-  // a full stage: the code and digit copies' tx arrives, the scale warps
-  static constexpr int kFullCount = 2 + kMoeScaleWarps + kMoeDigitWarps;
+  // a full stage: the codes' tx arrive, the scale and digit warps (and the digits' bytes)
+  static constexpr int kFullCount = 1 + kMoeScaleWarps + kMoeDigitWarps;
 };
 
 struct MoeCtl {
@@ -849,8 +868,8 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
       if (!ok) break;
     }
   } else if (warp < kMoeMmaWarp) {
-    // ---------------------------------------------- activation digits: scales; codes by the first
-    // Warp `part`: tokens part + 4 i (+ 16), lane = 8 i + digit: again the four row groups of a line
+    // ---------------------------------------------------------------- activation digits and scales
+    // Warp `part`: tokens part + 4 i. Scales: lane = 8 i + digit, again the four row groups of a line
     // side by side.
     const int part = warp - kMoeDigitWarp0;
     constexpr int kSets = Cfg::kBlocks;
@@ -871,7 +890,9 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
           const int pr = pl.pairs[gm.off + n0 + i];
           return base + (t.phase == 0 ? pr / p.k : pr) * moe_image_row(gm.K);
         };
-        const uint8_t* codes = part == 0 && lane < n ? image(lane) : nullptr;
+        // codes of tokens part + 4 lane
+        const uint8_t* codes = part + 4 * lane < n ? image(part + 4 * lane) : nullptr;
+        const uint32_t code_bytes = (n - part + 3) / 4 * kMoeChunkCodes;
         const uint8_t* src[kSets];
         uint32_t at[kSets];
         uint4 w[kMoeAhead][kSets];
@@ -894,14 +915,15 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
             if (c0 + j >= gm.c1) break;
             if (!(ok = moe_warp_wait(ctl.empty[r.slot], r.phase ^ 1u, kErrWaitEmpty, ctl, p.err))) break;
             const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
-            if (part == 0) {
-              const uint32_t fb = smem_u32(&ctl.full[r.slot]);
-              if (lane == 0) mbar_arrive_expect_tx(fb, n * kMoeChunkCodes);
-              __syncwarp();
-              if (codes != nullptr)
-                bulk_load(st + Cfg::oB + lane * kMoeChunkCodes,
-                          codes + static_cast<int64_t>(c0 + j) * kMoeChunk, kMoeChunkCodes, fb);
-            }
+            const uint32_t fb = smem_u32(&ctl.full[r.slot]);
+            if (lane == 0)
+              asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(fb),
+                           "r"(code_bytes)
+                           : "memory");
+            __syncwarp();
+            if (codes != nullptr)
+              bulk_load(st + Cfg::oB + (part + 4 * lane) * kMoeChunkCodes,
+                        codes + static_cast<int64_t>(c0 + j) * kMoeChunk, kMoeChunkCodes, fb);
 #pragma unroll
             for (int k = 0; k < kSets; ++k)
               if (src[k] != nullptr)

@@ -139,8 +139,33 @@ int launch_gemm(GemmFp4Params p, const uint8_t* a, const uint8_t* b, bool overla
 }
 
 template <int kFmt>
+int launch_pair(GemmFp4Params p, const uint8_t* a, const uint8_t* b, bool overlap,
+                const DeviceInfo* d, cudaStream_t s) {
+  using Cfg = PairFp4Cfg<kFmt>;
+  static std::atomic<uint64_t> configured{0};
+  if (!allow_smem(w4a4_pair_kernel<kFmt>, Cfg::kSmem, configured)) return BD_ERR_CUDA;
+  p.n_tiles = (p.N + 255) / 256;
+  p.m_tiles = (p.M + 255) / 256;
+  const int64_t tiles = static_cast<int64_t>(p.n_tiles) * p.m_tiles;
+  if (tiles > 0x7FFFFFFF) return BD_ERR_SHAPE;
+  CUtensorMap mw, mt;
+  if (!codes_map(&mw, b, p.N, p.K, 128) || !codes_map(&mt, a, p.M, p.K, 128)) return BD_ERR_CUDA;
+  const int grid = 2 * static_cast<int>(std::min<int64_t>(tiles, d->sm_count / 2));
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg =
+      launch_config(grid, kPairThreads, Cfg::kSmem, s, attr, overlap, 2);
+  if (cudaLaunchKernelEx(&cfg, w4a4_pair_kernel<kFmt>, mw, mt, p) != cudaSuccess)
+    return BD_ERR_CUDA;
+  return last_status();
+}
+
+template <int kFmt>
 int launch_gemm_any(const GemmFp4Params& p, const uint8_t* a, const uint8_t* b, bool overlap,
                     const DeviceInfo* d, cudaStream_t s) {
+  // 256 x 256 tiles where they occupy at least half of the SM pairs
+  const int64_t pair_tiles =
+      static_cast<int64_t>((p.N + 255) / 256) * ((p.M + 255) / 256);
+  if (p.M > 128 && 4 * pair_tiles >= d->sm_count) return launch_pair<kFmt>(p, a, b, overlap, d, s);
   if (p.M <= 16) return launch_gemm<16, kFmt>(p, a, b, overlap, d, s);
   if (p.M <= 32) return launch_gemm<32, kFmt>(p, a, b, overlap, d, s);
   if (p.M <= 64) return launch_gemm<64, kFmt>(p, a, b, overlap, d, s);
@@ -275,6 +300,7 @@ int bd_w4a4_gemm(void* c, const uint8_t* a, const uint8_t* a_scales, const float
   p.words = sf_words(K, fmt);
   p.out_dtype = out_dtype;
   p.epilogue = epilogue;
+  p.vec_out = aligned(c, 16) && static_cast<int64_t>(N) * (out_dtype == BD_OUT_F32 ? 4 : 2) % 16 == 0;
   p.weights_early = (flags & BD_GEMM_WEIGHTS_STATIC) ? 1 : 0;
   p.err = d->err;
   const bool overlap = (flags & BD_GEMM_OVERLAP_PREV) != 0;

@@ -5,6 +5,8 @@
 //
 //   C[m, n] = act(acc[m, n] * ((s_m * ts) * s_n) + bias[n]),  acc = sum_k a b in fp32
 //
+// Two kernels: w4a4_pair_kernel where 256 x 256 tiles fill the machine, w4a4_gemm_kernel else.
+//
 // w4a4_gemm_kernel: tiles of 128 weight rows (the MMA's M) x BN tokens (its N), so a decode batch
 // of 16 tokens pads to 16 columns instead of 128 rows. One CTA computes one K slice of one tile;
 // the `split` CTAs of a cluster share a tile, and exchange their fp32 partials through distributed
@@ -32,6 +34,7 @@ struct GemmFp4Params {
   int M, N, K, words;
   int n_tiles, m_tiles;
   int out_dtype, epilogue;
+  int vec_out;                // rows of C are 16-byte aligned
   int weights_early;
   uint32_t* err;
 };
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
       for (int c0 = 0; c0 < cols; c0 += 16) {
         uint32_t r[16];
         tmem_ld_x16(taddr + c0, r);
-        tmem_ld_wait();
+        tmem_ld_wait_x16(r);
 #pragma unroll
         for (int j = 0; j < 16; ++j) finish(c0 + j, __uint_as_float(r[j]));
       }
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
     for (int c0 = 0; c0 < BN; c0 += 16) {
       uint32_t r[16];
       tmem_ld_x16(taddr + c0, r);
-      tmem_ld_wait();
+      tmem_ld_wait_x16(r);
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int owner = (c0 + j) / width, col = (c0 + j) % width;
@@ -286,6 +289,243 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
     tc_fence_after();
     tmem_dealloc(tb, Cfg::kTmemCols);
   }
+}
+
+// w4a4_pair_kernel: tiles of 256 tokens x 256 weight rows on clusters of two CTAs (cta_group::2): CTA
+// rank r loads tokens 128 r .. and weight rows 128 r .. of the tile (and the scales of all 256 weight
+// rows), each stage 38 KB for 512 cycles of MMA; rank 0 issues the MMAs. Persistent, tiles dealt
+// round-robin over the clusters, tokens fastest.
+//
+// Tensor memory: one 256-column accumulator and two sets of scale words (a second accumulator would
+// leave no room for scales), so the next tile's MMAs wait for the drain: eight epilogue warps take a
+// tile's 128 columns each into 128 registers in one go and release the accumulator before they scale,
+// convert and store (about 300 cycles of a 4096-deep tile's 8200).
+//
+// Warps: 0 producer, 1 MMA (rank 0), 2 relay (rank 1: tells rank 0 that a stage of rank 1 has
+// landed), 3 idle, 4..11 epilogue.
+constexpr int kPairThreads = 384;
+
+template <int kFmt>
+struct PairFp4Cfg {
+  static constexpr int kWords = kFmt == kNvfp4 ? 4 : 2;
+  static constexpr int kCodes = 128 * 128;        // codes of 128 rows, 256 of K
+  static constexpr int kSf = 512 * kWords;        // scales of 128 rows
+  static constexpr int oW = kCodes;               // tokens first
+  static constexpr int oSt = 2 * kCodes;
+  static constexpr int oSw = oSt + kSf;           // two blocks of 128 weight rows
+  static constexpr int kStage = cround_up(oSw + 2 * kSf, 1024);
+  static constexpr int kStages = 5;
+  static constexpr int kSmem = kStages * kStage + 1024;
+  static constexpr int kSfSet = 12 * kWords;      // scale words of a stage in tensor memory
+  static constexpr int kSfCol0 = 256;
+  static_assert(kSfCol0 + 2 * kSfSet <= 512, "tensor memory budget");
+  static_assert(kStage % 1024 == 0, "1 KB swizzle atoms");
+};
+
+struct PairFp4Ctl {
+  uint64_t full[5], peer_full[5], empty[5], acc_full, acc_empty, drain;
+  uint32_t tmem_base, abort_flag;
+};
+
+template <int kFmt>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    w4a4_pair_kernel(const __grid_constant__ CUtensorMap tm_w,
+                     const __grid_constant__ CUtensorMap tm_t, const GemmFp4Params p) {
+  using Cfg = PairFp4Cfg<kFmt>;
+  constexpr bool kNv = kFmt == kNvfp4;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ PairFp4Ctl ctl;
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
+  const int tiles = p.n_tiles * p.m_tiles;
+  const int chunks = (p.K + kF4ChunkK - 1) / kF4ChunkK;
+  volatile uint32_t* abort_flag = &ctl.abort_flag;
+  if (tid == 0) {
+    ctl.abort_flag = 0;
+    for (int s = 0; s < Cfg::kStages; ++s) {
+      mbar_init(smem_u32(&ctl.full[s]), 1);
+      mbar_init(smem_u32(&ctl.peer_full[s]), 1);
+      mbar_init(smem_u32(&ctl.empty[s]), 1);
+    }
+    mbar_init(smem_u32(&ctl.acc_full), 1);
+    mbar_init(smem_u32(&ctl.acc_empty), 16);  // the epilogue warps of both CTAs
+    mbar_init(smem_u32(&ctl.drain), 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&ctl.tmem_base), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers are initialised before anyone arrives
+  tc_fence_after();
+  const uint32_t tb = ctl.tmem_base;
+  grid_dep_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tmap(&tm_w);
+      prefetch_tmap(&tm_t);
+      // weights never wait for the previous grid apart from the tokens here: a stage has both
+      grid_dep_wait();
+      RingPos<Cfg::kStages> r;
+      int issued = 0;
+      bool ok = true;
+      for (int tile = cluster; tile < tiles && ok; tile += clusters) {
+        const int m0 = tile % p.m_tiles * 256 + 128 * static_cast<int>(rank);
+        const int n0 = tile / p.m_tiles * 256;
+        const int t_blocks = m0 < p.M ? 1 : 0, w_blocks = n0 + 128 < p.N ? 2 : 1;
+        const uint8_t* sf_t = p.sf_t + static_cast<int64_t>(m0 / 128) * p.words * 512;
+        const uint8_t* sf_w = p.sf_w + static_cast<int64_t>(n0 / 128) * p.words * 512;
+        const int64_t w_next = static_cast<int64_t>(p.words) * 512;
+        for (int k = 0; k < chunks; ++k) {
+          if (!(ok = mbar_wait(smem_u32(&ctl.empty[r.slot]), r.phase ^ 1u, p.err, kErrWaitEmpty,
+                               abort_flag)))
+            break;
+          const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
+          const uint32_t fb = smem_u32(&ctl.full[r.slot]);
+          const uint32_t sfb = 512u * min(Cfg::kWords, p.words - k * Cfg::kWords);
+          mbar_arrive_expect_tx(fb, 2 * Cfg::kCodes + sfb * (t_blocks + w_blocks));
+          tma_load_2d(st, &tm_t, k * 128, m0, fb);
+          tma_load_2d(st + Cfg::oW, &tm_w, k * 128, n0 + 128 * static_cast<int>(rank), fb);
+          const int64_t at = static_cast<int64_t>(k) * Cfg::kSf;
+          if (t_blocks) bulk_load(st + Cfg::oSt, sf_t + at, sfb, fb);
+          for (int b = 0; b < w_blocks; ++b)
+            bulk_load(st + Cfg::oSw + b * Cfg::kSf, sf_w + b * w_next + at, sfb, fb);
+          r.next();
+          ++issued;
+        }
+      }
+      // every copy issued has landed before the CTA exits (also after a wait ran out)
+      for (int j = max(0, issued - Cfg::kStages); j < issued; ++j)
+        mbar_wait(smem_u32(&ctl.full[j % Cfg::kStages]), (j / Cfg::kStages) & 1, p.err, kErrWaitTma,
+                  nullptr);
+    }
+  } else if (warp == 2) {
+    if (lane == 0 && rank == 1) {
+      RingPos<Cfg::kStages> r;
+      bool ok = true;
+      for (int tile = cluster; tile < tiles && ok; tile += clusters)
+        for (int k = 0; k < chunks; ++k) {
+          if (!(ok = mbar_wait(smem_u32(&ctl.full[r.slot]), r.phase, p.err, kErrWaitTma, abort_flag)))
+            break;
+          mbar_arrive_remote_release(mapa_shared(smem_u32(&ctl.peer_full[r.slot]), 0));
+          r.next();
+        }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      RingPos<Cfg::kStages> r;
+      uint32_t aph = 0, set = 0;
+      bool ok = true;
+      for (int tile = cluster; tile < tiles && ok; tile += clusters) {
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl.acc_empty), aph ^ 1u, p.err,
+                                                           kErrWaitAccum, abort_flag))))
+          break;
+        aph ^= 1u;
+        tc_fence_after();
+        for (int k = 0; k < chunks; ++k) {
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.full[r.slot]), r.phase, p.err,
+                                                 kErrWaitTma, abort_flag)) &&
+               __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl.peer_full[r.slot]), r.phase,
+                                                       p.err, kErrWaitTma, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
+          const uint32_t sft = tb + Cfg::kSfCol0 + set * Cfg::kSfSet, sfw = sft + 4 * Cfg::kWords;
+          const int words = min(Cfg::kWords, p.words - k * Cfg::kWords);
+          const int steps = min(4, (p.K - k * kF4ChunkK + 63) / 64);
+          if (elect_one()) {
+            for (int w = 0; w < words; ++w) {
+              tmem_cp_32x128b_x4_pair(sft + 4 * w, sdesc_sf(st + Cfg::oSt + 512 * w));
+              tmem_cp_32x128b_x4_pair(sfw + 8 * w, sdesc_sf(st + Cfg::oSw + 512 * w));
+              tmem_cp_32x128b_x4_pair(sfw + 8 * w + 4, sdesc_sf(st + Cfg::oSw + Cfg::kSf + 512 * w));
+            }
+            for (int kk = 0; kk < steps; ++kk) {
+              const int w = kNv ? kk : kk >> 1;
+              const uint32_t idesc = idesc_mxf4(256, 256, !kNv, kNv ? 0 : 2 * (kk & 1));
+              mma_mxf4_ss<kNv, true>(tb, sdesc_sw128(st + kk * 32), sdesc_sw128(st + Cfg::oW + kk * 32),
+                                     idesc, sft + 4 * w, sfw + 8 * w, (k > 0 || kk > 0) ? 1u : 0u);
+            }
+            tc_commit_pair(smem_u32(&ctl.empty[r.slot]), 3);
+            if (k + 1 == chunks) tc_commit_pair(smem_u32(&ctl.acc_full), 3);
+          }
+          __syncwarp();
+          r.next();
+          set ^= 1u;
+        }
+      }
+      // arrives once every tcgen05 operation this warp issued has completed
+      if (elect_one()) tc_commit_pair(smem_u32(&ctl.drain), 3);
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    const int quarter = warp & 3, group = (warp - 4) >> 2;
+    const uint32_t acc = tb + (static_cast<uint32_t>(32 * quarter) << 16) + 128 * group;
+    const uint32_t acc_empty = mapa_shared(smem_u32(&ctl.acc_empty), 0);
+    uint32_t aph = 0;
+    grid_dep_wait();  // C, bias and the row scales belong to the previous grid until it ends
+    for (int tile = cluster; tile < tiles; tile += clusters) {
+      const int m = tile % p.m_tiles * 256 + 128 * static_cast<int>(rank) + 32 * quarter + lane;
+      const int n0 = tile / p.m_tiles * 256 + 128 * group;
+      const float scale = p.row_scale_t != nullptr && m < p.M
+                              ? __fmul_rn(p.row_scale_t[m], p.tensor_scale)
+                              : p.tensor_scale;
+      if (!__all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl.acc_full), aph, p.err, kErrWaitAccum,
+                                                   abort_flag)))
+        break;
+      aph ^= 1u;
+      tc_fence_after();
+      uint32_t r[4][32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld_x32(acc + 32 * i, r[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld_wait_x32(r[i]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(acc_empty);
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = n0 + 32 * i;
+        if (n >= p.N) break;
+        const int64_t at = static_cast<int64_t>(m) * p.N + n;
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(__uint_as_float(r[i][j]), scale);
+        if (n + 32 <= p.N) {
+          if (p.row_scale_w != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(v[j], p.row_scale_w[n + j]);
+          }
+          apply_epilogue_row<32>(v, 1.0f, p.epilogue, p.bias, n);
+          store_row<32>(p.out, at, v, p.out_dtype, p.vec_out);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (n + j < p.N) {
+              float x = p.row_scale_w != nullptr ? __fmul_rn(v[j], p.row_scale_w[n + j]) : v[j];
+              store_out(p.out, at + j, apply_epilogue(x, p.epilogue, p.bias, n + j), p.out_dtype);
+            }
+        }
+      }
+    }
+  }
+  // ---- teardown
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (lane == 0) mbar_wait(smem_u32(&ctl.drain), 0, p.err, kErrWaitMma, nullptr);
+    __syncwarp();
+    tc_fence_after();
+  }
+  // neither CTA frees its tensor memory or exits while the peer may still arrive on its barriers
+  cluster_sync_all();
+  if (warp == 1) tmem_dealloc_pair(tb, 512);
 }
 
 }  // namespace bd

@@ -1084,7 +1084,8 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
               uint32_t d0[16], d1[16];
               tmem_ld_x16(acc + (up ? 64 * group + 16 * j : 128 * group + 32 * j), d0);
               tmem_ld_x16(acc + (up ? 128 + 64 * group + 16 * j : 128 * group + 32 * j + 16), d1);
-              tmem_ld_wait();
+              tmem_ld_wait_x16(d0);
+              tmem_ld_wait_x16(d1);
               moe_lane_sums(d0, v[4 * j], v[4 * j + 1]);
               moe_lane_sums(d1, v[4 * j + 2], v[4 * j + 3]);
             }
@@ -1131,7 +1132,8 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
               tmem_ld_x8(acc + (up ? 0 : group * Cfg::kN) + c * kMoeDigitRows, d0);
               tmem_ld_x8(acc + (up ? Cfg::kN + c * kMoeDigitRows
                                    : group * Cfg::kN + (c + 1) * kMoeDigitRows), d1);
-              tmem_ld_wait();
+              tmem_ld_wait_x8(d0);
+              tmem_ld_wait_x8(d1);
               sum[2 * j] = moe_sum8(d0);
               sum[2 * j + 1] = moe_sum8(d1);
             }

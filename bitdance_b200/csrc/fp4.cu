@@ -111,6 +111,13 @@ bool codes_map(CUtensorMap* m, const uint8_t* codes, int rows, int K, int box_ro
                      K / 2, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Scale tiles as rows of 512 bytes (one word of 128 rows), boxes of box_words of them.
+bool scales_map(CUtensorMap* m, const uint8_t* sf, int rows, int words, int box_words) {
+  return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, const_cast<uint8_t*>(sf), 128,
+                     (static_cast<uint64_t>(rows) + 127) / 128 * words, 512, 128, box_words,
+                     CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 template <int BN, int kFmt>
 int launch_gemm(GemmFp4Params p, const uint8_t* a, const uint8_t* b, bool overlap,
                 const DeviceInfo* d, cudaStream_t s) {
@@ -148,13 +155,16 @@ int launch_pair(GemmFp4Params p, const uint8_t* a, const uint8_t* b, bool overla
   p.m_tiles = (p.M + 255) / 256;
   const int64_t tiles = static_cast<int64_t>(p.n_tiles) * p.m_tiles;
   if (tiles > 0x7FFFFFFF) return BD_ERR_SHAPE;
-  CUtensorMap mw, mt;
-  if (!codes_map(&mw, b, p.N, p.K, 128) || !codes_map(&mt, a, p.M, p.K, 128)) return BD_ERR_CUDA;
+  CUtensorMap mw, mt, sw, st;
+  if (!codes_map(&mw, b, p.N, p.K, 128) || !codes_map(&mt, a, p.M, p.K, 128) ||
+      !scales_map(&sw, p.sf_w, p.N, p.words, Cfg::kWords) ||
+      !scales_map(&st, p.sf_t, p.M, p.words, Cfg::kWords))
+    return BD_ERR_CUDA;
   const int grid = 2 * static_cast<int>(std::min<int64_t>(tiles, d->sm_count / 2));
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg =
       launch_config(grid, kPairThreads, Cfg::kSmem, s, attr, overlap, 2);
-  if (cudaLaunchKernelEx(&cfg, w4a4_pair_kernel<kFmt>, mw, mt, p) != cudaSuccess)
+  if (cudaLaunchKernelEx(&cfg, w4a4_pair_kernel<kFmt>, mw, mt, sw, st, p) != cudaSuccess)
     return BD_ERR_CUDA;
   return last_status();
 }

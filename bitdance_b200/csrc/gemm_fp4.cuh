@@ -301,8 +301,10 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
 // tile's 128 columns each into 128 registers in one go and release the accumulator before they scale,
 // convert and store (about 300 cycles of a 4096-deep tile's 8200).
 //
-// Warps: 0 producer, 1 MMA (rank 0), 2 relay (rank 1: tells rank 0 that a stage of rank 1 has
-// landed), 3 idle, 4..11 epilogue.
+// Both CTAs' loads complete on rank 0's barrier (a relay warp in rank 1 that passed arrivals on was
+// 840 cycles a stage).
+//
+// Warps: 0 producer, 1 MMA (rank 0), 2 and 3 idle, 4..11 epilogue.
 constexpr int kPairThreads = 384;
 
 template <int kFmt>
@@ -323,14 +325,16 @@ struct PairFp4Cfg {
 };
 
 struct PairFp4Ctl {
-  uint64_t full[5], peer_full[5], empty[5], acc_full, acc_empty, drain;
+  uint64_t full[5], empty[5], acc_full, acc_empty, drain;
   uint32_t tmem_base, abort_flag;
 };
 
 template <int kFmt>
 __global__ void __launch_bounds__(kPairThreads, 1)
     w4a4_pair_kernel(const __grid_constant__ CUtensorMap tm_w,
-                     const __grid_constant__ CUtensorMap tm_t, const GemmFp4Params p) {
+                     const __grid_constant__ CUtensorMap tm_t,
+                     const __grid_constant__ CUtensorMap tm_sw,
+                     const __grid_constant__ CUtensorMap tm_st, const GemmFp4Params p) {
   using Cfg = PairFp4Cfg<kFmt>;
   constexpr bool kNv = kFmt == kNvfp4;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -346,7 +350,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     ctl.abort_flag = 0;
     for (int s = 0; s < Cfg::kStages; ++s) {
       mbar_init(smem_u32(&ctl.full[s]), 1);
-      mbar_init(smem_u32(&ctl.peer_full[s]), 1);
       mbar_init(smem_u32(&ctl.empty[s]), 1);
     }
     mbar_init(smem_u32(&ctl.acc_full), 1);
@@ -369,7 +372,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (lane == 0) {
       prefetch_tmap(&tm_w);
       prefetch_tmap(&tm_t);
-      // weights never wait for the previous grid apart from the tokens here: a stage has both
+      prefetch_tmap(&tm_sw);
+      prefetch_tmap(&tm_st);
       grid_dep_wait();
       RingPos<Cfg::kStages> r;
       int issued = 0;
@@ -377,44 +381,31 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int tile = cluster; tile < tiles && ok; tile += clusters) {
         const int m0 = tile % p.m_tiles * 256 + 128 * static_cast<int>(rank);
         const int n0 = tile / p.m_tiles * 256;
-        const int t_blocks = m0 < p.M ? 1 : 0, w_blocks = n0 + 128 < p.N ? 2 : 1;
-        const uint8_t* sf_t = p.sf_t + static_cast<int64_t>(m0 / 128) * p.words * 512;
-        const uint8_t* sf_w = p.sf_w + static_cast<int64_t>(n0 / 128) * p.words * 512;
-        const int64_t w_next = static_cast<int64_t>(p.words) * 512;
         for (int k = 0; k < chunks; ++k) {
           if (!(ok = mbar_wait(smem_u32(&ctl.empty[r.slot]), r.phase ^ 1u, p.err, kErrWaitEmpty,
                                abort_flag)))
             break;
           const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
-          const uint32_t fb = smem_u32(&ctl.full[r.slot]);
-          const uint32_t sfb = 512u * min(Cfg::kWords, p.words - k * Cfg::kWords);
-          mbar_arrive_expect_tx(fb, 2 * Cfg::kCodes + sfb * (t_blocks + w_blocks));
-          tma_load_2d(st, &tm_t, k * 128, m0, fb);
-          tma_load_2d(st + Cfg::oW, &tm_w, k * 128, n0 + 128 * static_cast<int>(rank), fb);
-          const int64_t at = static_cast<int64_t>(k) * Cfg::kSf;
-          if (t_blocks) bulk_load(st + Cfg::oSt, sf_t + at, sfb, fb);
-          for (int b = 0; b < w_blocks; ++b)
-            bulk_load(st + Cfg::oSw + b * Cfg::kSf, sf_w + b * w_next + at, sfb, fb);
+          const uint32_t fb = mapa_shared(smem_u32(&ctl.full[r.slot]), 0);
+          if (rank == 0)
+            mbar_arrive_expect_tx(smem_u32(&ctl.full[r.slot]), 2 * (2 * Cfg::kCodes + 3 * Cfg::kSf));
+          tma_load_2d_pair(st, &tm_t, k * 128, m0, fb);
+          tma_load_2d_pair(st + Cfg::oW, &tm_w, k * 128, n0 + 128 * static_cast<int>(rank), fb);
+          // scale boxes of kWords words: past a row's last word they take words of the next 128 rows
+          // (or zeros), which no MMA reads
+          const int w0 = k * Cfg::kWords;
+          tma_load_2d_pair(st + Cfg::oSt, &tm_st, 0, m0 / 128 * p.words + w0, fb);
+          tma_load_2d_pair(st + Cfg::oSw, &tm_sw, 0, n0 / 128 * p.words + w0, fb);
+          tma_load_2d_pair(st + Cfg::oSw + Cfg::kSf, &tm_sw, 0, (n0 / 128 + 1) * p.words + w0, fb);
           r.next();
           ++issued;
         }
       }
-      // every copy issued has landed before the CTA exits (also after a wait ran out)
-      for (int j = max(0, issued - Cfg::kStages); j < issued; ++j)
-        mbar_wait(smem_u32(&ctl.full[j % Cfg::kStages]), (j / Cfg::kStages) & 1, p.err, kErrWaitTma,
-                  nullptr);
-    }
-  } else if (warp == 2) {
-    if (lane == 0 && rank == 1) {
-      RingPos<Cfg::kStages> r;
-      bool ok = true;
-      for (int tile = cluster; tile < tiles && ok; tile += clusters)
-        for (int k = 0; k < chunks; ++k) {
-          if (!(ok = mbar_wait(smem_u32(&ctl.full[r.slot]), r.phase, p.err, kErrWaitTma, abort_flag)))
-            break;
-          mbar_arrive_remote_release(mapa_shared(smem_u32(&ctl.peer_full[r.slot]), 0));
-          r.next();
-        }
+      // a wait ran out: every copy issued lands before the CTA exits (rank 0's barriers say so)
+      if (*abort_flag && rank == 0)
+        for (int j = max(0, issued - Cfg::kStages); j < issued; ++j)
+          mbar_wait(smem_u32(&ctl.full[j % Cfg::kStages]), (j / Cfg::kStages) & 1, p.err, kErrWaitTma,
+                    nullptr);
     }
   } else if (warp == 1) {
     if (rank == 0) {
@@ -428,11 +419,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         aph ^= 1u;
         tc_fence_after();
         for (int k = 0; k < chunks; ++k) {
-          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl.full[r.slot]), r.phase, p.err,
-                                                 kErrWaitTma, abort_flag)) &&
-               __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl.peer_full[r.slot]), r.phase,
-                                                       p.err, kErrWaitTma, abort_flag));
-          if (!ok) break;
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl.full[r.slot]), r.phase,
+                                                             p.err, kErrWaitTma, abort_flag))))
+            break;
           tc_fence_after();
           const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
           const uint32_t sft = tb + Cfg::kSfCol0 + set * Cfg::kSfSet, sfw = sft + 4 * Cfg::kWords;

@@ -64,8 +64,8 @@ cudaLaunchConfig_t launch_config(int grid, int threads, int smem, cudaStream_t s
 
 template <int kIn, int kFmt>
 int launch_quantize(const QuantFp4Params& p, bool overlap, const DeviceInfo* d, cudaStream_t s) {
-  // up to 64 pieces of a row a warp keeps the row (two per lane); longer rows take a whole CTA
-  const bool warp_rows = p.K <= 1024;
+  // a warp per row where the rows give every SM four warps, or a row is short; else a CTA per row
+  const bool warp_rows = p.K <= 1024 || p.M >= 4 * d->sm_count;
   const int rows_per_cta = warp_rows ? kQ4Threads / 32 : 1;
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg =
@@ -84,26 +84,33 @@ int launch_quantize_in(int in, const QuantFp4Params& p, bool overlap, const Devi
   return launch_quantize<kInF16, kFmt>(p, overlap, d, s);
 }
 
-template <int kFmt>
-int launch_dequantize(int out_dtype, const uint8_t* codes, const uint8_t* tiled, const float* rs,
-                      float ts, void* out, int M, int K, bool overlap, const DeviceInfo* d,
+template <int kFmt, int kOut>
+int launch_dequantize(const uint8_t* codes, const uint8_t* tiled, const float* rs, float ts,
+                      void* out, int M, int K, bool overlap, const DeviceInfo* d,
                       cudaStream_t s) {
-  const int64_t total = static_cast<int64_t>(M) * (K / 16);
+  const bool warp_rows = K <= 1024;  // a warp per row, else a CTA
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg =
-      launch_config(grid_for(total, 256, d), 256, 0, s, attr, overlap);
-  const int pieces = K / 16, words = sf_words(K, kFmt);
-  cudaError_t e;
-  if (out_dtype == BD_OUT_BF16)
-    e = cudaLaunchKernelEx(&cfg, dequantize_fp4_kernel<kFmt, 0>, codes, tiled, rs, ts, out, total,
-                           pieces, words);
-  else if (out_dtype == BD_OUT_F16)
-    e = cudaLaunchKernelEx(&cfg, dequantize_fp4_kernel<kFmt, 1>, codes, tiled, rs, ts, out, total,
-                           pieces, words);
-  else
-    e = cudaLaunchKernelEx(&cfg, dequantize_fp4_kernel<kFmt, 2>, codes, tiled, rs, ts, out, total,
-                           pieces, words);
+      launch_config(grid_for(M, warp_rows ? 8 : 1, d), 256, 0, s, attr, overlap);
+  uint8_t* o = static_cast<uint8_t*>(out);
+  const int words = sf_words(K, kFmt);
+  const cudaError_t e =
+      warp_rows ? cudaLaunchKernelEx(&cfg, dequantize_fp4_kernel<kFmt, kOut, 32>, codes, tiled, rs,
+                                     ts, o, M, K, words)
+                : cudaLaunchKernelEx(&cfg, dequantize_fp4_kernel<kFmt, kOut, 256>, codes, tiled, rs,
+                                     ts, o, M, K, words);
   return e == cudaSuccess ? last_status() : BD_ERR_CUDA;
+}
+
+template <int kFmt>
+int launch_dequantize_out(int out_dtype, const uint8_t* codes, const uint8_t* tiled,
+                          const float* rs, float ts, void* out, int M, int K, bool overlap,
+                          const DeviceInfo* d, cudaStream_t s) {
+  if (out_dtype == BD_OUT_BF16)
+    return launch_dequantize<kFmt, 0>(codes, tiled, rs, ts, out, M, K, overlap, d, s);
+  if (out_dtype == BD_OUT_F16)
+    return launch_dequantize<kFmt, 1>(codes, tiled, rs, ts, out, M, K, overlap, d, s);
+  return launch_dequantize<kFmt, 2>(codes, tiled, rs, ts, out, M, K, overlap, d, s);
 }
 
 bool codes_map(CUtensorMap* m, const uint8_t* codes, int rows, int K, int box_rows) {
@@ -276,9 +283,9 @@ int bd_dequantize_fp4(const uint8_t* codes, const uint8_t* scales_tiled, const f
   if (st != BD_OK) return st;
   const bool overlap = (flags & BD_GEMM_OVERLAP_PREV) != 0;
   return fmt == BD_FP4_NVFP4
-             ? launch_dequantize<kNvfp4>(out_dtype, codes, scales_tiled, row_scale, tensor_scale,
+             ? launch_dequantize_out<kNvfp4>(out_dtype, codes, scales_tiled, row_scale, tensor_scale,
                                          out, M, K, overlap, d, as_stream(stream))
-             : launch_dequantize<kMxfp4>(out_dtype, codes, scales_tiled, row_scale, tensor_scale,
+             : launch_dequantize_out<kMxfp4>(out_dtype, codes, scales_tiled, row_scale, tensor_scale,
                                          out, M, K, overlap, d, as_stream(stream));
 }
 

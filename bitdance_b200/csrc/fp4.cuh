@@ -18,11 +18,11 @@
 // E2M1 of x * 2^-e, a tie to the lower magnitude. x * 2^-e is exact (values that leave the normal
 // range are far below the first midpoint).
 //
-// Element code on float bits: for y >= 1 the E2M1 index is (exponent field - 126) * 2 + the top
-// mantissa bit, rounded up when the 22 bits below are strictly above half: adding 0x1FFFFF
-// carries into bit 22 exactly then, so idx = ((bits(y) + 0x1FFFFF) >> 22) - 252, capped at 7.
-// For y < 1 (step 1/2) the same holds of z = (y + 1) / 2 in [0.5, 1), rounded up to float32 so
-// that "strictly above half" is kept; max(y, z) picks the right one.
+// Element code: y = x * r rounded to float32 goes through the hardware's conversion to E2M1, which
+// rounds to nearest, a tie to the even code. A tie always has its low 21 mantissa bits zero, and so
+// does every E2M1 value; a y with those bits zero is first multiplied by 1 - 2^-24, which takes it to
+// the float below: a tie then rounds down, an E2M1 value back to itself. (Integer rounding on float
+// bits instead took 11 instructions an element for 6, and the quantiser was bound by them.)
 //
 // Scale tiles (both formats): [ceil(rows / 128)][ceil(scales per row / 4)][512 bytes], row r of a
 // tile at 16 (r % 32) + 4 (r / 32 % 4), its four scales side by side: the image tcgen05.cp
@@ -93,10 +93,17 @@ struct Raw16 {
   }
 };
 
-__device__ __forceinline__ uint32_t e2m1_mag(float a, float r) {
-  const float y = fabsf(a) * r;
-  const float z = __fmaf_ru(y, 0.5f, 0.5f);
-  return min((__float_as_uint(fmaxf(y, z)) + (0x1FFFFFu - (252u << 22))) >> 22, 7u);
+// Four codes bytes of eight scaled elements, sign kept on non-zero magnitudes only.
+__device__ __forceinline__ uint32_t e2m1_pack8(const float (&y)[8]) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(w)
+      : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+  // a nibble's magnitude + 7 has bit 3 set exactly when it is not 0
+  return w & ((((w & 0x77777777u) + 0x77777777u) & 0x88888888u) | 0x77777777u);
 }
 
 // 16 elements times r -> 8 code bytes.
@@ -105,15 +112,13 @@ __device__ __forceinline__ uint2 e2m1_encode16(const Raw16<kIn>& x, float r) {
   uint32_t o[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t m = 0, sg = 0;
+    float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float v = x.get(8 * h + j);
-      m |= e2m1_mag(v, r) << (4 * j);
-      sg |= (__float_as_uint(v) >> (28 - 4 * j)) & (8u << (4 * j));
+      y[j] = __fmul_rn(x.get(8 * h + j), r);
+      if ((__float_as_uint(y[j]) & 0x1FFFFFu) == 0) y[j] = __fmul_rn(y[j], 0.99999994f);  // 1 - 2^-24
     }
-    // the sign stays on nibbles whose magnitude is not 0 (n + 7 has bit 3 set exactly then)
-    o[h] = m | ((m + 0x77777777u) & sg & 0x88888888u);
+    o[h] = e2m1_pack8(y);
   }
   return make_uint2(o[0], o[1]);
 }
@@ -135,15 +140,16 @@ struct QuantFp4Params {
   uint32_t* err;
 };
 
-// Quantiser. G threads share a row (G = 32: eight rows per CTA; G = 256: the CTA's eight warps
-// share one, their maxima meeting in shared memory). A thread takes 16-element pieces tid, tid + G,
-// ..., keeps the first kKeep of them in registers between the maximum and the codes, and reads
-// the rest of a long row twice (the second time from L1 / L2). Bound by the bytes of x.
+// Quantiser. G threads share a row: a warp where there are rows enough to fill the machine (no
+// barriers, kKeep pieces of each lane in flight), else a CTA of eight warps, their maxima meeting in
+// shared memory. A thread takes 16-element pieces t, t + G, ..., keeps the first kKeep of them in
+// registers between the maximum and the codes, and reads the rest of a long row twice (the second time
+// from L2). Bound by the bytes of x.
 constexpr int kQ4Threads = 256;
 
 template <int kIn, int kFmt, int G>
-__global__ void __launch_bounds__(kQ4Threads) quantize_fp4_kernel(const QuantFp4Params p) {
-  constexpr int kKeep = kIn == kInF32 ? 2 : 4;
+__global__ void __launch_bounds__(kQ4Threads, 2) quantize_fp4_kernel(const QuantFp4Params p) {
+  constexpr int kKeep = kIn == kInF32 ? 4 : 8;
   __shared__ uint32_t part[2][kQ4Threads / 32];
   const int sub = threadIdx.x / G, t = threadIdx.x % G;
   const int pieces = p.K / 16;
@@ -158,22 +164,21 @@ __global__ void __launch_bounds__(kQ4Threads) quantize_fp4_kernel(const QuantFp4
     const bool row_ok = m < p.M;
     const int64_t e0 = m * p.K;
     Raw16<kIn> keep[kKeep];
-    float inv = 1.0f;
+    auto fetch = [&](int c0) {
 #pragma unroll
-    for (int u = 0; u < kKeep; ++u)
-      if (row_ok && t + u * G < pieces)
-        keep[u].load(p.x, e0 + static_cast<int64_t>(t + u * G) * 16);
+      for (int u = 0; u < kKeep; ++u)
+        if (row_ok && c0 + u * G < pieces)
+          keep[u].load(p.x, e0 + static_cast<int64_t>(c0 + u * G) * 16);
+    };
+    float inv = 1.0f;
     if constexpr (kFmt == kNvfp4) {
+      // the row's maximum, last pieces first: the first kKeep stay in registers
       uint32_t am = 0;
-      if (row_ok) {
+      for (int c0 = (pieces - 1) / (kKeep * G) * (kKeep * G) + t; c0 >= 0; c0 -= kKeep * G) {
+        fetch(c0);
 #pragma unroll
         for (int u = 0; u < kKeep; ++u)
-          if (t + u * G < pieces) am = max(am, keep[u].amax_bits());
-        for (int c = t + kKeep * G; c < pieces; c += G) {
-          Raw16<kIn> r;
-          r.load(p.x, e0 + static_cast<int64_t>(c) * 16);
-          am = max(am, r.amax_bits());
-        }
+          if (row_ok && c0 + u * G < pieces) am = max(am, keep[u].amax_bits());
       }
       am = __reduce_max_sync(0xFFFFFFFFu, am);
       if constexpr (G > 32) {
@@ -192,6 +197,8 @@ __global__ void __launch_bounds__(kQ4Threads) quantize_fp4_kernel(const QuantFp4
                    : fmaxf(__fdiv_rn(__uint_as_float(am), kFp4RowMax), 7.52316385e-37f);  // 2^-120
       inv = __frcp_rn(s);
       if (row_ok && t == 0) p.row_scale[m] = s;
+    } else {
+      fetch(t);
     }
     if (!row_ok) continue;  // whole warps (G is a multiple of 32)
     // Piece c of the row. Lanes of a group of eight pieces come together (pieces_pad and G are
@@ -237,13 +244,11 @@ __global__ void __launch_bounds__(kQ4Threads) quantize_fp4_kernel(const QuantFp4
         }
       }
     };
+    for (int c0 = t; c0 < pieces_pad; c0 += kKeep * G) {
+      if (c0 != t) fetch(c0);
 #pragma unroll
-    for (int u = 0; u < kKeep; ++u)
-      if (t + u * G < pieces_pad) encode(t + u * G, keep[u]);
-    for (int c = t + kKeep * G; c < pieces_pad; c += G) {
-      Raw16<kIn> r = {};
-      if (c < pieces) r.load(p.x, e0 + static_cast<int64_t>(c) * 16);
-      encode(c, r);
+      for (int u = 0; u < kKeep; ++u)
+        if (c0 + u * G < pieces_pad) encode(c0 + u * G, keep[u]);
     }
   }
   if (bad) atomicOr(p.err, kErrNonFinite);
@@ -287,48 +292,65 @@ __device__ __forceinline__ float e8m0_value(uint32_t b) {
 }
 
 // Dequantiser: out (M, K) = (code * block scale) * (row scale * tensor scale), the first product
-// exact. One thread per 16 elements (8 code bytes in, 32 or 64 bytes out); bound by the bytes
-// written.
-template <int kFmt, int kOut>
+// exact. G threads share a row, each turn 16 bytes of output a thread (side by side); bound by the
+// bytes written.
+template <int kFmt, int kOut, int G>
 __global__ void __launch_bounds__(256)
     dequantize_fp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ tiled,
                           const float* __restrict__ row_scale, float tensor_scale,
-                          void* __restrict__ out, int64_t total, int pieces, int words) {
+                          uint8_t* __restrict__ out, int M, int K, int words) {
+  constexpr int kElems = kOut == 2 ? 4 : 8;      // per thread and turn
+  constexpr int kPer = (kFmt == kNvfp4 ? 16 : 32) / kElems;  // threads per block scale
+  constexpr int kTurns = 4;
+  const int t = threadIdx.x % G, groups = K / kElems;
   grid_dep_wait();
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t m = i / pieces;
-    const int c = static_cast<int>(i - m * pieces);
-    const uint32_t b = tiled[sf_tile_offset(m, kFmt == kNvfp4 ? c : c / 2, words)];
-    const float sc = kFmt == kNvfp4 ? e4m3_value(b) : e8m0_value(b);
+  for (int64_t m = static_cast<int64_t>(blockIdx.x) * (256 / G) + threadIdx.x / G; m < M;
+       m += static_cast<int64_t>(gridDim.x) * (256 / G)) {
     const float s = row_scale != nullptr ? __fmul_rn(row_scale[m], tensor_scale) : tensor_scale;
-    const uint2 q = reinterpret_cast<const uint2*>(codes)[i];
-    float v[16];
+    const uint8_t* src = codes + m * (K / 2);
+    const int64_t tile = sf_tile_offset(m, 0, words);
+    uint8_t* dst = out + m * K * (16 / kElems);
+    for (int g0 = t; g0 < groups; g0 += kTurns * G) {
+      uint32_t q[kTurns], b[kTurns];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t n = ((j < 8 ? q.x : q.y) >> (4 * (j & 7))) & 15u;
-      v[j] = __fmul_rn(__fmul_rn(e2m1_value(n), sc), s);
-    }
-    if constexpr (kOut == 2) {
-      float4* o = reinterpret_cast<float4*>(out) + i * 4;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-    } else {
-      uint32_t w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if constexpr (kOut == 0) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-          const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+      for (int u = 0; u < kTurns; ++u) {
+        const int g = g0 + u * G;
+        if (g < groups) {
+          q[u] = kElems == 8 ? reinterpret_cast<const uint32_t*>(src)[g]
+                             : reinterpret_cast<const uint16_t*>(src)[g];
+          const int sc = g / kPer;
+          b[u] = tiled[tile + static_cast<int64_t>(sc >> 2) * 512 + (sc & 3)];
         }
       }
-      uint4* o = reinterpret_cast<uint4*>(out) + i * 2;
-      o[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      o[1] = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u) {
+        const int g = g0 + u * G;
+        if (g >= groups) break;
+        const float sc = kFmt == kNvfp4 ? e4m3_value(b[u]) : e8m0_value(b[u]);
+        float v[kElems];
+#pragma unroll
+        for (int j = 0; j < kElems; ++j)
+          v[j] = __fmul_rn(__fmul_rn(e2m1_value((q[u] >> (4 * j)) & 15u), sc), s);
+        uint4 w;
+        if constexpr (kOut == 2) {
+          w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                         __float_as_uint(v[3]));
+        } else {
+          uint32_t h[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (kOut == 0) {
+              const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+              h[j] = *reinterpret_cast<const uint32_t*>(&x);
+            } else {
+              const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+              h[j] = *reinterpret_cast<const uint32_t*>(&x);
+            }
+          }
+          w = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        __stcs(reinterpret_cast<uint4*>(dst) + g, w);
+      }
     }
   }
 }

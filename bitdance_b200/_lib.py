@@ -113,8 +113,15 @@ def check(fn: str, status: int) -> None:
         raise BitdanceError(fn, status, status_text(status))
 
 
+_fns: dict = {}
+
+
 def call(fn: str, *args) -> int:
     """Call an int-returning entry point and raise BitdanceError on a non-zero status."""
-    st = getattr(load(), fn)(*args)
-    check(fn, st)
+    f = _fns.get(fn)
+    if f is None:
+        f = _fns[fn] = getattr(load(), fn)
+    st = f(*args)
+    if st != BD_OK:
+        check(fn, st)
     return st

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import call
-from .ops import EPILOGUES, _OUT, _need, _p, _stream, quantize_nvfp4, tensor_scale_of
+from .ops import EPILOGUES, _OUT, _need, quantize_nvfp4, tensor_scale_of
 
 FP4_FORMATS = {"nvfp4": _lib.BD_FP4_NVFP4, "mxfp4": _lib.BD_FP4_MXFP4}
 _BLOCK = {"nvfp4": 16, "mxfp4": 32}
@@ -46,14 +46,36 @@ def _scale_bytes(rows: int, K: int, fmt: str) -> int:
     return (rows + 127) // 128 * ((K // _BLOCK[fmt] + 3) // 4) * 512
 
 
-def _on(stream, device):
-    """Context in which new tensors belong to the stream the kernels run on (their memory is
-    reused in that stream's order)."""
+# These entry points serve single tokens, where a call's time is the host's: addresses go to the
+# library as integers, the current stream and device come from torch's C layer.
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _stream_ptr(stream) -> int:
     if stream is None:
-        return torch.cuda.stream(None)
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
+def _empty(shape, dtype, device, stream):
+    """A new tensor that belongs to the stream the kernels run on (its memory is reused in that
+    stream's order)."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
-    return torch.cuda.stream(stream)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _have(t, dtype, what: str, numel: int) -> None:
+    """``ops._need`` with its common case first."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.is_contiguous()
+            and t.numel() >= numel and t.get_device() == torch._C._cuda_getDevice()):
+        _need(t, dtype, what, numel)
 
 
 def _check_x4(x: torch.Tensor):
@@ -61,7 +83,7 @@ def _check_x4(x: torch.Tensor):
         raise ValueError("x must be a 2-D tensor (M, K)")
     if x.dtype not in _IN4:
         raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    _need(x, x.dtype, "x")
+    _have(x, x.dtype, "x", 0)
     M, K = x.shape
     if K == 0 or K % 32:
         raise ValueError(f"K must be a positive multiple of 32, got {K}")
@@ -72,10 +94,10 @@ def _check_operand(op: Fp4Operand, what: str) -> None:
     _fmt(op.fmt)
     if op.rows < 0 or op.K <= 0 or op.K % 32:
         raise ValueError(f"{what}: K must be a positive multiple of 32, got {op.K}")
-    _need(op.codes, torch.uint8, f"{what}.codes", op.rows * op.K // 2)
-    _need(op.scales, torch.uint8, f"{what}.scales", _scale_bytes(op.rows, op.K, op.fmt))
+    _have(op.codes, torch.uint8, f"{what}.codes", op.rows * op.K // 2)
+    _have(op.scales, torch.uint8, f"{what}.scales", _scale_bytes(op.rows, op.K, op.fmt))
     if op.row_scale is not None:
-        _need(op.row_scale, torch.float32, f"{what}.row_scale", op.rows)
+        _have(op.row_scale, torch.float32, f"{what}.row_scale", op.rows)
 
 
 def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", stream=None,
@@ -86,14 +108,13 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", stream=None,
     word and leaves its row undefined."""
     code = _fmt(fmt)
     M, K = _check_x4(x)
-    with _on(stream, x.device):
-        codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
-        scales = torch.empty(_scale_bytes(M, K, fmt), dtype=torch.uint8, device=x.device)
-        row_scale = None
-        if fmt == "nvfp4":
-            row_scale = torch.empty(M, dtype=torch.float32, device=x.device)
-    call("bd_quantize_fp4", _p(x), _IN4[x.dtype], code, _p(codes), None, _p(scales), _p(row_scale),
-         M, K, _lib.BD_GEMM_OVERLAP_PREV if overlap_prev else 0, _stream(stream))
+    device = x.device
+    codes = _empty((M, K // 2), torch.uint8, device, stream)
+    scales = _empty(_scale_bytes(M, K, fmt), torch.uint8, device, stream)
+    row_scale = _empty(M, torch.float32, device, stream) if fmt == "nvfp4" else None
+    call("bd_quantize_fp4", x.data_ptr(), _IN4[x.dtype], code, codes.data_ptr(), None,
+         scales.data_ptr(), _ptr(row_scale), M, K,
+         _lib.BD_GEMM_OVERLAP_PREV if overlap_prev else 0, _stream_ptr(stream))
     return Fp4Operand(codes, scales, M, K, fmt, row_scale)
 
 
@@ -102,11 +123,10 @@ def quantize_mxfp4(x: torch.Tensor, stream=None):
     ``quantize_fp4(x, "mxfp4")`` in the natural layout (the reference's quantize(x, E8M0, E2M1),
     vector_quant_error.py:283-319)."""
     M, K = _check_x4(x)
-    with _on(stream, x.device):
-        codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
-        e8m0 = torch.empty((M, K // 32), dtype=torch.uint8, device=x.device)
-    call("bd_quantize_fp4", _p(x), _IN4[x.dtype], _lib.BD_FP4_MXFP4, _p(codes), _p(e8m0), None,
-         None, M, K, 0, _stream(stream))
+    codes = _empty((M, K // 2), torch.uint8, x.device, stream)
+    e8m0 = _empty((M, K // 32), torch.uint8, x.device, stream)
+    call("bd_quantize_fp4", x.data_ptr(), _IN4[x.dtype], _lib.BD_FP4_MXFP4, codes.data_ptr(),
+         e8m0.data_ptr(), None, None, M, K, 0, _stream_ptr(stream))
     return codes, e8m0
 
 
@@ -125,9 +145,9 @@ def pack_fp4(codes: torch.Tensor, scales: torch.Tensor, fmt: str = "nvfp4",
     _need(scales, torch.uint8, "scales", rows * (K // _BLOCK[fmt]))
     if row_scale is not None:
         _need(row_scale, torch.float32, "row_scale", rows)
-    with _on(stream, codes.device):
-        tiled = torch.empty(_scale_bytes(rows, K, fmt), dtype=torch.uint8, device=codes.device)
-    call("bd_tile_scales_fp4", _p(scales), _p(tiled), rows, K, code, _stream(stream))
+    tiled = _empty(_scale_bytes(rows, K, fmt), torch.uint8, codes.device, stream)
+    call("bd_tile_scales_fp4", scales.data_ptr(), tiled.data_ptr(), rows, K, code,
+         _stream_ptr(stream))
     return Fp4Operand(codes, tiled, rows, K, fmt, row_scale, float(tensor_scale))
 
 
@@ -136,9 +156,12 @@ def quantize_weights_fp4(w: torch.Tensor, fmt: str = "nvfp4", stream=None) -> Fp
     fp32 scale for the tensor, read back to the host once); "mxfp4": ``quantize_fp4``."""
     if _fmt(fmt) == _lib.BD_FP4_MXFP4:
         return quantize_fp4(w, fmt, stream)
-    with _on(stream, w.device):
-        codes, scales, tstat = quantize_nvfp4(w, stream)
-        return pack_fp4(codes, scales, fmt, tensor_scale_of(tstat), stream=stream)
+    if stream is not None:  # quantize_nvfp4 allocates on the current stream
+        with torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else
+                               torch.cuda.ExternalStream(int(stream), device=w.device)):
+            return quantize_weights_fp4(w, fmt)
+    codes, scales, tstat = quantize_nvfp4(w)
+    return pack_fp4(codes, scales, fmt, tensor_scale_of(tstat))
 
 
 def dequantize_fp4(op: Fp4Operand, out_dtype=torch.float32, out: Optional[torch.Tensor] = None,
@@ -148,12 +171,12 @@ def dequantize_fp4(op: Fp4Operand, out_dtype=torch.float32, out: Optional[torch.
     if out_dtype not in _OUT:
         raise TypeError(f"unsupported output dtype {out_dtype}")
     if out is None:
-        with _on(stream, op.codes.device):
-            out = torch.empty((op.rows, op.K), dtype=out_dtype, device=op.codes.device)
-    _need(out, out_dtype, "out", op.rows * op.K)
-    call("bd_dequantize_fp4", _p(op.codes), _p(op.scales), _p(op.row_scale),
-         float(op.tensor_scale), _p(out), _OUT[out_dtype], FP4_FORMATS[op.fmt], op.rows, op.K, 0,
-         _stream(stream))
+        out = _empty((op.rows, op.K), out_dtype, op.codes.device, stream)
+    else:
+        _have(out, out_dtype, "out", op.rows * op.K)
+    call("bd_dequantize_fp4", op.codes.data_ptr(), op.scales.data_ptr(), _ptr(op.row_scale),
+         float(op.tensor_scale), out.data_ptr(), _OUT[out_dtype], FP4_FORMATS[op.fmt], op.rows,
+         op.K, 0, _stream_ptr(stream))
     return out
 
 
@@ -162,7 +185,7 @@ def _epilogue(epilogue: str, bias, N: int) -> int:
         raise ValueError(f"unknown epilogue {epilogue!r}")
     epi = EPILOGUES[epilogue]
     if bias is not None:
-        _need(bias, torch.bfloat16, "bias", N)
+        _have(bias, torch.bfloat16, "bias", N)
     if epi != _lib.BD_EPI_NONE and bias is None:
         raise ValueError(f"epilogue {epilogue!r} needs a bias")
     return epi
@@ -172,9 +195,8 @@ def _output(out, M: int, N: int, out_dtype, device, stream):
     if out_dtype not in _OUT:
         raise TypeError(f"unsupported output dtype {out_dtype}")
     if out is None:
-        with _on(stream, device):
-            return torch.empty((M, N), dtype=out_dtype, device=device)
-    _need(out, out_dtype, "out", M * N)
+        return _empty((M, N), out_dtype, device, stream)
+    _have(out, out_dtype, "out", M * N)
     return out
 
 
@@ -195,10 +217,11 @@ def w4a4_gemm(acts: Fp4Operand, weights: Fp4Operand, bias: Optional[torch.Tensor
     out = _output(out, M, N, out_dtype, acts.codes.device, stream)
     flags = (_lib.BD_GEMM_OVERLAP_PREV if overlap_prev else 0) | \
         (_lib.BD_GEMM_WEIGHTS_STATIC if weights_static else 0)
-    call("bd_w4a4_gemm", _p(out), _p(acts.codes), _p(acts.scales), _p(acts.row_scale),
-         _p(weights.codes), _p(weights.scales), _p(weights.row_scale),
-         float(acts.tensor_scale) * float(weights.tensor_scale), _p(bias), M, N, K,
-         FP4_FORMATS[acts.fmt], _OUT[out_dtype], epi, flags, _stream(stream))
+    call("bd_w4a4_gemm", out.data_ptr(), acts.codes.data_ptr(), acts.scales.data_ptr(),
+         _ptr(acts.row_scale), weights.codes.data_ptr(), weights.scales.data_ptr(),
+         _ptr(weights.row_scale), float(acts.tensor_scale) * float(weights.tensor_scale),
+         _ptr(bias), M, N, K, FP4_FORMATS[acts.fmt], _OUT[out_dtype], epi, flags,
+         _stream_ptr(stream))
     return out
 
 
@@ -218,11 +241,12 @@ def w4a4_linear(x: torch.Tensor, weights: Fp4Operand, bias: Optional[torch.Tenso
     out = _output(out, M, N, out_dtype, x.device, stream)
     if M == 0:
         return out
-    with _on(stream, x.device):
-        ws = torch.empty(_linear_workspace(M, K, weights.fmt), dtype=torch.uint8, device=x.device)
-    call("bd_w4a4_linear", _p(out), _p(x), _IN4[x.dtype], _p(weights.codes), _p(weights.scales),
-         _p(weights.row_scale), float(weights.tensor_scale), _p(bias), M, N, K,
-         FP4_FORMATS[weights.fmt], _OUT[out_dtype], epi, _p(ws), ws.numel(), _stream(stream))
+    nbytes = _linear_workspace(M, K, weights.fmt)
+    ws = _empty(nbytes, torch.uint8, x.device, stream)
+    call("bd_w4a4_linear", out.data_ptr(), x.data_ptr(), _IN4[x.dtype], weights.codes.data_ptr(),
+         weights.scales.data_ptr(), _ptr(weights.row_scale), float(weights.tensor_scale),
+         _ptr(bias), M, N, K, FP4_FORMATS[weights.fmt], _OUT[out_dtype], epi, ws.data_ptr(),
+         nbytes, _stream_ptr(stream))
     return out
 
 

@@ -9,8 +9,8 @@ import torch
 
 from . import _lib
 from ._lib import call
-from .fp4 import _on
-from .ops import _OUT, _need, _p, _stream, quantize_nvfp4
+from .fp4 import _empty, _have, _ptr, _stream_ptr
+from .ops import _OUT, quantize_nvfp4
 
 MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 64, 512, 16
 SCORINGS = {"softmax": _lib.BD_MOE_SOFTMAX, "sigmoid": _lib.BD_MOE_SIGMOID}
@@ -38,12 +38,15 @@ def quantize_moe_weights(gate_up: torch.Tensor, down: torch.Tensor, stream=None)
     E, two_i, H = gate_up.shape
     if two_i % 2 or down.shape != (E, H, two_i // 2):
         raise ValueError(f"gate_up {tuple(gate_up.shape)} and down {tuple(down.shape)} do not match")
+    if stream is not None:  # quantize_nvfp4 allocates on the current stream
+        with torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else
+                               torch.cuda.ExternalStream(int(stream), device=gate_up.device)):
+            return quantize_moe_weights(gate_up, down)
     parts = []
-    with _on(stream, gate_up.device):
-        for w in (gate_up, down):
-            q = [quantize_nvfp4(w[e], stream) for e in range(E)]
-            parts += [torch.stack([c for c, _, _ in q]), torch.stack([s for _, s, _ in q]),
-                      torch.stack([t[:1].view(torch.float32)[0] for _, _, t in q])]
+    for w in (gate_up, down):
+        q = [quantize_nvfp4(w[e]) for e in range(E)]
+        parts += [torch.stack([c for c, _, _ in q]), torch.stack([s for _, s, _ in q]),
+                  torch.stack([t[:1].view(torch.float32)[0] for _, _, t in q])]
     return MoeWeights(*parts)
 
 
@@ -52,7 +55,7 @@ def _check(x: torch.Tensor, w: MoeWeights, top_k: int):
         raise ValueError("x must be a 2-D tensor (tokens, H)")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
-    _need(x, x.dtype, "x")
+    _have(x, x.dtype, "x", 0)
     T, H = x.shape
     if w.gate_up.dim() != 3 or w.down.dim() != 3:
         raise ValueError("expert weights must be (E, rows, K/2)")
@@ -69,12 +72,12 @@ def _check(x: torch.Tensor, w: MoeWeights, top_k: int):
         raise ValueError(f"1 to {MOE_MAX_EXPERTS} experts, got {E}")
     if not 1 <= top_k <= min(MOE_MAX_TOP_K, E):
         raise ValueError(f"top_k must be in 1..{min(MOE_MAX_TOP_K, E)}, got {top_k}")
-    _need(w.gate_up, torch.uint8, "gate_up")
-    _need(w.gate_up_scales, torch.uint8, "gate_up_scales", E * two_i * (H // 16))
-    _need(w.gate_up_tensor_scale, torch.float32, "gate_up_tensor_scale", E)
-    _need(w.down, torch.uint8, "down")
-    _need(w.down_scales, torch.uint8, "down_scales", E * H * (inter // 16))
-    _need(w.down_tensor_scale, torch.float32, "down_tensor_scale", E)
+    _have(w.gate_up, torch.uint8, "gate_up", 0)
+    _have(w.gate_up_scales, torch.uint8, "gate_up_scales", E * two_i * (H // 16))
+    _have(w.gate_up_tensor_scale, torch.float32, "gate_up_tensor_scale", E)
+    _have(w.down, torch.uint8, "down", 0)
+    _have(w.down_scales, torch.uint8, "down_scales", E * H * (inter // 16))
+    _have(w.down_tensor_scale, torch.float32, "down_tensor_scale", E)
     return T, H, inter, E
 
 
@@ -89,19 +92,19 @@ def _workspace_bytes(T: int, H: int, inter: int, E: int, top_k: int) -> int:
         up(4 * pairs * inter) + up(pairs * ((inter + 255) // 256) * 1152) + 4 * H * max(pairs, 256)
 
 
-def _out_tensor(out, x: torch.Tensor, out_dtype):
+def _out_tensor(out, x: torch.Tensor, out_dtype, stream):
     dtype = x.dtype if out_dtype is None else out_dtype
     if dtype not in _OUT:
         raise TypeError(f"unsupported output dtype {dtype}")
     if out is None:
-        return torch.empty(x.shape, dtype=dtype, device=x.device)
-    _need(out, dtype, "out", x.numel())
+        return _empty(x.shape, dtype, x.device, stream)
+    _have(out, dtype, "out", x.numel())
     return out
 
 
 def _weight_args(w: MoeWeights):
-    return (_p(w.gate_up), _p(w.gate_up_scales), _p(w.gate_up_tensor_scale), _p(w.down),
-            _p(w.down_scales), _p(w.down_tensor_scale))
+    return (w.gate_up.data_ptr(), w.gate_up_scales.data_ptr(), w.gate_up_tensor_scale.data_ptr(),
+            w.down.data_ptr(), w.down_scales.data_ptr(), w.down_tensor_scale.data_ptr())
 
 
 def moe_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
@@ -116,14 +119,14 @@ def moe_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Ten
         raise ValueError("topk_ids and topk_weights must be (tokens, top_k)")
     top_k = topk_ids.shape[1]
     T, H, inter, E = _check(x, experts, top_k)
-    _need(topk_ids, torch.int32, "topk_ids")
-    _need(topk_weights, torch.float32, "topk_weights")
-    with _on(stream, x.device):
-        out = _out_tensor(out, x, out_dtype)
-        ws = torch.empty(_workspace_bytes(T, H, inter, E, top_k), dtype=torch.uint8, device=x.device)
-    call("bd_moe_experts", _p(out), _p(x), _IN_MOE[x.dtype], _p(topk_ids), _p(topk_weights),
-         *_weight_args(experts), T, H, inter, E, top_k, _OUT[out.dtype], _p(ws), ws.numel(),
-         _stream(stream))
+    _have(topk_ids, torch.int32, "topk_ids", 0)
+    _have(topk_weights, torch.float32, "topk_weights", 0)
+    out = _out_tensor(out, x, out_dtype, stream)
+    nbytes = _workspace_bytes(T, H, inter, E, top_k)
+    ws = _empty(nbytes, torch.uint8, x.device, stream)
+    call("bd_moe_experts", out.data_ptr(), x.data_ptr(), _IN_MOE[x.dtype], topk_ids.data_ptr(),
+         topk_weights.data_ptr(), *_weight_args(experts), T, H, inter, E, top_k, _OUT[out.dtype],
+         ws.data_ptr(), nbytes, _stream_ptr(stream))
     return out
 
 
@@ -145,16 +148,22 @@ def moe_layer(x: torch.Tensor, router: torch.Tensor, experts: MoeWeights, top_k:
         raise ValueError(f"router must be ({E}, {H}), got {tuple(router.shape)}")
     if router.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"router must be {x.dtype} or float32, got {router.dtype}")
-    _need(router, router.dtype, "router")
+    _have(router, router.dtype, "router", 0)
     if selection_bias is not None:
-        _need(selection_bias, torch.float32, "selection_bias", E)
-    with _on(stream, x.device):
-        out = _out_tensor(out, x, out_dtype)
-        ids = torch.empty((T, top_k), dtype=torch.int32, device=x.device)
-        weights = torch.empty((T, top_k), dtype=torch.float32, device=x.device)
-        ws = torch.empty(_workspace_bytes(T, H, inter, E, top_k), dtype=torch.uint8, device=x.device)
-    call("bd_moe_layer", _p(out), _p(ids), _p(weights), _p(x), _IN_MOE[x.dtype], _p(router),
-         _IN_MOE[router.dtype], _p(selection_bias), SCORINGS[scoring], 1 if renormalize else 0,
-         float(routed_scale), *_weight_args(experts), T, H, inter, E, top_k, _OUT[out.dtype],
-         _p(ws), ws.numel(), _stream(stream))
+        _have(selection_bias, torch.float32, "selection_bias", E)
+    out = _out_tensor(out, x, out_dtype, stream)
+    nbytes = _workspace_bytes(T, H, inter, E, top_k)
+    if return_routing:
+        ids = _empty((T, top_k), torch.int32, x.device, stream)
+        weights = _empty((T, top_k), torch.float32, x.device, stream)
+        ws = _empty(nbytes, torch.uint8, x.device, stream)
+        ids_at, weights_at = ids.data_ptr(), weights.data_ptr()
+    else:  # behind the workspace
+        ws = _empty(nbytes + 8 * T * top_k, torch.uint8, x.device, stream)
+        ids_at = ws.data_ptr() + nbytes
+        weights_at = ids_at + 4 * T * top_k
+    call("bd_moe_layer", out.data_ptr(), ids_at, weights_at, x.data_ptr(), _IN_MOE[x.dtype],
+         router.data_ptr(), _IN_MOE[router.dtype], _ptr(selection_bias), SCORINGS[scoring],
+         1 if renormalize else 0, float(routed_scale), *_weight_args(experts), T, H, inter, E,
+         top_k, _OUT[out.dtype], ws.data_ptr(), nbytes, _stream_ptr(stream))
     return (out, ids, weights) if return_routing else out

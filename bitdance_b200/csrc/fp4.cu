@@ -183,11 +183,12 @@ int launch_gemm_any(const GemmFp4Params& p, const uint8_t* a, const uint8_t* b, 
   const int64_t pair_tiles =
       static_cast<int64_t>((p.N + 255) / 256) * ((p.M + 255) / 256);
   if (p.M > 128 && 4 * pair_tiles >= d->sm_count) return launch_pair<kFmt>(p, a, b, overlap, d, s);
+  // else the smallest token tile that holds the batch (several tiles are of 128: a tile's scales are
+  // whole 128-row blocks)
   if (p.M <= 16) return launch_gemm<16, kFmt>(p, a, b, overlap, d, s);
   if (p.M <= 32) return launch_gemm<32, kFmt>(p, a, b, overlap, d, s);
   if (p.M <= 64) return launch_gemm<64, kFmt>(p, a, b, overlap, d, s);
-  if (p.M <= 128) return launch_gemm<128, kFmt>(p, a, b, overlap, d, s);
-  return launch_gemm<256, kFmt>(p, a, b, overlap, d, s);
+  return launch_gemm<128, kFmt>(p, a, b, overlap, d, s);
 }
 
 int check_gemm(const void* c, const void* bias, int M, int N, int K, int fmt, int out_dtype,

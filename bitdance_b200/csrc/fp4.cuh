@@ -148,8 +148,9 @@ struct QuantFp4Params {
 constexpr int kQ4Threads = 256;
 
 template <int kIn, int kFmt, int G>
-__global__ void __launch_bounds__(kQ4Threads, 2) quantize_fp4_kernel(const QuantFp4Params p) {
-  constexpr int kKeep = kIn == kInF32 ? 4 : 8;
+__global__ void __launch_bounds__(kQ4Threads, kIn == kInF32 ? 2 : 3)
+    quantize_fp4_kernel(const QuantFp4Params p) {
+  constexpr int kKeep = 4;
   __shared__ uint32_t part[2][kQ4Threads / 32];
   const int sub = threadIdx.x / G, t = threadIdx.x % G;
   const int pieces = p.K / 16;

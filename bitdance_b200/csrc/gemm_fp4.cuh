@@ -59,7 +59,7 @@ struct GemmFp4Cfg {
   static constexpr int kBudget = (kCtasPerSm == 2 ? 113 : 226) * 1024 - 2048 - 1024;
   static constexpr int kStages = kBudget / kStage > 8 ? 8 : kBudget / kStage;
   static constexpr int kRing = kStages * kStage;
-  // column slices of the partial exchange: [split][BN / split][128] fp32, over the ring
+  // partial exchange: [split][BN / split / 2][128][2] fp32, over the ring
   static_assert(BN * 128 * 4 <= kRing, "exchange buffer fits the ring");
   static constexpr int kSmemBytes = kRing + 2048 + 1024;
   // tensor memory: accumulator, then two sets of scale words
@@ -68,7 +68,7 @@ struct GemmFp4Cfg {
   static constexpr int kUsedCols = kSfCol0 + 2 * kSfSet;
   static constexpr int kTmemCols = kUsedCols <= 128 ? 128 : kUsedCols <= 256 ? 256 : 512;
   static_assert(kUsedCols <= 512, "tensor memory budget");
-  static_assert(BN % 16 == 0 && BN <= 256, "MMA N");
+  static_assert(BN % 16 == 0 && BN <= 128, "MMA N");
   static_assert(kStage % 1024 == 0 && kWBytes % 1024 == 0 && kTBytes % 1024 == 0,
                 "1 KB swizzle atoms");
 };
@@ -76,7 +76,7 @@ struct GemmFp4Cfg {
 struct GemmFp4Ctl {
   uint64_t full[8], empty[8], done;
   uint32_t tmem_base, abort_flag;
-  float tok_scale[256];
+  float tok_scale[128];
 };
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -84,9 +84,6 @@ __device__ __forceinline__ void cluster_arrive() {
 }
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
 __device__ __forceinline__ float activate(float v, int epi) {
@@ -236,13 +233,33 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
   ok = __syncthreads_and(ok) && !*abort_flag;
   tc_fence_after();
   const uint32_t taddr = tb + (static_cast<uint32_t>(32 * warp) << 16);
-  auto finish = [&](int j, float acc) {
-    const int m = m0 + j;
-    if (m >= p.M || n >= p.N) return;
-    float v = __fmul_rn(acc, ctl.tok_scale[j]);
-    if (p.row_scale_w != nullptr) v = __fmul_rn(v, wscale);
-    if (p.epilogue != 0) v = activate(__fadd_rn(v, bias), p.epilogue);
-    store_out(p.out, static_cast<int64_t>(m) * p.N + n, v, p.out_dtype);
+  // NC finished columns j .. of this thread's weight row: a warp's stores of a column are side by side
+  auto finish = [&](int j, auto& acc) {
+    constexpr int NC = sizeof(acc) / sizeof(acc[0]);
+    float v[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) v[i] = __fmul_rn(acc[i], ctl.tok_scale[j + i]);
+    if (p.row_scale_w != nullptr) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) v[i] = __fmul_rn(v[i], wscale);
+    }
+    if (p.epilogue != 0) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) v[i] = activate(__fadd_rn(v[i], bias), p.epilogue);
+    }
+    const int cols = min(NC, p.M - m0 - j);
+    if (n >= p.N) return;
+    const int64_t at = static_cast<int64_t>(m0 + j) * p.N + n;
+    auto store = [&](auto* out, auto convert) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (i < cols) out[at + static_cast<int64_t>(i) * p.N] = convert(v[i]);
+    };
+    if (p.out_dtype == 0)
+      store(static_cast<__nv_bfloat16*>(p.out), [](float x) { return __float2bfloat16_rn(x); });
+    else if (p.out_dtype == 1)
+      store(static_cast<__half*>(p.out), [](float x) { return __float2half_rn(x); });
+    else store(static_cast<float*>(p.out), [](float x) { return x; });
   };
   if (split == 1) {
     if (ok) {
@@ -252,35 +269,48 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
         uint32_t r[16];
         tmem_ld_x16(taddr + c0, r);
         tmem_ld_wait_x16(r);
+        float acc[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) finish(c0 + j, __uint_as_float(r[j]));
+        for (int j = 0; j < 16; ++j) acc[j] = __uint_as_float(r[j]);
+        finish(c0, acc);
       }
     }
   } else {
     // every CTA of the cluster is past its last MMA: the rings may be overwritten
     cluster_arrive();
     cluster_wait();
-    const int width = BN / split;  // columns per rank
-    float* part = reinterpret_cast<float*>(smem);
+    // partials to the owner of the columns, pairs of columns side by side: [rank][pair][row][2]
+    const int width = BN / split;  // columns per rank, at least two
+    const uint32_t part = smem_u32(smem);
+    const int row = 32 * warp + lane;
 #pragma unroll 1
     for (int c0 = 0; c0 < BN; c0 += 16) {
       uint32_t r[16];
       tmem_ld_x16(taddr + c0, r);
       tmem_ld_wait_x16(r);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int owner = (c0 + j) / width, col = (c0 + j) % width;
-        const uint32_t at = smem_u32(part + (rank * width + col) * 128 + 32 * warp + lane);
-        st_shared_cluster_f32(mapa_shared(at, owner), ok ? __uint_as_float(r[j]) : 0.0f);
+      for (int j = 0; j < 16; j += 2) {
+        const int owner = (c0 + j) / width, pair = ((c0 + j) % width) / 2;
+        const uint32_t at = part + ((rank * (width / 2) + pair) * 128 + row) * 8;
+        asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(mapa_shared(at, owner)),
+                     "r"(ok ? r[j] : 0u), "r"(ok ? r[j + 1] : 0u)
+                     : "memory");
       }
     }
     cluster_arrive();
     cluster_wait();
     if (ok)
-      for (int col = 0; col < width; ++col) {
-        float acc = 0.0f;
-        for (int s = 0; s < split; ++s) acc += part[(s * width + col) * 128 + 32 * warp + lane];
-        finish(rank * width + col, acc);
+      for (int pair = 0; pair < width / 2; ++pair) {
+        float acc[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          if (s < split) {
+            const float2 v = *reinterpret_cast<const float2*>(
+                smem + ((s * (width / 2) + pair) * 128 + row) * 8);
+            acc[0] += v.x;
+            acc[1] += v.y;
+          }
+        finish(rank * width + 2 * pair, acc);
       }
   }
   tc_fence_before();

@@ -349,8 +349,9 @@ struct PairFp4Cfg {
   static constexpr int kStages = 5;
   static constexpr int kSmem = kStages * kStage + 1024;
   static constexpr int kSfSet = 12 * kWords;      // scale words of a stage in tensor memory
+  static constexpr int kBatch = 2;                // stages whose scales are copied at once
   static constexpr int kSfCol0 = 256;
-  static_assert(kSfCol0 + 2 * kSfSet <= 512, "tensor memory budget");
+  static_assert(kSfCol0 + 2 * kBatch * kSfSet <= 512, "tensor memory budget");
   static_assert(kStage % 1024 == 0, "1 KB swizzle atoms");
 };
 
@@ -448,32 +449,57 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           break;
         aph ^= 1u;
         tc_fence_after();
-        for (int k = 0; k < chunks; ++k) {
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl.full[r.slot]), r.phase,
-                                                             p.err, kErrWaitTma, abort_flag))))
-            break;
+        // kBatch stages at a time: their scale copies, then their MMAs. Every change between copies
+        // and MMAs costs the tensor core about 100 cycles (copies issued between the MMAs of the
+        // stage before took 1.6 times as long).
+        for (int k0 = 0; k0 < chunks && ok; k0 += Cfg::kBatch) {
+          uint32_t st[Cfg::kBatch], free[Cfg::kBatch];
+#pragma unroll
+          for (int b = 0; b < Cfg::kBatch; ++b) {
+            if (k0 + b >= chunks) break;
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait<true>(smem_u32(&ctl.full[r.slot]), r.phase,
+                                                               p.err, kErrWaitTma, abort_flag))))
+              break;
+            st[b] = smem_u32(smem + r.slot * Cfg::kStage);
+            free[b] = smem_u32(&ctl.empty[r.slot]);
+            r.next();
+          }
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t st = smem_u32(smem + r.slot * Cfg::kStage);
-          const uint32_t sft = tb + Cfg::kSfCol0 + set * Cfg::kSfSet, sfw = sft + 4 * Cfg::kWords;
-          const int words = min(Cfg::kWords, p.words - k * Cfg::kWords);
-          const int steps = min(4, (p.K - k * kF4ChunkK + 63) / 64);
+          const uint32_t sf = tb + Cfg::kSfCol0 + set * Cfg::kBatch * Cfg::kSfSet;
           if (elect_one()) {
-            for (int w = 0; w < words; ++w) {
-              tmem_cp_32x128b_x4_pair(sft + 4 * w, sdesc_sf(st + Cfg::oSt + 512 * w));
-              tmem_cp_32x128b_x4_pair(sfw + 8 * w, sdesc_sf(st + Cfg::oSw + 512 * w));
-              tmem_cp_32x128b_x4_pair(sfw + 8 * w + 4, sdesc_sf(st + Cfg::oSw + Cfg::kSf + 512 * w));
+#pragma unroll
+            for (int b = 0; b < Cfg::kBatch; ++b) {
+              if (k0 + b >= chunks) break;
+              const uint32_t sft = sf + b * Cfg::kSfSet, sfw = sft + 4 * Cfg::kWords;
+#pragma unroll
+              for (int w = 0; w < Cfg::kWords; ++w) {  // (words past a row's last: copied, not used)
+                tmem_cp_32x128b_x4_pair(sft + 4 * w, sdesc_sf(st[b] + Cfg::oSt + 512 * w));
+                tmem_cp_32x128b_x4_pair(sfw + 8 * w, sdesc_sf(st[b] + Cfg::oSw + 512 * w));
+                tmem_cp_32x128b_x4_pair(sfw + 8 * w + 4,
+                                        sdesc_sf(st[b] + Cfg::oSw + Cfg::kSf + 512 * w));
+              }
             }
-            for (int kk = 0; kk < steps; ++kk) {
-              const int w = kNv ? kk : kk >> 1;
-              const uint32_t idesc = idesc_mxf4(256, 256, !kNv, kNv ? 0 : 2 * (kk & 1));
-              mma_mxf4_ss<kNv, true>(tb, sdesc_sw128(st + kk * 32), sdesc_sw128(st + Cfg::oW + kk * 32),
-                                     idesc, sft + 4 * w, sfw + 8 * w, (k > 0 || kk > 0) ? 1u : 0u);
+#pragma unroll
+            for (int b = 0; b < Cfg::kBatch; ++b) {
+              const int k = k0 + b;
+              if (k >= chunks) break;
+              const uint32_t sft = sf + b * Cfg::kSfSet, sfw = sft + 4 * Cfg::kWords;
+              const int steps = min(4, (p.K - k * kF4ChunkK + 63) / 64);
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) {
+                if (kk >= steps) break;
+                const int w = kNv ? kk : kk >> 1;
+                const uint32_t idesc = idesc_mxf4(256, 256, !kNv, kNv ? 0 : 2 * (kk & 1));
+                mma_mxf4_ss<kNv, true>(tb, sdesc_sw128(st[b] + kk * 32),
+                                       sdesc_sw128(st[b] + Cfg::oW + kk * 32), idesc, sft + 4 * w,
+                                       sfw + 8 * w, (k > 0 || kk > 0) ? 1u : 0u);
+              }
+              tc_commit_pair(free[b], 3);
+              if (k + 1 == chunks) tc_commit_pair(smem_u32(&ctl.acc_full), 3);
             }
-            tc_commit_pair(smem_u32(&ctl.empty[r.slot]), 3);
-            if (k + 1 == chunks) tc_commit_pair(smem_u32(&ctl.acc_full), 3);
           }
           __syncwarp();
-          r.next();
           set ^= 1u;
         }
       }

@@ -62,14 +62,23 @@ cudaLaunchConfig_t config(int grid, int threads, int smem, cudaStream_t s, cudaL
   return cfg;
 }
 
+template <class X, class W, int TB, int parts>
+int launch_route_parts(const MoeRouteParams& p, cudaStream_t s) {
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg =
+      config((p.T + TB - 1) / TB * kRouteCluster, kMoeThreads,
+             (parts + 1) * p.E * static_cast<int>(sizeof(double)), s, attr, kRouteCluster);
+  return cudaLaunchKernelEx(&cfg, moe_route_kernel<X, W, TB, parts>, p) == cudaSuccess
+             ? last_status()
+             : BD_ERR_CUDA;
+}
+
+// Eight parts of K per expert where one warp per expert leaves most of a CTA's warps idle (rows shorter
+// than one round of 8 x 32 lanes x 8 elements have nothing to split).
 template <class X, class W, int TB>
 int launch_route(const MoeRouteParams& p, cudaStream_t s) {
-  cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t cfg = config((p.T + TB - 1) / TB * kRouteCluster, kMoeThreads,
-                                        2 * p.E * static_cast<int>(sizeof(double)), s, attr,
-                                        kRouteCluster);
-  return cudaLaunchKernelEx(&cfg, moe_route_kernel<X, W, TB>, p) == cudaSuccess ? last_status()
-                                                                              : BD_ERR_CUDA;
+  return p.E <= 4 * kRouteCluster && p.H >= 2048 ? launch_route_parts<X, W, TB, 8>(p, s)
+                                                 : launch_route_parts<X, W, TB, 1>(p, s);
 }
 
 template <class X, class W>

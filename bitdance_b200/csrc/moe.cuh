@@ -166,7 +166,6 @@ template <class X>
 __device__ void moe_convert_token(const X* x, uint8_t* xs, float* x_scale, int t, int H,
                                   uint32_t* part) {
   const X* row = x + static_cast<int64_t>(t) * H;
-  uint8_t* img = xs + t * moe_image_row(H);
   uint32_t am = 0;
   for (int c = threadIdx.x; c < H / 8; c += kMoeThreads) {
     float v[8];
@@ -187,7 +186,7 @@ __device__ void moe_convert_token(const X* x, uint8_t* xs, float* x_scale, int t
     load8(row + 16 * b + 8, *reinterpret_cast<float(*)[8]>(v + 8));
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] *= up;
-    moe_digits(v, img, b);
+    moe_digits(v, xs + t * moe_image_row(H), b);
   }
   if (threadIdx.x == 0) x_scale[t] = moe_row_factor(am);
 }
@@ -224,14 +223,17 @@ __device__ __forceinline__ double block_reduce(double v, double* part) {
 }
 
 // Router: a cluster of eight CTAs per TB tokens; a CTA takes every eighth expert (every seventh, and
-// the last CTA none, where one token's digits keep that CTA busy), one per warp at a time, for all TB
-// tokens; the logits of token i of the group go to CTA i's shared memory, which selects for it. Two
-// logits may be arbitrarily close, so they are kept in 64 bits: eight products are summed in fp32 and
-// added to a double, an error near 1e-8 of the logits' spread. Bound by the latency of one pass over
-// the router weights and of the selection's steps.
-template <class X, class W, int TB>
+// the last CTA none, where one token's digits keep that CTA busy) for all TB tokens, a warp per expert
+// and part of K (of eight where the experts are few: 8 of them, H 4096, 64 tokens took
+// 14.8 us for 21.4); the partial logits of token i of the group go to CTA i's shared
+// memory, which adds and selects for it. Two logits may be arbitrarily close, so
+// they are kept in 64 bits: eight products are summed in fp32 and added to a double, an error near 1e-8
+// of the logits' spread. Bound by latency: of one pass over the router weights, of the selection's
+// steps. (A share of every token's digits in each CTA took longer than one CTA's whole token beside
+// the others' products: 17 for 14 us at seven tokens.)
+template <class X, class W, int TB, int parts>
 __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRouteParams p) {
-  extern __shared__ double sh[];  // scores [E] (logits of this CTA's token), keys [E]
+  extern __shared__ double sh[];  // partial logits [parts][E] of this CTA's token, then keys [E]
   __shared__ double part[kMoeWarps];
   __shared__ uint32_t upart[kMoeWarps];
   __shared__ double sel[kMoeMaxTopK];
@@ -247,11 +249,13 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
   cluster_sync_all();  // every CTA of the cluster runs: its shared memory may be written
   const int pieces = p.H / 8;
   constexpr int kRanks = TB == 1 ? kRouteCluster - 1 : kRouteCluster;
-  for (int e = rank + kRanks * warp; rank < kRanks && e < p.E; e += kRanks * kMoeWarps) {
+  const int experts = rank < kRanks ? (p.E - static_cast<int>(rank) + kRanks - 1) / kRanks : 0;
+  for (int job = warp; job < experts * parts; job += kMoeWarps) {
+    const int e = static_cast<int>(rank) + kRanks * (job / parts), q = job % parts;
     double acc[TB] = {};
     const W* row = wr + static_cast<int64_t>(e) * p.H;
 #pragma unroll(TB == 1 ? 8 : 4)
-    for (int c = lane; c < pieces; c += 32) {
+    for (int c = 32 * q + lane; c < pieces; c += 32 * parts) {
       float w[8];
       load8(row + 8 * c, w);
 #pragma unroll
@@ -270,7 +274,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xFFFFFFFFu, acc[i], o);
       if (lane == 0) {
-        const uint32_t at = mapa_shared(smem_u32(&sh[e]), i);
+        const uint32_t at = mapa_shared(smem_u32(&sh[q * p.E + e]), i);
         asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(acc[i]) : "memory");
       }
     }
@@ -285,7 +289,12 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
   // rounds), else score + bias; a NaN ranks last. Where the weights are renormalised softmax scores
   // ranked by logit, exp(logit - largest) of the chosen ones is all that is needed.
   double* score = sh;
-  double* key = sh + p.E;
+  double* key = sh + parts * p.E;
+  if constexpr (parts > 1) {
+    for (int e = threadIdx.x; e < p.E; e += kMoeThreads)
+      for (int q = 1; q < parts; ++q) score[e] += sh[q * p.E + e];
+    __syncthreads();
+  }
   const bool lazy = !p.sigmoid && p.bias == nullptr && p.renormalize;
   if (!lazy) {
     double m = 0.0, z = 1.0;

@@ -272,6 +272,21 @@ def test_scorings(scoring, renormalize, with_bias, router):
 
 
 @gpu
+@pytest.mark.parametrize("T", [1, 16, 17, 33])
+@pytest.mark.parametrize("H,E", [(2048, 32), (2176, 7), (2048, 33)])
+def test_routing_where_experts_are_few_and_rows_long(T, H, E):
+    """The router may split K there; the sigmoid of every chosen logit shows in its weight."""
+    import bitdance_b200 as bd
+    case = Case(T, H, 128, E, torch.bfloat16, seed=T + H + E)
+    y, ids, weights = bd.moe_layer(case.x, case.router, case.w, 5, scoring="sigmoid",
+                                   renormalize=False, return_routing=True)
+    want_ids, want = routing(case, 5, "sigmoid", renormalize=False)
+    assert torch.equal(ids, want_ids)
+    assert weights_match(weights, want, case)
+    check(y, case, ids, weights)
+
+
+@gpu
 def test_equal_scores_take_the_lowest_experts():
     import bitdance_b200 as bd
     case = Case(6, 256, 128, 48, seed=4)

@@ -155,8 +155,10 @@ __global__ void __launch_bounds__(kQ4Threads, kIn == kInF32 ? 2 : 3)
   const int sub = threadIdx.x / G, t = threadIdx.x % G;
   const int pieces = p.K / 16;
   const int pieces_pad = (pieces + 7) & ~7;  // whole groups of eight: lanes past the end pad tiles
-  grid_dep_launch_dependents();
+  // In this order: a W4A4 GEMM behind this grid may load weights before it waits, and they may be the
+  // output of the grid before this one.
   grid_dep_wait();
+  grid_dep_launch_dependents();
   bool bad = false;
   int flip = 0;
   for (int64_t m0 = static_cast<int64_t>(blockIdx.x) * (kQ4Threads / G); m0 < p.M;

@@ -325,9 +325,8 @@ int bd_w4a4_gemm(void* c, const uint8_t* a, const uint8_t* a_scales, const float
                  int out_dtype, int epilogue, unsigned flags, bd_stream_t stream);
 
 /* bd_quantize_fp4 of x (M, K), then bd_w4a4_gemm, launched so that the GEMM streams its first
- * weights while the quantiser runs (b and b_scales must not be written by work still running
- * on the stream). workspace: bd_query_w4a4_linear_workspace bytes, 256-byte aligned, contents
- * irrelevant before and after; concurrent calls must not share one. */
+ * weights while the quantiser runs. workspace: bd_query_w4a4_linear_workspace bytes, 256-byte
+ * aligned, contents irrelevant before and after; concurrent calls must not share one. */
 size_t bd_query_w4a4_linear_workspace(int M, int K, int fmt);
 int bd_w4a4_linear(void* c, const void* x, int x_dtype, const uint8_t* b, const uint8_t* b_scales,
                    const float* b_row_scale, float tensor_scale, const void* bias, int M, int N,

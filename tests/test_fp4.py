@@ -364,3 +364,24 @@ def test_streams_and_graph_replay():
         torch.cuda.synchronize()
         assert torch.equal(c, want[j])
     assert bd.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_linear_right_behind_its_weights(fmt):
+    """Weights written by the launch just before the linear: its early loads wait for them."""
+    import bitdance_b200 as bd
+    x = matrix(3, 2048, torch.bfloat16, 1, 0.5).cuda()
+    ws = [matrix(4096, 2048, torch.float32, s, 0.5).cuda() for s in range(3)]
+    want = []
+    for w in ws:
+        q = bd.quantize_fp4(w, fmt)
+        torch.cuda.synchronize()
+        want.append(bd.w4a4_linear(x, q))
+        torch.cuda.synchronize()
+    del q
+    got = []
+    for i in range(24):  # the operand's memory is reused from turn to turn
+        got.append(bd.w4a4_linear(x, bd.quantize_fp4(ws[i % 3], fmt, overlap_prev=i % 2 == 1)))
+    for i, c in enumerate(got):
+        assert torch.equal(c, want[i % 3])

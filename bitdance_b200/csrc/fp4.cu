@@ -139,7 +139,7 @@ int launch_gemm(GemmFp4Params p, const uint8_t* a, const uint8_t* b, bool overla
   const int chunks = (p.K + kF4ChunkK - 1) / kF4ChunkK;
   int split = 1;
   while (split < 8 && tiles * split * 2 <= static_cast<int64_t>(d->sm_count) * Cfg::kCtasPerSm &&
-         chunks >= split * 4)
+         chunks >= split * 2)
     split *= 2;
   if (tiles * split > 0x7FFFFFFF) return BD_ERR_SHAPE;
   CUtensorMap mw, mt;

@@ -299,19 +299,35 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
     }
     cluster_arrive();
     cluster_wait();
-    if (ok)
-      for (int pair = 0; pair < width / 2; ++pair) {
-        float acc[2] = {0.0f, 0.0f};
+    // columns 2 pair .. of this rank: the partials in rank order, four pairs at a time where there are
+    // as many (one pair's epilogue is a chain of dependent steps, and a warp has its scheduler alone)
+    auto join = [&](int pair, auto& acc) {
+      constexpr int NP = sizeof(acc) / sizeof(acc[0]) / 2;
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
-          if (s < split) {
+      for (int s = 0; s < 8; ++s)
+        if (s < split) {
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
             const float2 v = *reinterpret_cast<const float2*>(
-                smem + ((s * (width / 2) + pair) * 128 + row) * 8);
-            acc[0] += v.x;
-            acc[1] += v.y;
+                smem + ((s * (width / 2) + pair + i) * 128 + row) * 8);
+            acc[2 * i] = s ? acc[2 * i] + v.x : v.x;
+            acc[2 * i + 1] = s ? acc[2 * i + 1] + v.y : v.y;
           }
-        finish(rank * width + 2 * pair, acc);
+        }
+      finish(rank * width + 2 * pair, acc);
+    };
+    if (ok && width % 8 == 0) {
+#pragma unroll 1
+      for (int pair = 0; pair < width / 2; pair += 4) {
+        float acc[8];
+        join(pair, acc);
       }
+    } else if (ok) {
+      for (int pair = 0; pair < width / 2; ++pair) {
+        float acc[2];
+        join(pair, acc);
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();

@@ -560,10 +560,12 @@ struct MoeCfg {
 };
 
 struct MoeCtl {
-  uint64_t full[4], empty[4], raw_full[4], acc_full, acc_empty, qfull[kMoeQueue], qempty[kMoeQueue], drain;
+  uint64_t full[4], empty[4], raw_full[4], acc_full, acc_empty, qfull[kMoeQueue], qempty[kMoeQueue], drain,
+      down_ready;
   uint32_t queue[kMoeQueue];
   uint32_t abort_flag, tmem_base;
   uint32_t warps;  // epilogue warps that finished their part of a down task
+  uint32_t digits_seen;  // down tasks whose digits are there, or kMoeAllSeen
 };
 constexpr int kMoeQueueReaders = kMoeScaleWarps + kMoeDigitWarps + 1 + kMoeEpiWarps;
 
@@ -636,12 +638,22 @@ __device__ __forceinline__ bool moe_next_task(MoeTask& t, RingPos<kMoeQueue>& q,
   return true;
 }
 
-// A whole warp: until *counter >= target, bounded.
+// A whole warp: until *counter >= target (counter of this grid, or kCta of this CTA), bounded. A counter
+// of the grid is read again only after a pause: a poll takes its turn in the same L2 slice as the
+// additions it waits for. (One warp per CTA polls for the others where they wait for the same: with all
+// eight epilogue warps of 148 CTAs polling, the combine phase began 1.5 us later.)
+template <bool kCta>
 __device__ __forceinline__ bool moe_wait(const uint32_t* counter, uint32_t target, MoeCtl& ctl,
                                          uint32_t* err) {
   bool ok = true;
   const long long c0 = clock64();
-  while (ld_acquire_gpu(counter) < target) {
+  while (true) {
+    uint32_t v;
+    if constexpr (kCta)
+      asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(counter)) : "memory");
+    else
+      v = ld_acquire_gpu(counter);
+    if (v >= target) break;
     if (*reinterpret_cast<volatile uint32_t*>(&ctl.abort_flag)) {
       ok = false;
       break;
@@ -652,8 +664,18 @@ __device__ __forceinline__ bool moe_wait(const uint32_t* counter, uint32_t targe
       ok = false;
       break;
     }
+    __nanosleep(kCta ? 20 : 60);
   }
   return __all_sync(0xFFFFFFFFu, ok);
+}
+constexpr uint32_t kMoeAllSeen = 1u << 30;
+
+// A warp's stores, then the count (lane 0's release covers what the others stored before the
+// __syncwarp).
+__device__ __forceinline__ void moe_count(uint32_t* counter) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0)
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
 }
 
 __device__ __forceinline__ uint32_t moe_ticket(uint32_t* counter) {
@@ -664,11 +686,15 @@ __device__ __forceinline__ uint32_t moe_ticket(uint32_t* counter) {
 // An epilogue warp's part of a down task is done: its stores before the count. The last of eight
 // parts counts for the CTA (parts of two tasks may mix; the phase's total is what is waited for).
 __device__ __forceinline__ void moe_count_down(uint32_t* counter, uint32_t* warps) {
-  __threadfence();
   __syncwarp();
-  if ((threadIdx.x & 31) == 0 && (atomicAdd(warps, 1u) & (kMoeEpiWarps - 1)) == kMoeEpiWarps - 1) {
-    __threadfence();
-    atomicAdd(counter, 1u);
+  if ((threadIdx.x & 31) == 0) {
+    uint32_t before;
+    asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;"
+                 : "=r"(before)
+                 : "r"(smem_u32(warps))
+                 : "memory");
+    if ((before & (kMoeEpiWarps - 1)) == kMoeEpiWarps - 1)
+      asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
   }
 }
 
@@ -743,7 +769,9 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
       mbar_init(smem_u32(&ctl.qempty[s]), kMoeQueueReaders);
     }
     mbar_init(smem_u32(&ctl.drain), 1);
+    mbar_init(smem_u32(&ctl.down_ready), 1);
     ctl.warps = 0;
+    ctl.digits_seen = 0;
     fence_mbar_init();
   }
   if (warp == kMoeMmaWarp) {
@@ -883,11 +911,25 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     const int part = warp - kMoeDigitWarp0;
     constexpr int kSets = Cfg::kBlocks;
     bool ready = false;  // the digits of all experts
+    uint32_t seen = 0;
     while (moe_next_task(t, q, ctl, p.err) && t.phase != 2) {
       const MoeGeom gm = sh.geom(p, pl, t);
       if (t.phase == 1 && !ready) {
-        ready = __all_sync(0xFFFFFFFFu, ld_acquire_gpu(p.counters + kMoeDigitsDone) >= total_d);
-        if (!ready && !moe_wait(digits_done + gm.a, pl.dig[gm.a + 1] - pl.dig[gm.a], ctl, p.err)) break;
+        ++seen;
+        if (part == 0) {
+          ready = __all_sync(0xFFFFFFFFu, ld_acquire_gpu(p.counters + kMoeDigitsDone) >= total_d);
+          if (!ready &&
+              !moe_wait<false>(digits_done + gm.a, pl.dig[gm.a + 1] - pl.dig[gm.a], ctl, p.err))
+            break;
+          if (lane == 0)
+            asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(&ctl.digits_seen)),
+                         "r"(ready ? kMoeAllSeen : seen)
+                         : "memory");
+        } else {
+          if (!moe_wait<true>(&ctl.digits_seen, seen, ctl, p.err)) break;
+          ready = __all_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t*>(&ctl.digits_seen) ==
+                                              kMoeAllSeen);
+        }
         // written by ordinary stores of this grid; the bulk copies read through the async proxy
         asm volatile("fence.proxy.async;" ::: "memory");
       }
@@ -1017,7 +1059,7 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
         if (pl.dig[mid] <= k) a = mid;
         else hi = mid;
       }
-      if (!moe_wait(gate_up_done + a, sh.blocks1 * kMoeEpiWarps, ctl, p.err)) break;
+      if (!moe_wait<false>(gate_up_done + a, sh.blocks1 * kMoeEpiWarps, ctl, p.err)) break;
       const int e = pl.act[a];
 #pragma unroll 1
       for (int i = 0; i < kMoeDigitBlocks; i += 32) {
@@ -1039,12 +1081,8 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
         }
       }
       asm volatile("fence.proxy.async;" ::: "memory");
-      __threadfence();
-      __syncwarp();
-      if (lane == 0) {
-        atomicAdd(digits_done + a, 1u);
-        atomicAdd(p.counters + kMoeDigitsDone, 1u);
-      }
+      moe_count(digits_done + a);
+      moe_count(p.counters + kMoeDigitsDone);
     }
   } else {
     // ------------------------------------------------------------------------------ epilogue
@@ -1173,19 +1211,19 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
         }
       }
       if (!ok) break;
-      if (t.phase == 0) {
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) atomicAdd(gate_up_done + gm.a, 1u);
-      } else {
-        moe_count_down(p.counters + kMoeDownDone, &ctl.warps);
-      }
+      if (t.phase == 0) moe_count(gate_up_done + gm.a);
+      else moe_count_down(p.counters + kMoeDownDone, &ctl.warps);
     }
 
     // combine: 128 outputs of a token per warp and turn, dealt by index (no one waits for these),
     // eight partial sums in flight
     const int blocks3 = p.H / 128, terms = p.k * sh.slices;
-    ok = ok && moe_wait(p.counters + kMoeDownDone, sh.total2, ctl, p.err);
+    if (warp == kMoeEpiWarp0) {
+      ok = ok && moe_wait<false>(p.counters + kMoeDownDone, sh.total2, ctl, p.err);
+      if (ok && lane == 0) mbar_arrive(smem_u32(&ctl.down_ready));
+    } else {
+      ok = ok && moe_warp_wait(ctl.down_ready, 0, kErrWaitOperand, ctl, p.err);
+    }
     for (int task = blockIdx.x + gridDim.x * (warp - kMoeEpiWarp0); ok && task < p.T * blocks3;
          task += gridDim.x * kMoeEpiWarps) {
       const int tok = task / blocks3, h0 = (task % blocks3) * 128 + 4 * lane;

@@ -846,6 +846,13 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
       const int pitch = gm.K / 16, half = 8 * (lane & 1);
       const uint8_t* base = (t.phase == 0 ? p.s13 : p.s2) + (lane >> 1) * pitch + half;
       const uint8_t *sa = base + gm.ra * pitch, *sb = base + gm.rb * pitch;
+      if (lane < (gm.two ? 2 : 1)) {  // all of the task's scales towards L2: 16 bytes a row come slowly
+        const uint8_t* rows = (t.phase == 0 ? p.s13 : p.s2) + (lane == 0 ? gm.ra : gm.rb) * pitch;
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
+                         reinterpret_cast<uint64_t>(rows) & ~15ull),
+                     "r"(128 * pitch)
+                     : "memory");
+      }
       for (int n0 = 0; n0 < gm.cnt && ok; n0 += TOK)
         for (int c = gm.c0; c < gm.c1; ++c) {
           // (an empty stage's raw scales are read too: they were repacked before its MMAs)

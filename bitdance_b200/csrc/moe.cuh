@@ -536,6 +536,11 @@ constexpr int kMoeEpiWarp0 = kMoeMakeWarp0 + kMoeMakeWarps, kMoeEpiWarps = 8;
 constexpr int kMoeExpertThreads = 32 * (kMoeEpiWarp0 + kMoeEpiWarps);
 constexpr int kMoeQueue = 4;
 
+// 32 lanes x 16 columns of a digit sum: 20 words a lane, 16 more behind every eight lanes, so that
+// neither the stores nor the loads have bank conflicts.
+constexpr int kMoeSumLane = 20, kMoeSumToken = 8 * kMoeSumLane + 16;
+constexpr int kMoeSumBytes = 4 * kMoeSumToken * 4;
+
 template <int TOK>
 struct MoeCfg {
   static constexpr bool kSwap = TOK <= 16;
@@ -549,7 +554,8 @@ struct MoeCfg {
   static constexpr int kStages = 3;
   static constexpr int kRaw = 256 * 16;                      // natural weight scales of a stage
   static constexpr int oRaw = kStages * kStage;
-  static constexpr int kSmem = oRaw + kStages * kRaw + 1024;
+  static constexpr int oSum = oRaw + kStages * kRaw;         // a digit sum's buffer per epilogue warp
+  static constexpr int kSmem = oSum + (kSwap ? kMoeEpiWarps * kMoeSumBytes : 0) + 1024;
   static constexpr int kSfCol0 = 2 * kN;                     // after the two tiles' accumulators
   static constexpr int kSfSet = 2 * 16 + kBlocks * 16;       // scale words of a stage in tensor memory
   static_assert(kSfCol0 + 2 * kSfSet <= 512, "tensor memory budget");
@@ -706,27 +712,30 @@ __device__ __forceinline__ float moe_sum8(const uint32_t* r) {
   return s;
 }
 
-// 16 columns of eight lanes' digits: lane p of the eight gets the sums over the eight lanes of columns
-// p and 8 + p (each step halves the columns a lane keeps, adding what the other half's lane had).
-__device__ __forceinline__ void moe_lane_sums(const uint32_t (&d)[16], float& s0, float& s1) {
+// 16 columns of eight lanes' digits: lane c of the eight gets the sums over them of columns 2 c and
+// 2 c + 1, by way of shared memory. (In registers, by three exchanges of halves, it took 14 shuffles
+// and 28 selects: with one to four tokens all of that is the work of one scheduler's warps, and the
+// accumulator is busy until it ends.)
+__device__ __forceinline__ float2 moe_lane_sums(const uint32_t (&d)[16], float* buf) {
   const int lane = threadIdx.x & 31;
-  float v[16];
+  float* own = buf + (lane >> 3) * kMoeSumToken;
+  uint4* dst = reinterpret_cast<uint4*>(own + (lane & 7) * kMoeSumLane);
+  if ((lane & 7) < kMoeDigitCount) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(d[i]);
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
-    const bool high = (lane & o) != 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < o; ++i) {
-        const float keep = high ? v[8 * h + o + i] : v[8 * h + i];
-        const float give = high ? v[8 * h + i] : v[8 * h + o + i];
-        v[8 * h + i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
-      }
+    for (int i = 0; i < 4; ++i) dst[i] = make_uint4(d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]);
   }
-  s0 = v[0];
-  s1 = v[8];
+  __syncwarp();
+  const float2* src = reinterpret_cast<const float2*>(own) + (lane & 7);
+  float2 v[kMoeDigitCount];
+#pragma unroll
+  for (int p = 0; p < kMoeDigitCount; ++p) v[p] = src[p * (kMoeSumLane / 2)];
+  __syncwarp();
+#pragma unroll
+  for (int p = kMoeDigitCount - 2; p >= 0; --p) {
+    v[p].x += v[p + 1].x;
+    v[p].y += v[p + 1].y;
+  }
+  return v[0];
 }
 
 // Four scale words (a row's 16 scales of a stage) into their tiles, 512 bytes apart.
@@ -1128,20 +1137,26 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
           // Lanes 8 i .. 8 i + 7 of a quarter: the digits of token 4 quarter + i; columns: weight
           // rows. Up: this group of four warps takes 64 hidden units, both tiles; down: the 128
           // rows of its own tile. Four pieces of 16 + 16 columns, summed over the digits so that
-          // lane p of eight ends with columns p and 8 + p of each 16.
+          // lane p of eight ends with columns 2 p and 2 p + 1 of each 16.
           const int c = 4 * quarter + (lane >> 3);
           const bool work = 4 * quarter < n && (up || group == 0 || gm.two);
-          float v[16];
+          // piece i of eight: 16 columns of the first tile (even i) or the second; a piece is loaded while
+          // the one before is summed
+          float2 v[8];
           if (work) {
+            float* buf = reinterpret_cast<float*>(smem + Cfg::oSum) +
+                         (warp - kMoeEpiWarp0) * (kMoeSumBytes / 4);
+            uint32_t d[2][16];
+            auto load = [&](int i) {
+              tmem_ld_x16(acc + (up ? 128 * (i & 1) + 64 * group + 16 * (i >> 1) : 128 * group + 16 * i),
+                          d[i & 1]);
+            };
+            load(0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t d0[16], d1[16];
-              tmem_ld_x16(acc + (up ? 64 * group + 16 * j : 128 * group + 32 * j), d0);
-              tmem_ld_x16(acc + (up ? 128 + 64 * group + 16 * j : 128 * group + 32 * j + 16), d1);
-              tmem_ld_wait_x16(d0);
-              tmem_ld_wait_x16(d1);
-              moe_lane_sums(d0, v[4 * j], v[4 * j + 1]);
-              moe_lane_sums(d1, v[4 * j + 2], v[4 * j + 3]);
+            for (int i = 0; i < 8; ++i) {
+              tmem_ld_wait_x16(d[i & 1]);
+              if (i < 7) load(i + 1);
+              v[i] = moe_lane_sums(d[i & 1], buf);
             }
           }
           release();
@@ -1152,21 +1167,21 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
             float* dst = up ? p.h + static_cast<int64_t>(pr) * p.I + gm.row0 + 64 * group
                             : p.part + (static_cast<int64_t>(gm.z) * p.T * p.k + pr) * p.H + gm.row0 +
                                   128 * group;
-            dst += lane & 7;
+            float2* out = reinterpret_cast<float2*>(dst) + (lane & 7);
             if (c < n) {
+              if (up) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                  if (up) {
-                    const float h = silu_rn(v[4 * j + half] * g0) * (v[4 * j + 2 + half] * g0) * g1;
-                    dst[16 * j + 8 * half] = h;
-                    hm = max(hm, __float_as_uint(h) & 0x7FFFFFFFu);
-                  } else {
-                    dst[32 * j + 8 * half] = v[4 * j + half] * g0;
-                    dst[32 * j + 16 + 8 * half] = v[4 * j + 2 + half] * g0;
-                  }
+                for (int j = 0; j < 4; ++j) {
+                  const float2 g = v[2 * j], u = v[2 * j + 1];
+                  const float2 h = make_float2(silu_rn(g.x * g0) * (u.x * g0) * g1,
+                                               silu_rn(g.y * g0) * (u.y * g0) * g1);
+                  out[8 * j] = h;
+                  hm = max(hm, max(__float_as_uint(h.x) & 0x7FFFFFFFu, __float_as_uint(h.y) & 0x7FFFFFFFu));
                 }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) out[8 * i] = make_float2(v[i].x * g0, v[i].y * g0);
+              }
             }
             if (up) {
 #pragma unroll

@@ -222,15 +222,15 @@ __device__ __forceinline__ double block_reduce(double v, double* part) {
   return v;
 }
 
-// Router: a cluster of eight CTAs per TB tokens; a CTA takes every eighth expert (every seventh, and
-// the last CTA none, where one token's digits keep that CTA busy) for all TB tokens, a warp per expert
-// and part of K (of eight where the experts are few: 8 of them, H 4096, 64 tokens took
-// 14.8 us for 21.4); the partial logits of token i of the group go to CTA i's shared
-// memory, which adds and selects for it. Two logits may be arbitrarily close, so
-// they are kept in 64 bits: eight products are summed in fp32 and added to a double, an error near 1e-8
-// of the logits' spread. Bound by latency: of one pass over the router weights, of the selection's
-// steps. (A share of every token's digits in each CTA took longer than one CTA's whole token beside
-// the others' products: 17 for 14 us at seven tokens.)
+// Router: a cluster of eight CTAs per TB tokens; a CTA takes every eighth expert for all TB tokens (every
+// seventh, and the last CTA none, where one token's digits keep that CTA busy and seven CTAs' warps
+// hold all experts at once), a warp per expert and part of K (of eight where the experts are few: 8 of
+// them, H 4096, 64 tokens took 14.8 us for 21.4); the partial logits of token i of the group go to CTA
+// i's shared memory, which adds and selects for it. Two logits may be arbitrarily close, so they are
+// kept in 64 bits: eight products are summed in fp32 and added to a double, an error near 1e-8 of the
+// logits' spread. Bound by latency: one pass over the router weights is half of it (3 of 5 us for one
+// token and 64 experts), the selection's steps the rest. (A share of every token's digits in each CTA
+// took longer than one CTA's whole token beside the others' products: 17 for 14 us at seven tokens.)
 template <class X, class W, int TB, int parts>
 __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRouteParams p) {
   extern __shared__ double sh[];  // partial logits [parts][E] of this CTA's token, then keys [E]
@@ -248,10 +248,10 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
     for (int i = threadIdx.x; i < moe_counters(p.E); i += kMoeThreads) p.counters[i] = 0;
   cluster_sync_all();  // every CTA of the cluster runs: its shared memory may be written
   const int pieces = p.H / 8;
-  constexpr int kRanks = TB == 1 ? kRouteCluster - 1 : kRouteCluster;
-  const int experts = rank < kRanks ? (p.E - static_cast<int>(rank) + kRanks - 1) / kRanks : 0;
+  const int ranks = TB == 1 && p.E <= (kRouteCluster - 1) * kMoeWarps ? kRouteCluster - 1 : kRouteCluster;
+  const int experts = static_cast<int>(rank) < ranks ? (p.E - static_cast<int>(rank) + ranks - 1) / ranks : 0;
   for (int job = warp; job < experts * parts; job += kMoeWarps) {
-    const int e = static_cast<int>(rank) + kRanks * (job / parts), q = job % parts;
+    const int e = static_cast<int>(rank) + ranks * (job / parts), q = job % parts;
     double acc[TB] = {};
     const W* row = wr + static_cast<int64_t>(e) * p.H;
 #pragma unroll(TB == 1 ? 8 : 4)
@@ -1240,6 +1240,7 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     // combine: 128 outputs of a token per warp and turn, dealt by index (no one waits for these),
     // eight partial sums in flight
     const int blocks3 = p.H / 128, terms = p.k * sh.slices;
+    const int slice_bits = 31 - __clz(sh.slices);  // a power of two
     if (warp == kMoeEpiWarp0) {
       ok = ok && moe_wait<false>(p.counters + kMoeDownDone, sh.total2, ctl, p.err);
       if (ok && lane == 0) mbar_arrive(smem_u32(&ctl.down_ready));
@@ -1254,7 +1255,7 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
         uint4 v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int i = i0 + j, s = i / sh.slices, z = i - s * sh.slices;
+          const int i = i0 + j, s = i >> slice_bits, z = i & (sh.slices - 1);
           const int pr = tok * p.k + s;
           v[j] = i < terms && pl.used[pr]
                      ? ld_cg(p.part + (static_cast<int64_t>(z) * p.T * p.k + pr) * p.H + h0)

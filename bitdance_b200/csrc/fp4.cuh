@@ -106,8 +106,11 @@ __device__ __forceinline__ uint32_t e2m1_pack8(const float (&y)[8]) {
   return w & ((((w & 0x77777777u) + 0x77777777u) & 0x88888888u) | 0x77777777u);
 }
 
-// 16 elements times r -> 8 code bytes.
-template <int kIn>
+// 16 elements times r -> 8 code bytes. The conversion rounds ties to even, the rule to the lower
+// magnitude, so a product that is a tie (its low 21 mantissa bits are zero) is made a little smaller.
+// kLow: r is already 2^-20 too small, which does it for 16-bit elements and a power of two: a product
+// has at most 11 significant bits, so it is a tie or at least 2^-11 of itself away from one.
+template <int kIn, bool kLow>
 __device__ __forceinline__ uint2 e2m1_encode16(const Raw16<kIn>& x, float r) {
   uint32_t o[2];
 #pragma unroll
@@ -116,7 +119,7 @@ __device__ __forceinline__ uint2 e2m1_encode16(const Raw16<kIn>& x, float r) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       y[j] = __fmul_rn(x.get(8 * h + j), r);
-      if ((__float_as_uint(y[j]) & 0x1FFFFFu) == 0) y[j] = __fmul_rn(y[j], 0.99999994f);  // 1 - 2^-24
+      if (!kLow && (__float_as_uint(y[j]) & 0x1FFFFFu) == 0) y[j] = __fmul_rn(y[j], 0.99999994f);  // 1 - 2^-24
     }
     o[h] = e2m1_pack8(y);
   }
@@ -140,17 +143,17 @@ struct QuantFp4Params {
   uint32_t* err;
 };
 
-// Quantiser. G threads share a row: a warp where there are rows enough to fill the machine (no
-// barriers, kKeep pieces of each lane in flight), else a CTA of eight warps, their maxima meeting in
-// shared memory. A thread takes 16-element pieces t, t + G, ..., keeps the first kKeep of them in
+// Quantiser. G threads share a row: a warp (eight to a CTA, no barriers), or a CTA of four or eight
+// warps, their maxima meeting in shared memory; kKeep pieces of each thread are in flight. A thread takes 16-element pieces t, t + G, ..., keeps the first kKeep of them in
 // registers between the maximum and the codes, and reads the rest of a long row twice (the second time
 // from L2). Bound by the bytes of x.
-constexpr int kQ4Threads = 256;
+__host__ __device__ constexpr int q4_threads(int G) { return G == 32 ? 256 : G; }
 
 template <int kIn, int kFmt, int G>
-__global__ void __launch_bounds__(kQ4Threads, kIn == kInF32 ? 2 : 3)
+__global__ void __launch_bounds__(q4_threads(G), (kIn == kInF32 ? 2 : 3) * 256 / q4_threads(G))
     quantize_fp4_kernel(const QuantFp4Params p) {
-  constexpr int kKeep = 4;
+  constexpr int kKeep = 4, kQ4Threads = q4_threads(G);
+  constexpr bool kLow = kFmt == kMxfp4 && kIn != kInF32;
   __shared__ uint32_t part[2][kQ4Threads / 32];
   const int sub = threadIdx.x / G, t = threadIdx.x % G;
   const int pieces = p.K / 16;
@@ -221,11 +224,12 @@ __global__ void __launch_bounds__(kQ4Threads, kIn == kInF32 ? 2 : 3)
         const int e = mxfp4_block_exp(am);
         byte = static_cast<uint32_t>(e + 127);
         mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        if (kLow) mul *= 0.99999905f;  // 1 - 2^-20
       }
       if (!ok) byte = 0;
       if (ok)
         *reinterpret_cast<uint2*>(p.codes + (e0 >> 1) + static_cast<int64_t>(c) * 8) =
-            e2m1_encode16<kIn>(r, mul);
+            e2m1_encode16<kIn, kLow>(r, mul);
       if constexpr (kFmt == kNvfp4) {
         if (p.scales != nullptr && ok) p.scales[m * pieces + c] = static_cast<uint8_t>(byte);
         if (p.scales_tiled != nullptr) {

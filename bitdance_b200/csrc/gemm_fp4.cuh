@@ -14,6 +14,10 @@
 // the same bits whatever the timing.
 //
 // Warps: 0 producer (TMA), 1 MMA, all four drain the accumulator (lane = weight row).
+//
+// Bound by latency and, where there are weights enough, their bytes. Measured with the quantiser in
+// front, one call after another: 1 token, 4096 -> 14336 (33 MB) 11 us, 3.0 TB/s; 32 tokens, 14336 ->
+// 4096 (31 MB) 12 to 14 us; 128 tokens, 4096 -> 4096 12 us; 333 tokens, 1056 -> 1000 18 us.
 #pragma once
 #include <cstdint>
 
@@ -346,6 +350,10 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
 // leave no room for scales), so the next tile's MMAs wait for the drain: eight epilogue warps take a
 // tile's 128 columns each into 128 registers in one go and release the accumulator before they scale,
 // convert and store (about 300 cycles of a 4096-deep tile's 8200).
+//
+// Measured: 8192 x 14336 x 4096 NVFP4 213 us (4.5 PFLOP/s, the tensor pipe 58 % busy), 8192 x 4096 x
+// 14336 MXFP4 183 us (5.3 PFLOP/s, 68 %). The scale copies share the tensor core with the MMAs, but
+// little of the rest is theirs: without any, NVFP4 took 5 % less and MXFP4 the same.
 //
 // Both CTAs' loads complete on rank 0's barrier (a relay warp in rank 1 that passed arrivals on was
 // 840 cycles a stage).

@@ -222,23 +222,22 @@ __device__ __forceinline__ double block_reduce(double v, double* part) {
   return v;
 }
 
-// Router: a cluster of eight CTAs per TB tokens; a CTA takes every eighth expert for all TB tokens (every
-// seventh, and the last CTA none, where one token's digits keep that CTA busy and seven CTAs' warps
-// hold all experts at once), a warp per expert and part of K (of eight where the experts are few: 8 of
-// them, H 4096, 64 tokens took 14.8 us for 21.4); the partial logits of token i of the group go to CTA
-// i's shared memory, which adds and selects for it. Two logits may be arbitrarily close, so they are
-// kept in 64 bits: eight products are summed in fp32 and added to a double, an error near 1e-8 of the
-// logits' spread. Bound by latency: one pass over the router weights is half of it (3 of 5 us for one
-// token and 64 experts), the selection's steps the rest. (A share of every token's digits in each CTA
-// took longer than one CTA's whole token beside the others' products: 17 for 14 us at seven tokens.)
-template <class X, class W, int TB, int parts>
+// Router: a cluster of eight CTAs per token; a CTA takes every eighth expert (every seventh, and the last
+// CTA none, where seven CTAs' warps hold all experts at once), a warp per expert and part of K (of
+// eight where the experts are few); the partial logits go to CTA 0's shared memory, which adds and selects. The last CTA makes the token's digits
+// meanwhile. Two logits may be arbitrarily close, so they are kept in 64 bits: eight products are
+// summed in fp32 and added to a double, an error near 1e-8 of the logits' spread. Bound by latency: one
+// pass over the router weights is half of it (3 of 5 us for one token and 64 experts), the selection's
+// steps the rest. (Two or four tokens per cluster, for fewer passes over the weights: 64 tokens, 64
+// experts, H 4096 took the layer 127 us for 118. A share of the token's digits in each CTA took longer
+// than one CTA's whole token beside the others' products: 17 for 14 us at seven tokens.)
+template <class X, class W, int parts>
 __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRouteParams p) {
-  extern __shared__ double sh[];  // partial logits [parts][E] of this CTA's token, then keys [E]
+  extern __shared__ double sh[];  // partial logits [parts][E], then keys [E]
   __shared__ double part[kMoeWarps];
   __shared__ uint32_t upart[kMoeWarps];
   __shared__ double sel[kMoeMaxTopK];
-  const uint32_t rank = cluster_ctarank();
-  const int t0 = blockIdx.x / kRouteCluster * TB;
+  const int rank = static_cast<int>(cluster_ctarank()), t = blockIdx.x / kRouteCluster;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const X* x = static_cast<const X*>(p.x);
   const W* wr = static_cast<const W*>(p.router);
@@ -248,43 +247,32 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
     for (int i = threadIdx.x; i < moe_counters(p.E); i += kMoeThreads) p.counters[i] = 0;
   cluster_sync_all();  // every CTA of the cluster runs: its shared memory may be written
   const int pieces = p.H / 8;
-  const int ranks = TB == 1 && p.E <= (kRouteCluster - 1) * kMoeWarps ? kRouteCluster - 1 : kRouteCluster;
-  const int experts = static_cast<int>(rank) < ranks ? (p.E - static_cast<int>(rank) + ranks - 1) / ranks : 0;
+  const int ranks = p.E <= (kRouteCluster - 1) * kMoeWarps ? kRouteCluster - 1 : kRouteCluster;
+  const int experts = rank < ranks ? (p.E - rank + ranks - 1) / ranks : 0;
   for (int job = warp; job < experts * parts; job += kMoeWarps) {
-    const int e = static_cast<int>(rank) + ranks * (job / parts), q = job % parts;
-    double acc[TB] = {};
+    const int e = rank + ranks * (job / parts), q = job % parts;
+    double acc = 0.0;
     const W* row = wr + static_cast<int64_t>(e) * p.H;
-#pragma unroll(TB == 1 ? 8 : 4)
+    const X* xt = x + static_cast<int64_t>(t) * p.H;
+#pragma unroll 8
     for (int c = 32 * q + lane; c < pieces; c += 32 * parts) {
-      float w[8];
+      float w[8], v[8], s = 0.0f;
       load8(row + 8 * c, w);
+      load8(xt + 8 * c, v);
 #pragma unroll
-      for (int i = 0; i < TB; ++i) {
-        if (t0 + i < p.T) {
-          float v[8], s = 0.0f;
-          load8(x + static_cast<int64_t>(t0 + i) * p.H + 8 * c, v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) s = fmaf(w[j], v[j], s);
-          acc[i] += static_cast<double>(s);
-        }
-      }
+      for (int j = 0; j < 8; ++j) s = fmaf(w[j], v[j], s);
+      acc += static_cast<double>(s);
     }
 #pragma unroll
-    for (int i = 0; i < TB; ++i) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xFFFFFFFFu, acc[i], o);
-      if (lane == 0) {
-        const uint32_t at = mapa_shared(smem_u32(&sh[q * p.E + e]), i);
-        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(acc[i]) : "memory");
-      }
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xFFFFFFFFu, acc, o);
+    if (lane == 0) {
+      const uint32_t at = mapa_shared(smem_u32(&sh[q * p.E + e]), 0);
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(acc) : "memory");
     }
   }
-  // the digits of token i by CTA 7 - i, while the others may still multiply
-  const int mine = kRouteCluster - 1 - static_cast<int>(rank);
-  if (mine < TB && t0 + mine < p.T) moe_convert_token(x, p.xs, p.x_scale, t0 + mine, p.H, upart);
+  if (rank == kRouteCluster - 1) moe_convert_token(x, p.xs, p.x_scale, t, p.H, upart);
   cluster_sync_all();
-  const int t = t0 + static_cast<int>(rank);
-  if (static_cast<int>(rank) >= TB || t >= p.T) return;
+  if (rank != 0) return;
   // Scores and keys. The key ranks: the logit itself (softmax without bias: the same order, nothing
   // rounds), else score + bias; a NaN ranks last. Where the weights are renormalised softmax scores
   // ranked by logit, exp(logit - largest) of the chosen ones is all that is needed.
@@ -524,10 +512,19 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
 // 5..8 activation digits, waiting for those of a down task's expert while the weights of the next
 // stages already arrive. 9 MMA. 10, 11 digits of the hidden values, as experts finish. 12..19 epilogue
 // and combine.
-// An MMA of this kind takes the same time (about 128 cycles) for 16 columns as for 256, so the weights
-// are its 256 columns and the digits its 128 rows where a pass has at most 16 tokens (kSwap: half the
-// MMAs a stage; the digits' sum then runs over lanes); with 24 tokens a pass the weights are two
-// tiles of 128 rows and the digits 192 columns.
+// An MMA of this kind takes about as long for 16 columns as for 128, so the weights are its 256 columns
+// and the digits its 128 rows where a pass has at most 16 tokens (kSwap: half the MMAs a stage; the
+// digits' sum then runs over lanes); with 24 tokens a pass the weights are two tiles of 128 rows and the
+// digits 192 columns.
+// Measured (the layer, GPU time, one call after another): 1 token, 8 of 64 experts of 2048 x 768: 34 us
+// for 21 MB of weights: a chain of latencies (routing 5 to 9, plan 2.4, first stage 3, gate / up 5,
+// epilogue, digits 4, down, combine 3). 7 tokens, 6 of 128 of 4096 x 1408: 84 us (5.2 TB/s while the
+// weights stream); 48 tokens, 8 of 128 of 2048 x 1024: 108 us (4.4 TB/s over this kernel); 64 tokens, 2
+// of 8 of 4096 x 14336: 198 us (4.2 TB/s): there a stage's MMAs (1000 to 1250 cycles) and the drain of
+// the one accumulator that fits tensor memory beside the scales take nearly as long as its bytes.
+// Tried, no gain: a fourth stage of weights (93 us for 91 at seven tokens); scales stored to tensor
+// memory from registers instead of tcgen05.cp (equal with four sets of scale words, 25 % slower with
+// the two that fit beside 24 tokens).
 constexpr int kMoeScaleWarp0 = 1, kMoeScaleWarps = 4;
 constexpr int kMoeDigitWarp0 = kMoeScaleWarp0 + kMoeScaleWarps, kMoeDigitWarps = 4;
 constexpr int kMoeMmaWarp = kMoeDigitWarp0 + kMoeDigitWarps;

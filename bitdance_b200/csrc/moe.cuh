@@ -523,7 +523,7 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
 // of 8 of 4096 x 14336: 198 us (4.2 TB/s): there a stage's MMAs (1000 to 1250 cycles) and the drain of
 // the one accumulator that fits tensor memory beside the scales take nearly as long as its bytes.
 // Tried, no gain: a fourth stage of weights (93 us for 91 at seven tokens); scales stored to tensor
-// memory from registers instead of tcgen05.cp (equal with four sets of scale words, 25 % slower with
+// memory from registers instead of tcgen05.cp (equal with four sets of scale words, 211 us for 199 with
 // the two that fit beside 24 tokens).
 constexpr int kMoeScaleWarp0 = 1, kMoeScaleWarps = 4;
 constexpr int kMoeDigitWarp0 = kMoeScaleWarp0 + kMoeScaleWarps, kMoeDigitWarps = 4;

@@ -17,8 +17,6 @@ namespace {
 
 constexpr int kMaxRows = 1 << 28, kMaxK = 1 << 24;
 
-int last_status() { return cudaPeekAtLastError() == cudaSuccess ? BD_OK : BD_ERR_CUDA; }
-
 // Scale tiles (of four scales) along a row of K elements.
 int sf_words(int K, int fmt) {
   const int block = fmt == BD_FP4_NVFP4 ? 16 : 32;
@@ -34,8 +32,7 @@ bool allow_smem(K kernel, int bytes, std::atomic<uint64_t>& configured) {
   if (cudaGetDevice(&dev) != cudaSuccess) return false;
   const uint64_t bit = 1ull << (dev & 63);
   if (configured.load() & bit) return true;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
-      cudaSuccess)
+  if (launch_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)))
     return false;
   configured.fetch_or(bit);
   return true;
@@ -80,7 +77,7 @@ int launch_quantize(const QuantFp4Params& p, bool overlap, const DeviceInfo* d, 
   const cudaError_t e = warp_rows                ? launch(quantize_fp4_kernel<kIn, kFmt, 32>, 32)
                         : p.M >= 4 * d->sm_count ? launch(quantize_fp4_kernel<kIn, kFmt, 128>, 128)
                                                  : launch(quantize_fp4_kernel<kIn, kFmt, 256>, 256);
-  return e == cudaSuccess ? last_status() : BD_ERR_CUDA;
+  return launch_status(e);
 }
 
 template <int kFmt>
@@ -106,7 +103,7 @@ int launch_dequantize(const uint8_t* codes, const uint8_t* tiled, const float* r
                                      ts, o, M, K, words)
                 : cudaLaunchKernelEx(&cfg, dequantize_fp4_kernel<kFmt, kOut, 256>, codes, tiled, rs,
                                      ts, o, M, K, words);
-  return e == cudaSuccess ? last_status() : BD_ERR_CUDA;
+  return launch_status(e);
 }
 
 template <int kFmt>
@@ -154,9 +151,7 @@ int launch_gemm(GemmFp4Params p, const uint8_t* a, const uint8_t* b, bool overla
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = launch_config(static_cast<int>(tiles * split), 128,
                                                Cfg::kSmemBytes, s, attr, overlap, split);
-  if (cudaLaunchKernelEx(&cfg, w4a4_gemm_kernel<BN, kFmt>, mw, mt, p, split) != cudaSuccess)
-    return BD_ERR_CUDA;
-  return last_status();
+  return launch_status(cudaLaunchKernelEx(&cfg, w4a4_gemm_kernel<BN, kFmt>, mw, mt, p, split));
 }
 
 template <int kFmt>
@@ -178,9 +173,7 @@ int launch_pair(GemmFp4Params p, const uint8_t* a, const uint8_t* b, bool overla
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg =
       launch_config(grid, kPairThreads, Cfg::kSmem, s, attr, overlap, 2);
-  if (cudaLaunchKernelEx(&cfg, w4a4_pair_kernel<kFmt>, mw, mt, sw, st, p) != cudaSuccess)
-    return BD_ERR_CUDA;
-  return last_status();
+  return launch_status(cudaLaunchKernelEx(&cfg, w4a4_pair_kernel<kFmt>, mw, mt, sw, st, p));
 }
 
 template <int kFmt>
@@ -273,9 +266,11 @@ int bd_tile_scales_fp4(const uint8_t* scales, uint8_t* scales_tiled, int rows, i
   if (st != BD_OK) return st;
   const int words = sf_words(K, fmt);
   const int64_t work = static_cast<int64_t>(rows) * words;
-  tile_scales_kernel<<<grid_for(work, 256, d), 256, 0, as_stream(stream)>>>(
-      scales, scales_tiled, rows, K / (fmt == BD_FP4_NVFP4 ? 16 : 32), words);
-  return last_status();
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg =
+      launch_config(grid_for(work, 256, d), 256, 0, as_stream(stream), attr, false);
+  return launch_status(cudaLaunchKernelEx(&cfg, tile_scales_kernel, scales, scales_tiled, rows,
+                                          K / (fmt == BD_FP4_NVFP4 ? 16 : 32), words));
 }
 
 int bd_dequantize_fp4(const uint8_t* codes, const uint8_t* scales_tiled, const float* row_scale,

@@ -36,4 +36,12 @@ bool make_map_2d(CUtensorMap* m, CUtensorMapDataType dt, void* base, uint64_t d0
 // Blocks for `work` items, per_block at a time, at most eight per SM.
 int grid_for(int64_t work, int per_block, const DeviceInfo* d);
 
+// Status of a launch (or of another runtime call) that returned e. A failed one leaves its error in the
+// runtime's record as well: cleared here, so that no later call takes it for its own.
+inline int launch_status(cudaError_t e) {
+  if (e == cudaSuccess) return BD_OK;
+  cudaGetLastError();
+  return BD_ERR_CUDA;
+}
+
 }  // namespace bd

@@ -12,8 +12,6 @@
 namespace bd {
 namespace {
 
-int last_status() { return cudaPeekAtLastError() == cudaSuccess ? BD_OK : BD_ERR_CUDA; }
-
 // Workspace: counters | row maxima of h | row factors of x | digits of x | h | digits of h | partial
 // sums, each 256-byte aligned. Few pairs may split the down product: at least kPartRows rows of
 // partials.
@@ -68,8 +66,7 @@ int launch_route_parts(const MoeRouteParams& p, cudaStream_t s) {
   const cudaLaunchConfig_t cfg =
       config(p.T * kRouteCluster, kMoeThreads, (parts + 1) * p.E * static_cast<int>(sizeof(double)), s,
              attr, kRouteCluster);
-  return cudaLaunchKernelEx(&cfg, moe_route_kernel<X, W, parts>, p) == cudaSuccess ? last_status()
-                                                                                : BD_ERR_CUDA;
+  return launch_status(cudaLaunchKernelEx(&cfg, moe_route_kernel<X, W, parts>, p));
 }
 
 // Eight parts of K per expert where one warp per expert leaves most of a CTA's warps idle (rows shorter
@@ -120,17 +117,15 @@ int launch_experts(const CUtensorMap& m13, const CUtensorMap& m2, const MoeExper
   if (cudaGetDevice(&dev) != cudaSuccess) return BD_ERR_CUDA;
   const uint64_t bit = 1ull << (dev & 63);
   if (!(configured.load() & bit)) {
-    if (cudaFuncSetAttribute(moe_experts_kernel<TOK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             MoeCfg<TOK>::kSmem) != cudaSuccess)
-      return BD_ERR_CUDA;
+    const int st = launch_status(cudaFuncSetAttribute(
+        moe_experts_kernel<TOK>, cudaFuncAttributeMaxDynamicSharedMemorySize, MoeCfg<TOK>::kSmem));
+    if (st != BD_OK) return st;
     configured.fetch_or(bit);
   }
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg =
       config(d->sm_count, kMoeExpertThreads, MoeCfg<TOK>::kSmem, s, attr, 1);
-  return cudaLaunchKernelEx(&cfg, moe_experts_kernel<TOK>, m13, m2, p) == cudaSuccess
-             ? last_status()
-             : BD_ERR_CUDA;
+  return launch_status(cudaLaunchKernelEx(&cfg, moe_experts_kernel<TOK>, m13, m2, p));
 }
 
 int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
@@ -213,7 +208,7 @@ int bd_moe_experts(void* y, const void* x, int x_dtype, const int* ids, const fl
                                H, E, top_k)
           : cudaLaunchKernelEx(&cfg, moe_prepare_kernel<__half>, static_cast<const __half*>(x),
                                ws + w.xs, x_scale, hmax, counters, H, E, top_k);
-  if (e != cudaSuccess) return BD_ERR_CUDA;
+  if (e != cudaSuccess) return launch_status(e);
   return run_experts(y, out_dtype, ids, weights, a, T, H, I, E, top_k, ws, d, s);
 }
 

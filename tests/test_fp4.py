@@ -209,6 +209,18 @@ def test_quantise_and_back(rows, K, fmt, dtype):
 
 @gpu
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("dtype,rows,K", [
+    (torch.float32, 600, 1056), (torch.bfloat16, 600, 1056), (torch.float16, 601, 1056),
+    (torch.bfloat16, 593, 9248), (torch.float32, 4737, 1056), (torch.bfloat16, 4737, 1088)])
+def test_quantise_many_rows(rows, K, fmt, dtype):
+    import bitdance_b200 as bd
+    op, code, byte, s = operand(matrix(rows, K, dtype, 3), fmt)
+    want = (f.values(code, byte, fmt) * s[:, None]).astype(np.float32)
+    assert np.array_equal(bd.dequantize_fp4(op).cpu().numpy(), want)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 def test_quantise_ties_zeros_and_extremes(fmt):
     import bitdance_b200 as bd
     x = tie_matrix()
@@ -317,6 +329,29 @@ def test_gemm_epilogues_and_tensor_scales(epilogue, act, lip, M):
 
 @gpu
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("M,N,K", [
+    (9473, 8, 96), (2500, 1000, 1056), (1300, 1801, 320), (300, 4900, 288), (2560, 1024, 64),
+    (257, 4864, 2592), (5121, 513, 512)])
+def test_gemm_of_many_tiles(M, N, K, fmt):
+    """Products that CTA pairs share, with ragged last tiles and stages."""
+    import bitdance_b200 as bd
+    a, *an = operand(matrix(M, K, torch.bfloat16, 1, 0.7), fmt)
+    w, *wn = operand(matrix(N, K, torch.float32, 2, 0.7), fmt)
+    av, wv = value_of(*an, fmt), value_of(*wn, fmt)
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.full((M + 2, N), 7.0, dtype=dtype, device="cuda")
+        c = bd.w4a4_gemm(a, w, out_dtype=dtype, out=out[1:M + 1])
+        gemm_check(c, av, wv, K, dtype)
+        assert (out[0] == 7).all() and (out[M + 1] == 7).all()
+    bias = torch.linspace(-2, 2, N).to(torch.bfloat16)
+    c = bd.w4a4_gemm(a, w, bias=bias.cuda(), epilogue="bias_silu", out_dtype=torch.float16)
+    gemm_check(c, av, wv, K, torch.float16, bias.double().numpy(),
+               lambda v: v / (1 + np.exp(-np.clip(v, -700, None))), 1.1)
+    assert bd.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("M,N,K", [(1, 512, 2048), (40, 300, 1056), (600, 1024, 512)])
 def test_linear_is_quantise_then_gemm(M, N, K, fmt):
     import bitdance_b200 as bd
@@ -385,3 +420,33 @@ def test_linear_right_behind_its_weights(fmt):
         got.append(bd.w4a4_linear(x, bd.quantize_fp4(ws[i % 3], fmt, overlap_prev=i % 2 == 1)))
     for i, c in enumerate(got):
         assert torch.equal(c, want[i % 3])
+
+
+@gpu
+def test_a_refused_launch_leaves_no_error_behind():
+    """A launch into the legacy stream while a blocking stream is being captured is refused by the
+    runtime; the next call is not."""
+    import bitdance_b200 as bd
+    L = lib()
+    x = torch.randn(4, 64, device="cuda")
+    want = bd.quantize_fp4(x)
+    codes, scales = torch.zeros_like(want.codes), torch.zeros_like(want.scales)
+    row_scale = torch.zeros_like(want.row_scale)
+    torch.cuda.synchronize()
+
+    def quantize(stream):
+        P = ctypes.c_void_p
+        return L.bd_quantize_fp4(P(x.data_ptr()), 0, 0, P(codes.data_ptr()), None,
+                                 P(scales.data_ptr()), P(row_scale.data_ptr()), 4, 64, 0, P(stream))
+    rt = ctypes.CDLL("libcudart.so.12")
+    s, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    assert rt.cudaStreamCreate(ctypes.byref(s)) == 0
+    assert rt.cudaStreamBeginCapture(s, 0) == 0
+    refused = quantize(1)  # the legacy stream
+    rt.cudaStreamEndCapture(s, ctypes.byref(graph))
+    rt.cudaGetLastError()
+    assert refused == -5
+    assert quantize(s.value) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(codes, want.codes) and torch.equal(row_scale, want.row_scale)
+    assert rt.cudaStreamDestroy(s) == 0

@@ -276,7 +276,8 @@ int bd_splitk_reduce(const float* partials, void* c, const void* bias, float b_t
 
 /* ---- 4-bit activations: W4A4 ----------------------------------------------------------------
  * Operand formats: E2M1 codes (rows, K/2), element 2j in the low nibble of byte j, with
- *   BD_FP4_NVFP4  one E4M3 scale byte per 16 elements, an fp32 scale per row and / or per tensor;
+ *   BD_FP4_NVFP4  one E4M3 scale byte (of a number >= 0) per 16 elements, an fp32 scale per row and
+ *                 / or per tensor;
  *   BD_FP4_MXFP4  one E8M0 scale byte per 32 elements.
  * Scale tiles (what the GEMM reads; bd_query_fp4_scales bytes):
  *   [ceil(rows/128)][ceil(scales per row / 4)][512]: row r of a tile at byte
@@ -335,7 +336,7 @@ int bd_w4a4_linear(void* c, const void* x, int x_dtype, const uint8_t* b, const 
 
 /* ---- mixture of experts for a few tokens ----------------------------------------------------
  * Expert weights in NVFP4, natural layout (what bd_quantize_b_nvfp4 writes, one expert after the
- * other): gate_up (E, 2I, H/2) codes (I gate rows, then I up rows) and (E, 2I, H/16) E4M3 scales;
+ * other): gate_up (E, 2I, H/2) codes (I gate rows, then I up rows) and (E, 2I, H/16) E4M3 scales >= 0;
  * down (E, H, I/2) and (E, H, I/16); one fp32 tensor scale per expert and matrix, device arrays.
  * T <= 64 tokens, E <= 512, top_k <= min(16, E), H % 128 == 0, I % 128 == 0; T == 0: nothing is
  * done. x bf16 or fp16 (T, H); y (T, H) in out_dtype. Weights enter the products exactly, x and the

@@ -278,13 +278,15 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
   // ranked by logit, exp(logit - largest) of the chosen ones is all that is needed.
   double* score = sh;
   double* key = sh + parts * p.E;
-  if constexpr (parts > 1) {
-    for (int e = threadIdx.x; e < p.E; e += kMoeThreads)
-      for (int q = 1; q < parts; ++q) score[e] += sh[q * p.E + e];
-    __syncthreads();
-  }
   const bool lazy = !p.sigmoid && p.bias == nullptr && p.renormalize;
-  if (!lazy) {
+  for (int e = threadIdx.x; e < p.E; e += kMoeThreads) {
+    double l = score[e];
+#pragma unroll
+    for (int q = 1; q < parts; ++q) l += sh[q * p.E + e];
+    if (parts > 1) score[e] = l;
+    key[e] = l == l ? l : -INFINITY;
+  }
+  if (!lazy) {  // (every loop gives a thread the same experts)
     double m = 0.0, z = 1.0;
     if (!p.sigmoid) {
       m = -INFINITY;
@@ -301,23 +303,21 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
       score[e] = s;
       key[e] = v == v ? v : -INFINITY;
     }
-    __syncthreads();
   }
+  __syncthreads();
   // rank of an expert: how many stand before it (ties to the lowest index); ranks are distinct.
   // `team` threads (a power of two up to 32) share an expert.
   int team = 32;
   while (team > 1 && team * p.E > kMoeThreads) team >>= 1;
   const int sub = threadIdx.x & (team - 1);
-  const double* by = lazy ? score : key;
   for (int e0 = 0; e0 < p.E; e0 += kMoeThreads / team) {
     const int e = e0 + threadIdx.x / team;
     int r = 0;
     if (e < p.E) {
-      double v = by[e];
-      if (v != v) v = -INFINITY;
+      const double v = key[e];
+#pragma unroll 8
       for (int j = sub; j < p.E; j += team) {
-        double u = by[j];
-        if (u != u) u = -INFINITY;
+        const double u = key[j];
         r += (u > v || (u == v && j < e)) ? 1 : 0;
       }
     }
@@ -328,17 +328,18 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
     }
   }
   __syncthreads();
-  if (threadIdx.x < p.k) {
+  if (warp == 0) {
     // lazy: sel holds logits, the first the largest (all NaN or -inf: the weights are NaN, as theirs)
-    const double mine = lazy ? exp(sel[threadIdx.x] - sel[0]) : sel[threadIdx.x];
-    double sum = 1.0;
+    double mine = lane < p.k ? sel[lane] : 0.0, sum = 1.0;
+    if (lazy && lane < p.k) mine = exp(mine - sel[0]);
     if (p.renormalize) {
       sum = 0.0;
-      for (int r = 0; r < p.k; ++r) sum += lazy ? exp(sel[r] - sel[0]) : sel[r];
+      for (int r = 0; r < p.k; ++r) sum += __shfl_sync(0xFFFFFFFFu, mine, r);
     }
-    p.hmax[t * p.k + threadIdx.x] = 0;
-    p.weights[t * p.k + threadIdx.x] =
-        static_cast<float>(mine / sum * static_cast<double>(p.routed_scale));
+    if (lane < p.k) {
+      p.hmax[t * p.k + lane] = 0;
+      p.weights[t * p.k + lane] = static_cast<float>(mine / sum * static_cast<double>(p.routed_scale));
+    }
   }
 }
 

@@ -47,7 +47,15 @@ def _scale_bytes(rows: int, K: int, fmt: str) -> int:
 
 
 # These entry points serve single tokens, where a call's time is the host's: addresses go to the
-# library as integers, the current stream and device come from torch's C layer.
+# library as integers, and the current stream and device come from torch's C layer, as do new tensors
+# where it has a call for them (0.8 us; torch.empty reads its arguments for another 0.8, and for 1.5
+# and 2.3 more where the sizes are a tuple or a torch.Size).
+_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else \
+    torch.cuda.current_device
+try:
+    from torch._C._dynamo.guards import _empty_strided_cuda as _alloc
+except ImportError:
+    _alloc = None
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -56,25 +64,28 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 
 def _stream_ptr(stream) -> int:
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+        return torch._C._cuda_getCurrentRawStream(_device())
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
-def _empty(shape, dtype, device, stream):
-    """A new tensor that belongs to the stream the kernels run on (its memory is reused in that
-    stream's order)."""
+def _empty(stream, dtype, device, *shape):
+    """A new tensor of one or two dimensions that belongs to the stream the kernels run on (its memory
+    is reused in that stream's order), on the current device (``device``: the arguments were checked
+    to be there)."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        if _alloc is not None:
+            return _alloc(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype)
+        return torch.empty(*shape, dtype=dtype, device=device)
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty(*shape, dtype=dtype, device=device)
 
 
 def _have(t, dtype, what: str, numel: int) -> None:
     """``ops._need`` with its common case first."""
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.is_contiguous()
-            and t.numel() >= numel and t.get_device() == torch._C._cuda_getDevice()):
+            and t.numel() >= numel and t.get_device() == _device()):
         _need(t, dtype, what, numel)
 
 
@@ -109,9 +120,9 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", stream=None,
     code = _fmt(fmt)
     M, K = _check_x4(x)
     device = x.device
-    codes = _empty((M, K // 2), torch.uint8, device, stream)
-    scales = _empty(_scale_bytes(M, K, fmt), torch.uint8, device, stream)
-    row_scale = _empty(M, torch.float32, device, stream) if fmt == "nvfp4" else None
+    codes = _empty(stream, torch.uint8, device, M, K // 2)
+    scales = _empty(stream, torch.uint8, device, _scale_bytes(M, K, fmt))
+    row_scale = _empty(stream, torch.float32, device, M) if fmt == "nvfp4" else None
     call("bd_quantize_fp4", x.data_ptr(), _IN4[x.dtype], code, codes.data_ptr(), None,
          scales.data_ptr(), _ptr(row_scale), M, K,
          _lib.BD_GEMM_OVERLAP_PREV if overlap_prev else 0, _stream_ptr(stream))
@@ -123,8 +134,8 @@ def quantize_mxfp4(x: torch.Tensor, stream=None):
     ``quantize_fp4(x, "mxfp4")`` in the natural layout (the reference's quantize(x, E8M0, E2M1),
     vector_quant_error.py:283-319)."""
     M, K = _check_x4(x)
-    codes = _empty((M, K // 2), torch.uint8, x.device, stream)
-    e8m0 = _empty((M, K // 32), torch.uint8, x.device, stream)
+    codes = _empty(stream, torch.uint8, x.device, M, K // 2)
+    e8m0 = _empty(stream, torch.uint8, x.device, M, K // 32)
     call("bd_quantize_fp4", x.data_ptr(), _IN4[x.dtype], _lib.BD_FP4_MXFP4, codes.data_ptr(),
          e8m0.data_ptr(), None, None, M, K, 0, _stream_ptr(stream))
     return codes, e8m0
@@ -145,7 +156,7 @@ def pack_fp4(codes: torch.Tensor, scales: torch.Tensor, fmt: str = "nvfp4",
     _need(scales, torch.uint8, "scales", rows * (K // _BLOCK[fmt]))
     if row_scale is not None:
         _need(row_scale, torch.float32, "row_scale", rows)
-    tiled = _empty(_scale_bytes(rows, K, fmt), torch.uint8, codes.device, stream)
+    tiled = _empty(stream, torch.uint8, codes.device, _scale_bytes(rows, K, fmt))
     call("bd_tile_scales_fp4", scales.data_ptr(), tiled.data_ptr(), rows, K, code,
          _stream_ptr(stream))
     return Fp4Operand(codes, tiled, rows, K, fmt, row_scale, float(tensor_scale))
@@ -171,7 +182,7 @@ def dequantize_fp4(op: Fp4Operand, out_dtype=torch.float32, out: Optional[torch.
     if out_dtype not in _OUT:
         raise TypeError(f"unsupported output dtype {out_dtype}")
     if out is None:
-        out = _empty((op.rows, op.K), out_dtype, op.codes.device, stream)
+        out = _empty(stream, out_dtype, op.codes.device, op.rows, op.K)
     else:
         _have(out, out_dtype, "out", op.rows * op.K)
     call("bd_dequantize_fp4", op.codes.data_ptr(), op.scales.data_ptr(), _ptr(op.row_scale),
@@ -195,7 +206,7 @@ def _output(out, M: int, N: int, out_dtype, device, stream):
     if out_dtype not in _OUT:
         raise TypeError(f"unsupported output dtype {out_dtype}")
     if out is None:
-        return _empty((M, N), out_dtype, device, stream)
+        return _empty(stream, out_dtype, device, M, N)
     _have(out, out_dtype, "out", M * N)
     return out
 
@@ -241,7 +252,7 @@ def w4a4_linear(x: torch.Tensor, weights: Fp4Operand, bias: Optional[torch.Tenso
     if M == 0:
         return out
     nbytes = _linear_workspace(M, K, weights.fmt)
-    ws = _empty(nbytes, torch.uint8, x.device, stream)
+    ws = _empty(stream, torch.uint8, x.device, nbytes)
     call("bd_w4a4_linear", out.data_ptr(), x.data_ptr(), _IN4[x.dtype], weights.codes.data_ptr(),
          weights.scales.data_ptr(), _ptr(weights.row_scale), float(weights.tensor_scale),
          _ptr(bias), M, N, K, FP4_FORMATS[weights.fmt], _OUT[out_dtype], epi, ws.data_ptr(),

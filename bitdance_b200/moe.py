@@ -61,7 +61,7 @@ def _check(x: torch.Tensor, w: MoeWeights, top_k: int):
         raise ValueError("expert weights must be (E, rows, K/2)")
     E, two_i, half = w.gate_up.shape
     inter = two_i // 2
-    if two_i % 2 or half * 2 != H or tuple(w.down.shape) != (E, H, inter // 2):
+    if two_i % 2 or half * 2 != H or w.down.shape != (E, H, inter // 2):
         raise ValueError(f"x has {H} columns, gate_up {tuple(w.gate_up.shape)}, down "
                          f"{tuple(w.down.shape)}: expected (E, 2I, H/2) and (E, H, I/2)")
     if H == 0 or inter == 0 or H % 128 or inter % 128:
@@ -92,13 +92,13 @@ def _workspace_bytes(T: int, H: int, inter: int, E: int, top_k: int) -> int:
         up(4 * pairs * inter) + up(pairs * ((inter + 255) // 256) * 1152) + 4 * H * max(pairs, 256)
 
 
-def _out_tensor(out, x: torch.Tensor, out_dtype, stream):
+def _out_tensor(out, x: torch.Tensor, T: int, H: int, out_dtype, stream):
     dtype = x.dtype if out_dtype is None else out_dtype
     if dtype not in _OUT:
         raise TypeError(f"unsupported output dtype {dtype}")
     if out is None:
-        return _empty(x.shape, dtype, x.device, stream)
-    _have(out, dtype, "out", x.numel())
+        return _empty(stream, dtype, x.device, T, H)
+    _have(out, dtype, "out", T * H)
     return out
 
 
@@ -121,9 +121,9 @@ def moe_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Ten
     T, H, inter, E = _check(x, experts, top_k)
     _have(topk_ids, torch.int32, "topk_ids", 0)
     _have(topk_weights, torch.float32, "topk_weights", 0)
-    out = _out_tensor(out, x, out_dtype, stream)
+    out = _out_tensor(out, x, T, H, out_dtype, stream)
     nbytes = _workspace_bytes(T, H, inter, E, top_k)
-    ws = _empty(nbytes, torch.uint8, x.device, stream)
+    ws = _empty(stream, torch.uint8, x.device, nbytes)
     call("bd_moe_experts", out.data_ptr(), x.data_ptr(), _IN_MOE[x.dtype], topk_ids.data_ptr(),
          topk_weights.data_ptr(), *_weight_args(experts), T, H, inter, E, top_k, _OUT[out.dtype],
          ws.data_ptr(), nbytes, _stream_ptr(stream))
@@ -144,22 +144,22 @@ def moe_layer(x: torch.Tensor, router: torch.Tensor, experts: MoeWeights, top_k:
     if scoring not in SCORINGS:
         raise ValueError(f"unknown scoring {scoring!r}: 'softmax' or 'sigmoid'")
     T, H, inter, E = _check(x, experts, top_k)
-    if tuple(router.shape) != (E, H):
+    if router.shape != (E, H):
         raise ValueError(f"router must be ({E}, {H}), got {tuple(router.shape)}")
     if router.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"router must be {x.dtype} or float32, got {router.dtype}")
     _have(router, router.dtype, "router", 0)
     if selection_bias is not None:
         _have(selection_bias, torch.float32, "selection_bias", E)
-    out = _out_tensor(out, x, out_dtype, stream)
+    out = _out_tensor(out, x, T, H, out_dtype, stream)
     nbytes = _workspace_bytes(T, H, inter, E, top_k)
     if return_routing:
-        ids = _empty((T, top_k), torch.int32, x.device, stream)
-        weights = _empty((T, top_k), torch.float32, x.device, stream)
-        ws = _empty(nbytes, torch.uint8, x.device, stream)
+        ids = _empty(stream, torch.int32, x.device, T, top_k)
+        weights = _empty(stream, torch.float32, x.device, T, top_k)
+        ws = _empty(stream, torch.uint8, x.device, nbytes)
         ids_at, weights_at = ids.data_ptr(), weights.data_ptr()
     else:  # behind the workspace
-        ws = _empty(nbytes + 8 * T * top_k, torch.uint8, x.device, stream)
+        ws = _empty(stream, torch.uint8, x.device, nbytes + 8 * T * top_k)
         ids_at = ws.data_ptr() + nbytes
         weights_at = ids_at + 4 * T * top_k
     call("bd_moe_layer", out.data_ptr(), ids_at, weights_at, x.data_ptr(), _IN_MOE[x.dtype],

@@ -82,10 +82,10 @@ def _empty(stream, dtype, device, *shape):
         return torch.empty(*shape, dtype=dtype, device=device)
 
 
-def _have(t, dtype, what: str, numel: int) -> None:
-    """``ops._need`` with its common case first."""
-    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.is_contiguous()
-            and t.numel() >= numel and t.get_device() == _device()):
+def _have(t, dtype, what: str, numel: int, dev: int) -> None:
+    """``ops._need`` with its common case first: on device dev, the current one."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev
+            and t.is_contiguous() and t.numel() >= numel):
         _need(t, dtype, what, numel)
 
 
@@ -94,21 +94,28 @@ def _check_x4(x: torch.Tensor):
         raise ValueError("x must be a 2-D tensor (M, K)")
     if x.dtype not in _IN4:
         raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    _have(x, x.dtype, "x", 0)
+    if not (x.is_cuda and x.is_contiguous() and x.get_device() == _device()):
+        _need(x, x.dtype, "x")
     M, K = x.shape
     if K == 0 or K % 32:
         raise ValueError(f"K must be a positive multiple of 32, got {K}")
     return M, K
 
 
-def _check_operand(op: Fp4Operand, what: str) -> None:
+def _check_operand(op: Fp4Operand, what: str, dev: Optional[int] = None) -> int:
+    """The operand's device, the current one (dev: already known)."""
     _fmt(op.fmt)
+    if dev is None:
+        if not (isinstance(op.codes, torch.Tensor) and op.codes.is_cuda):
+            _need(op.codes, torch.uint8, f"{what}.codes")
+        dev = _device()
     if op.rows < 0 or op.K <= 0 or op.K % 32:
         raise ValueError(f"{what}: K must be a positive multiple of 32, got {op.K}")
-    _have(op.codes, torch.uint8, f"{what}.codes", op.rows * op.K // 2)
-    _have(op.scales, torch.uint8, f"{what}.scales", _scale_bytes(op.rows, op.K, op.fmt))
+    _have(op.codes, torch.uint8, f"{what}.codes", op.rows * op.K // 2, dev)
+    _have(op.scales, torch.uint8, f"{what}.scales", _scale_bytes(op.rows, op.K, op.fmt), dev)
     if op.row_scale is not None:
-        _have(op.row_scale, torch.float32, f"{what}.row_scale", op.rows)
+        _have(op.row_scale, torch.float32, f"{what}.row_scale", op.rows, dev)
+    return dev
 
 
 def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", stream=None,
@@ -178,36 +185,36 @@ def quantize_weights_fp4(w: torch.Tensor, fmt: str = "nvfp4", stream=None) -> Fp
 def dequantize_fp4(op: Fp4Operand, out_dtype=torch.float32, out: Optional[torch.Tensor] = None,
                    stream=None) -> torch.Tensor:
     """The values of an operand, (rows, K) in out_dtype (fp32, bf16 or fp16)."""
-    _check_operand(op, "operand")
+    dev = _check_operand(op, "operand")
     if out_dtype not in _OUT:
         raise TypeError(f"unsupported output dtype {out_dtype}")
     if out is None:
         out = _empty(stream, out_dtype, op.codes.device, op.rows, op.K)
     else:
-        _have(out, out_dtype, "out", op.rows * op.K)
+        _have(out, out_dtype, "out", op.rows * op.K, dev)
     call("bd_dequantize_fp4", op.codes.data_ptr(), op.scales.data_ptr(), _ptr(op.row_scale),
          float(op.tensor_scale), out.data_ptr(), _OUT[out_dtype], FP4_FORMATS[op.fmt], op.rows,
          op.K, 0, _stream_ptr(stream))
     return out
 
 
-def _epilogue(epilogue: str, bias, N: int) -> int:
+def _epilogue(epilogue: str, bias, N: int, dev: int) -> int:
     if epilogue not in EPILOGUES:
         raise ValueError(f"unknown epilogue {epilogue!r}")
     epi = EPILOGUES[epilogue]
     if bias is not None:
-        _have(bias, torch.bfloat16, "bias", N)
+        _have(bias, torch.bfloat16, "bias", N, dev)
     if epi != _lib.BD_EPI_NONE and bias is None:
         raise ValueError(f"epilogue {epilogue!r} needs a bias")
     return epi
 
 
-def _output(out, M: int, N: int, out_dtype, device, stream):
+def _output(out, M: int, N: int, out_dtype, device, dev: int, stream):
     if out_dtype not in _OUT:
         raise TypeError(f"unsupported output dtype {out_dtype}")
     if out is None:
         return _empty(stream, out_dtype, device, M, N)
-    _have(out, out_dtype, "out", M * N)
+    _have(out, out_dtype, "out", M * N, dev)
     return out
 
 
@@ -221,11 +228,11 @@ def w4a4_gemm(acts: Fp4Operand, weights: Fp4Operand, bias: Optional[torch.Tensor
         raise ValueError(f"format mismatch: activations {acts.fmt}, weights {weights.fmt}")
     if acts.K != weights.K:
         raise ValueError(f"K mismatch: activations {acts.K}, weights {weights.K}")
-    _check_operand(acts, "acts")
-    _check_operand(weights, "weights")
+    dev = _check_operand(acts, "acts")
+    _check_operand(weights, "weights", dev)
     M, N, K = acts.rows, weights.rows, acts.K
-    epi = _epilogue(epilogue, bias, N)
-    out = _output(out, M, N, out_dtype, acts.codes.device, stream)
+    epi = _epilogue(epilogue, bias, N, dev)
+    out = _output(out, M, N, out_dtype, acts.codes.device, dev, stream)
     flags = (_lib.BD_GEMM_OVERLAP_PREV if overlap_prev else 0) | \
         (_lib.BD_GEMM_WEIGHTS_STATIC if weights_static else 0)
     call("bd_w4a4_gemm", out.data_ptr(), acts.codes.data_ptr(), acts.scales.data_ptr(),
@@ -245,10 +252,10 @@ def w4a4_linear(x: torch.Tensor, weights: Fp4Operand, bias: Optional[torch.Tenso
     M, K = _check_x4(x)
     if weights.K != K:
         raise ValueError(f"K mismatch: activations {K}, weights {weights.K}")
-    _check_operand(weights, "weights")
+    dev = _check_operand(weights, "weights", x.get_device())
     N = weights.rows
-    epi = _epilogue(epilogue, bias, N)
-    out = _output(out, M, N, out_dtype, x.device, stream)
+    epi = _epilogue(epilogue, bias, N, dev)
+    out = _output(out, M, N, out_dtype, x.device, dev, stream)
     if M == 0:
         return out
     nbytes = _linear_workspace(M, K, weights.fmt)

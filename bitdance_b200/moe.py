@@ -9,8 +9,8 @@ import torch
 
 from . import _lib
 from ._lib import call
-from .fp4 import _empty, _have, _ptr, _stream_ptr
-from .ops import _OUT, quantize_nvfp4
+from .fp4 import _device, _empty, _have, _ptr, _stream_ptr
+from .ops import _OUT, _need, quantize_nvfp4
 
 MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 64, 512, 16
 SCORINGS = {"softmax": _lib.BD_MOE_SOFTMAX, "sigmoid": _lib.BD_MOE_SIGMOID}
@@ -55,7 +55,9 @@ def _check(x: torch.Tensor, w: MoeWeights, top_k: int):
         raise ValueError("x must be a 2-D tensor (tokens, H)")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
-    _have(x, x.dtype, "x", 0)
+    if not (x.is_cuda and x.is_contiguous() and x.get_device() == _device()):
+        _need(x, x.dtype, "x")
+    dev = x.get_device()
     T, H = x.shape
     if w.gate_up.dim() != 3 or w.down.dim() != 3:
         raise ValueError("expert weights must be (E, rows, K/2)")
@@ -72,13 +74,13 @@ def _check(x: torch.Tensor, w: MoeWeights, top_k: int):
         raise ValueError(f"1 to {MOE_MAX_EXPERTS} experts, got {E}")
     if not 1 <= top_k <= min(MOE_MAX_TOP_K, E):
         raise ValueError(f"top_k must be in 1..{min(MOE_MAX_TOP_K, E)}, got {top_k}")
-    _have(w.gate_up, torch.uint8, "gate_up", 0)
-    _have(w.gate_up_scales, torch.uint8, "gate_up_scales", E * two_i * (H // 16))
-    _have(w.gate_up_tensor_scale, torch.float32, "gate_up_tensor_scale", E)
-    _have(w.down, torch.uint8, "down", 0)
-    _have(w.down_scales, torch.uint8, "down_scales", E * H * (inter // 16))
-    _have(w.down_tensor_scale, torch.float32, "down_tensor_scale", E)
-    return T, H, inter, E
+    _have(w.gate_up, torch.uint8, "gate_up", 0, dev)
+    _have(w.gate_up_scales, torch.uint8, "gate_up_scales", E * two_i * (H // 16), dev)
+    _have(w.gate_up_tensor_scale, torch.float32, "gate_up_tensor_scale", E, dev)
+    _have(w.down, torch.uint8, "down", 0, dev)
+    _have(w.down_scales, torch.uint8, "down_scales", E * H * (inter // 16), dev)
+    _have(w.down_tensor_scale, torch.float32, "down_tensor_scale", E, dev)
+    return T, H, inter, E, dev
 
 
 def _workspace_bytes(T: int, H: int, inter: int, E: int, top_k: int) -> int:
@@ -92,13 +94,13 @@ def _workspace_bytes(T: int, H: int, inter: int, E: int, top_k: int) -> int:
         up(4 * pairs * inter) + up(pairs * ((inter + 255) // 256) * 1152) + 4 * H * max(pairs, 256)
 
 
-def _out_tensor(out, x: torch.Tensor, T: int, H: int, out_dtype, stream):
+def _out_tensor(out, x: torch.Tensor, T: int, H: int, out_dtype, dev: int, stream):
     dtype = x.dtype if out_dtype is None else out_dtype
     if dtype not in _OUT:
         raise TypeError(f"unsupported output dtype {dtype}")
     if out is None:
         return _empty(stream, dtype, x.device, T, H)
-    _have(out, dtype, "out", T * H)
+    _have(out, dtype, "out", T * H, dev)
     return out
 
 
@@ -118,10 +120,10 @@ def moe_experts(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Ten
             topk_weights.shape != topk_ids.shape:
         raise ValueError("topk_ids and topk_weights must be (tokens, top_k)")
     top_k = topk_ids.shape[1]
-    T, H, inter, E = _check(x, experts, top_k)
-    _have(topk_ids, torch.int32, "topk_ids", 0)
-    _have(topk_weights, torch.float32, "topk_weights", 0)
-    out = _out_tensor(out, x, T, H, out_dtype, stream)
+    T, H, inter, E, dev = _check(x, experts, top_k)
+    _have(topk_ids, torch.int32, "topk_ids", 0, dev)
+    _have(topk_weights, torch.float32, "topk_weights", 0, dev)
+    out = _out_tensor(out, x, T, H, out_dtype, dev, stream)
     nbytes = _workspace_bytes(T, H, inter, E, top_k)
     ws = _empty(stream, torch.uint8, x.device, nbytes)
     call("bd_moe_experts", out.data_ptr(), x.data_ptr(), _IN_MOE[x.dtype], topk_ids.data_ptr(),
@@ -143,15 +145,15 @@ def moe_layer(x: torch.Tensor, router: torch.Tensor, experts: MoeWeights, top_k:
     return_routing, best expert first."""
     if scoring not in SCORINGS:
         raise ValueError(f"unknown scoring {scoring!r}: 'softmax' or 'sigmoid'")
-    T, H, inter, E = _check(x, experts, top_k)
+    T, H, inter, E, dev = _check(x, experts, top_k)
     if router.shape != (E, H):
         raise ValueError(f"router must be ({E}, {H}), got {tuple(router.shape)}")
     if router.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"router must be {x.dtype} or float32, got {router.dtype}")
-    _have(router, router.dtype, "router", 0)
+    _have(router, router.dtype, "router", 0, dev)
     if selection_bias is not None:
-        _have(selection_bias, torch.float32, "selection_bias", E)
-    out = _out_tensor(out, x, T, H, out_dtype, stream)
+        _have(selection_bias, torch.float32, "selection_bias", E, dev)
+    out = _out_tensor(out, x, T, H, out_dtype, dev, stream)
     nbytes = _workspace_bytes(T, H, inter, E, top_k)
     if return_routing:
         ids = _empty(stream, torch.int32, x.device, T, top_k)

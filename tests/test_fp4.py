@@ -174,6 +174,15 @@ def test_python_refusals():
         bd.dequantize_fp4(a)
 
 
+def test_operands_off_the_gpu_are_refused():
+    import bitdance_b200 as bd
+    u8 = torch.zeros(4096, dtype=torch.uint8)
+    op = bd.Fp4Operand(u8[:1024].view(4, 256), u8[:4096], 4, 512, "nvfp4", torch.ones(4))
+    for call in (lambda: bd.dequantize_fp4(op), lambda: bd.w4a4_gemm(op, op)):
+        with pytest.raises(TypeError, match="CUDA"):
+            call()
+
+
 # --------------------------------------------------------------------------------------- GPU
 
 gpu = pytest.mark.gpu
@@ -450,3 +459,20 @@ def test_a_refused_launch_leaves_no_error_behind():
     torch.cuda.synchronize()
     assert torch.equal(codes, want.codes) and torch.equal(row_scale, want.row_scale)
     assert rt.cudaStreamDestroy(s) == 0
+
+
+@gpu
+@pytest.mark.parametrize("which", ["codes", "scales", "row_scale"])
+def test_one_tensor_off_the_gpu_is_refused(which):
+    import bitdance_b200 as bd
+    good = bd.quantize_fp4(torch.ones(4, 512, device="cuda"))
+    bad = bd.Fp4Operand(good.codes, good.scales, 4, 512, "nvfp4", good.row_scale)
+    setattr(bad, which, getattr(good, which).cpu())
+    x = torch.ones(1, 512, device="cuda")
+    for call in (lambda: bd.dequantize_fp4(bad), lambda: bd.w4a4_gemm(good, bad),
+                 lambda: bd.w4a4_linear(x, bad),
+                 lambda: bd.w4a4_linear(x, good, bias=torch.ones(4, dtype=torch.bfloat16)),
+                 lambda: bd.w4a4_linear(x.cpu(), good),
+                 lambda: bd.dequantize_fp4(good, out=torch.empty(4, 512))):
+        with pytest.raises(TypeError, match="CUDA"):
+            call()

@@ -321,6 +321,27 @@ def test_given_routing_empty_slots_repeats_and_bad_ids():
 
 
 @gpu
+def test_one_tensor_off_the_gpu_is_refused():
+    import dataclasses
+
+    import bitdance_b200 as bd
+    case = Case(2, 128, 128, 4)
+    ids, w = torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, 2)
+    calls = [lambda: bd.moe_layer(case.x, case.router.cpu(), case.w, 2),
+             lambda: bd.moe_layer(case.x.cpu(), case.router, case.w, 2),
+             lambda: bd.moe_layer(case.x, case.router, case.w, 2, selection_bias=torch.zeros(4)),
+             lambda: bd.moe_layer(case.x, case.router, case.w, 2, out=torch.empty(2, 128).bfloat16()),
+             lambda: bd.moe_experts(case.x, ids, w.cuda(), case.w),
+             lambda: bd.moe_experts(case.x, ids.cuda(), w, case.w)]
+    for field in dataclasses.fields(case.w):
+        bad = dataclasses.replace(case.w, **{field.name: getattr(case.w, field.name).cpu()})
+        calls.append(lambda bad=bad: bd.moe_layer(case.x, case.router, bad, 2))
+    for call in calls:
+        with pytest.raises(TypeError, match="CUDA"):
+            call()
+
+
+@gpu
 def test_no_tokens():
     import bitdance_b200 as bd
     case = Case(2, 128, 128, 4)

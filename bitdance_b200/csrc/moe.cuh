@@ -125,7 +125,9 @@ __device__ __forceinline__ uint32_t e2m1_pair(float lo, float hi, float& vlo, fl
 
 // Digits of the 16-block `blk` of a row (values v already times the row's 2^shift) into its image.
 // Lanes 4 i .. 4 i + 3 hold four consecutive blocks (one scale word); all lanes of a group come
-// together.
+// together. kUnroll: digits side by side in the code; one at a time where a warp comes by once or twice
+// and the instructions' way from memory counts (48 tokens 107 us for 108; large experts 199 for 196).
+template <int kUnroll>
 __device__ __forceinline__ void moe_digits(float (&v)[16], uint8_t* img, int blk) {
   float a = 0.0f;
 #pragma unroll
@@ -137,7 +139,7 @@ __device__ __forceinline__ void moe_digits(float (&v)[16], uint8_t* img, int blk
   uint8_t* chunk = img + static_cast<int64_t>(blk >> 4) * kMoeChunk;
   const int piece = (blk & 15) >> 1;  // 16-byte piece of the 128-byte row; this block is half of it
   const uint32_t group = 0xFu << (threadIdx.x & 28);
-#pragma unroll
+#pragma unroll kUnroll
   for (int p = 0; p < kMoeDigitRows; ++p) {
     const int ep = e - 3 * p;
     uint32_t w[2] = {0, 0}, byte = 0;
@@ -186,7 +188,7 @@ __device__ void moe_convert_token(const X* x, uint8_t* xs, float* x_scale, int t
     load8(row + 16 * b + 8, *reinterpret_cast<float(*)[8]>(v + 8));
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] *= up;
-    moe_digits(v, xs + t * moe_image_row(H), b);
+    moe_digits<1>(v, xs + t * moe_image_row(H), b);
   }
   if (threadIdx.x == 0) x_scale[t] = moe_row_factor(am);
 }
@@ -394,6 +396,68 @@ struct MoePlan {
 };
 constexpr int kMoeDigitBlocks = 64;  // 16-blocks of hidden values per digit task
 
+// moe_plan for up to 32 pairs: a lane per pair of one warp (2.4 us by the whole CTA, with a barrier
+// between any two steps).
+__device__ __forceinline__ void moe_plan_warp(const MoeExpertsParams& p, MoePlan& pl) {
+  const int lane = threadIdx.x & 31, npairs = p.T * p.k;
+  constexpr uint32_t kAll = 0xFFFFFFFFu;
+  int e = -1;
+  float w = 0.0f;
+  if (lane < npairs) {
+    e = p.ids[lane];
+    w = p.weights[lane];
+    if (e < 0 || e >= p.E) {
+      if (e != -1) atomicOr(p.err, kErrRange);
+      e = -1;
+    }
+  }
+  // the first pair of a token that names this expert keeps the sum of the weights
+  const int token = lane / p.k;
+  bool first = e >= 0;
+  for (int j = 0; j < npairs; ++j) {
+    const int ej = __shfl_sync(kAll, e, j);
+    const float wj = __shfl_sync(kAll, w, j);  // (of a later pair: still its own)
+    if (j / p.k == token && ej == e) {
+      if (j < lane) first = false;
+      if (j > lane) w += wj;
+    }
+  }
+  if (!first) e = -1;
+  const uint32_t same = __match_any_sync(kAll, e), before = same & ((1u << lane) - 1u);
+  const int cnt = __popc(same);
+  const bool lead = first && before == 0;
+  const uint32_t tasks =
+      (static_cast<uint32_t>(cnt) * (p.I / 16) + kMoeDigitBlocks - 1) / kMoeDigitBlocks;
+  int place = 0, off = 0;  // touched experts and pairs of smaller experts, and their digit tasks
+  uint32_t dig = 0;
+  for (int j = 0; j < npairs; ++j) {
+    const int ej = __shfl_sync(kAll, e, j);
+    const int cj = __shfl_sync(kAll, lead ? cnt : 0, j);
+    if (cj > 0 && ej < e) {
+      ++place;
+      off += cj;
+      dig += (static_cast<uint32_t>(cj) * (p.I / 16) + kMoeDigitBlocks - 1) / kMoeDigitBlocks;
+    }
+  }
+  const int nact = __popc(__ballot_sync(kAll, lead));
+  const uint32_t total = __reduce_add_sync(kAll, lead ? tasks : 0u);
+  if (lead) {
+    pl.cnt[e] = cnt;
+    pl.off[e] = static_cast<uint16_t>(off);
+    pl.act[place] = static_cast<uint16_t>(e);
+    pl.dig[place] = dig;
+  }
+  if (first) {
+    pl.pairs[off + __popc(before)] = static_cast<uint16_t>(lane);
+    pl.w[lane] = w;
+  }
+  if (lane < npairs) pl.used[lane] = first;
+  if (lane == 0) {
+    pl.nact = nact;
+    pl.dig[nact] = total;
+  }
+}
+
 // Pairs by expert, by kThreads >= kMoeMaxExperts threads; pl.cnt is zero and visible before. A token
 // that names an expert twice keeps the first pair with the sum of the weights; ids outside [0, E) are
 // no pair (-1 quietly, others reported). Ends with a barrier.
@@ -402,6 +466,11 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
   static_assert(kThreads >= kMoeMaxExperts, "an expert per thread");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int npairs = p.T * p.k;
+  if (npairs <= 32) {
+    if (warp == 0) moe_plan_warp(p, pl);
+    __syncthreads();
+    return;
+  }
   constexpr int kPer = (kMoeMaxTokens * kMoeMaxTopK + kThreads - 1) / kThreads;
   float w[kPer] = {};
 #pragma unroll
@@ -1091,7 +1160,7 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
             v[4 * j + 2] = __uint_as_float(u.z) * up;
             v[4 * j + 3] = __uint_as_float(u.w) * up;
           }
-          moe_digits(v, p.hs + pr * moe_image_row(p.I), blk);
+          moe_digits<Cfg::kSwap ? 1 : kMoeDigitRows>(v, p.hs + pr * moe_image_row(p.I), blk);
         }
       }
       asm volatile("fence.proxy.async;" ::: "memory");

@@ -321,6 +321,21 @@ def test_given_routing_empty_slots_repeats_and_bad_ids():
 
 
 @gpu
+@pytest.mark.parametrize("T,k,E", [(1, 16, 16), (2, 16, 16), (8, 4, 5), (11, 3, 3), (33, 4, 6), (64, 16, 20)])
+def test_random_routing_with_repeats_and_empty_slots(T, k, E):
+    """Both ways of sorting the pairs by expert (up to 32 pairs, and more)."""
+    import bitdance_b200 as bd
+    case = Case(T, 256, 256, E, seed=T)
+    g = torch.Generator(device="cuda").manual_seed(T + k)
+    ids = torch.randint(-1, E, (T, k), device="cuda", dtype=torch.int32, generator=g)
+    w = torch.rand(T, k, device="cuda", generator=g) - 0.3
+    y = bd.moe_experts(case.x, ids, w, case.w, out_dtype=torch.float32)
+    check(y, case, ids, w)
+    assert torch.equal(bd.moe_experts(case.x, ids, w, case.w, out_dtype=torch.float32), y)
+    assert bd.device_error() == 0
+
+
+@gpu
 def test_one_tensor_off_the_gpu_is_refused():
     import dataclasses
 

@@ -586,11 +586,11 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
 // and the digits its 128 rows where a pass has at most 16 tokens (kSwap: half the MMAs a stage; the
 // digits' sum then runs over lanes); with 24 tokens a pass the weights are two tiles of 128 rows and the
 // digits 192 columns.
-// Measured (the layer, GPU time, one call after another): 1 token, 8 of 64 experts of 2048 x 768: 34 us
-// for 21 MB of weights: a chain of latencies (routing 5 to 9, plan 2.4, first stage 3, gate / up 5,
-// epilogue, digits 4, down, combine 3). 7 tokens, 6 of 128 of 4096 x 1408: 84 us (5.2 TB/s while the
-// weights stream); 48 tokens, 8 of 128 of 2048 x 1024: 108 us (4.4 TB/s over this kernel); 64 tokens, 2
-// of 8 of 4096 x 14336: 198 us (4.2 TB/s): there a stage's MMAs (1000 to 1250 cycles) and the drain of
+// Measured (the layer, GPU time, one call after another): 1 token, 8 of 64 experts of 2048 x 768: 33 us
+// for 21 MB of weights: a chain of latencies (routing 5 to 9, plan 1.5, first stage 3, gate / up 5,
+// epilogue, digits 4, down, combine 3), most of its code run once, from cold instruction caches. 7
+// tokens, 6 of 128 of 4096 x 1408: 84 us (5.2 TB/s while the weights stream); 48 tokens, 8 of 128 of
+// 2048 x 1024: 107 us (4.4 TB/s over this kernel); 64 tokens, 2 of 8 of 4096 x 14336: 196 us (4.2 TB/s): there a stage's MMAs (1000 to 1250 cycles) and the drain of
 // the one accumulator that fits tensor memory beside the scales take nearly as long as its bytes.
 // Tried, no gain: a fourth stage of weights (93 us for 91 at seven tokens); scales stored to tensor
 // memory from registers instead of tcgen05.cp (equal with four sets of scale words, 211 us for 199 with

@@ -5,6 +5,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -45,13 +46,16 @@ def _run(cmd) -> str:
 def build_library(force: bool = False, verbose: bool = False) -> str:
     if force or stale():
         flags = [f for f in NVCC_FLAGS if f != "-shared"] + (["-Xptxas=-v"] if verbose else [])
-        objs = [os.path.splitext(f)[0] + ".o" for f in SOURCES]
-        with ThreadPoolExecutor(len(SOURCES)) as pool:  # one nvcc per source
-            logs = list(pool.map(lambda so: _run([nvcc(), *flags, "-c", "-o", so[1], so[0]]),
-                                 zip(SOURCES, objs)))
-        _run([nvcc(), *NVCC_FLAGS, "-o", LIB, *objs])
-        for o in objs:
-            os.remove(o)
+        # objects and the new library beside no one else's: processes may build at the same time, and
+        # one may have the old library open
+        with tempfile.TemporaryDirectory() as tmp:
+            objs = [os.path.join(tmp, os.path.basename(f)[:-3] + ".o") for f in SOURCES]
+            with ThreadPoolExecutor(len(SOURCES)) as pool:  # one nvcc per source
+                logs = list(pool.map(lambda so: _run([nvcc(), *flags, "-c", "-o", so[1], so[0]]),
+                                     zip(SOURCES, objs)))
+            new = f"{LIB[:-3]}.{os.getpid()}.so"
+            _run([nvcc(), *NVCC_FLAGS, "-o", new, *objs])
+            os.replace(new, LIB)
         if verbose:
             print("".join(logs))
     return LIB

@@ -223,7 +223,9 @@ def w4a4_gemm(acts: Fp4Operand, weights: Fp4Operand, bias: Optional[torch.Tensor
               out: Optional[torch.Tensor] = None, stream=None, overlap_prev: bool = False,
               weights_static: bool = False) -> torch.Tensor:
     """C[M, N] = act(A . B^T + bias) of two 4-bit operands of one format on the tensor cores (any
-    M and N, K % 32 == 0; no workspace). overlap_prev, weights_static: as in ``w4a6_gemm``."""
+    M and N, K % 32 == 0; no workspace). bias (N,) bf16 is added by the epilogues "bias", "bias_relu",
+    "bias_silu" and "bias_gelu" ("none" leaves it unread). overlap_prev, weights_static: as in
+    ``w4a6_gemm``."""
     if acts.fmt != weights.fmt:
         raise ValueError(f"format mismatch: activations {acts.fmt}, weights {weights.fmt}")
     if acts.K != weights.K:
@@ -248,7 +250,7 @@ def w4a4_linear(x: torch.Tensor, weights: Fp4Operand, bias: Optional[torch.Tenso
                 out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """C = act(quantize_fp4(x) . W^T + bias) from raw activations x (M, K) fp32 / bf16 / fp16, in
     the weights' format: the quantiser, then the W4A4 GEMM, which streams its first weights while
-    the quantiser runs."""
+    the quantiser runs. bias, epilogue: as in ``w4a4_gemm``."""
     M, K = _check_x4(x)
     if weights.K != K:
         raise ValueError(f"K mismatch: activations {K}, weights {weights.K}")

@@ -336,6 +336,35 @@ def test_random_routing_with_repeats_and_empty_slots(T, k, E):
 
 
 @gpu
+def test_largest_counts():
+    import bitdance_b200 as bd
+    case = Case(64, 128, 128, 512, seed=9)
+    y, ids, weights = bd.moe_layer(case.x, case.router, case.w, 16, return_routing=True)
+    want_ids, want_w = routing(case, 16)
+    assert torch.equal(ids, want_ids)
+    assert weights_match(weights, want_w, case)
+    check(y, case, ids, weights)
+    assert bd.device_error() == 0
+
+
+@gpu
+def test_two_layers_and_a_linear_at_once_on_three_streams():
+    import bitdance_b200 as bd
+    cases = [Case(9, 512, 256, 12, seed=1), Case(40, 256, 512, 6, seed=2)]
+    w4 = bd.quantize_weights_fp4(torch.randn(1024, 512, device="cuda"))
+    calls = [lambda s=None, c=c: bd.moe_layer(c.x, c.router, c.w, 3, stream=s) for c in cases]
+    calls.append(lambda s=None: bd.w4a4_linear(cases[0].x, w4, stream=s))
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [(i, call(s)) for _ in range(20) for i, (call, s) in enumerate(zip(calls, streams))]
+    torch.cuda.synchronize()
+    for i, y in got:
+        assert torch.equal(y, want[i])
+    assert bd.device_error() == 0
+
+
+@gpu
 def test_one_tensor_off_the_gpu_is_refused():
     import dataclasses
 

@@ -9,12 +9,13 @@
 // cp.async to shared memory and from there to tcgen05.mma kind::mxf4nvf4 as they are. What that MMA
 // wants besides is a second operand in 4 bits, and it has columns to spare: a token becomes eight
 // columns, six of them digits of its values. With s = 2^e the scale of a 16-block (amax <= 4 s),
-//   x = s (d_0 + d_1 / 8 + ... + d_5 / 8^5) + r,   d_p = E2M1 round of what is left, |r| <= s 2^-16,
-// each digit's scale 2^(e - 3 p) an E4M3 power of two, and the columns' sum is the product with x
-// to 2^-17 of the block's largest value (digits whose scale would fall below E4M3's 2^-9 are dropped:
-// 2^-20 of the row's largest): activations of 16 bits against 4-bit weights (W4A16) on the FP4
-// tensor cores without unpacking a weight. (Unpacking them into fp16 fragments for mma.sync took
-// 140 to 175 instructions per 2048 weights and ran at 40 % of the memory rate.)
+//   x = s (d_0 + d_1 / 8 + ... + d_5 / 8^5) + r,   d_p = E2M1 round of what is left, |r| <= s 2^-16.
+// All six digits carry the block's scale s, an E4M3 power of two; a digit's factor 8^-p is common to its
+// column, so it is applied to the column's finished sum. The product is then one with x to 2^-17 of the
+// block's largest value, or to 2^-34 of the row's where E4M3's smallest scale is larger than the block
+// wants: activations of 16 bits against 4-bit weights (W4A16) on the FP4 tensor cores without unpacking
+// a weight. (Unpacking them into fp16 fragments for mma.sync took 140 to 175 instructions per 2048
+// weights and ran at 40 % of the memory rate.)
 //
 // Kernel 1 (moe_route_kernel, or moe_prepare_kernel where the caller brings the routing): router
 // products, selection, digits of x, counters to zero.
@@ -51,7 +52,8 @@ enum : int {
 __host__ __device__ constexpr int moe_counters(int E) { return kMoeCounters + 2 * E; }
 
 // Digits of a row of K activations: per 256 elements the 8 x 128 bytes of codes (row p: digit p; rows
-// 6 and 7 are zero), 128B-swizzled as the MMA's operand tile, then 8 x 4 words of scales.
+// 6 and 7 are zero), 128B-swizzled as the MMA's operand tile, then 8 x 4 words of scales (the same
+// for every row).
 constexpr int kMoeDigitRows = 8, kMoeDigitCount = 6;
 constexpr int kMoeChunkCodes = 1024;
 constexpr int kMoeChunk = kMoeChunkCodes + 128;
@@ -101,7 +103,8 @@ __device__ __forceinline__ float pow2f(int e) {
 }
 // Row factor: with 2^E <= amax < 2^(E+1) the row times 2^(9 - E) is below 2^10 = 4 * 2^8, so that its
 // largest block's scale is E4M3's 2^8. Returns 9 - E; the factor back is 2^(E - 9), and NaN for a
-// row with a NaN or Inf (its digits are finite: the factor carries the NaN into every product).
+// row with a NaN or Inf (its digits are finite: the factor carries the NaN into every product). Rows
+// below 2^-100 get the factor of 2^-100.
 __device__ __forceinline__ int moe_row_shift(uint32_t amax_bits) {
   return 9 - min(127, max(-100, static_cast<int>(amax_bits >> 23) - 127));
 }
@@ -139,11 +142,17 @@ __device__ __forceinline__ void moe_digits(float (&v)[16], uint8_t* img, int blk
   uint8_t* chunk = img + static_cast<int64_t>(blk >> 4) * kMoeChunk;
   const int piece = (blk & 15) >> 1;  // 16-byte piece of the 128-byte row; this block is half of it
   const uint32_t group = 0xFu << (threadIdx.x & 28);
+  const uint32_t byte = e >= -6 ? static_cast<uint32_t>(e + 7) << 3 : 1u << (e + 9);  // E4M3 2^e
+  uint32_t word = byte << (8 * (blk & 3));
+  word |= __shfl_xor_sync(group, word, 1);
+  word |= __shfl_xor_sync(group, word, 2);
+  uint8_t* scales = chunk + kMoeChunkCodes + (blk & 12);  // rows 2 i and 2 i + 1 by lane i of the four
+  *reinterpret_cast<uint32_t*>(scales + (blk & 3) * 32) = word;
+  *reinterpret_cast<uint32_t*>(scales + (blk & 3) * 32 + 16) = word;
 #pragma unroll kUnroll
   for (int p = 0; p < kMoeDigitRows; ++p) {
-    const int ep = e - 3 * p;
-    uint32_t w[2] = {0, 0}, byte = 0;
-    if (p < kMoeDigitCount && ep >= -9) {
+    uint32_t w[2] = {0, 0};
+    if (p < kMoeDigitCount) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float d0, d1;
@@ -151,15 +160,9 @@ __device__ __forceinline__ void moe_digits(float (&v)[16], uint8_t* img, int blk
         v[2 * j] = (v[2 * j] - d0) * 8.0f;
         v[2 * j + 1] = (v[2 * j + 1] - d1) * 8.0f;
       }
-      byte = ep >= -6 ? static_cast<uint32_t>(ep + 7) << 3 : 1u << (ep + 9);
     }
     *reinterpret_cast<uint2*>(chunk + p * 128 + ((piece ^ p) << 4) + (blk & 1) * 8) =
         make_uint2(w[0], w[1]);
-    uint32_t word = byte << (8 * (blk & 3));
-    word |= __shfl_xor_sync(group, word, 1);
-    word |= __shfl_xor_sync(group, word, 2);
-    if ((blk & 3) == 0)
-      *reinterpret_cast<uint32_t*>(chunk + kMoeChunkCodes + p * 16 + (blk & 15)) = word;
   }
 }
 
@@ -771,16 +774,16 @@ __device__ __forceinline__ void moe_count_down(uint32_t* counter, uint32_t* warp
   }
 }
 
-// Sum of a token's eight digit columns.
+// Sum of a token's digit columns, digit p times 8^-p (the product by 1/8 is exact).
 __device__ __forceinline__ float moe_sum8(const uint32_t* r) {
   float s = __uint_as_float(r[kMoeDigitCount - 1]);
 #pragma unroll
-  for (int p = kMoeDigitCount - 2; p >= 0; --p) s += __uint_as_float(r[p]);
+  for (int p = kMoeDigitCount - 2; p >= 0; --p) s = fmaf(s, 0.125f, __uint_as_float(r[p]));
   return s;
 }
 
-// 16 columns of eight lanes' digits: lane c of the eight gets the sums over them of columns 2 c and
-// 2 c + 1, by way of shared memory. (In registers, by three exchanges of halves, it took 14 shuffles
+// 16 columns of eight lanes' digits: lane c of the eight gets the sums over them (digit p times 8^-p) of
+// columns 2 c and 2 c + 1, by way of shared memory. (In registers, by three exchanges of halves, it took 14 shuffles
 // and 28 selects: with one to four tokens all of that is the work of one scheduler's warps, and the
 // accumulator is busy until it ends.)
 __device__ __forceinline__ float2 moe_lane_sums(const uint32_t (&d)[16], float* buf) {
@@ -799,8 +802,8 @@ __device__ __forceinline__ float2 moe_lane_sums(const uint32_t (&d)[16], float* 
   __syncwarp();
 #pragma unroll
   for (int p = kMoeDigitCount - 2; p >= 0; --p) {
-    v[p].x += v[p + 1].x;
-    v[p].y += v[p + 1].y;
+    v[p].x = fmaf(v[p + 1].x, 0.125f, v[p].x);
+    v[p].y = fmaf(v[p + 1].y, 0.125f, v[p].y);
   }
   return v[0];
 }

@@ -340,8 +340,8 @@ int bd_w4a4_linear(void* c, const void* x, int x_dtype, const uint8_t* b, const 
  * down (E, H, I/2) and (E, H, I/16); one fp32 tensor scale per expert and matrix, device arrays.
  * T <= 64 tokens, E <= 512, top_k <= min(16, E), H % 128 == 0, I % 128 == 0; T == 0: nothing is
  * done. x bf16 or fp16 (T, H); y (T, H) in out_dtype. Weights enter the products exactly, x and the
- * hidden values to 2^-17 of the largest magnitude of their 16-block (values below 2^-20 of their
- * row's largest may drop out); sums fp32; a token with a NaN or Inf gives a row of NaN; results do
+ * hidden values to 2^-17 of the largest magnitude of their 16-block, 2^-34 of their row's or 2^-134,
+ * whichever is largest; sums fp32; a token with a NaN or Inf gives a row of NaN; results do
  * not depend on timing. Codes, x and router 16-byte aligned, scales 8-byte. workspace:
  * bd_query_moe_workspace bytes, 256-byte aligned, contents irrelevant before and after; concurrent
  * calls must not share one. No reference counterpart. */

@@ -227,15 +227,41 @@ __device__ __forceinline__ double block_reduce(double v, double* part) {
   return v;
 }
 
+// A lane's part of a logit in 64 bits: 8-element pieces c, c + step, ... kExact: each product in 64 bits
+// too; else in fp32, where a product of two 16-bit numbers is exact unless it leaves fp32's range.
+template <bool kExact, int kUnroll, class X, class W>
+__device__ __forceinline__ double route_dot(const W* row, const X* x, int c, int step, int pieces) {
+  double sum[4] = {};
+#pragma unroll kUnroll
+  for (; c < pieces; c += step) {
+    float w[8], v[8];
+    load8(row + 8 * c, w);
+    load8(x + 8 * c, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (kExact) sum[j & 3] = fma(static_cast<double>(w[j]), static_cast<double>(v[j]), sum[j & 3]);
+      else sum[j & 3] += static_cast<double>(__fmul_rn(w[j], v[j]));
+    }
+  }
+  double all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
+  return all;
+}
+
 // Router: a cluster of eight CTAs per token; a CTA takes every eighth expert (every seventh, and the last
-// CTA none, where seven CTAs' warps hold all experts at once), a warp per expert and part of K (of
-// eight where the experts are few); the partial logits go to CTA 0's shared memory, which adds and selects. The last CTA makes the token's digits
-// meanwhile. Two logits may be arbitrarily close, so they are kept in 64 bits: eight products are
-// summed in fp32 and added to a double, an error near 1e-8 of the logits' spread. Bound by latency: one
-// pass over the router weights is half of it (3 of 5 us for one token and 64 experts), the selection's
-// steps the rest. (Two or four tokens per cluster, for fewer passes over the weights: 64 tokens, 64
-// experts, H 4096 took the layer 127 us for 118. A share of the token's digits in each CTA took longer
-// than one CTA's whole token beside the others' products: 17 for 14 us at seven tokens.)
+// CTA none, where seven CTAs' warps hold all experts at once), a warp per expert and part of K (of eight
+// where the experts are few); the partial logits go to CTA 0's shared memory, which adds and selects. The
+// last CTA makes the token's digits meanwhile. Two logits may be arbitrarily close, so they are sums in 64
+// bits of exact products: of 16-bit routers in fp32, one conversion each (eight products summed in fp32
+// first misplaced logits closer than 2^-24 of their terms; the layer of 48 tokens and 128 experts takes 105
+// us either way, of 7 tokens, H 4096, 83 for 81, of 64 tokens and 512 experts 144 for 140), again with 64-bit products where one may have left
+// fp32's range (a sum that is not finite, or so small that what underflowed could count); of fp32 routers in
+// 64 bits (16 tokens, 256 experts, H 4096 89 us for 85). Bound by latency: one pass over the router
+// weights is half of it (3 of 5 us for one token and 64 experts), the selection's steps the rest. (Two or
+// four tokens per cluster, for fewer passes over the weights: 64 tokens, 64 experts, H 4096 took the layer
+// 127 us for 118. A share of the token's digits in each CTA took longer than one CTA's whole token beside
+// the others' products: 17 for 14 us at seven tokens.)
 template <class X, class W, int parts>
 __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRouteParams p) {
   extern __shared__ double sh[];  // partial logits [parts][E], then keys [E]
@@ -256,20 +282,13 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
   const int experts = rank < ranks ? (p.E - rank + ranks - 1) / ranks : 0;
   for (int job = warp; job < experts * parts; job += kMoeWarps) {
     const int e = rank + ranks * (job / parts), q = job % parts;
-    double acc = 0.0;
     const W* row = wr + static_cast<int64_t>(e) * p.H;
     const X* xt = x + static_cast<int64_t>(t) * p.H;
-#pragma unroll 8
-    for (int c = 32 * q + lane; c < pieces; c += 32 * parts) {
-      float w[8], v[8], s = 0.0f;
-      load8(row + 8 * c, w);
-      load8(xt + 8 * c, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s = fmaf(w[j], v[j], s);
-      acc += static_cast<double>(s);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xFFFFFFFFu, acc, o);
+    constexpr bool kExact = sizeof(W) == 4;
+    double acc = route_dot<kExact, 8>(row, xt, 32 * q + lane, 32 * parts, pieces);
+    // 2^20 products below 2^-126 lose 2^-130 in all: nothing beside 2^-60 in 64 bits
+    if (!kExact && !(fabs(acc) > 8.7e-19 && fabs(acc) < INFINITY))
+      acc = route_dot<true, 1>(row, xt, 32 * q + lane, 32 * parts, pieces);
     if (lane == 0) {
       const uint32_t at = mapa_shared(smem_u32(&sh[q * p.E + e]), 0);
       asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(acc) : "memory");

@@ -361,8 +361,8 @@ int bd_moe_experts(void* y, const void* x, int x_dtype, const int* ids, const fl
                    int I, int E, int top_k, int out_dtype, void* workspace,
                    size_t workspace_bytes, bd_stream_t stream);
 
-/* The whole layer in two kernels: logits = x . router^T (router (E, H) in x's type or fp32), score =
- * softmax over the experts or sigmoid; the top_k experts by score (+ selection_bias[e], NULL: none),
+/* The whole layer in two kernels: logits = x . router^T in 64 bits (router (E, H) in x's type or fp32),
+ * score = softmax over the experts or sigmoid; the top_k experts by score (+ selection_bias[e], NULL: none),
  * ties to the lowest index, a NaN last; weights = score, divided by their sum when renormalize,
  * times routed_scale. Writes ids and weights (T, top_k), best first, then y as bd_moe_experts. */
 int bd_moe_layer(void* y, int* ids, float* weights, const void* x, int x_dtype,

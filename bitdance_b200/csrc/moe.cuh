@@ -26,6 +26,7 @@
 // runs, so the waits end without any guarantee that the whole grid is resident.
 #pragma once
 #include <cstdint>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -227,16 +228,22 @@ __device__ __forceinline__ double block_reduce(double v, double* part) {
   return v;
 }
 
-// A lane's part of a logit in 64 bits: 8-element pieces c, c + step, ... kExact: each product in 64 bits
-// too; else in fp32, where a product of two 16-bit numbers is exact unless it leaves fp32's range.
+// A logit in 64 bits, by a warp: a lane's 8-element pieces c, c + step, ... kExact: each product in 64 bits
+// too; else in fp32, where a product of two 16-bit numbers is exact unless it leaves fp32's range. some: x
+// is not zero throughout.
 template <bool kExact, int kUnroll, class X, class W>
-__device__ __forceinline__ double route_dot(const W* row, const X* x, int c, int step, int pieces) {
+__device__ __forceinline__ double route_dot(const W* row, const X* x, int c, int step, int pieces,
+                                            bool& some) {
   double sum[4] = {};
+  uint32_t bits = 0;
 #pragma unroll kUnroll
   for (; c < pieces; c += step) {
     float w[8], v[8];
     load8(row + 8 * c, w);
-    load8(x + 8 * c, v);
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(x + 8 * c));
+    bits |= q.x | q.y | q.z | q.w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f32(reinterpret_cast<const X*>(&q)[j]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if constexpr (kExact) sum[j & 3] = fma(static_cast<double>(w[j]), static_cast<double>(v[j]), sum[j & 3]);
@@ -246,6 +253,7 @@ __device__ __forceinline__ double route_dot(const W* row, const X* x, int c, int
   double all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
+  some = __any_sync(0xFFFFFFFFu, bits != 0);
   return all;
 }
 
@@ -255,13 +263,13 @@ __device__ __forceinline__ double route_dot(const W* row, const X* x, int c, int
 // last CTA makes the token's digits meanwhile. Two logits may be arbitrarily close, so they are sums in 64
 // bits of exact products: of 16-bit routers in fp32, one conversion each (eight products summed in fp32
 // first misplaced logits closer than 2^-24 of their terms; the layer of 48 tokens and 128 experts takes 105
-// us either way, of 7 tokens, H 4096, 83 for 81, of 64 tokens and 512 experts 144 for 140), again with 64-bit products where one may have left
-// fp32's range (a sum that is not finite, or so small that what underflowed could count); of fp32 routers in
-// 64 bits (16 tokens, 256 experts, H 4096 89 us for 85). Bound by latency: one pass over the router
-// weights is half of it (3 of 5 us for one token and 64 experts), the selection's steps the rest. (Two or
-// four tokens per cluster, for fewer passes over the weights: 64 tokens, 64 experts, H 4096 took the layer
-// 127 us for 118. A share of the token's digits in each CTA took longer than one CTA's whole token beside
-// the others' products: 17 for 14 us at seven tokens.)
+// us either way, of 7 tokens, H 4096, 83 for 81, of 64 tokens and 512 experts 144 for 140), again with
+// 64-bit products where one may have left fp32's range (a sum that is not finite, or so small that what
+// underflowed could count); of fp32 routers in 64 bits (16 tokens, 256 experts, H 4096 89 us for 85). Bound
+// by latency: one pass over the router weights is half of it (3 of 5 us for one token and 64 experts), the
+// selection's steps the rest. (Two or four tokens per cluster, for fewer passes over the weights: 64
+// tokens, 64 experts, H 4096 took the layer 127 us for 118. A share of the token's digits in each CTA took
+// longer than one CTA's whole token beside the others' products: 17 for 14 us at seven tokens.)
 template <class X, class W, int parts>
 __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRouteParams p) {
   extern __shared__ double sh[];  // partial logits [parts][E], then keys [E]
@@ -285,10 +293,14 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
     const W* row = wr + static_cast<int64_t>(e) * p.H;
     const X* xt = x + static_cast<int64_t>(t) * p.H;
     constexpr bool kExact = sizeof(W) == 4;
-    double acc = route_dot<kExact, 8>(row, xt, 32 * q + lane, 32 * parts, pieces);
-    // 2^20 products below 2^-126 lose 2^-130 in all: nothing beside 2^-60 in 64 bits
-    if (!kExact && !(fabs(acc) > 8.7e-19 && fabs(acc) < INFINITY))
-      acc = route_dot<true, 1>(row, xt, 32 * q + lane, 32 * parts, pieces);
+    bool some;
+    double acc = route_dot<kExact, 8>(row, xt, 32 * q + lane, 32 * parts, pieces, some);
+    // products of two bf16 numbers may leave fp32's range (of fp16 none does): 2^20 of them below 2^-126 lose
+    // 2^-130 in all, nothing beside 2^-60 in 64 bits. (Zero rows pad a batch: they cost no second pass.)
+    if constexpr (!kExact && std::is_same_v<X, __nv_bfloat16>) {
+      if (some && !(fabs(acc) > 8.7e-19 && fabs(acc) < INFINITY))
+        acc = route_dot<true, 1>(row, xt, 32 * q + lane, 32 * parts, pieces, some);
+    }
     if (lane == 0) {
       const uint32_t at = mapa_shared(smem_u32(&sh[q * p.E + e]), 0);
       asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(acc) : "memory");

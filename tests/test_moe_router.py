@@ -74,3 +74,20 @@ def test_products_beyond_fp32(size):
     want = score / score.sum(dim=1, keepdim=True)
     # fp32 rounding, and logits of 2^140 leave the first alone
     assert ((weights.cpu().double() - want).abs() <= 2.0 ** -23 * want).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_zero_rows_in_a_batch(dtype):
+    """Rows of zeros, as a padded batch has them: every logit is equal, the output row is zero."""
+    import bitdance_b200 as bd
+    from test_moe import Case, check, routing
+    case = Case(6, 256, 128, 9, dtype, seed=3)
+    case.x[1] = 0
+    case.x[4] = -0.0
+    y, ids, weights = bd.moe_layer(case.x, case.router, case.w, 4, return_routing=True)
+    want_ids, _ = routing(case, 4)
+    assert torch.equal(ids, want_ids)
+    for t in (1, 4):
+        assert ids[t].tolist() == [0, 1, 2, 3] and (weights[t] == 0.25).all() and (y[t] == 0).all()
+    check(y, case, ids, weights)

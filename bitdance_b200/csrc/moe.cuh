@@ -311,16 +311,19 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
   if (rank != 0) return;
   // Scores and keys. The key ranks: the logit itself (softmax without bias: the same order, nothing
   // rounds), else score + bias; a NaN ranks last. Where the weights are renormalised softmax scores
-  // ranked by logit, exp(logit - largest) of the chosen ones is all that is needed.
+  // ranked by logit, exp(logit - largest) of the chosen ones is all that is needed (and whether any logit
+  // is a NaN: then every score is).
   double* score = sh;
   double* key = sh + parts * p.E;
   const bool lazy = !p.sigmoid && p.bias == nullptr && p.renormalize;
+  bool nan = false;
   for (int e = threadIdx.x; e < p.E; e += kMoeThreads) {
     double l = score[e];
 #pragma unroll
     for (int q = 1; q < parts; ++q) l += sh[q * p.E + e];
     if (parts > 1) score[e] = l;
     key[e] = l == l ? l : -INFINITY;
+    nan |= l != l;
   }
   if (!lazy) {  // (every loop gives a thread the same experts)
     double m = 0.0, z = 1.0;
@@ -340,7 +343,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
       key[e] = v == v ? v : -INFINITY;
     }
   }
-  __syncthreads();
+  nan = __syncthreads_or(nan);
   // rank of an expert: how many stand before it (ties to the lowest index); ranks are distinct.
   // `team` threads (a power of two up to 32) share an expert.
   int team = 32;
@@ -371,6 +374,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeRoutePa
     if (p.renormalize) {
       sum = 0.0;
       for (int r = 0; r < p.k; ++r) sum += __shfl_sync(0xFFFFFFFFu, mine, r);
+      if (lazy && nan) sum = NAN;
     }
     if (lane < p.k) {
       p.hmax[t * p.k + lane] = 0;

@@ -363,8 +363,9 @@ int bd_moe_experts(void* y, const void* x, int x_dtype, const int* ids, const fl
 
 /* The whole layer in two kernels: logits = x . router^T in 64 bits (router (E, H) in x's type or fp32),
  * score = softmax over the experts or sigmoid; the top_k experts by score (+ selection_bias[e], NULL: none),
- * ties to the lowest index, a NaN last; weights = score, divided by their sum when renormalize,
- * times routed_scale. Writes ids and weights (T, top_k), best first, then y as bd_moe_experts. */
+ * ties to the lowest index, a NaN last (a NaN logit makes every softmax score of its token NaN);
+ * weights = score, divided by their sum when renormalize, times routed_scale. Writes ids and weights
+ * (T, top_k), best first, then y as bd_moe_experts. */
 int bd_moe_layer(void* y, int* ids, float* weights, const void* x, int x_dtype,
                  const void* router, int router_dtype, const float* selection_bias, int scoring,
                  int renormalize, float routed_scale, const uint8_t* gate_up,

@@ -91,3 +91,22 @@ def test_zero_rows_in_a_batch(dtype):
     for t in (1, 4):
         assert ids[t].tolist() == [0, 1, 2, 3] and (weights[t] == 0.25).all() and (y[t] == 0).all()
     check(y, case, ids, weights)
+
+
+@gpu
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_a_nan_logit_shows_in_the_softmax_weights(renormalize):
+    """softmax over the experts of logits with a NaN is NaN, whether that expert is chosen or not."""
+    import bitdance_b200 as bd
+    E, H = 12, 256
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(2, H, generator=g).to(torch.bfloat16)
+    r = torch.randn(E, H, generator=g).to(torch.bfloat16)
+    r[5, 100] = float("nan")
+    _, ids, weights = bd.moe_layer(x.cuda(), r.cuda(), experts(E, H), 3, renormalize=renormalize,
+                                   return_routing=True)
+    assert weights.isnan().all()
+    assert not (ids == 5).any()  # a NaN ranks last
+    _, ids, weights = bd.moe_layer(x.cuda(), r.cuda(), experts(E, H), 3, scoring="sigmoid",
+                                   return_routing=True)
+    assert weights.isfinite().all() and not (ids == 5).any()

@@ -749,22 +749,25 @@ __device__ __forceinline__ bool moe_next_task(MoeTask& t, RingPos<kMoeQueue>& q,
   return true;
 }
 
-// A whole warp: until *counter >= target (counter of this grid, or kCta of this CTA), bounded. A counter
+// A whole warp: until *counter >= target (counter of this grid, or kCta of this CTA), bounded; `seen` is
+// the value that ended the lane's wait, and only that one was acquired. A counter
 // of the grid is read again only after a pause: a poll takes its turn in the same L2 slice as the
 // additions it waits for. (One warp per CTA polls for the others where they wait for the same: with all
 // eight epilogue warps of 148 CTAs polling, the combine phase began 1.5 us later.)
 template <bool kCta>
 __device__ __forceinline__ bool moe_wait(const uint32_t* counter, uint32_t target, MoeCtl& ctl,
-                                         uint32_t* err) {
+                                         uint32_t* err, uint32_t& seen) {
   bool ok = true;
   const long long c0 = clock64();
   while (true) {
-    uint32_t v;
     if constexpr (kCta)
-      asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(counter)) : "memory");
+      asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];"
+                   : "=r"(seen)
+                   : "r"(smem_u32(counter))
+                   : "memory");
     else
-      v = ld_acquire_gpu(counter);
-    if (v >= target) break;
+      seen = ld_acquire_gpu(counter);
+    if (seen >= target) break;
     if (*reinterpret_cast<volatile uint32_t*>(&ctl.abort_flag)) {
       ok = false;
       break;
@@ -778,6 +781,12 @@ __device__ __forceinline__ bool moe_wait(const uint32_t* counter, uint32_t targe
     __nanosleep(kCta ? 20 : 60);
   }
   return __all_sync(0xFFFFFFFFu, ok);
+}
+template <bool kCta>
+__device__ __forceinline__ bool moe_wait(const uint32_t* counter, uint32_t target, MoeCtl& ctl,
+                                         uint32_t* err) {
+  uint32_t seen;
+  return moe_wait<kCta>(counter, target, ctl, err, seen);
 }
 constexpr uint32_t kMoeAllSeen = 1u << 30;
 
@@ -1047,9 +1056,9 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
                          "r"(ready ? kMoeAllSeen : seen)
                          : "memory");
         } else {
-          if (!moe_wait<true>(&ctl.digits_seen, seen, ctl, p.err)) break;
-          ready = __all_sync(0xFFFFFFFFu, *reinterpret_cast<volatile uint32_t*>(&ctl.digits_seen) ==
-                                              kMoeAllSeen);
+          uint32_t now;
+          if (!moe_wait<true>(&ctl.digits_seen, seen, ctl, p.err, now)) break;
+          ready = __all_sync(0xFFFFFFFFu, now == kMoeAllSeen);
         }
         // written by ordinary stores of this grid; the bulk copies read through the async proxy
         asm volatile("fence.proxy.async;" ::: "memory");

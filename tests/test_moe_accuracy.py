@@ -137,3 +137,19 @@ def test_one_expert_with_more_tokens_than_a_pass(T, H, I):
     y = bd.moe_experts(case.x, ids, w, case.w, out_dtype=torch.float32)
     check(y, case, ids, w)
     assert bd.device_error() == 0
+
+
+@gpu
+def test_experts_that_finish_far_apart_repeat_their_bits():
+    """One expert with every token beside many with one: down tasks wait for digits made long apart."""
+    import bitdance_b200 as bd
+    from test_moe import Case, check
+    T, E = 64, 96
+    case = Case(T, 1024, 768, E, seed=2)
+    ids = torch.stack([torch.full((T,), 95), torch.arange(T), torch.full((T,), 3)], dim=1).int().cuda()
+    w = torch.rand(T, 3, device="cuda") + 0.25
+    want = bd.moe_experts(case.x, ids, w, case.w, out_dtype=torch.float32)
+    check(want, case, ids, w)
+    for _ in range(100):
+        assert torch.equal(bd.moe_experts(case.x, ids, w, case.w, out_dtype=torch.float32), want)
+    assert bd.device_error() == 0

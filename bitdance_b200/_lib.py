@@ -42,6 +42,7 @@ SIGNATURES = {
     "bd_status_string": (ctypes.c_char_p, [_I]),
     "bd_device_error": (_I, [ctypes.POINTER(ctypes.c_uint32), _I]),
     "bd_selftest_bounded_wait": (_I, [_I64, _P]),
+    "bd_selftest_cluster_wait": (_I, [_I64, _I, _I, _P, _P]),
     "bd_probe_mma_peak": (_I, [_I64, _I, _I, _P]),
     "bd_transcode_nvfp4_to_mxfp6": (_I, [_P, _P, _P, _P, _I64, _I, _P]),
     "bd_pack_b": (_I, [_P, _P, _P, _P, _I, _I, _P]),

@@ -330,6 +330,22 @@ int bd_w4a4_gemm(void* c, const uint8_t* a, const uint8_t* a_scales, const float
                              : launch_gemm_any<kMxfp4>(p, a, b, overlap, d, as_stream(stream));
 }
 
+int bd_selftest_cluster_wait(int64_t limit_cycles, int ctas, int failing, uint32_t* stored,
+                             bd_stream_t stream) {
+  if (limit_cycles < 1000 || static_cast<unsigned long long>(limit_cycles) > kWaitLimitCycles)
+    return BD_ERR_INVALID_ARG;
+  if ((ctas != 2 && ctas != 4 && ctas != 8) || failing < -1 || failing >= ctas || !stored)
+    return BD_ERR_INVALID_ARG;
+  if (!aligned(stored, 4)) return BD_ERR_ALIGNMENT;
+  DeviceInfo* d = nullptr;
+  const int st = device_info(&d);
+  if (st != BD_OK) return st;
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = launch_config(ctas, 128, 0, as_stream(stream), attr, false, ctas);
+  return launch_status(cudaLaunchKernelEx(&cfg, cluster_wait_selftest_kernel, stored, ctas, failing,
+                                          static_cast<unsigned long long>(limit_cycles), d->err));
+}
+
 size_t bd_query_w4a4_linear_workspace(int M, int K, int fmt) {
   if (bad_fmt(fmt) || M <= 0 || K <= 0 || K % 32) return 0;
   return linear_ws(M, K, fmt).total;

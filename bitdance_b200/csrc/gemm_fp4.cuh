@@ -80,6 +80,7 @@ struct GemmFp4Cfg {
 struct GemmFp4Ctl {
   uint64_t full[8], empty[8], done;
   uint32_t tmem_base, abort_flag;
+  uint32_t peer_failed;  // set by a CTA of the cluster whose partial is not there
   float tok_scale[128];
 };
 
@@ -88,6 +89,14 @@ __device__ __forceinline__ void cluster_arrive() {
 }
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// CTAs of a cluster that add one another's partials: between the barrier after which partials are written
+// and the one after which they are read, a CTA without one (a wait ran out) says so to all; `failed` (zero
+// before the first barrier) is then set in every CTA after the second.
+__device__ __forceinline__ void cluster_report_failure(uint32_t* failed, int ctas) {
+  if (static_cast<int>(threadIdx.x) < ctas)
+    st_shared_cluster_u32(mapa_shared(smem_u32(failed), threadIdx.x), 1u);
 }
 
 __device__ __forceinline__ float activate(float v, int epi) {
@@ -119,6 +128,7 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
 
   if (tid == 0) {
     ctl.abort_flag = 0;
+    ctl.peer_failed = 0;
     for (int s = 0; s < Cfg::kStages; ++s) {
       mbar_init(smem_u32(&ctl.full[s]), 1);
       mbar_init(smem_u32(&ctl.empty[s]), 1);
@@ -232,8 +242,8 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
   const float wscale = p.row_scale_w != nullptr && n < p.N ? p.row_scale_w[n] : 1.0f;
   const float bias = p.epilogue != 0 && n < p.N ? __bfloat162float(p.bias[n]) : 0.0f;
   bool ok = mbar_wait(smem_u32(&ctl.done), 0, p.err, kErrWaitAccum, abort_flag);
-  // the barrier publishes tok_scale; nothing is stored after a wait that ran out (here, or in a
-  // peer of the cluster: its partial then holds whatever its accumulator held)
+  // the barrier publishes tok_scale; nothing is stored after a wait that ran out, here or in a peer of
+  // the cluster
   ok = __syncthreads_and(ok) && !*abort_flag;
   tc_fence_after();
   const uint32_t taddr = tb + (static_cast<uint32_t>(32 * warp) << 16);
@@ -287,8 +297,9 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
     const int width = BN / split;  // columns per rank, at least two
     const uint32_t part = smem_u32(smem);
     const int row = 32 * warp + lane;
+    if (!ok) cluster_report_failure(&ctl.peer_failed, split);
 #pragma unroll 1
-    for (int c0 = 0; c0 < BN; c0 += 16) {
+    for (int c0 = 0; ok && c0 < BN; c0 += 16) {
       uint32_t r[16];
       tmem_ld_x16(taddr + c0, r);
       tmem_ld_wait_x16(r);
@@ -297,12 +308,13 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
         const int owner = (c0 + j) / width, pair = ((c0 + j) % width) / 2;
         const uint32_t at = part + ((rank * (width / 2) + pair) * 128 + row) * 8;
         asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(mapa_shared(at, owner)),
-                     "r"(ok ? r[j] : 0u), "r"(ok ? r[j + 1] : 0u)
+                     "r"(r[j]), "r"(r[j + 1])
                      : "memory");
       }
     }
     cluster_arrive();
     cluster_wait();
+    ok = *reinterpret_cast<volatile uint32_t*>(&ctl.peer_failed) == 0;
     // columns 2 pair .. of this rank: the partials in rank order, four pairs at a time where there are
     // as many (one pair's epilogue is a chain of dependent steps, and a warp has its scheduler alone)
     auto join = [&](int pair, auto& acc) {
@@ -339,6 +351,30 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
     tc_fence_after();
     tmem_dealloc(tb, Cfg::kTmemCols);
   }
+}
+
+// Diagnostic of the exchange above: a cluster whose CTA `failing` waits for an arrival that never comes, with
+// a limit of `limit` cycles; every CTA writes whether it would store.
+__global__ void __launch_bounds__(128) cluster_wait_selftest_kernel(uint32_t* stored, int ctas, int failing,
+                                                                    unsigned long long limit, uint32_t* err) {
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ uint32_t failed;
+  const int rank = static_cast<int>(cluster_ctarank());
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&bar), 1);
+    failed = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const bool ok = rank != failing || mbar_wait(smem_u32(&bar), 0, err, kErrWaitAccum, nullptr, limit);
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (!ok) cluster_report_failure(&failed, ctas);
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (threadIdx.x == 0) stored[rank] = *reinterpret_cast<volatile uint32_t*>(&failed) == 0 ? 1u : 0u;
 }
 
 // w4a4_pair_kernel: tiles of 256 tokens x 256 weight rows on clusters of two CTAs (cta_group::2): CTA

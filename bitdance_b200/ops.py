@@ -409,3 +409,15 @@ def selftest_bounded_wait(limit_cycles: int = 2_000_000, stream=None) -> int:
         raise RuntimeError("device error word already set before the self-test")
     call("bd_selftest_bounded_wait", int(limit_cycles), _stream(stream))
     return device_error(clear=True)
+
+
+def selftest_cluster_wait(ctas: int, failing: int = -1, limit_cycles: int = 2_000_000,
+                          stream=None) -> tuple[int, list[int]]:
+    """Run the diagnostic of partial sums shared by a cluster (bd_selftest_cluster_wait): the device
+    error word it leaves, cleared, and for each of the cluster's CTAs whether it would store."""
+    if device_error(clear=True) != 0:
+        raise RuntimeError("device error word already set before the self-test")
+    stored = torch.full((8,), 7, dtype=torch.int32, device="cuda")
+    call("bd_selftest_cluster_wait", int(limit_cycles), int(ctas), int(failing), _p(stored),
+         _stream(stream))
+    return device_error(clear=True), stored[:ctas].tolist()

@@ -102,6 +102,13 @@ int bd_device_error(uint32_t* word, int clear);
  * reads the status with bd_device_error. 1000 <= limit_cycles <= 4e9. */
 int bd_selftest_bounded_wait(int64_t limit_cycles, bd_stream_t stream);
 
+/* The same for the CTAs of a cluster that add one another's partial sums (bd_w4a4_gemm): in a cluster of
+ * `ctas` (2, 4 or 8) the CTA `failing` (-1: none) waits in vain, sets a bit of BD_DEVERR_WAIT_MASK and tells
+ * the others; stored[r] (a device array of `ctas` words) is 1 where CTA r would store its output, which is
+ * nowhere once one has failed. */
+int bd_selftest_cluster_wait(int64_t limit_cycles, int ctas, int failing, uint32_t* stored,
+                             bd_stream_t stream);
+
 /* Tensor-core peak probe (the FP6 = FP8-rate roofline of the GEMM): one CTA per SM, each
  * issuing mmas_per_cta block-scaled tcgen05.mma.kind::mxf8f6f4 (M = 128, N = n_cols, K = 32,
  * E2M3 x E4M3 operands, E8M0 scales) back to back into one fp32 accumulator, operands on chip;

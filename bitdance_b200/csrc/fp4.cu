@@ -138,8 +138,8 @@ int launch_gemm(GemmFp4Params p, const uint8_t* a, const uint8_t* b, bool overla
   p.n_tiles = (p.N + 127) / 128;
   p.m_tiles = (p.M + BN - 1) / BN;
   const int64_t tiles = static_cast<int64_t>(p.n_tiles) * p.m_tiles;
-  // K slices per tile (a cluster): doubled while the CTAs still fit the machine at once and each
-  // keeps at least two chunks
+  // K slices per tile (a cluster): doubled while the CTAs still fit the machine at once and each keeps a
+  // chunk of its own
   const int chunks = (p.K + kF4ChunkK - 1) / kF4ChunkK;
   int split = 1;
   while (split < 8 && tiles * split * 2 <= static_cast<int64_t>(d->sm_count) * Cfg::kCtasPerSm &&

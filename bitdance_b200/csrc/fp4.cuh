@@ -144,11 +144,12 @@ struct QuantFp4Params {
 };
 
 // Quantiser. G threads share a row: a warp (eight to a CTA, no barriers), or a CTA of four or eight
-// warps, their maxima meeting in shared memory; kKeep pieces of each thread are in flight. A thread takes 16-element pieces t, t + G, ..., keeps the first kKeep of them in
-// registers between the maximum and the codes, and reads the rest of a long row twice (the second time
-// from L2). Measured: 4099 x 14336 fp32 to MXFP4 47 us (5.6 TB/s), 8192 x 14336 bf16 to MXFP4 60 us
-// (5.0 TB/s), 8192 x 4096 bf16 to NVFP4 28 us (3.1 TB/s: two divisions a block and the row's maximum
-// first); 57 % of the issue slots, the integer pipe 60 % busy. Few rows are bound by the launch.
+// warps, their maxima meeting in shared memory; kKeep pieces of each thread are in flight. A thread takes
+// 16-element pieces t, t + G, ..., keeps the first kKeep of them in registers between the maximum and the
+// codes, and reads the rest of a long row twice (the second time from L2). Measured: 4099 x 14336 fp32 to
+// MXFP4 47 us (5.6 TB/s), 8192 x 14336 bf16 to MXFP4 60 us (5.0 TB/s), 8192 x 4096 bf16 to NVFP4 28 us
+// (3.1 TB/s: two divisions a block and the row's maximum first); 57 % of the issue slots, the integer pipe
+// 60 % busy. Few rows are bound by the launch.
 __host__ __device__ constexpr int q4_threads(int G) { return G == 32 ? 256 : G; }
 
 template <int kIn, int kFmt, int G>

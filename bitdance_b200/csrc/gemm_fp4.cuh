@@ -50,14 +50,13 @@ constexpr int cround_up(int x, int a) { return (x + a - 1) / a * a; }
 template <int BN, int kFmt>
 struct GemmFp4Cfg {
   static constexpr int kWords = kFmt == kNvfp4 ? 4 : 2;  // scale words per row and chunk
-  static constexpr int kTBlocks = (BN + 127) / 128;
   static constexpr int kWBytes = 128 * 128;              // weight codes of a stage
   static constexpr int kTBytes = BN * 128;               // token codes
   static constexpr int kSfBytes = 512 * kWords;          // scales of 128 rows
   static constexpr int oT = kWBytes;
   static constexpr int oSw = oT + kTBytes;
   static constexpr int oSt = oSw + kSfBytes;
-  static constexpr int kStage = cround_up(oSt + kTBlocks * kSfBytes, 1024);
+  static constexpr int kStage = cround_up(oSt + kSfBytes, 1024);
   // two CTAs per SM up to 64 tokens (weight streaming: twice the independent schedules), one above
   static constexpr int kCtasPerSm = BN <= 64 ? 2 : 1;
   static constexpr int kBudget = (kCtasPerSm == 2 ? 113 : 226) * 1024 - 2048 - 1024;
@@ -67,7 +66,7 @@ struct GemmFp4Cfg {
   static_assert(BN * 128 * 4 <= kRing, "exchange buffer fits the ring");
   static constexpr int kSmemBytes = kRing + 2048 + 1024;
   // tensor memory: accumulator, then two sets of scale words
-  static constexpr int kSfSet = 4 * kWords * (1 + kTBlocks);
+  static constexpr int kSfSet = 4 * kWords * 2;
   static constexpr int kSfCol0 = BN < 64 ? 64 : BN;
   static constexpr int kUsedCols = kSfCol0 + 2 * kSfSet;
   static constexpr int kTmemCols = kUsedCols <= 128 ? 128 : kUsedCols <= 256 ? 256 : 512;
@@ -150,14 +149,13 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
     if (lane == 0) {
       prefetch_tmap(&tm_w);
       prefetch_tmap(&tm_t);
-      const int t_blocks = min(Cfg::kTBlocks, (p.M - m0 + 127) / 128);
       // words of chunk k present in the tiles
       auto words_of = [&](int k) { return min(Cfg::kWords, p.words - k * Cfg::kWords); };
       auto load_weights = [&](int k, int slot) {
         uint8_t* st = smem + slot * Cfg::kStage;
         const uint32_t fb = smem_u32(&ctl.full[slot]);
         const uint32_t sfb = 512u * words_of(k);
-        mbar_arrive_expect_tx(fb, Cfg::kWBytes + Cfg::kTBytes + sfb * (1 + t_blocks));
+        mbar_arrive_expect_tx(fb, Cfg::kWBytes + Cfg::kTBytes + 2 * sfb);
         tma_load_2d(smem_u32(st), &tm_w, k * 128, n0, fb);
         bulk_load(smem_u32(st + Cfg::oSw),
                   p.sf_w + (static_cast<int64_t>(nt) * p.words + k * Cfg::kWords) * 512, sfb, fb);
@@ -167,10 +165,8 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
         const uint32_t fb = smem_u32(&ctl.full[slot]);
         const uint32_t sfb = 512u * words_of(k);
         tma_load_2d(smem_u32(st + Cfg::oT), &tm_t, k * 128, m0, fb);
-        for (int b = 0; b < t_blocks; ++b)
-          bulk_load(smem_u32(st + Cfg::oSt + b * Cfg::kSfBytes),
-                    p.sf_t + (static_cast<int64_t>(m0 / 128 + b) * p.words + k * Cfg::kWords) * 512,
-                    sfb, fb);
+        bulk_load(smem_u32(st + Cfg::oSt),
+                  p.sf_t + (static_cast<int64_t>(m0 / 128) * p.words + k * Cfg::kWords) * 512, sfb, fb);
       };
       // the first ring of weights before the wait for the previous grid (when it does not write
       // them), the tokens after it
@@ -209,16 +205,13 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
       if (elect_one()) {
         for (int w = 0; w < words; ++w) {
           tmem_cp_32x128b_x4(sfw + 4 * w, sdesc_sf(st + Cfg::oSw + 512 * w));
-#pragma unroll
-          for (int b = 0; b < Cfg::kTBlocks; ++b)
-            tmem_cp_32x128b_x4(sft + 4 * (w * Cfg::kTBlocks + b),
-                               sdesc_sf(st + Cfg::oSt + b * Cfg::kSfBytes + 512 * w));
+          tmem_cp_32x128b_x4(sft + 4 * w, sdesc_sf(st + Cfg::oSt + 512 * w));
         }
         for (int kk = 0; kk < steps; ++kk) {
           const int w = kNv ? kk : kk >> 1;
           const uint32_t idesc = idesc_mxf4(128, BN, !kNv, kNv ? 0 : 2 * (kk & 1));
           mma_mxf4_ss<kNv, false>(tb, sdesc_sw128(st + kk * 32), sdesc_sw128(st + Cfg::oT + kk * 32),
-                                  idesc, sfw + 4 * w, sft + 4 * Cfg::kTBlocks * w,
+                                  idesc, sfw + 4 * w, sft + 4 * w,
                                   (k > k0 || kk > 0) ? 1u : 0u);
         }
         tc_commit(smem_u32(&ctl.empty[r.slot]));

@@ -639,7 +639,7 @@ constexpr int kMoeMmaWarp = kMoeDigitWarp0 + kMoeDigitWarps;
 constexpr int kMoeMakeWarp0 = kMoeMmaWarp + 1, kMoeMakeWarps = 2;
 constexpr int kMoeEpiWarp0 = kMoeMakeWarp0 + kMoeMakeWarps, kMoeEpiWarps = 8;
 constexpr int kMoeExpertThreads = 32 * (kMoeEpiWarp0 + kMoeEpiWarps);
-constexpr int kMoeQueue = 4;
+constexpr int kMoeQueue = 4, kMoeStages = 3;
 
 // 32 lanes x 16 columns of a digit sum: 20 words a lane, 16 more behind every eight lanes, so that
 // neither the stores nor the loads have bank conflicts.
@@ -656,7 +656,7 @@ struct MoeCfg {
   static constexpr int oB = oSw + 2 * 4 * 512;               // digits
   static constexpr int oSb = oB + TOK * kMoeChunkCodes;      // digit scales [block][word][512]
   static constexpr int kStage = oSb + kBlocks * 4 * 512;
-  static constexpr int kStages = 3;
+  static constexpr int kStages = kMoeStages;
   static constexpr int kRaw = 256 * 16;                      // natural weight scales of a stage
   static constexpr int oRaw = kStages * kStage;
   static constexpr int oSum = oRaw + kStages * kRaw;         // a digit sum's buffer per epilogue warp
@@ -671,8 +671,8 @@ struct MoeCfg {
 };
 
 struct MoeCtl {
-  uint64_t full[4], empty[4], raw_full[4], acc_full, acc_empty, qfull[kMoeQueue], qempty[kMoeQueue], drain,
-      down_ready;
+  uint64_t full[kMoeStages], empty[kMoeStages], raw_full[kMoeStages], acc_full, acc_empty;
+  uint64_t qfull[kMoeQueue], qempty[kMoeQueue], drain, down_ready;
   uint32_t queue[kMoeQueue];
   uint32_t abort_flag, tmem_base;
   uint32_t warps;  // epilogue warps that finished their part of a down task

@@ -249,8 +249,8 @@ def w4a4_linear(x: torch.Tensor, weights: Fp4Operand, bias: Optional[torch.Tenso
                 out_dtype=torch.bfloat16, epilogue: str = "none",
                 out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """C = act(quantize_fp4(x) . W^T + bias) from raw activations x (M, K) fp32 / bf16 / fp16, in
-    the weights' format: the quantiser, then the W4A4 GEMM, which streams its first weights while
-    the quantiser runs. bias, epilogue: as in ``w4a4_gemm``."""
+    the weights' format: the quantiser, then the W4A4 GEMM, which for few tokens streams its first
+    weights while the quantiser runs. bias, epilogue: as in ``w4a4_gemm``."""
     M, K = _check_x4(x)
     if weights.K != K:
         raise ValueError(f"K mismatch: activations {K}, weights {weights.K}")

@@ -326,14 +326,14 @@ int bd_dequantize_fp4(const uint8_t* codes, const uint8_t* scales_tiled, const f
  * 4-bit tensor-core MMAs, fp32 accumulation, both operands in format `fmt`, scales tiled; the row
  * scales may be NULL (1). Any N >= 1; no workspace; results do not depend on timing. a, b and the
  * scale tiles 16-byte aligned. flags: BD_GEMM_OVERLAP_PREV, BD_GEMM_WEIGHTS_STATIC (as for
- * bd_w4a6_gemm_ex; b, b_scales). */
+ * bd_w4a6_gemm_ex; b, b_scales; products in tiles of 256 x 256 wait before they load weights too). */
 int bd_w4a4_gemm(void* c, const uint8_t* a, const uint8_t* a_scales, const float* a_row_scale,
                  const uint8_t* b, const uint8_t* b_scales, const float* b_row_scale,
                  float tensor_scale, const void* bias, int M, int N, int K, int fmt,
                  int out_dtype, int epilogue, unsigned flags, bd_stream_t stream);
 
-/* bd_quantize_fp4 of x (M, K), then bd_w4a4_gemm, launched so that the GEMM streams its first
- * weights while the quantiser runs. workspace: bd_query_w4a4_linear_workspace bytes, 256-byte
+/* bd_quantize_fp4 of x (M, K), then bd_w4a4_gemm, launched so that the GEMM starts while the quantiser
+ * runs and, where it is not in tiles of 256 x 256, streams its first weights meanwhile. workspace: bd_query_w4a4_linear_workspace bytes, 256-byte
  * aligned, contents irrelevant before and after; concurrent calls must not share one. */
 size_t bd_query_w4a4_linear_workspace(int M, int K, int fmt);
 int bd_w4a4_linear(void* c, const void* x, int x_dtype, const uint8_t* b, const uint8_t* b_scales,

@@ -207,6 +207,28 @@ int check_gemm(const void* c, const void* bias, int M, int N, int K, int fmt, in
   return BD_OK;
 }
 
+// bd_quantize_fp4; release: as in QuantFp4Params.
+int quantize(const void* x, int x_dtype, int fmt, uint8_t* codes, uint8_t* scales,
+             uint8_t* scales_tiled, float* row_scale, int M, int K, bool overlap,
+             bool release, bd_stream_t stream) {
+  if (bad_fmt(fmt) || x_dtype < BD_IN_F32 || x_dtype > BD_IN_F16) return BD_ERR_INVALID_ARG;
+  if (M < 0 || K <= 0 || K % 32 || M > kMaxRows || K > kMaxK) return BD_ERR_SHAPE;
+  if (M == 0) return BD_OK;
+  if (!x || !codes || (!scales && !scales_tiled)) return BD_ERR_INVALID_ARG;
+  if (fmt == BD_FP4_NVFP4 && !row_scale) return BD_ERR_INVALID_ARG;
+  if (!aligned(x, 16) || !aligned(codes, 16) || (scales_tiled && !aligned(scales_tiled, 16)) ||
+      (row_scale && !aligned(row_scale, 4)))
+    return BD_ERR_ALIGNMENT;
+  DeviceInfo* d = nullptr;
+  const int st = device_info(&d);
+  if (st != BD_OK) return st;
+  const QuantFp4Params p{x, codes, scales, scales_tiled, row_scale, M, K, sf_words(K, fmt),
+                         release ? 1 : 0, d->err};
+  return fmt == BD_FP4_NVFP4
+             ? launch_quantize_in<kNvfp4>(x_dtype, p, overlap, d, as_stream(stream))
+             : launch_quantize_in<kMxfp4>(x_dtype, p, overlap, d, as_stream(stream));
+}
+
 // Workspace of bd_w4a4_linear: codes | scale tiles | row scales, each 256-byte aligned.
 struct LinearWs {
   size_t codes, scales, total;
@@ -236,22 +258,8 @@ int bd_quantize_fp4(const void* x, int x_dtype, int fmt, uint8_t* codes, uint8_t
                     uint8_t* scales_tiled, float* row_scale, int M, int K, unsigned flags,
                     bd_stream_t stream) {
   if (flags & ~static_cast<unsigned>(BD_GEMM_OVERLAP_PREV)) return BD_ERR_INVALID_ARG;
-  if (bad_fmt(fmt) || x_dtype < BD_IN_F32 || x_dtype > BD_IN_F16) return BD_ERR_INVALID_ARG;
-  if (M < 0 || K <= 0 || K % 32 || M > kMaxRows || K > kMaxK) return BD_ERR_SHAPE;
-  if (M == 0) return BD_OK;
-  if (!x || !codes || (!scales && !scales_tiled)) return BD_ERR_INVALID_ARG;
-  if (fmt == BD_FP4_NVFP4 && !row_scale) return BD_ERR_INVALID_ARG;
-  if (!aligned(x, 16) || !aligned(codes, 16) || (scales_tiled && !aligned(scales_tiled, 16)) ||
-      (row_scale && !aligned(row_scale, 4)))
-    return BD_ERR_ALIGNMENT;
-  DeviceInfo* d = nullptr;
-  const int st = device_info(&d);
-  if (st != BD_OK) return st;
-  const QuantFp4Params p{x, codes, scales, scales_tiled, row_scale, M, K, sf_words(K, fmt), d->err};
-  const bool overlap = (flags & BD_GEMM_OVERLAP_PREV) != 0;
-  return fmt == BD_FP4_NVFP4
-             ? launch_quantize_in<kNvfp4>(x_dtype, p, overlap, d, as_stream(stream))
-             : launch_quantize_in<kMxfp4>(x_dtype, p, overlap, d, as_stream(stream));
+  return quantize(x, x_dtype, fmt, codes, scales, scales_tiled, row_scale, M, K,
+                  (flags & BD_GEMM_OVERLAP_PREV) != 0, false, stream);
 }
 
 int bd_tile_scales_fp4(const uint8_t* scales, uint8_t* scales_tiled, int rows, int K, int fmt,
@@ -364,8 +372,7 @@ int bd_w4a4_linear(void* c, const void* x, int x_dtype, const uint8_t* b, const 
   if (!aligned(workspace, 256) || !aligned(x, 16)) return BD_ERR_ALIGNMENT;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   float* row_scale = fmt == BD_FP4_NVFP4 ? reinterpret_cast<float*>(ws + w.scales) : nullptr;
-  st = bd_quantize_fp4(x, x_dtype, fmt, ws, nullptr, ws + w.codes, row_scale, M, K,
-                       BD_GEMM_OVERLAP_PREV, stream);
+  st = quantize(x, x_dtype, fmt, ws, nullptr, ws + w.codes, row_scale, M, K, true, true, stream);
   if (st != BD_OK) return st;
   return bd_w4a4_gemm(c, ws, ws + w.codes, row_scale, b, b_scales, b_row_scale, tensor_scale, bias,
                       M, N, K, fmt, out_dtype, epilogue,

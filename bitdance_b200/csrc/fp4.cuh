@@ -140,6 +140,7 @@ struct QuantFp4Params {
   uint8_t* scales_tiled;  // tiles, may be null
   float* row_scale;       // (M,), NVFP4
   int M, K, words;
+  int release;            // lets the next grid start early: the outputs are activations, not weights
   uint32_t* err;
 };
 
@@ -162,9 +163,11 @@ __global__ void __launch_bounds__(q4_threads(G), (kIn == kInF32 ? 2 : 3) * 256 /
   const int pieces = p.K / 16;
   const int pieces_pad = (pieces + 7) & ~7;  // whole groups of eight: lanes past the end pad tiles
   // In this order: a W4A4 GEMM behind this grid may load weights before it waits, and they may be the
-  // output of the grid before this one.
+  // output of the grid before this one. Where this grid's own output may be weights it releases nothing: the
+  // launch behind it may start the one after, which may stream weights early (weights_static is a promise
+  // about the launch just before).
   grid_dep_wait();
-  grid_dep_launch_dependents();
+  if (p.release) grid_dep_launch_dependents();
   bool bad = false;
   int flip = 0;
   for (int64_t m0 = static_cast<int64_t>(blockIdx.x) * (kQ4Threads / G); m0 < p.M;

@@ -143,7 +143,6 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
   __syncthreads();
   tc_fence_after();
   const uint32_t tb = ctl.tmem_base;
-  grid_dep_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -174,6 +173,8 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
       if (!p.weights_early) grid_dep_wait();
       for (int i = 0; i < first; ++i) load_weights(k0 + i, i);
       grid_dep_wait();
+      // only now: the next grid may load weights that the grid before this one wrote
+      grid_dep_launch_dependents();
       for (int i = 0; i < first; ++i) load_tokens(k0 + i, i);
       RingPos<Cfg::kStages> r;
       if (first == Cfg::kStages) r.phase = 1;
@@ -450,7 +451,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   cluster_sync_all();  // both CTAs' barriers are initialised before anyone arrives
   tc_fence_after();
   const uint32_t tb = ctl.tmem_base;
-  grid_dep_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -459,6 +459,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       prefetch_tmap(&tm_sw);
       prefetch_tmap(&tm_st);
       grid_dep_wait();
+      grid_dep_launch_dependents();
       RingPos<Cfg::kStages> r;
       int issued = 0;
       bool ok = true;

@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
       grid_dep_launch_dependents();
       for (int i = 0; i < first; ++i) load_tokens(k0 + i, i);
       RingPos<Cfg::kStages> r;
-      if (first == Cfg::kStages) r.phase = 1;
+      for (int i = 0; i < first; ++i) r.next();
       for (int k = k0 + first; k < k1; ++k) {
         if (!mbar_wait(smem_u32(&ctl.empty[r.slot]), r.phase ^ 1u, p.err, kErrWaitEmpty,
                        abort_flag))
@@ -186,10 +186,10 @@ __global__ void __launch_bounds__(128, (GemmFp4Cfg<BN, kFmt>::kCtasPerSm))
         load_tokens(k, r.slot);
         r.next();
       }
-      // every copy issued has landed before the CTA goes on (also after a wait ran out)
-      for (int i = max(0, k1 - k0 - Cfg::kStages); i < k1 - k0 && *abort_flag; ++i)
-        mbar_wait(smem_u32(&ctl.full[i % Cfg::kStages]), (i / Cfg::kStages) & 1, p.err, kErrWaitTma,
-                  nullptr);
+      // a wait ran out: what was issued last to each slot lands before the CTA goes on
+      for (int s = 0; s < Cfg::kStages && *abort_flag; ++s)
+        mbar_wait(smem_u32(&ctl.full[s]), r.last_parity(s), p.err, kErrWaitTma, nullptr,
+                  kWaitLimitCycles / 8);
     }
   } else if (warp == 1) {
     RingPos<Cfg::kStages> r;

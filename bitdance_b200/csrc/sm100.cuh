@@ -124,13 +124,35 @@ template <int N>
 struct RingPos {
   int slot = 0;
   uint32_t phase = 0;
-  __device__ __forceinline__ void next() {
+  __host__ __device__ constexpr void next() {
     if (++slot == N) {
       slot = 0;
       phase ^= 1u;
     }
   }
+  // Parity of the last pass that came by slot s: waiting for it on the slot's barrier waits for what was
+  // started there last (at once where nothing was yet: a fresh barrier lets parity 1 through).
+  __host__ __device__ constexpr uint32_t last_parity(int s) const {
+    return s < slot ? phase : phase ^ 1u;
+  }
 };
+// (checked against fills counted one by one)
+template <int N>
+constexpr bool ring_parities_right(int fills) {
+  RingPos<N> r;
+  int count[N] = {};
+  for (int i = 0; i < fills; ++i) {
+    ++count[r.slot];
+    r.next();
+  }
+  for (int s = 0; s < N; ++s)
+    if (r.last_parity(s) != ((count[s] + 1u) & 1u)) return false;
+  return true;
+}
+static_assert(ring_parities_right<3>(0) && ring_parities_right<3>(1) && ring_parities_right<3>(2) &&
+                  ring_parities_right<3>(3) && ring_parities_right<3>(4) && ring_parities_right<3>(7) &&
+                  ring_parities_right<8>(8) && ring_parities_right<8>(13) && ring_parities_right<5>(16),
+              "the last fill of every slot");
 
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

@@ -1387,12 +1387,15 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
     }
   }
   // ------------------------------------------------------------------------------- teardown
-  __syncwarp();
-  if (*abort_flag && warp == 0) {  // a wait ran out: the copies issued land before the CTA exits
-    for (int s = 0; s < Cfg::kStages; ++s)
-      mbar_wait(smem_u32(&ctl.full[s]), 0, p.err, kErrWaitTma, nullptr, kWaitLimitCycles / 8);
-  }
   tc_fence_before();
+  __syncthreads();
+  // A wait ran out: what this warp issued last to each slot (weights; digits) lands before the CTA exits.
+  // Limited: a slot that another role never arrived at does not complete, but its copies do land.
+  if (*abort_flag && (warp == 0 || (warp >= kMoeDigitWarp0 && warp < kMoeMmaWarp))) {
+    for (int s = 0; s < Cfg::kStages; ++s)
+      mbar_wait(smem_u32(&ctl.full[s]), r.last_parity(s), p.err, kErrWaitTma, nullptr,
+                kWaitLimitCycles / 8);
+  }
   __syncthreads();
   if (warp == kMoeMmaWarp) {
     tc_fence_after();

@@ -140,3 +140,39 @@ def test_two_graphs_of_a_layer_replayed_at_once():
     for (y, z), (wy, wz) in zip(got, want):
         assert torch.equal(y, wy) and torch.equal(z, wz)
     assert bd.device_error() == 0
+
+
+def test_every_entry_point_on_a_raw_stream_handle():
+    """stream= as an integer handle, the operands made on that stream too."""
+    import bitdance_b200 as bd
+    from test_moe import Case
+    case = Case(5, 256, 128, 4, seed=1)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(40, 256, device="cuda", generator=g)
+    w = torch.randn(96, 256, device="cuda", generator=g)
+    gate_up = torch.randn(2, 256, 128, device="cuda", generator=g)
+    down = torch.randn(2, 128, 128, device="cuda", generator=g)
+    ids = torch.tensor([[0, 1]] * 5, dtype=torch.int32, device="cuda")
+    weight = torch.rand(5, 2, device="cuda", generator=g)
+
+    def run(**kw):
+        a = bd.quantize_fp4(x, **kw)
+        m, e = bd.quantize_mxfp4(x, **kw)
+        q = [bd.quantize_weights_fp4(w, fmt, **kw) for fmt in ("nvfp4", "mxfp4")]
+        p = bd.pack_fp4(m, e, "mxfp4", **kw)
+        experts = bd.quantize_moe_weights(gate_up, down, **kw)
+        return [bd.w4a4_gemm(a, q[0], **kw), bd.w4a4_gemm(p, q[1], **kw), bd.w4a4_linear(x, q[1], **kw),
+                bd.dequantize_fp4(a, **kw), bd.dequantize_fp4(p, torch.bfloat16, **kw),
+                bd.moe_layer(case.x, case.router, case.w, 2, **kw),
+                bd.moe_experts(case.x, ids, weight, case.w, **kw), experts.gate_up, experts.down_scales]
+
+    want = run()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for stream in (s.cuda_stream, s, torch.cuda.default_stream().cuda_stream):
+        for _ in range(3):
+            got = run(stream=stream)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    assert bd.device_error() == 0

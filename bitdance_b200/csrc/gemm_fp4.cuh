@@ -96,6 +96,7 @@ __device__ __forceinline__ void cluster_wait() {
 __device__ __forceinline__ void cluster_report_failure(uint32_t* failed, int ctas) {
   if (static_cast<int>(threadIdx.x) < ctas)
     st_shared_cluster_u32(mapa_shared(smem_u32(failed), threadIdx.x), 1u);
+  __syncwarp();
 }
 
 __device__ __forceinline__ float activate(float v, int epi) {
@@ -365,7 +366,6 @@ __global__ void __launch_bounds__(128) cluster_wait_selftest_kernel(uint32_t* st
   cluster_arrive();
   cluster_wait();
   if (!ok) cluster_report_failure(&failed, ctas);
-  __syncwarp();
   cluster_arrive();
   cluster_wait();
   if (threadIdx.x == 0) stored[rank] = *reinterpret_cast<volatile uint32_t*>(&failed) == 0 ? 1u : 0u;

@@ -625,11 +625,14 @@ __device__ void moe_plan(const MoeExpertsParams& p, MoePlan& pl) {
 // digits' sum then runs over lanes); with 24 tokens a pass the weights are two tiles of 128 rows and the
 // digits 192 columns.
 // Measured (the layer, GPU time, one call after another): 1 token, 8 of 64 experts of 2048 x 768: 33 us
-// for 21 MB of weights: a chain of latencies (routing 5 to 9, plan 1.5, first stage 3, gate / up 5,
-// epilogue, digits 4, down, combine 3), most of its code run once, from cold instruction caches. 7
-// tokens, 6 of 128 of 4096 x 1408: 84 us (5.2 TB/s while the weights stream); 48 tokens, 8 of 128 of
-// 2048 x 1024: 107 us (4.4 TB/s over this kernel); 64 tokens, 2 of 8 of 4096 x 14336: 196 us (4.2 TB/s): there a stage's MMAs (1000 to 1250 cycles) and the drain of
-// the one accumulator that fits tensor memory beside the scales take nearly as long as its bytes.
+// for 21 MB of weights: a chain of latencies (routing 5 to 9, plan 1.5, first stage 3.5, gate / up 5.5,
+// epilogue and digits 6.5, down 4.5, combine 3), most of its code run once, from cold instruction caches. 7
+// tokens, 6 of 128 of 4096 x 1408: 80 to 85 us (5.5 TB/s while the weights stream); 48 tokens, 8 of 128 of
+// 2048 x 1024: 107 us (4.4 TB/s over this kernel); 64 tokens, 2 of 8 of 4096 x 14336: 180 to 192 us (4.6
+// TB/s): there a stage's MMAs (1000 to 1250 cycles) and the drain of the one accumulator that fits tensor
+// memory beside the scales take nearly as long as its bytes. A pass reads the expert's weights anew: 64
+// tokens of which every one names the same two of 64 experts of 4096 x 2048 take 88 us in four passes for
+// 28 MB of weights.
 // Tried, no gain: a fourth stage of weights (93 us for 91 at seven tokens); scales stored to tensor
 // memory from registers instead of tcgen05.cp (equal with four sets of scale words, 211 us for 199 with
 // the two that fit beside 24 tokens).

@@ -333,8 +333,9 @@ int bd_w4a4_gemm(void* c, const uint8_t* a, const uint8_t* a_scales, const float
                  int out_dtype, int epilogue, unsigned flags, bd_stream_t stream);
 
 /* bd_quantize_fp4 of x (M, K), then bd_w4a4_gemm, launched so that the GEMM starts while the quantiser
- * runs and, where it is not in tiles of 256 x 256, streams its first weights meanwhile. workspace: bd_query_w4a4_linear_workspace bytes, 256-byte
- * aligned, contents irrelevant before and after; concurrent calls must not share one. */
+ * runs and, where it is not in tiles of 256 x 256, streams its first weights meanwhile. workspace:
+ * bd_query_w4a4_linear_workspace bytes, 256-byte aligned, contents irrelevant before and after;
+ * concurrent calls must not share one. */
 size_t bd_query_w4a4_linear_workspace(int M, int K, int fmt);
 int bd_w4a4_linear(void* c, const void* x, int x_dtype, const uint8_t* b, const uint8_t* b_scales,
                    const float* b_row_scale, float tensor_scale, const void* bias, int M, int N,

@@ -71,7 +71,8 @@ int launch_route_parts(const MoeRouteParams& p, cudaStream_t s) {
 
 // Eight parts of K per expert where one warp per expert leaves most of a CTA's warps idle (rows shorter
 // than one round of 8 x 32 lanes x 8 elements have nothing to split). The layer with 8 experts, H 4096,
-// 8 / 32 / 64 tokens: 50 / 54 / 65 us for 51 / 57 / 65 in one part; with 64 experts 118 us for 117.
+// 8 / 32 / 64 tokens: 47 / 51 / 63 us for 50 / 53 / 69 in one part; with 32 of H 2048 equal; with 64 of
+// H 4096, 8 / 64 tokens: 80 / 125 for 76 / 119.
 template <class X, class W>
 int launch_route(const MoeRouteParams& p, cudaStream_t s) {
   return p.E <= 4 * kRouteCluster && p.H >= 2048 ? launch_route_parts<X, W, 8>(p, s)
@@ -162,7 +163,7 @@ int run_experts(void* y, int out_dtype, const int* ids, const float* weights,
     return BD_ERR_CUDA;
   // passes of 16 tokens (half the MMAs) where an expert is expected to have at most about ten, of 24
   // else; an expert with more takes several passes either way. 32 experts of 2048 x 1024 with 8 / 10 /
-  // 12 / 16 tokens each: 52 / 54 / 62 / 71 us in passes of 16, 53 / 55 / 57 / 61 us of 24
+  // 12 / 16 tokens each: 50 / 55 / 60 / 68 us in passes of 16, 56 / 55 / 57 / 62 us of 24
   return T <= 16 || T * k <= 10 * E ? launch_experts<16>(m13, m2, p, d, s)
                                     : launch_experts<24>(m13, m2, p, d, s);
 }

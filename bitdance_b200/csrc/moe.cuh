@@ -129,9 +129,8 @@ __device__ __forceinline__ uint32_t e2m1_pair(float lo, float hi, float& vlo, fl
 
 // Digits of the 16-block `blk` of a row (values v already times the row's 2^shift) into its image.
 // Lanes 4 i .. 4 i + 3 hold four consecutive blocks (one scale word); all lanes of a group come
-// together. kUnroll: digits side by side in the code; one at a time where a warp comes by once or twice
-// and the instructions' way from memory counts (48 tokens 107 us for 108; large experts 199 for 196).
-template <int kUnroll>
+// together. One digit after the other in the code: a warp comes by few times, and the instructions' way
+// from memory counts (side by side, 48 tokens 110 us for 108, 7 tokens 90 for 86.5, large experts equal).
 __device__ __forceinline__ void moe_digits(float (&v)[16], uint8_t* img, int blk) {
   float a = 0.0f;
 #pragma unroll
@@ -150,7 +149,7 @@ __device__ __forceinline__ void moe_digits(float (&v)[16], uint8_t* img, int blk
   uint8_t* scales = chunk + kMoeChunkCodes + (blk & 12);  // rows 2 i and 2 i + 1 by lane i of the four
   *reinterpret_cast<uint32_t*>(scales + (blk & 3) * 32) = word;
   *reinterpret_cast<uint32_t*>(scales + (blk & 3) * 32 + 16) = word;
-#pragma unroll kUnroll
+#pragma unroll 1
   for (int p = 0; p < kMoeDigitRows; ++p) {
     uint32_t w[2] = {0, 0};
     if (p < kMoeDigitCount) {
@@ -192,7 +191,7 @@ __device__ void moe_convert_token(const X* x, uint8_t* xs, float* x_scale, int t
     load8(row + 16 * b + 8, *reinterpret_cast<float(*)[8]>(v + 8));
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] *= up;
-    moe_digits<1>(v, xs + t * moe_image_row(H), b);
+    moe_digits(v, xs + t * moe_image_row(H), b);
   }
   if (threadIdx.x == 0) x_scale[t] = moe_row_factor(am);
 }
@@ -1210,7 +1209,7 @@ __global__ void __launch_bounds__(kMoeExpertThreads, 1)
             v[4 * j + 2] = __uint_as_float(u.z) * up;
             v[4 * j + 3] = __uint_as_float(u.w) * up;
           }
-          moe_digits<Cfg::kSwap ? 1 : kMoeDigitRows>(v, p.hs + pr * moe_image_row(p.I), blk);
+          moe_digits(v, p.hs + pr * moe_image_row(p.I), blk);
         }
       }
       asm volatile("fence.proxy.async;" ::: "memory");

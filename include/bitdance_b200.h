@@ -306,7 +306,8 @@ size_t bd_query_fp4_scales(int rows, int K, int fmt);
  * smallest integer in [-40, 40] with 6 * 2^e >= amax of the 32-block (0 for a zero block), code =
  * nearest E2M1 of x / 2^e. A tie goes to the lower magnitude, the sign is kept on non-zero codes
  * only. NaN / Inf in a row sets BD_DEVERR_NONFINITE and leaves that row's outputs undefined.
- * x, codes and scales_tiled 16-byte aligned. flags: BD_GEMM_OVERLAP_PREV. */
+ * x, codes and scales_tiled 16-byte aligned. flags: BD_GEMM_OVERLAP_PREV. (The output may be weights: a
+ * kernel behind this one starts only when it ends.) */
 int bd_quantize_fp4(const void* x, int x_dtype, int fmt, uint8_t* codes, uint8_t* scales,
                     uint8_t* scales_tiled, float* row_scale, int M, int K, unsigned flags,
                     bd_stream_t stream);
